@@ -233,6 +233,66 @@ int turbofno_query_2d_algo(int bs, int DX, int DY, int K, int N, int algo);
 int turbofno_query_1d_kernel(int logDY, long M, int N, int K, int compute_units, int exchange_attached);
 int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, int exchange_attached);
 
+/*
+ * Operators around the spectral layer: what else a Fourier block does at every position, in training and in serving (no counterpart in the
+ * reference, which stops at the layer). Fields are channel outermost, x[K][P] with P positions (batch and grid) in a row and `ld` elements from one
+ * channel to the next (ld >= P); weights are W[n][k], K in a row. Types: TURBOFNO_C64 (interleaved float re, im), TURBOFNO_F32, TURBOFNO_BF16; sums are
+ * fp32 for all of them, results are rounded once. Activations act on real and imaginary parts separately; TURBOFNO_ACT_GELU_TANH is
+ * z sigmoid(2 sqrt(2 / pi) (z + 0.044715 z^3)). Rows may start at any multiple of their elements' size; P, N and K are any sizes (at most 65536
+ * channels), and with P = 0 nothing is written but the gradients of weights, which are zeros. Pointers that may be NULL say so.
+ *
+ *   turbofno_mix             z = W x + bias + residual, y = act(z): x[K][P] -> y[N][P]. bias [N], residual [N][P] and z [N][P] may be NULL; z is the
+ *                            pre-activation that the gradient needs. residual may be y or z itself. 32-bit products are formed as those of the
+ *                            layer (see "Precision"), sums that come out infinite or NaN again in fp32; parts of operands below 2^-133 are lost.
+ *   turbofno_mix_8bit        the same from 8-bit operands (e4m3, complex values as (re, im) pairs): x = xscale[p] xq[k][p], W = wscale[n] Wq[n][k];
+ *                            type is that of bias, residual and y, ldx counts elements (pairs where they are complex).
+ *   turbofno_mix_input_grad  gz = gy act'(z) (re and im apart), gx[k] = sum_n conj(W[n][k]) gz[n]. gz is the gradient of residual, and what
+ *                            turbofno_mix_weight_grad takes. With TURBOFNO_ACT_NONE gz is gy: z and gz are not used and may be NULL. For bf16, gx is formed
+ *                            from gz as it was rounded.
+ *   turbofno_mix_weight_grad gW[n][k] = sum_p gz[n][p] conj(x[k][p]), gbias[n] = sum_p gz[n][p] (may be NULL), in the type of the fields. On truncated
+ *                            spectra (turbofno_fft_stride_DY, turbofno_fft2d_trunc) gW is also the gradient of the spectral layer's own weights.
+ *                            The sums do not depend on anything but the operands and sizes. Workspace: as queried, 4-byte aligned.
+ *   turbofno_rms_norm        s = x + residual, rstd[p] = 1 / sqrt(mean over k of |s[k][p]|^2 + eps), y[k] = gain[k] rstd s[k]; gain [K] in fp32 for every
+ *                            type. residual, s (not needed without residual) and rstd may be NULL. s and y may be x or residual themselves.
+ *   turbofno_rms_norm_8bit   the same with y in e4m3 and a scale per position: scale[p] = max over k of |y[k][p]| / 448 (real and imaginary parts; 1
+ *                            where that is no normal number), q = y / scale: what turbofno_mix_8bit takes.
+ *   turbofno_rms_norm_backward  gx = gradient of s: that of y through the norm, plus gs (what reaches s by the residual stream; may be NULL). It is
+ *                            that of x and of residual. ggain [K]: gradient of gain. gx may be gy, s or gs itself.
+ *   turbofno_clip_grad_norm  norm = sqrt(sum of |g|^2 over all tensors), on the device; out[i] = grads[i] min(1, max_norm / (norm + 1e-6)). Lists of
+ *                            `count` tensors, on the host, of sizes[i] elements; out[i] may be grads[i], which is left alone when nothing is scaled. The
+ *                            sum is formed in 64 bits. An infinite or NaN value makes norm the same, and every result follows the formula.
+ *                            Workspace: as queried, 8-byte aligned.
+ */
+#define TURBOFNO_C64  0
+#define TURBOFNO_F32  1
+#define TURBOFNO_BF16 2
+
+#define TURBOFNO_ACT_NONE      0
+#define TURBOFNO_ACT_RELU      1
+#define TURBOFNO_ACT_SILU      2
+#define TURBOFNO_ACT_GELU_TANH 3
+
+int turbofno_mix(int type, long P, int N, int K, const void* x, long ldx, const void* W, const void* bias, const void* residual, long ldr,
+                 int act, void* z, long ldz, void* y, long ldy, void* stream);
+int turbofno_mix_8bit(int type, long P, int N, int K, const void* xq, long ldx, const float* xscale, const void* Wq, const float* wscale,
+                      const void* bias, const void* residual, long ldr, int act, void* y, long ldy, void* stream);
+int turbofno_mix_input_grad(int type, long P, int N, int K, const void* gy, long ldgy, const void* z, long ldz, const void* W, int act,
+                            void* gz, long ldgz, void* gx, long ldgx, void* stream);
+size_t turbofno_mix_weight_grad_workspace_bytes(int type, long P, int N, int K);
+int turbofno_mix_weight_grad(int type, long P, int N, int K, const void* gz, long ldgz, const void* x, long ldx, void* gW, void* gbias,
+                             void* workspace, size_t workspace_bytes, void* stream);
+int turbofno_rms_norm(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, float eps,
+                      void* s, long lds, void* y, long ldy, float* rstd, void* stream);
+int turbofno_rms_norm_8bit(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, float eps,
+                           void* s, long lds, void* q, long ldq, float* scale, void* stream);
+size_t turbofno_rms_norm_backward_workspace_bytes(int type, long P, int K);
+int turbofno_rms_norm_backward(int type, long P, int K, const void* gy, long ldgy, const void* s, long lds, const float* gain,
+                               const float* rstd, const void* gs, long ldgs, void* gx, long ldgx, float* ggain, void* workspace,
+                               size_t workspace_bytes, void* stream);
+size_t turbofno_clip_grad_norm_workspace_bytes(int count);
+int turbofno_clip_grad_norm(int count, const void* const* grads, void* const* out, const long* sizes, const int* types, float max_norm,
+                            float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Explanation of the last non-zero return value on this thread ("" if none). Never NULL. */
 const char* turbofno_last_error_string(void);
 

@@ -32,5 +32,18 @@ from .api import (  # noqa: F401
     set_1d_algo,
     set_exchange_wait_us,
 )
+from .operators import (  # noqa: F401
+    clip_grad_norm,
+    mix,
+    mix_8bit,
+    mix_backward,
+    mix_input_grad,
+    mix_weight_grad,
+    mix_weight_grad_workspace_bytes,
+    rms_norm,
+    rms_norm_8bit,
+    rms_norm_backward,
+    rms_norm_backward_workspace_bytes,
+)
 
 ALGO_AUTO, ALGO_THREE_KERNEL, ALGO_WHOLE_IMAGE, ALGO_ROWS_FIRST = 0, 1, 2, 3

@@ -1,14 +1,17 @@
 // C ABI of the library: argument validation, dispatch by transform length, error strings.
 // Declarations and the reference interfaces each entry point replaces are in include/turbofno.h.
 #include "../../include/turbofno.h"
+#include "capi_error.h"
 #include "kernels.h"
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
 namespace {
-
 thread_local char g_err[512] = "";
+}
+
+namespace tfno {
 
 int fail(int code, const char* fmt, ...)
 {
@@ -24,6 +27,13 @@ int hip_status(hipError_t e, const char* what)
     if (e == hipSuccess) return TURBOFNO_OK;
     return fail(TURBOFNO_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
+
+}  // namespace tfno
+
+using tfno::fail;
+using tfno::hip_status;
+
+namespace {
 
 int log2_exact(long v)
 {

@@ -75,7 +75,7 @@ def test_channels_apart_and_rows_that_start_anywhere(kind):
 
 @pytest.mark.parametrize("kind", TYPES)
 def test_residual_in_place(kind):
-    for N, P in ((64, 1000), (150, 77)):
+    for N, P in ((64, 1000), (150, 77), (70, 60003)):
         x, W, b, r = operands(kind, 40, N, (P,), 5)
         want = tf.mix(x, W, b, r, "relu")
         stream = r.clone()

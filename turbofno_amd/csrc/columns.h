@@ -18,6 +18,7 @@ template <int IN> using RawOf = typename Columns<IN>::Raw;
 typedef float4_v float4_any __attribute__((aligned(4)));
 typedef uint2_v uint2_any __attribute__((aligned(2)));
 typedef unsigned uint_any __attribute__((aligned(1)));
+typedef uint2_v uint2_bytes __attribute__((aligned(1)));
 template <int IN> __device__ __forceinline__ RawOf<IN> load4(const void* row, long column)
 {
     const auto* p = static_cast<const typename Columns<IN>::Value*>(row) + column;
@@ -67,6 +68,34 @@ template <int IN> __device__ __forceinline__ RawOf<IN> zero4()
     if constexpr (IN == kIn32) return (float4_v){ 0.f, 0.f, 0.f, 0.f };
     else if constexpr (IN == kIn16) return (uint2_v){ 0u, 0u };
     else return 0u;
+}
+// The same at an address of two parts: one for the whole wave, in scalar registers, and the lane's, of 32 bits. Kept apart from the compiler, which
+// would add them per lane ahead of a loop and hold the 64-bit sums of every row in vector registers.
+#define TFNO_GLOBAL __attribute__((address_space(1)))
+typedef const TFNO_GLOBAL char* ScalarAddress;
+__device__ __forceinline__ long scalar(long v)
+{
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (long)((unsigned long)hi << 32 | lo);
+}
+__device__ __forceinline__ ScalarAddress scalar(const void* base, long bytes) { return reinterpret_cast<ScalarAddress>(scalar(reinterpret_cast<long>(base) + bytes)); }
+// a copy that the compiler does not know: what is made of it, its extension to 64 bits too, stays beside the access (which takes 32) instead of in
+// registers of its own from ahead of a loop
+__device__ __forceinline__ unsigned fresh(unsigned offset)
+{
+    asm volatile("" : "+v"(offset));
+    return offset;
+}
+template <int IN> __device__ __forceinline__ RawOf<IN> near_load4(ScalarAddress base, unsigned offset)
+{
+    if constexpr (IN == kIn32) return *reinterpret_cast<const TFNO_GLOBAL float4_any*>(base + offset);
+    else if constexpr (IN == kIn16) return *reinterpret_cast<const TFNO_GLOBAL uint2_any*>(base + offset);
+    else return *reinterpret_cast<const TFNO_GLOBAL uint_any*>(base + offset);
+}
+template <int IN> __device__ __forceinline__ void near_store4(ScalarAddress base, unsigned offset, RawOf<IN> v)
+{
+    if constexpr (IN == kIn32) *(TFNO_GLOBAL float4_any*)(base + offset) = v;
+    else *(TFNO_GLOBAL uint2_any*)(base + offset) = v;
 }
 __device__ __forceinline__ float value_of(float v) { return v; }
 __device__ __forceinline__ float value_of(unsigned short v) { return __builtin_bit_cast(float, (unsigned)v << 16); }

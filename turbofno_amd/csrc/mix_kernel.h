@@ -140,14 +140,25 @@ __device__ __forceinline__ void load_weights(const void* W, int row, int rows, i
     Value w[8];
     const Value* p = static_cast<const Value*>(W);
     const bool inside = row < rows;
+    if (!GRAD && inside && e + 8 <= count) {
+        p += (long)row * ld * V + e;
+        if constexpr (IN == kIn8) {
+            const RawOf<kIn16> raw = *reinterpret_cast<const uint2_bytes*>(p);
+            __builtin_memcpy(w, &raw, 8);
+        } else {
+            const RawOf<IN> lo = load4<IN>(p, 0), hi = load4<IN>(p, 4);
+            __builtin_memcpy(w, &lo, sizeof lo);
+            __builtin_memcpy(w + 4, &hi, sizeof hi);
+        }
+    } else
 #pragma unroll
-    for (int j = 0; j < 8; j += V) {
-        const int k = (e + j) / V;                       // channel of the contraction
-        const bool there = inside && e + j < count;
-        const long at = there ? (GRAD ? (long)k * ld + row : (long)row * ld + k) * V : 0;
+        for (int j = 0; j < 8; j += V) {
+            const int k = (e + j) / V;                   // channel of the contraction
+            const bool there = inside && e + j < count;
+            const long at = there ? (GRAD ? (long)k * ld + row : (long)row * ld + k) * V : 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) w[j + i] = there ? p[at + i] : (Value)0;
-    }
+            for (int i = 0; i < V; ++i) w[j + i] = there ? p[at + i] : (Value)0;
+        }
     if constexpr (IN == kIn32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -212,144 +223,363 @@ template <bool COMPLEX, bool GRAD> __device__ __forceinline__ float product_fp32
     return sum;
 }
 
-// What a wave does with its columns: the input of a step, and the results
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT> struct MixWave {
+// Columns of a wave: column0 ... column0 + 63, of which `there` exist
+struct Window {
+    long column0;
+    int there;
+};
+
+// What a wave does with its columns: the input of a step, and the results. An address is a uniform part, 64 bits in scalar registers, and the lane's
+// part; FAR: the lane's part may take more than 32 bits, and columns beyond the last may be asked for (the direct kernel).
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct MixWave {
     static constexpr int V = COMPLEX ? 2 : 1, CHANNELS = 32 / V, PER_LANE = 8 / V;      // channels of a step, of a lane
+    typedef RawOf<IN> Rows[PER_LANE];                   // a lane's part of a step
+    typedef typename Columns<OUT>::Value OutValue;
     const MixParams& q;
     int lane, c, kq;
     __device__ __forceinline__ MixWave(const MixParams& params) : q(params), lane(threadIdx.x & 63), c(lane & 15), kq(lane >> 4) { }
 
-    struct Input {
-        RawOf<IN> x[PER_LANE];
-        RawOf<IN> z[GRAD ? PER_LANE : 1];
-    };
-    // rows of step `step` at column0 ... column0 + 63
-    __device__ __forceinline__ void fetch(long column0, int step, Input& in) const
+    // four columns of row `row` (uniform) + lane_row of a field of `rows`; of row `row`, or the last one, where there is none (GUARD)
+    template <int TYPE, bool GUARD> __device__ __forceinline__ RawOf<TYPE> read(const void* base, long ld, int row, int lane_row, int rows, const Window& w) const
     {
-        const int first = step * CHANNELS + kq * PER_LANE;
-        const long column = column0 + 4 * c;
-        const auto* x = static_cast<const typename Columns<IN>::Value*>(q.x);
-        const auto* z = static_cast<const typename Columns<IN>::Value*>(q.zin);
-        const bool slopes = GRAD && q.act != kActNone;
-        if ((step + 1) * CHANNELS <= q.contraction && column0 + kColumns <= q.columns) {
-#pragma unroll
-            for (int j = 0; j < PER_LANE; ++j) in.x[j] = load4<IN>(x + (first + j) * q.ldx, column);
-            if constexpr (GRAD) if (slopes)
-#pragma unroll
-                for (int j = 0; j < PER_LANE; ++j) in.z[j] = load4<IN>(z + (first + j) * q.ldzin, column);
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < PER_LANE; ++j) {
-            const bool there = first + j < q.contraction;
-            const int k = there ? first + j : q.contraction - 1;
-            in.x[j] = load4_ragged<IN>(x + k * q.ldx, column, q.columns);
-            if constexpr (GRAD) if (slopes) in.z[j] = load4_ragged<IN>(z + k * q.ldzin, column, q.columns);
-            if (!there) {
-                in.x[j] = zero4<IN>();
-                if constexpr (GRAD) in.z[j] = zero4<IN>();
-            }
+        typedef typename Columns<TYPE>::Value Value;
+        const bool there = !GUARD || row + lane_row < rows;
+        if (GUARD) row = row < rows ? row : rows - 1;
+        const long at = row * ld + w.column0;
+        if constexpr (FAR) {
+            const Value* p = static_cast<const Value*>(base) + at + (there ? lane_row * ld : 0);
+            return w.there < kColumns ? load4_ragged<TYPE>(p, 4 * c, w.there) : load4<TYPE>(p, 4 * c);
+        } else {
+            unsigned offset = fresh(((unsigned)lane_row * (unsigned)ld + 4 * c) * (unsigned)sizeof(Value));
+            if (GUARD) offset = there ? offset : 4 * c * (unsigned)sizeof(Value);
+            return near_load4<TYPE>(scalar(base, at * (long)sizeof(Value)), offset);
         }
     }
-    // gradient: the input through the activation, written out by one of the waves that share these columns
-    __device__ __forceinline__ void slope(long column0, int step, Input& in, bool write) const
+    template <int TYPE> __device__ __forceinline__ void write(void* base, long ld, int row, int lane_row, const Window& w, RawOf<TYPE> v) const
     {
-        if constexpr (GRAD) {
-            if (q.act == kActNone) return;
-            const int first = step * CHANNELS + kq * PER_LANE;
-            auto* gz = static_cast<typename Columns<IN>::Value*>(q.z);
+        typedef typename Columns<TYPE>::Value Value;
+        const long at = row * ld + w.column0;
+        if constexpr (FAR) {
+            Value* p = static_cast<Value*>(base) + at + lane_row * ld;
+            if (w.there < kColumns) store4_ragged<TYPE>(p, 4 * c, w.there, v);
+            else store4<TYPE>(p, 4 * c, v);
+        } else near_store4<TYPE>(scalar(base, at * (long)sizeof(Value)), fresh(((unsigned)lane_row * (unsigned)ld + 4 * c) * (unsigned)sizeof(Value)), v);
+    }
+    // the lane's rows of step `step` of `base`: channels beyond the last are zeros
+    __device__ __forceinline__ void fetch(const void* base, long ld, const Window& w, int step, Rows& rows) const
+    {
+        const int first = step * CHANNELS, lane_row = kq * PER_LANE;
+        if (first + CHANNELS <= q.contraction) {
+#pragma unroll
+            for (int j = 0; j < PER_LANE; ++j) rows[j] = read<IN, false>(base, ld, first + j, lane_row, q.contraction, w);
+        } else
 #pragma unroll
             for (int j = 0; j < PER_LANE; ++j) {
-                const float4_v gy = to_float<IN>(in.x[j]), z = to_float<IN>(in.z[j]);
-                float4_v g;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) g[i] = through_activation(q.act, gy[i], z[i]);
-                in.x[j] = from_float<IN>(g);
-                if (write && first + j < q.contraction) {
-                    if (column0 + kColumns <= q.columns) store4<IN>(gz + (first + j) * q.ldz, column0 + 4 * c, in.x[j]);
-                    else store4_ragged<IN>(gz + (first + j) * q.ldz, column0 + 4 * c, q.columns, in.x[j]);
-                }
+                rows[j] = read<IN, true>(base, ld, first + j, lane_row, q.contraction, w);
+                if (first + j + lane_row >= q.contraction) rows[j] = zero4<IN>();
             }
+    }
+    // gradient: gy through the activation at z, written out by one of the waves that share these columns
+    __device__ __forceinline__ void slope(const Window& w, int step, Rows& x, const Rows& zin, bool writes) const
+    {
+        if (q.act == kActGeluTanh) slope_of<kActGeluTanh>(w, step, x, zin, writes);
+        else if (q.act == kActSilu) slope_of<kActSilu>(w, step, x, zin, writes);
+        else slope_of<kActRelu>(w, step, x, zin, writes);
+    }
+    template <int ACT> __device__ __forceinline__ void slope_of(const Window& w, int step, Rows& x, const Rows& zin, bool writes) const
+    {
+        const int first = step * CHANNELS, lane_row = kq * PER_LANE;
+        const bool whole = first + CHANNELS <= q.contraction;
+#pragma unroll
+        for (int j = 0; j < PER_LANE; ++j) {
+            const float4_v gy = to_float<IN>(x[j]), z = to_float<IN>(zin[j]);
+            float4_v g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) g[i] = through_activation(ACT, gy[i], z[i]);
+            x[j] = from_float<IN>(g);
+            if (writes && (whole || first + lane_row + j < q.contraction)) write<IN>(q.z, q.ldz, first + j, lane_row, w, x[j]);
         }
     }
-    // results of rows row0 + 16 t + 4 kq + i: acc[t][b][i] belongs to column 4 c + b
-    __device__ __forceinline__ void finish(long column0, int row0, float4_v (&acc)[NT][4]) const
+    // sums that are not finite, again in fp32
+    __device__ __forceinline__ void mend(const Window& w, int row0, float4_v (&acc)[NT][4]) const
     {
-        const long column = column0 + 4 * c;
-        const bool full = column0 + kColumns <= q.columns;
-        typedef typename Columns<OUT>::Value Value;
-        float4_v xs = { 1.f, 1.f, 1.f, 1.f };
-        if constexpr (IN == kIn8) {                     // scales of the lane's columns
-#pragma unroll
-            for (int b = 0; b < 4; ++b) xs[b] = q.xscale[(column + b < q.columns ? column + b : q.columns - 1) / V];
-        }
+        float high = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = row0 + 16 * t + 4 * kq + i;
-                if (row >= q.rows) continue;
-                float4_v v = { acc[t][0][i], acc[t][1][i], acc[t][2][i], acc[t][3][i] };
-                if constexpr (IN == kIn32) {
-                    if (__builtin_expect(not_finite(larger(0.f, v), 0.f), 0))
-                        for (int b = 0; b < 4; ++b)
-                            if (not_finite(__builtin_fabsf(v[b]), 0.f)) v[b] = product_fp32<COMPLEX, GRAD>(q, row, column + b < q.columns ? column + b : q.columns - 1);
-                }
-                if constexpr (IN == kIn8) v *= xs * q.wscale[row];
-                if constexpr (!GRAD) {
-                    if (q.bias) {
-                        const Value* bias = static_cast<const Value*>(q.bias) + (long)row * V;
-                        const float b0 = value_of(bias[0]), b1 = COMPLEX ? value_of(bias[V - 1]) : b0;
-                        v += (float4_v){ b0, b1, b0, b1 };
-                    }
-                    if (q.residual) {
-                        const Value* r = static_cast<const Value*>(q.residual) + row * q.ldr;
-                        v += to_float<OUT>(full ? load4<OUT>(r, column) : load4_ragged<OUT>(r, column, q.columns));
-                    }
-                    if (q.z) write(static_cast<Value*>(q.z) + row * q.ldz, column, full, from_float<OUT>(v));
-                    if (q.act != kActNone)
+            for (int b = 0; b < 4; ++b) high = larger(high, acc[t][b]);
+        if (__builtin_expect(!any_lane(not_finite(high, 0.f)), 1)) return;
+        unsigned long long wrong = 0;                   // a bit for each of the lane's sums
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) v[b] = activate(q.act, v[b]);
-                }
-                write(static_cast<Value*>(q.y) + row * q.ldy, column, full, from_float<OUT>(v));
-            }
+        for (int e = 0; e < 16 * NT; ++e)
+            if (not_finite(__builtin_fabsf(acc[e / 16][e / 4 % 4][e % 4]), 0.f)) wrong |= 1ull << e;
+#pragma unroll 1
+        for (int e = 0; e < 16 * NT; ++e) {
+            const bool here = wrong >> e & 1;
+            if (!any_lane(here)) continue;
+            const int row = row0 + 16 * (e / 16) + 4 * kq + e % 4, column = 4 * c + e / 4 % 4;
+            const float v = here && row < q.rows ? product_fp32<COMPLEX, GRAD>(q, row, w.column0 + (column < w.there ? column : w.there - 1)) : 0.f;
+#pragma unroll
+            for (int f = 0; f < 16 * NT; ++f)
+                if (here && f == e) acc[f / 16][f / 4 % 4][f % 4] = v;
+        }
     }
-    __device__ __forceinline__ void write(void* row, long column, bool full, RawOf<OUT> v) const
+    // results of rows row0 + 16 t + 4 kq + i: acc[t][b][i] belongs to column 4 c + b
+    // bias(t): the bias of the lane's four rows of 16 rows t, real and imaginary parts apart
+    template <typename Bias> __device__ __forceinline__ void finish(const Window& w, int row0, float4_v (&acc)[NT][4], Bias bias) const
     {
-        if (full) store4<OUT>(row, column, v);
-        else store4_ragged<OUT>(row, column, q.columns, v);
+        if constexpr (IN == kIn32) mend(w, row0, acc);
+        RawOf<OUT> residual[GRAD ? 1 : NT][4];          // all loads first
+        float4_v xs = { 1.f, 1.f, 1.f, 1.f }, ws[IN == kIn8 ? NT : 1];
+        if constexpr (!GRAD) {
+            if (q.residual)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int first = row0 + 16 * t;
+                    if (first + 16 <= q.rows)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) residual[t][i] = read<OUT, false>(q.residual, q.ldr, first + i, 4 * kq, q.rows, w);
+                    else if (first < q.rows)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) residual[t][i] = read<OUT, true>(q.residual, q.ldr, first + i, 4 * kq, q.rows, w);
+                }
+        }
+        if constexpr (IN == kIn8) {                     // scales of the lane's columns and rows
+#pragma unroll
+            for (int b = 0; b < 4; ++b) xs[b] = q.xscale[(w.column0 + (!FAR || 4 * c + b < w.there ? 4 * c + b : w.there - 1)) / V];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = row0 + 16 * t + 4 * kq + i;
+                    ws[t][i] = q.wscale[row < q.rows ? row : q.rows - 1];
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (row0 + 16 * t >= q.rows) break;
+            float4_v v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = (float4_v){ acc[t][0][i], acc[t][1][i], acc[t][2][i], acc[t][3][i] };
+                if constexpr (IN == kIn8) v[i] *= xs * ws[t][i];
+            }
+            if constexpr (!GRAD) {
+                if (q.bias) {
+                    const Parts p = bias(t);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] += (float4_v){ p.v[0][i], p.v[V - 1][i], p.v[0][i], p.v[V - 1][i] };
+                }
+                if (q.residual)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] += to_float<OUT>(residual[t][i]);
+                if (q.z) put(q.z, q.ldz, row0 + 16 * t, w, v);
+                if (q.act == kActGeluTanh) act_rows<kActGeluTanh>(v);
+                else if (q.act == kActSilu) act_rows<kActSilu>(v);
+                else if (q.act == kActRelu) act_rows<kActRelu>(v);
+            }
+            put(q.y, q.ldy, row0 + 16 * t, w, v);
+        }
+    }
+    struct Parts {
+        float4_v v[V];
+    };
+    __device__ __forceinline__ Parts bias_of(int first) const       // of rows first ... first + 3; of the last one beyond it
+    {
+        Parts p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) p.v[j][i] = value_of(static_cast<const OutValue*>(q.bias)[(long)(first + i < q.rows ? first + i : q.rows - 1) * V + j]);
+        return p;
+    }
+    template <int ACT> static __device__ __forceinline__ void act_rows(float4_v (&v)[4])
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) v[i][b] = activate(ACT, v[i][b]);
+    }
+    // rows first + 4 kq + i
+    __device__ __forceinline__ void put(void* base, long ld, int first, const Window& w, const float4_v (&v)[4]) const
+    {
+        if (first + 16 <= q.rows)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) write<OUT>(base, ld, first + i, 4 * kq, w, from_float<OUT>(v[i]));
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (first + 4 * kq + i < q.rows) write<OUT>(base, ld, first + i, 4 * kq, w, from_float<OUT>(v[i]));
     }
 };
 
-// A wave for 64 columns and 16 NT rows, weights from memory
+// Few columns: a wave for 64 columns and 16 NT rows, weights from memory
 template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT>
 __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, int row_groups)
 {
-    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT> Wave;
-    const Wave w(q);
-    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, true> Wave;
+    const Wave wave(q);
+    const long id = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long column0 = id / row_groups * kColumns;
     const int row0 = (int)(id % row_groups) * (16 * NT);
     if (column0 >= q.columns) return;
+    const Window w = { column0, q.columns - column0 < kColumns ? (int)(q.columns - column0) : (int)kColumns };
+    const bool slopes = GRAD && q.act != kActNone;
     const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
     float4_v acc[NT][4] = {};
-    typename Wave::Input in;
-    w.fetch(column0, 0, in);
+    typename Wave::Rows x, z, xnext, znext;
+    auto fetch = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
+        wave.fetch(q.x, q.ldx, w, s, x);
+        if (slopes) wave.fetch(q.zin, q.ldzin, w, s, z);
+    };
+    fetch(0, x, z);
     for (int s = 0; s < steps; ++s) {
-        typename Wave::Input next = in;
-        if (s + 1 < steps) w.fetch(column0, s + 1, next);
-        w.slope(column0, s, in, row0 == 0);
+        if (s + 1 < steps) fetch(s + 1, xnext, znext);
+        if constexpr (GRAD)
+            if (slopes) wave.slope(w, s, x, z, row0 == 0);
         Operand<IN> b[4];
-        make_operands<IN, COMPLEX, GRAD>(in.x, b);
+        make_operands<IN, COMPLEX, GRAD>(x, b);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             Operand<IN> a;
-            load_weights<IN, COMPLEX, GRAD>(q.W, row0 + 16 * t + w.c, q.rows, 32 * s + 8 * w.kq, q.contraction * Wave::V, q.ldw, a);
+            load_weights<IN, COMPLEX, GRAD>(q.W, row0 + 16 * t + wave.c, q.rows, 32 * s + 8 * wave.kq, q.contraction * Wave::V, q.ldw, a);
             multiply<IN>(a, b, acc[t]);
         }
-        in = next;
+#pragma unroll
+        for (int j = 0; j < Wave::PER_LANE; ++j) {
+            x[j] = xnext[j];
+            if constexpr (GRAD) z[j] = znext[j];
+        }
     }
-    w.finish(column0, row0, acc);
+    wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); });
+}
+
+// f(0) ... f(N - 1) with no loop left, so that registers are indexed by constants
+template <int N, int I = 0, typename F> __device__ __forceinline__ void unrolled(F&& f)
+{
+    if constexpr (I < N) {
+        f(I);
+        unrolled<N, I + 1>(f);
+    }
+}
+
+// Many columns: the operands of the block's rows of A stay in LDS, in the order in which lanes read them (16 bytes per lane, part, 16 rows and step), and
+// its waves walk the columns without meeting again. HELD steps of the input stay in registers while the rows are walked, and are asked for again for
+// the next columns as the last rows use them up; HELD = 0: steps are read as they are needed, once for every 16 NT rows.
+constexpr int kWaveParts(int in) { return in == kIn32 ? 3 : 1; }
+constexpr int kResidentThreads = 512;
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD>
+__global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const MixParams q, int block_rows, int tiles)
+{
+    extern __shared__ uint4_v weights[];
+    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, false> Wave;
+    constexpr int PARTS = kWaveParts(IN);
+    const Wave wave(q);
+    const int row_first = blockIdx.y * block_rows, groups = block_rows / (16 * NT);
+    const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
+    const bool slopes = GRAD && q.act != kActNone, writes = blockIdx.y == 0;
+    {
+        const int per_step = block_rows / 16 * 64, count = steps * per_step;
+#pragma unroll 4
+        for (int e = threadIdx.x; e < count; e += blockDim.x) {
+            const int s = e / per_step, rest = e % per_step, t = rest / 64, l = rest % 64;
+            Operand<IN> a;
+            load_weights<IN, COMPLEX, GRAD>(q.W, row_first + 16 * t + (l & 15), q.rows, 32 * s + 8 * (l >> 4), q.contraction * Wave::V, q.ldw, a);
+            uint4_v* to = weights + (long)(e / 64) * (64 * PARTS) + l;
+            if constexpr (IN == kIn32) { to[0] = a.h; to[64] = a.m; to[128] = a.l; }
+            else to[0] = a.v;
+        }
+    }
+    typedef typename Wave::Parts Parts;
+    Parts* biases = reinterpret_cast<Parts*>(weights + (long)steps * block_rows * (4 * PARTS));
+    if constexpr (!GRAD)
+        if (q.bias)
+            for (int e = threadIdx.x; e < block_rows / 4; e += blockDim.x) biases[e] = wave.bias_of(row_first + 4 * e);
+    __syncthreads();
+    auto weight = [&](int s, int t16) {                 // operand of step s, 16 rows t16
+        const uint4_v* from = weights + (long)(s * (block_rows / 16) + t16) * (64 * PARTS) + wave.lane;
+        Operand<IN> a;
+        if constexpr (IN == kIn32) { a.h = from[0]; a.m = from[64]; a.l = from[128]; }
+        else a.v = from[0];
+        return a;
+    };
+    // tiles are counted in 32 bits: 64-bit numbers are compared in vector registers. A last tile that is not whole ends with the columns
+    auto window = [&](int tile) { return Window{ scalar(tile < tiles - 1 ? (long)tile * kColumns : q.columns - kColumns), kColumns }; };
+    const int stride = gridDim.x * (blockDim.x >> 6);
+    int tile = blockIdx.x * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (tile >= tiles) return;
+    Window w = window(tile);
+    if constexpr (HELD > 0) {
+        typename Wave::Rows x[HELD];
+#pragma unroll
+        for (int s = 0; s < HELD; ++s)
+            if (s < steps) wave.fetch(q.x, q.ldx, w, s, x[s]);
+        for (;;) {
+            if constexpr (GRAD)
+                if (slopes) {
+                    constexpr int AHEAD = IN == kIn32 ? (COMPLEX ? 2 : 1) : HELD < 4 ? HELD : 4;          // steps of z on their way
+                    typename Wave::Rows z[AHEAD];
+#pragma unroll
+                    for (int s = 0; s < AHEAD; ++s)
+                        if (s < steps) wave.fetch(q.zin, q.ldzin, w, s, z[s]);
+                    unrolled<HELD>([&](int s) {
+                        if (s < steps) {
+                            wave.slope(w, s, x[s], z[s % AHEAD], writes);
+                            if (s + AHEAD < steps) wave.fetch(q.zin, q.ldzin, w, s + AHEAD, z[s % AHEAD]);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    });
+                }
+            const int next = tile + stride;
+            const bool more = next < tiles;
+            const Window wn = window(more ? next : tile);
+            for (int g = 0; g < groups; ++g) {
+                float4_v acc[NT][4] = {};
+                unrolled<HELD>([&](int s) {
+                    if (s < steps) {
+                        Operand<IN> b[4];
+                        make_operands<IN, COMPLEX, GRAD>(x[s], b);
+                        if (more && g == groups - 1) wave.fetch(q.x, q.ldx, wn, s, x[s]);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                });
+                wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; });
+            }
+            if (!more) return;
+            tile = next;
+            w = wn;
+        }
+    } else {
+        for (; tile < tiles; tile += stride) {
+            w = window(tile);
+            for (int g = 0; g < groups; ++g) {
+                float4_v acc[NT][4] = {};
+                typename Wave::Rows x, z, xnext, znext;
+                auto fetch = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
+                    wave.fetch(q.x, q.ldx, w, s, x);
+                    if (slopes) wave.fetch(q.zin, q.ldzin, w, s, z);
+                };
+                fetch(0, x, z);
+                for (int s = 0; s < steps; ++s) {
+                    if (s + 1 < steps) fetch(s + 1, xnext, znext);
+                    if constexpr (GRAD)
+                        if (slopes) wave.slope(w, s, x, z, writes && g == 0);
+                    Operand<IN> b[4];
+                    make_operands<IN, COMPLEX, GRAD>(x, b);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
+#pragma unroll
+                    for (int j = 0; j < Wave::PER_LANE; ++j) {
+                        x[j] = xnext[j];
+                        if constexpr (GRAD) z[j] = znext[j];
+                    }
+                }
+                wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; });
+            }
+        }
+    }
 }
 
 }  // namespace tfno

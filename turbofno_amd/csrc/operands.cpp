@@ -6,8 +6,11 @@
 // Nothing here decides that a call is wrong: whatever does not pass is handed back (None, or -1) and takes the checks in Python,
 // which raise. Only plain torch.Tensor / Parameter objects are looked at, so subclasses and wrappers keep their own behaviour, and
 // nothing is kept from one call to the next.
+#include "../../include/turbofno.h"
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty.h>
 #include <climits>
+#include <vector>
 
 namespace {
 
@@ -148,10 +151,315 @@ PyObject* layer_2d(PyObject*, PyObject* const* args, Py_ssize_t count)
     return PyLong_FromLong(rc);
 }
 
+// ---- the operators around the layer (turbofno_amd/operators.py): the same checks as there, in the same order of trust: whatever does not pass is
+// handed back as -1 ----
+
+using Mix = decltype(&turbofno_mix);
+using Mix8bit = decltype(&turbofno_mix_8bit);
+using InputGrad = decltype(&turbofno_mix_input_grad);
+using WeightGrad = decltype(&turbofno_mix_weight_grad);
+using WeightGradBytes = decltype(&turbofno_mix_weight_grad_workspace_bytes);
+using Norm = decltype(&turbofno_rms_norm);
+using NormGrad = decltype(&turbofno_rms_norm_backward);
+using NormGradBytes = decltype(&turbofno_rms_norm_backward_workspace_bytes);
+using Clip = decltype(&turbofno_clip_grad_norm);
+using ClipBytes = decltype(&turbofno_clip_grad_norm_workspace_bytes);
+
+struct NotHere { };                                     // an operand for Python to judge
+
+int type_of(const at::Tensor& t)
+{
+    switch (t.scalar_type()) {
+    case at::kComplexFloat: return TURBOFNO_C64;
+    case at::kFloat: return TURBOFNO_F32;
+    case at::kBFloat16: return TURBOFNO_BF16;
+    default: throw NotHere();
+    }
+}
+// a tensor of that type on that GPU whose memory holds its values
+const at::Tensor& on_gpu(PyObject* o, at::ScalarType type, int device)
+{
+    if (!THPVariable_CheckExact(o)) throw NotHere();
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || !t.is_cuda() || t.scalar_type() != type || t.get_device() != device || t.is_conj() || t.is_neg()) throw NotHere();
+    return t;
+}
+const at::Tensor& first_operand(PyObject* o, int device)
+{
+    if (!THPVariable_CheckExact(o)) throw NotHere();
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || t.dim() < 2 || t.size(0) <= 0) throw NotHere();
+    return on_gpu(o, t.scalar_type(), device);
+}
+struct Field {
+    void* data = nullptr;
+    long ld = 0;
+};
+// distance between channels; the dimensions after the first have to lie side by side
+long spread(const at::Tensor& t, long parts = 1)
+{
+    int64_t step = 1;
+    for (int64_t i = t.dim() - 1; i > 0; --i) {
+        if (t.size(i) != 1 && t.stride(i) != step) throw NotHere();
+        step *= t.size(i);
+    }
+    const int64_t ld = t.size(0) > 1 ? t.stride(0) : step;
+    if (ld % parts) throw NotHere();
+    return ld / parts;
+}
+// a field of `channels` channels with the positions of `like` (whose last dimension is (re, im) where `like_pairs`), with a last dimension of two where `pairs`
+Field field(PyObject* o, at::ScalarType type, int device, int64_t channels, const at::Tensor& like, bool pairs = false, bool like_pairs = false, bool optional = false)
+{
+    if (optional && o == Py_None) return {};
+    const at::Tensor& t = on_gpu(o, type, device);
+    const int64_t dims = like.dim() - (like_pairs ? 1 : 0);
+    if (t.dim() != dims + (pairs ? 1 : 0) || t.size(0) != channels || (pairs && t.size(dims) != 2)) throw NotHere();
+    for (int64_t i = 1; i < dims; ++i)
+        if (t.size(i) != like.size(i)) throw NotHere();
+    return { t.data_ptr(), spread(t, pairs ? 2 : 1) };
+}
+// a contiguous tensor of those sizes
+void* packed(PyObject* o, at::ScalarType type, int device, std::initializer_list<int64_t> sizes, bool optional = false)
+{
+    if (optional && o == Py_None) return nullptr;
+    const at::Tensor& t = on_gpu(o, type, device);
+    if (!t.is_contiguous() || t.sizes() != at::IntArrayRef(sizes)) throw NotHere();
+    return t.data_ptr();
+}
+// one value per position of `like`
+void* per_position(PyObject* o, int device, const at::Tensor& like, bool like_pairs = false)
+{
+    const at::Tensor& t = on_gpu(o, at::kFloat, device);
+    const int64_t dims = like.dim() - (like_pairs ? 1 : 0);
+    if (!t.is_contiguous() || t.dim() != dims - 1) throw NotHere();
+    for (int64_t i = 1; i < dims; ++i)
+        if (t.size(i - 1) != like.size(i)) throw NotHere();
+    return t.data_ptr();
+}
+long positions(const at::Tensor& t, bool pairs = false) { return t.numel() / t.size(0) / (pairs ? 2 : 1); }
+int channels(int64_t n)
+{
+    if (n <= 0 || !fits_int(n)) throw NotHere();
+    return (int)n;
+}
+template <typename F> F function(PyObject* o)
+{
+    bool ok;
+    void* p = pointer_value(o, ok);
+    if (!ok || !p) throw NotHere();
+    return reinterpret_cast<F>(p);
+}
+int small(PyObject* o)
+{
+    long long v;
+    if (!integer_value(o, v) || !fits_int(v)) throw NotHere();
+    return (int)v;
+}
+void* stream_of(PyObject* o)
+{
+    bool ok;
+    void* p = pointer_value(o, ok);
+    if (!ok) throw NotHere();
+    return p;
+}
+float real_value(PyObject* o)
+{
+    const double v = PyFloat_AsDouble(o);
+    if (PyErr_Occurred()) throw NotHere();
+    return (float)v;
+}
+// the caller's workspace, or memory that is free again, in the order of the stream, when the call returns
+struct Workspace {
+    at::Tensor held;
+    void* data;
+    size_t bytes;
+    Workspace(PyObject* o, size_t need, const at::Tensor& like, int device)
+    {
+        if (o == Py_None) held = at::empty({ (int64_t)need }, like.options().dtype(at::kByte));
+        else {
+            held = on_gpu(o, at::kByte, device);
+            if (!held.is_contiguous()) throw NotHere();
+        }
+        data = held.data_ptr();
+        bytes = (size_t)held.numel();
+    }
+};
+// body() -> status; anything that it throws leaves the call to Python
+template <typename F> PyObject* judged(bool counted, F body)
+{
+    int rc = -1;
+    if (counted) {
+        try {
+            rc = body();
+        } catch (...) {
+            PyErr_Clear();
+            rc = -1;
+        }
+    }
+    return PyLong_FromLong(rc);
+}
+
+// mix(function, x, W, bias, residual, activation, y, z, device, stream)
+PyObject* mix(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 10, [&] {
+        const auto call = function<Mix>(args[0]);
+        const int device = small(args[8]), act = small(args[5]);
+        void* stream = stream_of(args[9]);
+        const at::Tensor& x = first_operand(args[1], device);
+        const at::ScalarType dt = x.scalar_type();
+        const int type = type_of(x), K = channels(x.size(0));
+        if (!THPVariable_CheckExact(args[2]) || THPVariable_Unpack(args[2]).dim() != 2) throw NotHere();
+        const int N = channels(THPVariable_Unpack(args[2]).size(0));
+        const void *W = packed(args[2], dt, device, { N, K }), *bias = packed(args[3], dt, device, { N }, true);
+        const Field fx = field(args[1], dt, device, K, x), r = field(args[4], dt, device, N, x, false, false, true);
+        const Field y = field(args[6], dt, device, N, x), z = field(args[7], dt, device, N, x, false, false, true);
+        const long P = positions(x);
+        const WithoutLock unlocked;
+        return call(type, P, N, K, fx.data, fx.ld, W, bias, r.data, r.ld, act, z.data, z.ld, y.data, y.ld, stream);
+    });
+}
+
+// mix_8bit(function, xq, xscale, Wq, wscale, bias, residual, activation, y, device, stream)
+PyObject* mix_8bit(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 11, [&] {
+        const auto call = function<Mix8bit>(args[0]);
+        const int device = small(args[9]), act = small(args[7]);
+        void* stream = stream_of(args[10]);
+        const at::Tensor& x = first_operand(args[1], device);
+        if (x.scalar_type() != at::kFloat8_e4m3fn || !THPVariable_CheckExact(args[8]) || !THPVariable_CheckExact(args[3])) throw NotHere();
+        const at::Tensor& out = THPVariable_Unpack(args[8]);
+        const int type = type_of(out), K = channels(x.size(0)), N = channels(THPVariable_Unpack(args[3]).size(0));
+        const bool pairs = type == TURBOFNO_C64;
+        const at::ScalarType dt = out.scalar_type();
+        if (pairs && (x.dim() < 3 || x.size(x.dim() - 1) != 2)) throw NotHere();
+        const void* W = pairs ? packed(args[3], at::kFloat8_e4m3fn, device, { N, K, 2 }) : packed(args[3], at::kFloat8_e4m3fn, device, { N, K });
+        const float *xs = static_cast<float*>(per_position(args[2], device, x, pairs)), *ws = static_cast<float*>(packed(args[4], at::kFloat, device, { N }));
+        const void* bias = packed(args[5], dt, device, { N }, true);
+        const Field r = field(args[6], dt, device, N, x, false, pairs, true), y = field(args[8], dt, device, N, x, false, pairs);
+        const long P = positions(x, pairs), ld = spread(x, pairs ? 2 : 1);
+        const void* xq = x.data_ptr();
+        const WithoutLock unlocked;
+        return call(type, P, N, K, xq, ld, xs, W, ws, bias, r.data, r.ld, act, y.data, y.ld, stream);
+    });
+}
+
+// mix_backward(input_grad, weight_grad, workspace_bytes, gy, x, W, z, activation, gz, gx, gW, gbias, workspace, device, stream); gz is gy where there is no activation
+PyObject* mix_backward(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 15, [&] {
+        const auto input = function<InputGrad>(args[0]);
+        const auto weight = function<WeightGrad>(args[1]);
+        const auto bytes = function<WeightGradBytes>(args[2]);
+        const int device = small(args[13]), act = small(args[7]);
+        void* stream = stream_of(args[14]);
+        const at::Tensor& gy = first_operand(args[3], device);
+        const at::Tensor& x = first_operand(args[4], device);
+        const at::ScalarType dt = gy.scalar_type();
+        const int type = type_of(gy), N = channels(gy.size(0)), K = channels(x.size(0));
+        const bool slopes = act != TURBOFNO_ACT_NONE;
+        const Field g = field(args[3], dt, device, N, gy), fx = field(args[4], dt, device, K, gy);
+        const Field z = slopes ? field(args[6], dt, device, N, gy) : Field(), gz = slopes ? field(args[8], dt, device, N, gy) : g, gx = field(args[9], dt, device, K, gy);
+        const void* W = packed(args[5], dt, device, { N, K });
+        void *gW = packed(args[10], dt, device, { N, K }), *gbias = packed(args[11], dt, device, { N });
+        const long P = positions(gy);
+        const Workspace ws(args[12], bytes(type, P, N, K), gy, device);
+        const WithoutLock unlocked;
+        const int rc = input(type, P, N, K, g.data, g.ld, z.data, z.ld, W, act, slopes ? gz.data : nullptr, gz.ld, gx.data, gx.ld, stream);
+        return rc ? rc : weight(type, P, N, K, gz.data, gz.ld, fx.data, fx.ld, gW, gbias, ws.data, ws.bytes, stream);
+    });
+}
+
+// rms_norm(function, eight bits, x, gain, residual, eps, s, y or q, rstd or scale, device, stream)
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 11, [&] {
+        const auto call = function<Norm>(args[0]);
+        const int eight = small(args[1]), device = small(args[9]);
+        void* stream = stream_of(args[10]);
+        const at::Tensor& x = first_operand(args[2], device);
+        const at::ScalarType dt = x.scalar_type();
+        const int type = type_of(x), K = channels(x.size(0));
+        const float* gain = static_cast<float*>(packed(args[3], at::kFloat, device, { K }));
+        const float eps = real_value(args[5]);
+        const Field fx = field(args[2], dt, device, K, x), r = field(args[4], dt, device, K, x, false, false, true), s = field(args[6], dt, device, K, x, false, false, true);
+        const Field y = eight ? field(args[7], at::kFloat8_e4m3fn, device, K, x, type == TURBOFNO_C64) : field(args[7], dt, device, K, x);
+        float* rstd = static_cast<float*>(per_position(args[8], device, x));
+        const long P = positions(x);
+        const WithoutLock unlocked;
+        return call(type, P, K, fx.data, fx.ld, r.data, r.ld, gain, eps, s.data, s.ld, y.data, y.ld, rstd, stream);
+    });
+}
+
+// rms_norm_backward(function, workspace_bytes, gy, s, gain, rstd, gs, gx, ggain, workspace, device, stream)
+PyObject* rms_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 12, [&] {
+        const auto call = function<NormGrad>(args[0]);
+        const auto bytes = function<NormGradBytes>(args[1]);
+        const int device = small(args[10]);
+        void* stream = stream_of(args[11]);
+        const at::Tensor& gy = first_operand(args[2], device);
+        const at::ScalarType dt = gy.scalar_type();
+        const int type = type_of(gy), K = channels(gy.size(0));
+        const Field g = field(args[2], dt, device, K, gy), s = field(args[3], dt, device, K, gy), gs = field(args[6], dt, device, K, gy, false, false, true);
+        const Field gx = field(args[7], dt, device, K, gy);
+        const float* gain = static_cast<float*>(packed(args[4], at::kFloat, device, { K }));
+        const float* rstd = static_cast<float*>(per_position(args[5], device, gy));
+        float* ggain = static_cast<float*>(packed(args[8], at::kFloat, device, { K }));
+        const long P = positions(gy);
+        const Workspace ws(args[9], bytes(type, P, K), gy, device);
+        const WithoutLock unlocked;
+        return call(type, P, K, g.data, g.ld, s.data, s.ld, gain, rstd, gs.data, gs.ld, gx.data, gx.ld, ggain, ws.data, ws.bytes, stream);
+    });
+}
+
+// clip_grad_norm(function, workspace_bytes, list of gradients, list of results, max_norm, norm, workspace, device, stream)
+PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 9, [&] {
+        const auto call = function<Clip>(args[0]);
+        const auto bytes = function<ClipBytes>(args[1]);
+        const int device = small(args[7]);
+        void* stream = stream_of(args[8]);
+        if (!PyList_CheckExact(args[2]) || !PyList_CheckExact(args[3]) || PyList_GET_SIZE(args[2]) != PyList_GET_SIZE(args[3]) || PyList_GET_SIZE(args[2]) > INT_MAX)
+            throw NotHere();
+        const int n = (int)PyList_GET_SIZE(args[2]);
+        const float max_norm = real_value(args[4]);
+        std::vector<const void*> grads(n);
+        std::vector<void*> out(n);
+        std::vector<long> sizes(n);
+        std::vector<int> types(n);
+        for (int i = 0; i < n; ++i) {
+            PyObject *go = PyList_GET_ITEM(args[2], i), *oo = PyList_GET_ITEM(args[3], i);
+            if (!THPVariable_CheckExact(go)) throw NotHere();
+            const at::Tensor& g = on_gpu(go, THPVariable_Unpack(go).scalar_type(), device);
+            const at::Tensor& o = go == oo ? g : on_gpu(oo, g.scalar_type(), device);
+            if (!g.is_contiguous() || !o.is_contiguous() || o.sizes() != g.sizes()) throw NotHere();
+            types[i] = type_of(g);
+            sizes[i] = g.numel();
+            grads[i] = g.data_ptr();
+            out[i] = o.data_ptr();
+        }
+        float* norm = static_cast<float*>(packed(args[5], at::kFloat, device, {}));
+        const Workspace ws(args[6], bytes(n), THPVariable_Unpack(args[5]), device);
+        const WithoutLock unlocked;
+        return call(n, grads.data(), out.data(), sizes.data(), types.data(), max_norm, norm, ws.data, ws.bytes, stream);
+    });
+}
+
 PyMethodDef methods[] = {
     { "operands", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(operands)), METH_FASTCALL, "addresses of complex64 GPU tensors of given sizes, or None" },
     { "layer_1d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_1d)), METH_FASTCALL, "turbofno_layer_1d on checked tensors, or -1" },
     { "layer_2d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_2d)), METH_FASTCALL, "turbofno_layer_2d on checked tensors, or -1" },
+#define TFNO_METHOD(name, text) { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, text }
+    TFNO_METHOD(mix, "turbofno_mix on checked tensors, or -1"),
+    TFNO_METHOD(mix_8bit, "turbofno_mix_8bit on checked tensors, or -1"),
+    TFNO_METHOD(mix_backward, "turbofno_mix_input_grad and turbofno_mix_weight_grad on checked tensors, or -1"),
+    TFNO_METHOD(rms_norm, "turbofno_rms_norm or turbofno_rms_norm_8bit on checked tensors, or -1"),
+    TFNO_METHOD(rms_norm_backward, "turbofno_rms_norm_backward on checked tensors, or -1"),
+    TFNO_METHOD(clip_grad_norm, "turbofno_clip_grad_norm on lists of checked tensors, or -1"),
     { nullptr, nullptr, 0, nullptr },
 };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_operands", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };

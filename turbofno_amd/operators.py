@@ -15,6 +15,7 @@ from .api import _check, _need, _stream
 _TYPES = {torch.complex64: 0, torch.float32: 1, torch.bfloat16: 2}
 _ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
 _LIB = None
+_AT = {}                                # addresses of the entry points, for the compiled checks (csrc/operands.cpp)
 
 
 def _lib():
@@ -38,8 +39,25 @@ def _lib():
             getattr(L, name).restype = i
         for name in ("mix_weight_grad", "rms_norm_backward", "clip_grad_norm"):
             getattr(L, "turbofno_%s_workspace_bytes" % name).restype = sz
+        for name in ("mix", "mix_8bit", "mix_input_grad", "mix_weight_grad", "mix_weight_grad_workspace_bytes", "rms_norm", "rms_norm_8bit",
+                     "rms_norm_backward", "rms_norm_backward_workspace_bytes", "clip_grad_norm", "clip_grad_norm_workspace_bytes"):
+            _AT[name] = ctypes.cast(getattr(L, "turbofno_" + name), vp).value
         _LIB = L
     return _LIB
+
+
+def _compiled(call, functions, *args):
+    """The call through the compiled checks: True, or False where an operand is for the checks here to judge. They do the same, without a trip
+    through Python for every attribute of a tensor."""
+    if api._operands is None:
+        return False
+    if _LIB is None:
+        _lib()
+    device = torch.cuda.current_device()
+    rc = getattr(api._operands, call)(*[_AT[f] for f in functions], *args, device, api._raw_stream(device) if api._raw_stream is not None else _stream())
+    if rc > 0:
+        _check(rc)
+    return rc == 0
 
 
 def _type(dtype, name):
@@ -119,6 +137,10 @@ def _workspace(t, need, device):
 def mix(x, W, bias=None, residual=None, activation="none", y=None, z=None):
     """z = W x + bias + residual, y = activation(z): x[K][...], W[N][K] -> y[N][...]. `z`, where passed, receives the pre-activation that
     mix_backward takes. `residual` may be `y` or `z` itself. Activations: none, relu, silu, gelu_tanh; on real and imaginary parts."""
+    if y is None and isinstance(x, torch.Tensor) and isinstance(W, torch.Tensor) and x.is_cuda and x.dim() and W.dim():
+        y = torch.empty(W.shape[:1] + x.shape[1:], dtype=x.dtype, device=x.device)
+    if getattr(y, "is_cuda", False) and _compiled("mix", ("mix",), x, W, bias, residual, _ACTIVATIONS.get(activation, -1), y, z):
+        return y
     kind, device, K, P = _input(x, "x")
     act = _activation(activation)
     _need(isinstance(W, torch.Tensor) and W.dim() == 2 and W.shape[1] == K and W.shape[0] > 0, "W must be [N][%d], one column per channel of x", K)
@@ -139,6 +161,8 @@ def mix_8bit(xq, xscale, Wq, wscale, bias=None, residual=None, activation="none"
     """mix from 8-bit operands: x = xscale[position] xq, W = wscale[n] Wq, all of float8_e4m3fn with float32 scales; xq and xscale as
     rms_norm_8bit gives them. The result has the type of `y`, `residual` or `dtype`, whichever is there (bfloat16 if none is). Complex
     operands are (re, im) pairs along a last dimension of two: xq[K][...][2], Wq[N][K][2]."""
+    if getattr(y, "is_cuda", False) and _compiled("mix_8bit", ("mix_8bit",), xq, xscale, Wq, wscale, bias, residual, _ACTIVATIONS.get(activation, -1), y):
+        return y
     if dtype is None:
         dtype = next((t.dtype for t in (y, residual) if isinstance(t, torch.Tensor)), torch.bfloat16)
     kind = _type(dtype, "the result")
@@ -208,12 +232,22 @@ def mix_weight_grad(gz, x, gW=None, gbias=None, workspace=None):
 
 def mix_backward(gy, x, W, z=None, activation="none", gz=None, gx=None, gW=None, gbias=None, workspace=None):
     """(gx, gW, gbias, gz) from the gradient of y, and the x, W and z of mix; gz is the gradient of its residual."""
+    act = _ACTIVATIONS.get(activation, -1)
+    if isinstance(gy, torch.Tensor) and isinstance(x, torch.Tensor) and isinstance(W, torch.Tensor) and gy.is_cuda:
+        gz = gy if act == 0 else _result(gz, gy.shape, gy.dtype, gy.device)
+        gx, gW, gbias = _result(gx, x.shape, x.dtype, x.device), _result(gW, W.shape, W.dtype, W.device), _result(gbias, gy.shape[:1], gy.dtype, gy.device)
+        if _compiled("mix_backward", ("mix_input_grad", "mix_weight_grad", "mix_weight_grad_workspace_bytes"), gy, x, W, z, act, gz, gx, gW, gbias, workspace):
+            return gx, gW, gbias, gz
     gx, gz = mix_input_grad(gy, W, z=z, activation=activation, gz=gz, gx=gx)
     gW, gbias = mix_weight_grad(gz, x, gW=gW, gbias=gbias, workspace=workspace)
     return gx, gW, gbias, gz
 
 
 def _norm(x, gain, residual, eps, y, scale, s, rstd, eight):
+    row = scale if eight else rstd
+    if row is not None and (residual is None or s is not None) and getattr(y, "is_cuda", False):
+        if _compiled("rms_norm", ("rms_norm_8bit" if eight else "rms_norm",), int(eight), x, gain, residual, eps, s, y, row):
+            return y, row, x if s is None else s
     kind, device, K, P = _input(x, "x")
     dtype = x.dtype
     places = tuple(x.shape[1:])
@@ -262,6 +296,9 @@ def rms_norm_backward_workspace_bytes(K, P, dtype):
 def rms_norm_backward(gy, s, gain, rstd, gs=None, gx=None, ggain=None, workspace=None):
     """(gx, ggain) from the gradient of y, the s and rstd of rms_norm, and gs, what reaches s by the residual stream. gx is the gradient of x and of
     residual; it may be gy, s or gs itself."""
+    if ggain is not None and getattr(gx, "is_cuda", False):
+        if _compiled("rms_norm_backward", ("rms_norm_backward", "rms_norm_backward_workspace_bytes"), gy, s, gain, rstd, gs, gx, ggain, workspace):
+            return gx, ggain
     kind, device, K, P = _input(gy, "gy")
     dtype, places = gy.dtype, tuple(gy.shape[1:])
     if not all(isinstance(t, torch.Tensor) for t in (s, gain, rstd)):
@@ -286,6 +323,10 @@ def clip_grad_norm(grads, max_norm, out=None, norm=None, workspace=None):
     grads = list(grads)
     out = grads if out is None else list(out)
     _need(len(out) == len(grads), "out has %d tensors, grads %d", len(out), len(grads))
+    if grads and isinstance(grads[0], torch.Tensor) and grads[0].is_cuda:
+        norm = _result(norm, (), torch.float32, grads[0].device)
+        if _compiled("clip_grad_norm", ("clip_grad_norm", "clip_grad_norm_workspace_bytes"), grads, out, max_norm, norm, workspace):
+            return norm
     device = grads[0].device if grads and isinstance(grads[0], torch.Tensor) else torch.device("cuda", torch.cuda.current_device())
     count = len(grads)
     kinds, sizes = (ctypes.c_int * count)(), (ctypes.c_long * count)()

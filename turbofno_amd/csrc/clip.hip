@@ -14,7 +14,7 @@ namespace tfno {
 
 namespace {
 
-constexpr int kTensors = 96, kUnit = 4096, kBlocks = 1024;
+constexpr int kTensors = 96, kUnit = 4096, kBlocks = 2048;
 
 struct ClipParams {
     const void* grads[kTensors];

@@ -6,8 +6,9 @@
 // x, the quarters of a wave 32 of them, and has the operands of its matrix instructions. Complex rows are (re, im) pairs: gz as it is against
 // (re, im) of x for the real part, against (-im, re) for the imaginary part. 32-bit values are split into bf16 parts (bf16_split.h), 16-bit ones
 // are exact; sums are fp32. gbias takes its sums from the values of gz that pass by.
-// A block takes a tile of 64 rows n and 64 real (32 complex) rows k and a part of the positions, its four waves every fourth step of 32 real values,
-// so that a block reads 512 consecutive bytes of a row. The blocks' sums go to the workspace and are added in a second kernel, always in the
+// A block takes a tile of 64 rows n and 64 real (32 complex) rows k and a part of the positions: its four waves four steps of 32 real values side by
+// side, then those as many steps further as all blocks take together. So the blocks move through the rows as one window: with a contiguous part for each
+// block they all would stand at the same offset of their parts, on the same few memory channels. The blocks' sums go to the workspace and are added in a second kernel, always in the
 // same order: results do not change from call to call.
 // An infinite operand, or one above the largest bf16 number (3.3895e38), makes the sums it takes part in infinite or NaN.
 #include "columns.h"
@@ -24,7 +25,6 @@ struct GradParams {
     long ldg, ldx, columns;                             // real values
     int N, K;
     float* sums;                                        // [splits][N K V + N V]
-    long steps_per_split;
     int splits, ktiles, tiles;
 };
 
@@ -134,8 +134,7 @@ template <int IN, bool COMPLEX> __global__ __launch_bounds__(256, 1) void weight
 
     float4_v acc[4][4] = {};
     float bias_re[4] = {}, bias_im[4] = {};
-    const long steps = (q.columns + kStep - 1) / kStep, first = split * q.steps_per_split;
-    const long last = first + q.steps_per_split < steps ? first + q.steps_per_split : steps;
+    const long steps = (q.columns + kStep - 1) / kStep, stride = 4l * q.splits;
     Eight<IN> gv[4], xv[KT];
     auto fetch = [&](long s, Eight<IN> (&gv)[4], Eight<IN> (&xv)[KT]) {
         const long column = s * kStep + 8 * kq;
@@ -145,10 +144,11 @@ template <int IN, bool COMPLEX> __global__ __launch_bounds__(256, 1) void weight
 #pragma unroll
         for (int t = 0; t < KT; ++t) xv[t] = load8<IN>(x[t], column, q.columns, inside);
     };
-    if (first + wave < last) fetch(first + wave, gv, xv);
-    for (long s = first + wave; s < last; s += 4) {
+    const long first = 4l * split + wave;
+    if (first < steps) fetch(first, gv, xv);
+    for (long s = first; s < steps; s += stride) {
         Eight<IN> gn[4], xn[KT];
-        if (s + 4 < last) fetch(s + 4, gn, xn);
+        if (s + stride < steps) fetch(s + stride, gn, xn);
         Op b[4];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
@@ -218,8 +218,10 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict_
     const long e = (long)blockIdx.x * 64 + (threadIdx.x & 63);
     const int quarter = threadIdx.x >> 6;
     float sum = 0.f;
-    if (e < count)
+    if (e < count) {
+#pragma unroll 16
         for (int s = quarter; s < splits; s += 4) sum += sums[s * count + e];
+    }
     part[quarter][threadIdx.x & 63] = sum;
     __syncthreads();
     if (quarter == 0 && e < count) {
@@ -261,10 +263,8 @@ hipError_t launch_mix_weight_grad(int type, long P, int N, int K, const void* gz
                                   hipStream_t stream)
 {
     const int v = values_of(type);
-    GradParams q = { gz, x, ldgz * v, ldx * v, P * v, N, K, static_cast<float*>(workspace), 0, splits_of(type, P, N, K), 0, 0 };
+    GradParams q = { gz, x, ldgz * v, ldx * v, P * v, N, K, static_cast<float*>(workspace), splits_of(type, P, N, K), 0, 0 };
     q.tiles = tiles_of(type, N, K, q.ktiles);
-    const long steps = (q.columns + kStep - 1) / kStep;
-    q.steps_per_split = (steps + q.splits - 1) / q.splits;
     const dim3 grid((unsigned)(q.splits * q.tiles));
     switch (type) {
     case kC64: hipLaunchKernelGGL((weight_grad_kernel<kIn32, true>), grid, dim3(256), 0, stream, q); break;

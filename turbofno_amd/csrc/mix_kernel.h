@@ -265,19 +265,20 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
             else store4<TYPE>(p, 4 * c, v);
         } else near_store4<TYPE>(scalar(base, at * (long)sizeof(Value)), fresh(((unsigned)lane_row * (unsigned)ld + 4 * c) * (unsigned)sizeof(Value)), v);
     }
-    // the lane's rows of step `step` of `base`: channels beyond the last are zeros
-    __device__ __forceinline__ void fetch(const void* base, long ld, const Window& w, int step, Rows& rows) const
+    // the lane's rows of step `step` of `base`. GUARD: channels beyond the last may be among them; then some other row is read, and clear() has to follow.
+    // No branch: a load whose result meets another one where branches join is waited for there
+    template <bool GUARD> __device__ __forceinline__ void fetch(const void* base, long ld, const Window& w, int step, Rows& rows) const
     {
-        const int first = step * CHANNELS, lane_row = kq * PER_LANE;
-        if (first + CHANNELS <= q.contraction) {
 #pragma unroll
-            for (int j = 0; j < PER_LANE; ++j) rows[j] = read<IN, false>(base, ld, first + j, lane_row, q.contraction, w);
-        } else
+        for (int j = 0; j < PER_LANE; ++j) rows[j] = read<IN, GUARD>(base, ld, step * CHANNELS + j, kq * PER_LANE, q.contraction, w);
+    }
+    // channels beyond the last: zeros
+    __device__ __forceinline__ void clear(int step, Rows& rows) const
+    {
+        if ((step + 1) * CHANNELS <= q.contraction) return;
 #pragma unroll
-            for (int j = 0; j < PER_LANE; ++j) {
-                rows[j] = read<IN, true>(base, ld, first + j, lane_row, q.contraction, w);
-                if (first + j + lane_row >= q.contraction) rows[j] = zero4<IN>();
-            }
+        for (int j = 0; j < PER_LANE; ++j)
+            if (step * CHANNELS + j + kq * PER_LANE >= q.contraction) rows[j] = zero4<IN>();
     }
     // gradient: gy through the activation at z, written out by one of the waves that share these columns
     __device__ __forceinline__ void slope(const Window& w, int step, Rows& x, const Rows& zin, bool writes) const
@@ -334,15 +335,9 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
         if constexpr (!GRAD) {
             if (q.residual)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const int first = row0 + 16 * t;
-                    if (first + 16 <= q.rows)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) residual[t][i] = read<OUT, false>(q.residual, q.ldr, first + i, 4 * kq, q.rows, w);
-                    else if (first < q.rows)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) residual[t][i] = read<OUT, true>(q.residual, q.ldr, first + i, 4 * kq, q.rows, w);
-                }
+                    for (int i = 0; i < 4; ++i) residual[t][i] = read<OUT, true>(q.residual, q.ldr, row0 + 16 * t + i, 4 * kq, q.rows, w);
         }
         if constexpr (IN == kIn8) {                     // scales of the lane's columns and rows
 #pragma unroll
@@ -413,6 +408,15 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
     }
 };
 
+// f(0) ... f(N - 1) with no loop left, so that registers are indexed by constants
+template <int N, int I = 0, typename F> __device__ __forceinline__ void unrolled(F&& f)
+{
+    if constexpr (I < N) {
+        f(I);
+        unrolled<N, I + 1>(f);
+    }
+}
+
 // Few columns: a wave for 64 columns and 16 NT rows, weights from memory
 template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT>
 __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, int row_groups)
@@ -427,16 +431,16 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     const bool slopes = GRAD && q.act != kActNone;
     const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
     float4_v acc[NT][4] = {};
-    typename Wave::Rows x, z, xnext, znext;
+    typename Wave::Rows x0, z0, x1, z1;
     auto fetch = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
-        wave.fetch(q.x, q.ldx, w, s, x);
-        if (slopes) wave.fetch(q.zin, q.ldzin, w, s, z);
+        s = s < steps ? s : steps - 1;
+        wave.template fetch<true>(q.x, q.ldx, w, s, x);
+        if (slopes) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
     };
-    fetch(0, x, z);
-    for (int s = 0; s < steps; ++s) {
-        if (s + 1 < steps) fetch(s + 1, xnext, znext);
+    auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
         if constexpr (GRAD)
             if (slopes) wave.slope(w, s, x, z, row0 == 0);
+        wave.clear(s, x);
         Operand<IN> b[4];
         make_operands<IN, COMPLEX, GRAD>(x, b);
 #pragma unroll
@@ -445,39 +449,47 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
             load_weights<IN, COMPLEX, GRAD>(q.W, row0 + 16 * t + wave.c, q.rows, 32 * s + 8 * wave.kq, q.contraction * Wave::V, q.ldw, a);
             multiply<IN>(a, b, acc[t]);
         }
-#pragma unroll
-        for (int j = 0; j < Wave::PER_LANE; ++j) {
-            x[j] = xnext[j];
-            if constexpr (GRAD) z[j] = znext[j];
-        }
+    };
+    fetch(0, x0, z0);
+    for (int s = 0; s < steps; s += 2) {
+        fetch(s + 1, x1, z1);
+        product(s, x0, z0);
+        if (s + 1 >= steps) break;
+        fetch(s + 2, x0, z0);
+        product(s + 1, x1, z1);
     }
     wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); });
 }
 
-// f(0) ... f(N - 1) with no loop left, so that registers are indexed by constants
-template <int N, int I = 0, typename F> __device__ __forceinline__ void unrolled(F&& f)
-{
-    if constexpr (I < N) {
-        f(I);
-        unrolled<N, I + 1>(f);
-    }
-}
-
 // Many columns: the operands of the block's rows of A stay in LDS, in the order in which lanes read them (16 bytes per lane, part, 16 rows and step), and
-// its waves walk the columns without meeting again. HELD steps of the input stay in registers while the rows are walked, and are asked for again for
-// the next columns as the last rows use them up; HELD = 0: steps are read as they are needed, once for every 16 NT rows.
+// its waves walk the columns without meeting again. All steps of the input, HELD or up to `SPARE` fewer, stay in registers while the rows are walked, and
+// are asked for again for the next columns as the last rows use them up; HELD = 0: steps are read as they are needed, again for every 16 NT rows.
 constexpr int kWaveParts(int in) { return in == kIn32 ? 3 : 1; }
 constexpr int kResidentThreads = 512;
+// numbers of steps that there are kernels for
+constexpr int held_for(int steps) { return steps <= 4 ? steps : steps <= 6 ? 6 : 8; }
 template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD>
 __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const MixParams q, int block_rows, int tiles)
 {
     extern __shared__ uint4_v weights[];
     typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, false> Wave;
-    constexpr int PARTS = kWaveParts(IN);
+    typedef typename Wave::Parts Parts;
+    constexpr int PARTS = kWaveParts(IN), SPARE = HELD > 4 ? 2 : 1;     // steps from HELD - SPARE on may reach beyond the last channel
     const Wave wave(q);
     const int row_first = blockIdx.y * block_rows, groups = block_rows / (16 * NT);
-    const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
+    const int steps = HELD ? HELD : (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
     const bool slopes = GRAD && q.act != kActNone, writes = blockIdx.y == 0;
+    // tiles are counted in 32 bits: 64-bit numbers are compared in vector registers. A last tile that is not whole ends with the columns; tiles beyond it are it
+    auto window = [&](int tile) { return Window{ scalar(tile < tiles - 1 ? (long)tile * kColumns : q.columns - kColumns), kColumns }; };
+    const int stride = gridDim.x * (blockDim.x >> 6);
+    int tile = blockIdx.x * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Window w = window(tile);
+    auto fetch = [&](const void* base, long ld, const Window& w, int s, typename Wave::Rows& rows) {
+        if (s < HELD - SPARE) wave.template fetch<false>(base, ld, w, s, rows);
+        else wave.template fetch<true>(base, ld, w, s, rows);
+    };
+    typename Wave::Rows x[HELD ? HELD : 1];
+    unrolled<HELD>([&](int s) { fetch(q.x, q.ldx, w, s, x[s]); });      // on their way while the operands of A are formed
     {
         const int per_step = block_rows / 16 * 64, count = steps * per_step;
 #pragma unroll 4
@@ -490,12 +502,13 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
             else to[0] = a.v;
         }
     }
-    typedef typename Wave::Parts Parts;
     Parts* biases = reinterpret_cast<Parts*>(weights + (long)steps * block_rows * (4 * PARTS));
     if constexpr (!GRAD)
         if (q.bias)
             for (int e = threadIdx.x; e < block_rows / 4; e += blockDim.x) biases[e] = wave.bias_of(row_first + 4 * e);
     __syncthreads();
+    if (tile >= tiles) return;
+
     auto weight = [&](int s, int t16) {                 // operand of step s, 16 rows t16
         const uint4_v* from = weights + (long)(s * (block_rows / 16) + t16) * (64 * PARTS) + wave.lane;
         Operand<IN> a;
@@ -503,52 +516,59 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
         else a.v = from[0];
         return a;
     };
-    // tiles are counted in 32 bits: 64-bit numbers are compared in vector registers. A last tile that is not whole ends with the columns
-    auto window = [&](int tile) { return Window{ scalar(tile < tiles - 1 ? (long)tile * kColumns : q.columns - kColumns), kColumns }; };
-    const int stride = gridDim.x * (blockDim.x >> 6);
-    int tile = blockIdx.x * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (tile >= tiles) return;
-    Window w = window(tile);
+    auto finish = [&](int g, float4_v (&acc)[NT][4]) {
+        wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; });
+    };
     if constexpr (HELD > 0) {
-        typename Wave::Rows x[HELD];
-#pragma unroll
-        for (int s = 0; s < HELD; ++s)
-            if (s < steps) wave.fetch(q.x, q.ldx, w, s, x[s]);
         for (;;) {
             if constexpr (GRAD)
                 if (slopes) {
-                    constexpr int AHEAD = IN == kIn32 ? (COMPLEX ? 2 : 1) : HELD < 4 ? HELD : 4;          // steps of z on their way
+                    constexpr int AHEAD = IN == kIn32 ? (COMPLEX && HELD > 1 ? 2 : 1) : HELD < 4 ? HELD : 4;      // steps of z on their way
                     typename Wave::Rows z[AHEAD];
-#pragma unroll
-                    for (int s = 0; s < AHEAD; ++s)
-                        if (s < steps) wave.fetch(q.zin, q.ldzin, w, s, z[s]);
+                    unrolled<AHEAD>([&](int s) { fetch(q.zin, q.ldzin, w, s, z[s]); });
                     unrolled<HELD>([&](int s) {
-                        if (s < steps) {
-                            wave.slope(w, s, x[s], z[s % AHEAD], writes);
-                            if (s + AHEAD < steps) wave.fetch(q.zin, q.ldzin, w, s + AHEAD, z[s % AHEAD]);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
+                        wave.slope(w, s, x[s], z[s % AHEAD], writes);
+                        if (s + AHEAD < HELD) fetch(q.zin, q.ldzin, w, s + AHEAD, z[s % AHEAD]);
+                        __builtin_amdgcn_sched_barrier(0);
                     });
                 }
-            const int next = tile + stride;
-            const bool more = next < tiles;
-            const Window wn = window(more ? next : tile);
-            for (int g = 0; g < groups; ++g) {
-                float4_v acc[NT][4] = {};
+            const Window wn = window(tile + stride);
+            if constexpr (GRAD && IN == kIn16) {
+                // gz is not to be read again: its operands take the place of its rows
+                Operand<IN> b[HELD][4];
                 unrolled<HELD>([&](int s) {
-                    if (s < steps) {
+                    if (s >= HELD - SPARE) wave.clear(s, x[s]);
+                    make_operands<IN, COMPLEX, GRAD>(x[s], b[s]);
+                });
+                for (int g = 0; g < groups; ++g) {
+                    float4_v acc[NT][4] = {};
+                    unrolled<HELD>([&](int s) {
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b[s], acc[t]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                    finish(g, acc);
+                }
+                unrolled<HELD>([&](int s) { fetch(q.x, q.ldx, wn, s, x[s]); });
+            } else
+                for (int g = 0; g < groups; ++g) {
+                    // asked for again as they are used up: for the rows that follow, out of the caches, or for the next columns (after the last tile, the
+                    // last one again). Without a branch: loads whose results meet others where branches join are waited for there
+                    const Window wf = g < groups - 1 ? w : wn;
+                    float4_v acc[NT][4] = {};
+                    unrolled<HELD>([&](int s) {
+                        if (s >= HELD - SPARE) wave.clear(s, x[s]);
                         Operand<IN> b[4];
                         make_operands<IN, COMPLEX, GRAD>(x[s], b);
-                        if (more && g == groups - 1) wave.fetch(q.x, q.ldx, wn, s, x[s]);
+                        fetch(q.x, q.ldx, wf, s, x[s]);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
                         __builtin_amdgcn_sched_barrier(0);
-                    }
-                });
-                wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; });
-            }
-            if (!more) return;
-            tile = next;
+                    });
+                    finish(g, acc);
+                }
+            tile += stride;
+            if (tile >= tiles) return;
             w = wn;
         }
     } else {
@@ -556,27 +576,30 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
             w = window(tile);
             for (int g = 0; g < groups; ++g) {
                 float4_v acc[NT][4] = {};
-                typename Wave::Rows x, z, xnext, znext;
-                auto fetch = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
-                    wave.fetch(q.x, q.ldx, w, s, x);
-                    if (slopes) wave.fetch(q.zin, q.ldzin, w, s, z);
+                typename Wave::Rows x0, z0, x1, z1;
+                auto ahead = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
+                    s = s < steps ? s : steps - 1;
+                    wave.template fetch<true>(q.x, q.ldx, w, s, x);
+                    if (slopes) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
                 };
-                fetch(0, x, z);
-                for (int s = 0; s < steps; ++s) {
-                    if (s + 1 < steps) fetch(s + 1, xnext, znext);
+                auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
                     if constexpr (GRAD)
                         if (slopes) wave.slope(w, s, x, z, writes && g == 0);
+                    wave.clear(s, x);
                     Operand<IN> b[4];
                     make_operands<IN, COMPLEX, GRAD>(x, b);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
-#pragma unroll
-                    for (int j = 0; j < Wave::PER_LANE; ++j) {
-                        x[j] = xnext[j];
-                        if constexpr (GRAD) z[j] = znext[j];
-                    }
+                };
+                ahead(0, x0, z0);
+                for (int s = 0; s < steps; s += 2) {
+                    ahead(s + 1, x1, z1);
+                    product(s, x0, z0);
+                    if (s + 1 >= steps) break;
+                    ahead(s + 2, x0, z0);
+                    product(s + 1, x1, z1);
                 }
-                wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; });
+                finish(g, acc);
             }
         }
     }

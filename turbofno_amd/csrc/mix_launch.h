@@ -32,22 +32,46 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t
     return hipGetLastError();
 }
 
+// steps that registers hold, and beyond how many of them the sums of 64 rows find no room beside them
+template <int IN, bool COMPLEX> constexpr int kMostSteps = IN == kIn32 && !COMPLEX ? 4 : 8;
+template <int IN, bool COMPLEX> constexpr int kMostWideSteps = IN != kIn32 ? 8 : COMPLEX ? 4 : 2;
+
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int HELD = kMostSteps<IN, COMPLEX>>
+hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, size_t lds, hipStream_t stream)
+{
+    if constexpr (HELD != held_for(HELD)) return launch_steps<IN, OUT, COMPLEX, GRAD, HELD - 1>(q, nt, held, block_rows, lds, stream);
+    else {
+        if (held == HELD) {
+            if constexpr (HELD <= kMostWideSteps<IN, COMPLEX>)
+                if (nt == 4) return launch_resident<IN, OUT, COMPLEX, GRAD, 4, HELD>(q, block_rows, lds, stream);
+            return launch_resident<IN, OUT, COMPLEX, GRAD, 2, HELD>(q, block_rows, lds, stream);
+        }
+        if constexpr (HELD > 0) return launch_steps<IN, OUT, COMPLEX, GRAD, HELD - 1>(q, nt, held, block_rows, lds, stream);
+        else return hipErrorInvalidValue;
+    }
+}
+
 template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const MixParams& q, hipStream_t stream)
 {
     if (q.columns == 0) return hipSuccess;
     constexpr int CHANNELS = COMPLEX ? 16 : 32;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
-    const size_t lds16 = (size_t)steps * kWaveParts(IN) * 1024;         // of 16 rows
-    constexpr int MOST = IN == kIn32 && !COMPLEX ? 4 : 8;               // steps that registers hold
-    // 32 rows at a time where 64 are too many, or where the held steps leave no registers for the sums of 64
-    const bool narrow = IN == kIn32 && steps > MOST / 2 && steps <= MOST;
-    const int nt = tiles16 <= 2 || narrow ? 2 : 4;
+    const size_t lds16 = (size_t)(steps > kMostSteps<IN, COMPLEX> ? steps : held_for(steps)) * kWaveParts(IN) * 1024;         // of 16 rows
+    constexpr int MOST = kMostSteps<IN, COMPLEX>;
+    const int nt = tiles16 <= 2 || (steps > kMostWideSteps<IN, COMPLEX> && steps <= MOST) ? 2 : 4;
     // the lane's part of an address, up to 24 rows of the input or 12 of the results, in 32 bits
     const long widest = std::max(std::max(std::max(q.ldx, q.ldzin), q.ldr), std::max(q.ldy, q.ldz));
     const bool near = widest < (1L << 24) && tiles < (1L << 30);
-    if (near && q.columns >= kColumns && tiles * tiles16 > 4096 && nt * lds16 <= kResidentLds) {
-        const int groups = (tiles16 + nt - 1) / nt, fit = (int)(kResidentLds / (nt * lds16)), chunks = (groups + fit - 1) / fit;
+#ifndef RFROM
+#define RFROM 1024
+#define RWAVES 2048
+#endif
+    if (near && q.columns >= kColumns && tiles * tiles16 > RFROM && nt * lds16 <= kResidentLds) {
+        const int groups = (tiles16 + nt - 1) / nt, fit = (int)(kResidentLds / (nt * lds16));
+        int chunks = (groups + fit - 1) / fit;
+        while (chunks < groups && tiles * chunks < RWAVES) ++chunks;
+        if (GRAD && IN == kIn32) chunks = groups;       // the kernel walks 64 rows: what it made of gy and z is gone after them
         const int block_groups = (groups + chunks - 1) / chunks, block_rows = block_groups * nt * 16;
         const size_t lds = block_groups * nt * lds16 + block_rows * (COMPLEX ? 8 : 4);
         const long last = q.columns % kColumns;
@@ -66,15 +90,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
             if (hipError_t e = launch_mix<IN, OUT, COMPLEX, GRAD>(whole, stream); e != hipSuccess) return e;
             return launch_direct<IN, OUT, COMPLEX, GRAD, 1>(rest, stream);
         }
-#define TFNO_RESIDENT(NT, HELD) launch_resident<IN, OUT, COMPLEX, GRAD, NT, HELD>(q, block_rows, lds, stream)
-        if (steps > MOST) return nt == 2 ? TFNO_RESIDENT(2, 0) : TFNO_RESIDENT(4, 0);
-        if (steps <= 2) return nt == 2 ? TFNO_RESIDENT(2, 2) : TFNO_RESIDENT(4, 2);
-        if constexpr (MOST == 8) {
-            if (steps <= 4) return nt == 2 ? TFNO_RESIDENT(2, 4) : TFNO_RESIDENT(4, 4);
-            if constexpr (IN == kIn32) return TFNO_RESIDENT(2, 8);
-            else return nt == 2 ? TFNO_RESIDENT(2, 8) : TFNO_RESIDENT(4, 8);
-        } else return TFNO_RESIDENT(2, 4);
-#undef TFNO_RESIDENT
+        return launch_steps<IN, OUT, COMPLEX, GRAD>(q, nt, steps > MOST ? 0 : held_for(steps), block_rows, lds, stream);
     }
     if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1>(q, stream);
     if (tiles16 == 2 || tiles * tiles16 <= 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 2>(q, stream);

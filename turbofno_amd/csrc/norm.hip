@@ -256,7 +256,7 @@ template <int IN, bool COMPLEX, bool EIGHT> hipError_t launch_norm(const NormPar
     if (q.K <= 32) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 64, 4>), dim3((unsigned)wide), dim3(kThreads), 0, stream, q);
     else if (q.K <= 64) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 64, 8>), dim3((unsigned)wide), dim3(kThreads), 0, stream, q);
     else if (q.K <= 128) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 64, 16>), dim3((unsigned)wide), dim3(kThreads), 0, stream, q);
-    else if (q.K <= 256) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 16, 8>), dim3((unsigned)narrow), dim3(kThreads), 0, stream, q);
+    else if (q.K <= 256) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 32, 16>), dim3((unsigned)((q.columns + 127) / 128)), dim3(kThreads), 0, stream, q);
     else if (q.K <= 512) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 16, 16>), dim3((unsigned)narrow), dim3(kThreads), 0, stream, q);
     else hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 16, 0>), dim3((unsigned)narrow), dim3(kThreads), 0, stream, q);
     return hipGetLastError();

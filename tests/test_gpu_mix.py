@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 # K, N, positions: single elements, sizes around the tiles of 16 channels and 64 columns, steps that end inside, several row groups
 SIZES = [(1, 1, (1,)), (3, 5, (7,)), (8, 64, (128,)), (17, 33, (65,)), (64, 64, (10, 100)), (72, 200, (3, 111)), (130, 131, (129,)), (300, 40, (70,)),
-         (16, 300, (2, 5, 13)), (33, 16, (4099,)), (64, 128, (40001,))]
+         (16, 300, (2, 5, 13)), (33, 16, (4099,)), (64, 128, (40001,)), (20, 1500, (6001,))]
 
 
 def operands(kind, K, N, places, seed=0, bias=True, residual=True):

@@ -326,12 +326,13 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
         }
     }
     // results of rows row0 + 16 t + 4 kq + i: acc[t][b][i] belongs to column 4 c + b
-    // bias(t): the bias of the lane's four rows of 16 rows t, real and imaginary parts apart
-    template <typename Bias> __device__ __forceinline__ void finish(const Window& w, int row0, float4_v (&acc)[NT][4], Bias bias) const
+    // bias(t): the bias of the lane's four rows of 16 rows t, real and imaginary parts apart; row_scale(t): their scales, of 8-bit operands
+    template <typename Bias, typename Scale>
+    __device__ __forceinline__ void finish(const Window& w, int row0, float4_v (&acc)[NT][4], Bias bias, Scale row_scale) const
     {
         if constexpr (IN == kIn32) mend(w, row0, acc);
         RawOf<OUT> residual[GRAD ? 1 : NT][4];          // all loads first
-        float4_v xs = { 1.f, 1.f, 1.f, 1.f }, ws[IN == kIn8 ? NT : 1];
+        float4_v xs = { 1.f, 1.f, 1.f, 1.f };
         if constexpr (!GRAD) {
             if (q.residual)
 #pragma unroll
@@ -339,25 +340,19 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
 #pragma unroll
                     for (int i = 0; i < 4; ++i) residual[t][i] = read<OUT, true>(q.residual, q.ldr, row0 + 16 * t + i, 4 * kq, q.rows, w);
         }
-        if constexpr (IN == kIn8) {                     // scales of the lane's columns and rows
+        if constexpr (IN == kIn8)                       // scales of the lane's columns
 #pragma unroll
             for (int b = 0; b < 4; ++b) xs[b] = q.xscale[(w.column0 + (!FAR || 4 * c + b < w.there ? 4 * c + b : w.there - 1)) / V];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = row0 + 16 * t + 4 * kq + i;
-                    ws[t][i] = q.wscale[row < q.rows ? row : q.rows - 1];
-                }
-        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if (row0 + 16 * t >= q.rows) break;
             float4_v v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = (float4_v){ acc[t][0][i], acc[t][1][i], acc[t][2][i], acc[t][3][i] };
-                if constexpr (IN == kIn8) v[i] *= xs * ws[t][i];
+            for (int i = 0; i < 4; ++i) v[i] = (float4_v){ acc[t][0][i], acc[t][1][i], acc[t][2][i], acc[t][3][i] };
+            if constexpr (IN == kIn8) {
+                const float4_v ws = row_scale(t);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] *= xs * ws[i];
             }
             if constexpr (!GRAD) {
                 if (q.bias) {
@@ -387,6 +382,13 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
 #pragma unroll
             for (int j = 0; j < V; ++j) p.v[j][i] = value_of(static_cast<const OutValue*>(q.bias)[(long)(first + i < q.rows ? first + i : q.rows - 1) * V + j]);
         return p;
+    }
+    __device__ __forceinline__ float4_v scale_of(int first) const
+    {
+        float4_v v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = q.wscale[first + i < q.rows ? first + i : q.rows - 1];
+        return v;
     }
     template <int ACT> static __device__ __forceinline__ void act_rows(float4_v (&v)[4])
     {
@@ -459,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
         fetch(s + 2, x0, z0);
         product(s + 1, x1, z1);
     }
-    wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); });
+    wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); }, [&](int t) { return wave.scale_of(row0 + 16 * t + 4 * wave.kq); });
 }
 
 // Many columns: the operands of the block's rows of A stay in LDS, in the order in which lanes read them (16 bytes per lane, part, 16 rows and step), and
@@ -507,6 +509,9 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
     if constexpr (!GRAD)
         if (q.bias)
             for (int e = threadIdx.x; e < block_rows / 4; e += blockDim.x) biases[e] = wave.bias_of(row_first + 4 * e);
+    float4_v* scales = reinterpret_cast<float4_v*>(biases + block_rows / 4);
+    if constexpr (IN == kIn8)
+        for (int e = threadIdx.x; e < block_rows / 4; e += blockDim.x) scales[e] = wave.scale_of(row_first + 4 * e);
     __syncthreads();
     if (tile >= tiles) return;
 
@@ -518,7 +523,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
         return a;
     };
     auto finish = [&](int g, float4_v (&acc)[NT][4]) {
-        wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; });
+        wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; }, [&](int t) { return scales[(g * NT + t) * 4 + wave.kq]; });
     };
     if constexpr (HELD > 0) {
         for (;;) {
@@ -534,8 +539,8 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                     });
                 }
             const Window wn = window(tile + stride);
-            if constexpr (GRAD && IN == kIn16) {
-                // gz is not to be read again: its operands take the place of its rows
+            if constexpr (IN != kIn32) {
+                // 16- and 8-bit rows: all operands at once, in the registers that the rows leave
                 Operand<IN> b[HELD][4];
                 unrolled<HELD>([&](int s) {
                     if (s >= HELD - SPARE) wave.clear(s, x[s]);

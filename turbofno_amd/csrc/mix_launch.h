@@ -15,7 +15,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT> hipError_t launch_di
     return hipGetLastError();
 }
 
-constexpr size_t kResidentLds = 152 << 10, kResidentBias = 8 << 10;    // operands of A; a bias of up to 1024 complex rows
+constexpr size_t kResidentLds = 152 << 10, kResidentBias = 8 << 10;    // operands of A; bias and scales of up to 640 complex rows
 
 template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t launch_resident(const MixParams& q, int block_rows, size_t lds, hipStream_t stream)
 {
@@ -34,7 +34,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t
 
 // steps that registers hold, and beyond how many of them the sums of 64 rows find no room beside them
 template <int IN, bool COMPLEX> constexpr int kMostSteps = IN == kIn32 && !COMPLEX ? 4 : 8;
-template <int IN, bool COMPLEX> constexpr int kMostWideSteps = IN != kIn32 ? 8 : COMPLEX ? 4 : 2;
+template <int IN, int OUT, bool COMPLEX> constexpr int kMostWideSteps = IN == kIn32 ? (COMPLEX ? 4 : 2) : OUT == kIn32 ? 4 : 8;
 
 template <int IN, int OUT, bool COMPLEX, bool GRAD, int HELD = kMostSteps<IN, COMPLEX>>
 hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, size_t lds, hipStream_t stream)
@@ -42,7 +42,7 @@ hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, si
     if constexpr (HELD != held_for(HELD)) return launch_steps<IN, OUT, COMPLEX, GRAD, HELD - 1>(q, nt, held, block_rows, lds, stream);
     else {
         if (held == HELD) {
-            if constexpr (HELD <= kMostWideSteps<IN, COMPLEX>)
+            if constexpr (HELD <= kMostWideSteps<IN, OUT, COMPLEX>)
                 if (nt == 4) return launch_resident<IN, OUT, COMPLEX, GRAD, 4, HELD>(q, block_rows, lds, stream);
             return launch_resident<IN, OUT, COMPLEX, GRAD, 2, HELD>(q, block_rows, lds, stream);
         }
@@ -59,7 +59,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
     const size_t lds16 = (size_t)(steps > kMostSteps<IN, COMPLEX> ? steps : held_for(steps)) * kWaveParts(IN) * 1024;         // of 16 rows
     constexpr int MOST = kMostSteps<IN, COMPLEX>;
-    const int nt = tiles16 <= 2 || (steps > kMostWideSteps<IN, COMPLEX> && steps <= MOST) ? 2 : 4;
+    const int nt = tiles16 <= 2 || (steps > kMostWideSteps<IN, OUT, COMPLEX> && steps <= MOST) ? 2 : 4;
     // the lane's part of an address, up to 24 rows of the input or 12 of the results, in 32 bits
     const long widest = std::max(std::max(std::max(q.ldx, q.ldzin), q.ldr), std::max(q.ldy, q.ldz));
     const bool near = widest < (1L << 24) && tiles < (1L << 30);
@@ -68,12 +68,12 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
 #define RWAVES 2048
 #endif
     if (near && q.columns >= kColumns && tiles * tiles16 > RFROM && nt * lds16 <= kResidentLds) {
-        const int groups = (tiles16 + nt - 1) / nt, fit = (int)(kResidentLds / (nt * lds16));
+        const int groups = (tiles16 + nt - 1) / nt, fit = std::min((int)(kResidentLds / (nt * lds16)), 640 / (16 * nt));
         int chunks = (groups + fit - 1) / fit;
         while (chunks < groups && tiles * chunks < RWAVES) ++chunks;
         if (GRAD && IN == kIn32) chunks = groups;       // the kernel walks 64 rows: what it made of gy and z is gone after them
         const int block_groups = (groups + chunks - 1) / chunks, block_rows = block_groups * nt * 16;
-        const size_t lds = block_groups * nt * lds16 + block_rows * (COMPLEX ? 8 : 4);
+        const size_t lds = block_groups * nt * lds16 + block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
         const long last = q.columns % kColumns;
         if (last && q.residual && (q.residual == q.y || q.residual == q.z)) {
             // the last tile would start among columns of the one before it, whose residuals may be results by then: it goes to the direct kernel

@@ -263,13 +263,13 @@ int tiles_of(int N, int K, int& ktiles)
     ktiles = (K + kGradColumns - 1) / kGradColumns;
     return (N + kGradRows - 1) / kGradRows * ktiles;
 }
-// Parts of the positions: as many blocks as run at a time on 256 CUs (one or two on each, by their registers), at least four steps for each wave
+// Parts of the positions: as many blocks as run at a time on 256 CUs (one or two on each, by their registers), two steps for each wave at least
 int splits_of(int type, long P, int N, int K)
 {
     int ktiles;
     const long steps = (P * values_of(type) + kStep - 1) / kStep, tiles = tiles_of(N, K, ktiles);
     long splits = ((type == kC64 ? 256 : 512) + tiles - 1) / tiles;
-    if (splits > (steps + 15) / 16) splits = (steps + 15) / 16;
+    if (splits > (steps + 7) / 8) splits = (steps + 7) / 8;
     if (splits > 8) splits = splits / 8 * 8;
     return splits < 1 ? 1 : (int)splits;
 }

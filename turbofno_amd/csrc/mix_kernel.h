@@ -426,10 +426,12 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, true> Wave;
     const Wave wave(q);
     const long id = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long column0 = id / row_groups * kColumns;
+    const long column = id / row_groups * kColumns, left = q.columns - column;
     const int row0 = (int)(id % row_groups) * (16 * NT);
-    if (column0 >= q.columns) return;
-    const Window w = { column0, q.columns - column0 < kColumns ? (int)(q.columns - column0) : (int)kColumns };
+    if (left <= 0) return;
+    // a last tile that is not whole ends with the columns, if what the tile before it stores there cannot be a residual that it has yet to read
+    const bool back = left < kColumns && q.columns >= kColumns && !(q.residual && (q.residual == q.y || q.residual == q.z));
+    const Window w = { back ? q.columns - kColumns : column, left < kColumns && !back ? (int)left : (int)kColumns };
     const bool slopes = GRAD && q.act != kActNone;
     const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
     float4_v acc[NT][4] = {};

@@ -32,6 +32,13 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t
     return hipGetLastError();
 }
 
+// Up to this many tiles of 64 columns x 16 rows a wave of the direct kernel takes one of them: the resident one would form its operands of A on few CUs
+// first. complex64, gelu, residual: 64 to 64 channels at 200 ... 4096 positions 7.4 ... 7.7 us, 12.2 ... 12.6 in the resident one; 128 to 128 at
+// 4096 13.2 and 14.2; bf16, 256 to 256 at 4096 11.4 and 13.7. Above, the operands are formed once for all tiles of a block.
+constexpr long kFewTiles = 1024;
+// Fewer tiles than this number of waves (of 256 CUs): the rows of A are divided too
+constexpr long kWaves = 2048;
+
 // steps that registers hold, and beyond how many of them the sums of 64 rows find no room beside them
 template <int IN, bool COMPLEX> constexpr int kMostSteps = IN == kIn32 && !COMPLEX ? 4 : 8;
 template <int IN, int OUT, bool COMPLEX> constexpr int kMostWideSteps = IN == kIn32 ? (COMPLEX ? 4 : 2) : OUT == kIn32 ? 4 : 8;
@@ -57,20 +64,18 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     constexpr int CHANNELS = COMPLEX ? 16 : 32;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
-    const size_t lds16 = (size_t)(steps > kMostSteps<IN, COMPLEX> ? steps : held_for(steps)) * kWaveParts(IN) * 1024;         // of 16 rows
-    constexpr int MOST = kMostSteps<IN, COMPLEX>;
-    const int nt = tiles16 <= 2 || (steps > kMostWideSteps<IN, OUT, COMPLEX> && steps <= MOST) ? 2 : 4;
+    // gradients of 32-bit real rows with three or four steps are streamed in 64 rows instead of held in 32: the slopes are formed half as often
+    // (128 to 128 channels at 262144 positions, both gradients: 252 us, 264 held; 256 to 120 at 65536: 104 and 124)
+    const bool held = steps <= kMostSteps<IN, COMPLEX> && !(GRAD && IN == kIn32 && !COMPLEX && steps > 2);
+    const size_t lds16 = (size_t)(held ? held_for(steps) : steps) * kWaveParts(IN) * 1024;     // of 16 rows
+    const int nt = tiles16 <= 2 || (held && steps > kMostWideSteps<IN, OUT, COMPLEX>) ? 2 : 4;
     // the lane's part of an address, up to 24 rows of the input or 12 of the results, in 32 bits
     const long widest = std::max(std::max(std::max(q.ldx, q.ldzin), q.ldr), std::max(q.ldy, q.ldz));
     const bool near = widest < (1L << 24) && tiles < (1L << 30);
-#ifndef RFROM
-#define RFROM 1024
-#define RWAVES 2048
-#endif
-    if (near && q.columns >= kColumns && tiles * tiles16 > RFROM && nt * lds16 <= kResidentLds) {
+    if (near && q.columns >= kColumns && tiles * tiles16 > kFewTiles && nt * lds16 <= kResidentLds) {
         const int groups = (tiles16 + nt - 1) / nt, fit = std::min((int)(kResidentLds / (nt * lds16)), 640 / (16 * nt));
         int chunks = (groups + fit - 1) / fit;
-        while (chunks < groups && tiles * chunks < RWAVES) ++chunks;
+        while (chunks < groups && tiles * chunks < kWaves) ++chunks;
         if (GRAD && IN == kIn32) chunks = groups;       // the kernel walks 64 rows: what it made of gy and z is gone after them
         const int block_groups = (groups + chunks - 1) / chunks, block_rows = block_groups * nt * 16;
         const size_t lds = block_groups * nt * lds16 + block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
@@ -90,7 +95,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
             if (hipError_t e = launch_mix<IN, OUT, COMPLEX, GRAD>(whole, stream); e != hipSuccess) return e;
             return launch_direct<IN, OUT, COMPLEX, GRAD, 1>(rest, stream);
         }
-        return launch_steps<IN, OUT, COMPLEX, GRAD>(q, nt, steps > MOST ? 0 : held_for(steps), block_rows, lds, stream);
+        return launch_steps<IN, OUT, COMPLEX, GRAD>(q, nt, held ? held_for(steps) : 0, block_rows, lds, stream);
     }
     if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1>(q, stream);
     if (tiles16 == 2 || tiles * tiles16 <= 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 2>(q, stream);

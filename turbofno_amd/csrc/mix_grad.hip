@@ -6,8 +6,8 @@
 // x, the quarters of a wave 32 of them, and has the operands of its matrix instructions. Complex rows are (re, im) pairs: gz as it is against
 // (re, im) of x for the real part, against (-im, re) for the imaginary part. 32-bit values are split into bf16 parts (bf16_split.h), 16-bit ones
 // are exact; sums are fp32. gbias takes its sums from the values of gz that pass by.
-// A block takes a tile of 64 rows n and 64 rows k, so that up to 64 channels are read once, and a part of the positions: its four waves four steps of 32 real values side by
-// side, then those as many steps further as all blocks take together. So the blocks move through the rows as one window: with a contiguous part for each
+// A block takes a tile of 64 rows n and 64 rows k, so that up to 64 channels are read once (or of 32 and 32), and a part of the positions: its four waves two steps of 32
+// real values side by side, then those as many steps further as all blocks take together. So the blocks move through the rows as one window: with a contiguous part for each
 // block they all would stand at the same offset of their parts, on the same few memory channels. The blocks' sums go to the workspace and are added in a second kernel, always in the
 // same order: results do not change from call to call.
 // An infinite operand, or one above the largest bf16 number (3.3895e38), makes the sums it takes part in infinite or NaN.
@@ -18,7 +18,6 @@ namespace tfno {
 
 namespace {
 
-constexpr int kGradRows = 64, kGradColumns = 64;        // rows n and rows k of a tile
 constexpr int kStep = 32, kRun = 16;                    // real values of a step; steps of a run
 
 struct GradParams {
@@ -26,8 +25,19 @@ struct GradParams {
     long ldg, ldx, columns;                             // real values
     int N, K;
     float* sums;                                        // [splits][N K V + N V]
+    void *gW, *gbias;                                   // gbias may be null
     int splits, ktiles, tiles;
 };
+
+// result `at` of weights and bias, which follow one another
+template <bool B16> __device__ __forceinline__ void put_gradient(void* gW, void* gbias, long weights, long at, float sum)
+{
+    void* to = at < weights ? gW : gbias;
+    if (at >= weights) at -= weights;
+    if (!to) return;
+    if constexpr (B16) static_cast<__bf16*>(to)[at] = (__bf16)sum;
+    else static_cast<float*>(to)[at] = sum;
+}
 
 template <int IN> struct Eight;
 template <> struct Eight<kIn32> { float4_v lo, hi; };
@@ -45,18 +55,34 @@ template <int IN> __device__ __forceinline__ Eight<IN> load8(const typename Colu
     } else e.v = *reinterpret_cast<const uint4_any*>(p);
     return e;
 }
-// the first `there` of them, zeros for the others
-template <int IN> __device__ __forceinline__ Eight<IN> load8_ragged(const typename Columns<IN>::Value* p, int there)
+// which of a lane's values an index is, from the first
+template <int IN> constexpr int place(int i) { return IN == kIn32 && i >= 4 ? i + 12 : i; }
+// the same from a row that has fewer than a step's: the last one stands for those that there are not
+template <int IN> __device__ __forceinline__ Eight<IN> load8_short(const typename Columns<IN>::Value* p, int there)
 {
     Eight<IN> e;
-    auto at = [&](int i) { return i < there ? p[i] : (typename Columns<IN>::Value)0; };
+    auto at = [&](int i) { return p[place<IN>(i) < there ? place<IN>(i) : there - 1]; };
     if constexpr (IN == kIn32) {
         e.lo = (float4_v){ at(0), at(1), at(2), at(3) };
-        e.hi = (float4_v){ at(16), at(17), at(18), at(19) };
+        e.hi = (float4_v){ at(4), at(5), at(6), at(7) };
     } else
 #pragma unroll
         for (int j = 0; j < 4; ++j) e.v[j] = at(2 * j) | (unsigned)at(2 * j + 1) << 16;
     return e;
+}
+// zeros for the values at places below `from` and from `to` on
+template <int IN> __device__ __forceinline__ void keep(Eight<IN>& e, int from, int to)
+{
+    auto in = [&](int i) { return place<IN>(i) >= from && place<IN>(i) < to; };
+    if constexpr (IN == kIn32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            e.lo[i] = in(i) ? e.lo[i] : 0.f;
+            e.hi[i] = in(4 + i) ? e.hi[i] : 0.f;
+        }
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e.v[j] &= (in(2 * j) ? 0xffffu : 0u) | (in(2 * j + 1) ? 0xffff0000u : 0u);
 }
 __device__ __forceinline__ void operand(const Eight<kIn32>& e, SplitOperand& o)
 {
@@ -110,13 +136,14 @@ template <int B> __device__ __forceinline__ void multiply(uint4_v a, const uint4
     for (int i = 0; i < B; ++i) c[i] = mfma_bf16(a, b[i], c[i]);
 }
 
-template <int IN, bool COMPLEX> __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const GradParams q)
+// SHORT: rows of fewer than a step's values
+template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const GradParams q)
 {
-    constexpr int V = COMPLEX ? 2 : 1, KT = kGradColumns / 16;         // tiles of 16 rows k
+    constexpr int V = COMPLEX ? 2 : 1;
     constexpr int LANE = IN == kIn32 ? 4 : 8;           // consecutive values of a lane
     typedef typename std::conditional<IN == kIn32, SplitOperand, uint4_v>::type Op;
     typedef typename Columns<IN>::Value Value;
-    constexpr int ACC = 4 * KT * V;
+    constexpr int ACC = T * T * V;
     extern __shared__ float4_v totals[];                // [wave][sum][lane]
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
     // blocks of one part of the positions are eight apart, on one XCD: they read the same rows
@@ -131,36 +158,35 @@ template <int IN, bool COMPLEX> __global__ __launch_bounds__(256, 1) void weight
         split = full + rest / q.tiles;
         tile = rest % q.tiles;
     }
-    const int n0 = tile / q.ktiles * kGradRows, k0 = tile % q.ktiles * kGradColumns;
-    const Value* g[4];
-    const Value* x[KT];
+    const int n0 = tile / q.ktiles * (16 * T), k0 = tile % q.ktiles * (16 * T);
+    const Value* g[T];
+    const Value* x[T];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) g[t] = static_cast<const Value*>(q.g) + (n0 + 16 * t + c < q.N ? n0 + 16 * t + c : q.N - 1) * q.ldg + LANE * kq;
+    for (int t = 0; t < T; ++t) g[t] = static_cast<const Value*>(q.g) + (n0 + 16 * t + c < q.N ? n0 + 16 * t + c : q.N - 1) * q.ldg + LANE * kq;
 #pragma unroll
-    for (int t = 0; t < KT; ++t) x[t] = static_cast<const Value*>(q.x) + (k0 + 16 * t + c < q.K ? k0 + 16 * t + c : q.K - 1) * q.ldx + LANE * kq;
+    for (int t = 0; t < T; ++t) x[t] = static_cast<const Value*>(q.x) + (k0 + 16 * t + c < q.K ? k0 + 16 * t + c : q.K - 1) * q.ldx + LANE * kq;
 
-    float4_v acc[4][KT * V] = {};
-    float bias_re[4] = {}, bias_im[4] = {};
+    float4_v acc[T][T * V] = {};
+    float bias_re[T] = {}, bias_im[T] = {};
     struct Rows {
-        Eight<IN> g[4], x[KT];
+        Eight<IN> g[T], x[T];
     };
-    auto fetch = [&](long step, Rows& r) {
-        const long column = step * kStep;
+    auto fetch = [&](long column, Rows& r) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) r.g[t] = load8<IN>(g[t] + column);
+        for (int t = 0; t < T; ++t) r.g[t] = load8<IN>(g[t] + column);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) r.x[t] = load8<IN>(x[t] + column);
+        for (int t = 0; t < T; ++t) r.x[t] = load8<IN>(x[t] + column);
         __builtin_amdgcn_sched_barrier(0);              // the loads stay ahead of the products that follow
     };
     auto product = [&](const Rows& r) {
-        Op b[KT * V];
+        Op b[T * V];
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
+        for (int t = 0; t < T; ++t) {
             operand(r.x[t], b[V * t]);
             if constexpr (COMPLEX) b[V * t + 1] = imaginary(b[V * t]);
         }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < T; ++t) {
             Op a;
             operand(r.g[t], a);
             add_values<COMPLEX>(r.g[t], bias_re[t], bias_im[t]);
@@ -175,18 +201,18 @@ template <int IN, bool COMPLEX> __global__ __launch_bounds__(256, 1) void weight
     auto flush = [&] {
 #pragma unroll
         for (int t = 0; t < ACC; ++t) {
-            total[t * 64] = begun ? total[t * 64] + acc[t / (KT * V)][t % (KT * V)] : acc[t / (KT * V)][t % (KT * V)];
-            acc[t / (KT * V)][t % (KT * V)] = float4_v{};
+            total[t * 64] = begun ? total[t * 64] + acc[t / (T * V)][t % (T * V)] : acc[t / (T * V)][t % (T * V)];
+            acc[t / (T * V)][t % (T * V)] = float4_v{};
         }
         begun = true;
         run = 0;
     };
-    // whole steps, two on their way at a time (after the last one, the last one again: a branch around loads would be waited at); then the rest of the columns
+    // whole steps, two on their way at a time (after the last one, the last one again: a branch around loads would be waited at)
     const long steps = q.columns / kStep, stride = 8l * q.splits, first = 8l * split + 2 * __builtin_amdgcn_readfirstlane(wave);
-    if (first < steps) {
+    if (!SHORT && first < steps) {
         Rows r0, r1;
-        auto at = [&](long s) { return s < steps ? s : steps - 1; };
-        fetch(first, r0);
+        auto at = [&](long s) { return (s < steps ? s : steps - 1) * kStep; };
+        fetch(at(first), r0);
         for (long s = first;; s += stride) {
             fetch(at(s + 1), r1);
             product(r0);
@@ -197,40 +223,57 @@ template <int IN, bool COMPLEX> __global__ __launch_bounds__(256, 1) void weight
             if (s + stride >= steps) break;
         }
     }
-    if (steps * kStep < q.columns && steps % stride / 2 * 2 == first) {
+    // the rest of the columns: a step that ends with them, less what the one before it has had
+    const int rest = (int)(q.columns - steps * kStep);
+    if (rest && steps % stride / 2 * 2 == first) {
         Rows r;
-        const int rest = (int)(q.columns - steps * kStep) - LANE * kq;
+        if constexpr (SHORT) {
+            const int there = rest > LANE * kq ? rest - LANE * kq : 1, back = rest > LANE * kq ? 0 : LANE * kq;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) r.g[t] = load8_ragged<IN>(g[t] + steps * kStep, rest);
+            for (int t = 0; t < T; ++t) r.g[t] = load8_short<IN>(g[t] - back, there);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) r.x[t] = load8_ragged<IN>(x[t] + steps * kStep, rest);
+            for (int t = 0; t < T; ++t) r.x[t] = load8_short<IN>(x[t] - back, there);
+        } else fetch(q.columns - kStep, r);
+        const int from = SHORT ? 0 : kStep - rest - LANE * kq, to = SHORT ? rest - LANE * kq : (int)kStep;
+#pragma unroll
+        for (int t = 0; t < T; ++t) keep<IN>(r.g[t], from, to);
+#pragma unroll
+        for (int t = 0; t < T; ++t) keep<IN>(r.x[t], from, to);
         product(r);
     }
 
     flush();
     __syncthreads();
-    float* out = q.sums + (long)split * ((long)q.N * q.K + q.N) * V;
+    // to the workspace; the sums of all positions to the results
+    const long weights = (long)q.N * q.K * V;
+    float* out = q.sums + split * (weights + q.N * V);
+    auto put = [&](long at, float sum) {
+        if (T == 2 && q.splits == 1) put_gradient<IN == kIn16>(q.gW, q.gbias, weights, at, sum);
+        else out[at] = sum;
+    };
     for (int e = threadIdx.x; e < ACC * 64; e += 256) {
         const float4_v sum = (totals[e] + totals[ACC * 64 + e]) + (totals[2 * ACC * 64 + e] + totals[3 * ACC * 64 + e]);
-        const int l = e % 64, t = e / 64, n = n0 + 16 * (t / (KT * V)) + 4 * (l / 16), k = k0 + 16 * (t % (KT * V) / V) + l % 16;
+        const int l = e % 64, t = e / 64, n = n0 + 16 * (t / (T * V)) + 4 * (l / 16), k = k0 + 16 * (t % (T * V) / V) + l % 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (n + i < q.N && k < q.K) out[((long)(n + i) * q.K + k) * V + t % V] = sum[i];
+            if (n + i < q.N && k < q.K) put(((long)(n + i) * q.K + k) * V + t % V, sum[i]);
+    }
+    if (k0) return;
+    __syncthreads();
+    float* bias = reinterpret_cast<float*>(totals);     // [part][t][thread]
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        bias[t * 256 + threadIdx.x] = bias_re[t];
+        if constexpr (COMPLEX) bias[(T + t) * 256 + threadIdx.x] = bias_im[t];
     }
     __syncthreads();
-    float4_v* bias4 = totals;
-    if (k0 == 0) {
-        bias4[2 * threadIdx.x] = (float4_v){ bias_re[0], bias_re[1], bias_re[2], bias_re[3] };
-        bias4[2 * threadIdx.x + 1] = (float4_v){ bias_im[0], bias_im[1], bias_im[2], bias_im[3] };
-        __syncthreads();
-        // thread r: row n0 + r, over four waves and four quarters
-        if (threadIdx.x < 64 * V) {
-            const int r = threadIdx.x / V, part = threadIdx.x % V;
-            float sum = 0.f;
+    // thread r: row n0 + r, over four waves and four quarters
+    if (threadIdx.x < 16 * T * V) {
+        const int r = threadIdx.x / V, part = threadIdx.x % V;
+        float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < 16; ++w) sum += reinterpret_cast<const float*>(bias4)[(2 * (16 * w + r % 16) + part) * 4 + r / 16];
-            if (n0 + r < q.N) out[(long)q.N * q.K * V + (n0 + r) * V + part] = sum;
-        }
+        for (int w = 0; w < 16; ++w) sum += bias[(T * part + r / 16) * 256 + 16 * w + r % 16];
+        if (n0 + r < q.N) put(weights + (n0 + r) * V + part, sum);
     }
 }
 
@@ -249,53 +292,65 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict_
     __syncthreads();
     if (quarter == 0 && e < count) {
         sum = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-        void* to = e < weights ? gW : gbias;
-        const long at = e < weights ? e : e - weights;
-        if (to) {
-            if (type == kBF16) static_cast<__bf16*>(to)[at] = (__bf16)sum;
-            else static_cast<float*>(to)[at] = sum;
-        }
+        if (type == kBF16) put_gradient<true>(gW, gbias, weights, e, sum);
+        else put_gradient<false>(gW, gbias, weights, e, sum);
     }
 }
 
-int tiles_of(int N, int K, int& ktiles)
+// Up to this many steps of tiles of 32 x 32 such tiles are taken: a step of theirs is a quarter of the work, and the loads, of which there are twice as many,
+// come from the caches. Both gradients, complex64, gelu, 64 to 64 channels: 24.1 us at 200 positions with 64 x 64, 16.9 with 32 x 32; 50.0 and 36.6
+// at 30001; at 2^20, in HBM, 726 and 772 (bf16 206 and 250). Up to 32 x 32 channels there is one tile of either: 2^18 positions of 16 to 16 channels 94 and 61.
+constexpr long kSmallWork = 16384;
+// Tiles of a product: 16 t rows in both directions
+struct Tiling {
+    int t, ktiles, tiles, splits;
+};
+Tiling tiling_of(int type, long P, int N, int K)
 {
-    ktiles = (K + kGradColumns - 1) / kGradColumns;
-    return (N + kGradRows - 1) / kGradRows * ktiles;
-}
-// Parts of the positions: as many blocks as run at a time on 256 CUs (one or two on each, by their registers), two steps for each wave at least
-int splits_of(int type, long P, int N, int K)
-{
-    int ktiles;
-    const long steps = (P * values_of(type) + kStep - 1) / kStep, tiles = tiles_of(N, K, ktiles);
-    long splits = ((type == kC64 ? 256 : 512) + tiles - 1) / tiles;
+    Tiling g;
+    const long steps = (P * values_of(type) + kStep - 1) / kStep, small = (long)((N + 31) / 32) * ((K + 31) / 32);
+    g.t = small == 1 || small * steps <= kSmallWork ? 2 : 4;
+    g.ktiles = (K + 16 * g.t - 1) / (16 * g.t);
+    g.tiles = (N + 16 * g.t - 1) / (16 * g.t) * g.ktiles;
+    // Parts of the positions: as many blocks as run at a time on 256 CUs (one or two on each, by their registers), two steps for each wave at least;
+    // one part, without a second kernel, where each wave has up to four steps
+    long splits = ((type == kC64 && g.t == 4 ? 256 : 512) + g.tiles - 1) / g.tiles;
     if (splits > (steps + 7) / 8) splits = (steps + 7) / 8;
     if (splits > 8) splits = splits / 8 * 8;
-    return splits < 1 ? 1 : (int)splits;
+    g.splits = splits < 1 || (g.t == 2 && steps <= 16) ? 1 : (int)splits;
+    return g;
+}
+template <int IN, bool COMPLEX, int T> hipError_t launch_parts(const GradParams& q, hipStream_t stream)
+{
+    const bool few = q.columns < kStep;
+    const size_t lds = (size_t)4 * T * T * (COMPLEX ? 2 : 1) * 1024;
+    const auto kernel = few ? weight_grad_kernel<IN, COMPLEX, T, true> : weight_grad_kernel<IN, COMPLEX, T, false>;
+    static std::atomic<unsigned long long> served[2];
+    if (lds > (64 << 10))
+        if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, served[few]); e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(q.splits * q.tiles)), dim3(256), lds, stream, q);
+    return hipGetLastError();
+}
+template <int IN, bool COMPLEX> hipError_t launch_tiles(int t, const GradParams& q, hipStream_t stream)
+{
+    return t == 2 ? launch_parts<IN, COMPLEX, 2>(q, stream) : launch_parts<IN, COMPLEX, 4>(q, stream);
 }
 
 }  // namespace
 
 size_t mix_weight_grad_workspace(int type, long P, int N, int K)
 {
-    return (size_t)splits_of(type, P, N, K) * ((size_t)N * K + N) * values_of(type) * sizeof(float);
+    return (size_t)tiling_of(type, P, N, K).splits * ((size_t)N * K + N) * values_of(type) * sizeof(float);
 }
 
 hipError_t launch_mix_weight_grad(int type, long P, int N, int K, const void* gz, long ldgz, const void* x, long ldx, void* gW, void* gbias, void* workspace,
                                   hipStream_t stream)
 {
     const int v = values_of(type);
-    GradParams q = { gz, x, ldgz * v, ldx * v, P * v, N, K, static_cast<float*>(workspace), splits_of(type, P, N, K), 0, 0 };
-    q.tiles = tiles_of(N, K, q.ktiles);
-    const dim3 grid((unsigned)(q.splits * q.tiles));
-    const size_t lds = (size_t)4 * 4 * (kGradColumns / 16) * v * 1024;
-    if (type == kC64) {
-        static std::atomic<unsigned long long> served{ 0 };
-        if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(weight_grad_kernel<kIn32, true>), lds, served); e != hipSuccess) return e;
-        hipLaunchKernelGGL((weight_grad_kernel<kIn32, true>), grid, dim3(256), lds, stream, q);
-    } else if (type == kF32) hipLaunchKernelGGL((weight_grad_kernel<kIn32, false>), grid, dim3(256), lds, stream, q);
-    else hipLaunchKernelGGL((weight_grad_kernel<kIn16, false>), grid, dim3(256), lds, stream, q);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const Tiling g = tiling_of(type, P, N, K);
+    const GradParams q = { gz, x, ldgz * v, ldx * v, P * v, N, K, static_cast<float*>(workspace), gW, gbias, g.splits, g.ktiles, g.tiles };
+    const hipError_t e = type == kC64 ? launch_tiles<kIn32, true>(g.t, q, stream) : type == kF32 ? launch_tiles<kIn32, false>(g.t, q, stream) : launch_tiles<kIn16, false>(g.t, q, stream);
+    if (e != hipSuccess || (g.t == 2 && g.splits == 1)) return e;
     const long weights = (long)N * K * v, count = weights + (long)N * v;
     hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)((count + 63) / 64)), dim3(256), 0, stream, q.sums, q.splits, count, weights, type, gW, gbias);
     return hipGetLastError();

@@ -130,49 +130,69 @@ template <int IN, bool COMPLEX, bool CONJ> __device__ __forceinline__ void make_
     }
 }
 
-// eight consecutive values of the contraction of one row of A: entries e ... e + 7 of `count` real entries, zeros beyond. The row is row `row` of
-// W (forward), or column `row` of W (gradient; its entries are `ld` channels apart).
-template <int IN, bool COMPLEX, bool GRAD>
-__device__ __forceinline__ void load_weights(const void* W, int row, int rows, int e, int count, int ld, Operand<IN>& a)
+// Eight consecutive values of the contraction of one row of A: entries e ... e + 7 of `count` real entries. The row is row `row` of W (forward), or
+// column `row` of W (gradient; its entries are `ld` channels apart). First the loads, without a branch: entries that there are not are read from some
+// other place in W, of 8 values at least (FEW: of fewer), rows beyond the last from the last one.
+template <int IN> struct RawWeights {
+    typename Columns<IN>::Value w[8];
+};
+template <int IN, bool COMPLEX, bool GRAD, bool FEW>
+__device__ __forceinline__ void fetch_weights(const void* W, int row, int rows, int e, int count, int ld, RawWeights<IN>& r)
 {
     constexpr int V = COMPLEX ? 2 : 1;
-    typedef typename Columns<IN>::Value Value;
-    Value w[8];
-    const Value* p = static_cast<const Value*>(W);
-    const bool inside = row < rows;
-    if (!GRAD && inside && e + 8 <= count) {
-        p += (long)row * ld * V + e;
-        if constexpr (IN == kIn8) {
-            const RawOf<kIn16> raw = *reinterpret_cast<const uint2_bytes*>(p);
-            __builtin_memcpy(w, &raw, 8);
-        } else {
-            const RawOf<IN> lo = load4<IN>(p, 0), hi = load4<IN>(p, 4);
-            __builtin_memcpy(w, &lo, sizeof lo);
-            __builtin_memcpy(w + 4, &hi, sizeof hi);
-        }
-    } else
+    const auto* p = static_cast<const typename Columns<IN>::Value*>(W);
+    row = row < rows ? row : rows - 1;
+    if constexpr (GRAD || FEW) {
 #pragma unroll
         for (int j = 0; j < 8; j += V) {
-            const int k = (e + j) / V;                   // channel of the contraction
-            const bool there = inside && e + j < count;
-            const long at = there ? (GRAD ? (long)k * ld + row : (long)row * ld + k) * V : 0;
+            const int k = e + j < count ? (e + j) / V : count / V - 1;     // channel of the contraction
 #pragma unroll
-            for (int i = 0; i < V; ++i) w[j + i] = there ? p[at + i] : (Value)0;
+            for (int i = 0; i < V; ++i) r.w[j + i] = p[(GRAD ? (long)k * ld + row : (long)row * ld + k) * V + i];
         }
+    } else {
+        const long at = (long)row * ld * V + e, last = (long)(rows - 1) * ld * V + count - 8;
+        p += at < last ? at : last;
+        if constexpr (IN == kIn8) {
+            const RawOf<kIn16> raw = *reinterpret_cast<const uint2_bytes*>(p);
+            __builtin_memcpy(r.w, &raw, 8);
+        } else {
+            const RawOf<IN> lo = load4<IN>(p, 0), hi = load4<IN>(p, 4);
+            __builtin_memcpy(r.w, &lo, sizeof lo);
+            __builtin_memcpy(r.w + 4, &hi, sizeof hi);
+        }
+    }
+}
+// then the operand that they make, with zeros for entries that there are not
+template <int IN, bool COMPLEX, bool GRAD, bool FEW>
+__device__ __forceinline__ void form_weights(RawWeights<IN> r, int row, int rows, int e, int count, int ld, Operand<IN>& a)
+{
+    constexpr int V = COMPLEX ? 2 : 1;
+    if (e + 8 > count) {
+        if constexpr (!GRAD && !FEW) {                 // entries that were read from before their place
+            const long at = (long)(row < rows ? row : rows - 1) * ld * V + e, last = (long)(rows - 1) * ld * V + count - 8;
+            const int by = at <= last ? 0 : at - last < 8 ? (int)(at - last) : 7;
+#pragma unroll
+            for (int bit = 1; bit < 8; bit *= 2)
+#pragma unroll
+                for (int j = 0; j < 8 - bit; ++j) r.w[j] = by & bit ? r.w[j + bit] : r.w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r.w[j] = e + j < count ? r.w[j] : 0;
+    }
     if constexpr (IN == kIn32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             unsigned h, m, l;
-            split_bf16_pair(w[2 * j], w[2 * j + 1], h, m, l);
+            split_bf16_pair(r.w[2 * j], r.w[2 * j + 1], h, m, l);
             a.h[j] = h; a.m[j] = m; a.l[j] = l;
         }
     } else if constexpr (IN == kIn16) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a.v[j] = w[2 * j] | (unsigned)w[2 * j + 1] << 16;
+        for (int j = 0; j < 4; ++j) a.v[j] = r.w[2 * j] | (unsigned)r.w[2 * j + 1] << 16;
     } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint2_v v = widen(w[4 * j] | (unsigned)w[4 * j + 1] << 8 | (unsigned)w[4 * j + 2] << 16 | (unsigned)w[4 * j + 3] << 24);
+            const uint2_v v = widen(r.w[4 * j] | (unsigned)r.w[4 * j + 1] << 8 | (unsigned)r.w[4 * j + 2] << 16 | (unsigned)r.w[4 * j + 3] << 24);
             a.v[2 * j] = v[0];
             a.v[2 * j + 1] = v[1];
         }
@@ -230,8 +250,8 @@ struct Window {
 };
 
 // What a wave does with its columns: the input of a step, and the results. An address is a uniform part, 64 bits in scalar registers, and the lane's
-// part; FAR: the lane's part may take more than 32 bits, and columns beyond the last may be asked for (the direct kernel).
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct MixWave {
+// part; FAR: the lane's part may take more than 32 bits (the direct kernel), RAGGED: and columns beyond the last may be asked for.
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR, bool RAGGED> struct MixWave {
     static constexpr int V = COMPLEX ? 2 : 1, CHANNELS = 32 / V, PER_LANE = 8 / V;      // channels of a step, of a lane
     typedef RawOf<IN> Rows[PER_LANE];                   // a lane's part of a step
     typedef typename Columns<OUT>::Value OutValue;
@@ -248,7 +268,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
         const long at = row * ld + w.column0;
         if constexpr (FAR) {
             const Value* p = static_cast<const Value*>(base) + at + (there ? lane_row * ld : 0);
-            return w.there < kColumns ? load4_ragged<TYPE>(p, 4 * c, w.there) : load4<TYPE>(p, 4 * c);
+            return RAGGED ? load4_ragged<TYPE>(p, 4 * c, w.there) : load4<TYPE>(p, 4 * c);
         } else {
             unsigned offset = fresh(((unsigned)lane_row * (unsigned)ld + 4 * c) * (unsigned)sizeof(Value));
             if (GUARD) offset = there ? offset : 4 * c * (unsigned)sizeof(Value);
@@ -261,7 +281,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR> struct Mix
         const long at = row * ld + w.column0;
         if constexpr (FAR) {
             Value* p = static_cast<Value*>(base) + at + lane_row * ld;
-            if (w.there < kColumns) store4_ragged<TYPE>(p, 4 * c, w.there, v);
+            if constexpr (RAGGED) store4_ragged<TYPE>(p, 4 * c, w.there, v);
             else store4<TYPE>(p, 4 * c, v);
         } else near_store4<TYPE>(scalar(base, at * (long)sizeof(Value)), fresh(((unsigned)lane_row * (unsigned)ld + 4 * c) * (unsigned)sizeof(Value)), v);
     }
@@ -420,48 +440,55 @@ template <int N, int I = 0, typename F> __device__ __forceinline__ void unrolled
 }
 
 // Few columns: a wave for 64 columns and 16 NT rows, weights from memory
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT>
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool RAGGED, bool FEW>
 __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, int row_groups)
 {
-    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, true> Wave;
+    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, true, RAGGED> Wave;
     const Wave wave(q);
     const long id = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long column = id / row_groups * kColumns, left = q.columns - column;
     const int row0 = (int)(id % row_groups) * (16 * NT);
     if (left <= 0) return;
-    // a last tile that is not whole ends with the columns, if what the tile before it stores there cannot be a residual that it has yet to read
-    const bool back = left < kColumns && q.columns >= kColumns && !(q.residual && (q.residual == q.y || q.residual == q.z));
-    const Window w = { back ? q.columns - kColumns : column, left < kColumns && !back ? (int)left : (int)kColumns };
+    const Window w = { RAGGED || left >= kColumns ? column : q.columns - kColumns, RAGGED && left < kColumns ? (int)left : (int)kColumns };
     const bool slopes = GRAD && q.act != kActNone;
-    const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
+    const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS, count = q.contraction * Wave::V;
     float4_v acc[NT][4] = {};
-    typename Wave::Rows x0, z0, x1, z1;
-    auto fetch = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
+    constexpr bool AHEAD = NT == 1;                     // the weights of a step are asked for with its rows: there are registers for them
+    struct Step {
+        typename Wave::Rows x, z;
+        RawWeights<IN> a[NT];
+    } s0, s1;
+    auto fetch_a = [&](int s, int t, RawWeights<IN>& a) {
+        fetch_weights<IN, COMPLEX, GRAD, FEW>(q.W, row0 + 16 * t + wave.c, q.rows, 32 * s + 8 * wave.kq, count, q.ldw, a);
+    };
+    auto fetch = [&](int s, Step& r) {
         s = s < steps ? s : steps - 1;
-        wave.template fetch<true>(q.x, q.ldx, w, s, x);
-        if (slopes) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
+        wave.template fetch<true>(q.x, q.ldx, w, s, r.x);
+        if constexpr (GRAD) wave.template fetch<true>(slopes ? q.zin : q.x, slopes ? q.ldzin : q.ldx, w, s, r.z);
+        if constexpr (AHEAD) fetch_a(s, 0, r.a[0]);
         __builtin_amdgcn_sched_barrier(0);              // the loads stay ahead of the products that follow
     };
-    auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
+    auto product = [&](int s, Step& r) {
+        if constexpr (!AHEAD) unrolled<NT>([&](int t) { fetch_a(s, t, r.a[t]); });
         if constexpr (GRAD)
-            if (slopes) wave.slope(w, s, x, z, row0 == 0);
-        wave.clear(s, x);
+            if (slopes) wave.slope(w, s, r.x, r.z, row0 == 0);
+        wave.clear(s, r.x);
         Operand<IN> b[4];
-        make_operands<IN, COMPLEX, GRAD>(x, b);
+        make_operands<IN, COMPLEX, GRAD>(r.x, b);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             Operand<IN> a;
-            load_weights<IN, COMPLEX, GRAD>(q.W, row0 + 16 * t + wave.c, q.rows, 32 * s + 8 * wave.kq, q.contraction * Wave::V, q.ldw, a);
+            form_weights<IN, COMPLEX, GRAD, FEW>(r.a[t], row0 + 16 * t + wave.c, q.rows, 32 * s + 8 * wave.kq, count, q.ldw, a);
             multiply<IN>(a, b, acc[t]);
         }
     };
-    fetch(0, x0, z0);
+    fetch(0, s0);
     for (int s = 0; s < steps; s += 2) {
-        fetch(s + 1, x1, z1);
-        product(s, x0, z0);
+        fetch(s + 1, s1);
+        product(s, s0);
         if (s + 1 >= steps) break;
-        fetch(s + 2, x0, z0);
-        product(s + 1, x1, z1);
+        fetch(s + 2, s0);
+        product(s + 1, s1);
     }
     wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); }, [&](int t) { return wave.scale_of(row0 + 16 * t + 4 * wave.kq); });
 }
@@ -477,7 +504,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD>
 __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const MixParams q, int block_rows, int tiles)
 {
     extern __shared__ uint4_v weights[];
-    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, false> Wave;
+    typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, false, false> Wave;
     typedef typename Wave::Parts Parts;
     constexpr int PARTS = kWaveParts(IN), SPARE = HELD > 4 ? 2 : 1;     // steps from HELD - SPARE on may reach beyond the last channel
     const Wave wave(q);
@@ -499,9 +526,11 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
         const int per_step = block_rows / 16 * 64, count = steps * per_step;
 #pragma unroll 4
         for (int e = threadIdx.x; e < count; e += blockDim.x) {
-            const int s = e / per_step, rest = e % per_step, t = rest / 64, l = rest % 64;
+            const int s = e / per_step, rest = e % per_step, l = rest % 64, row = row_first + rest / 64 * 16 + (l & 15), entry = 32 * s + 8 * (l >> 4);
+            RawWeights<IN> raw;
             Operand<IN> a;
-            load_weights<IN, COMPLEX, GRAD>(q.W, row_first + 16 * t + (l & 15), q.rows, 32 * s + 8 * (l >> 4), q.contraction * Wave::V, q.ldw, a);
+            fetch_weights<IN, COMPLEX, GRAD, false>(q.W, row, q.rows, entry, q.contraction * Wave::V, q.ldw, raw);
+            form_weights<IN, COMPLEX, GRAD, false>(raw, row, q.rows, entry, q.contraction * Wave::V, q.ldw, a);
             uint4_v* to = weights + (long)(e / 64) * (64 * PARTS) + l;
             if constexpr (IN == kIn32) { to[0] = a.h; to[64] = a.m; to[128] = a.l; }
             else to[0] = a.v;

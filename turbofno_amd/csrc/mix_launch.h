@@ -6,12 +6,12 @@
 
 namespace tfno {
 
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT> hipError_t launch_direct(const MixParams& q, hipStream_t stream)
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool RAGGED, bool FEW> hipError_t launch_direct(const MixParams& q, hipStream_t stream)
 {
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int groups = (q.rows + 16 * NT - 1) / (16 * NT);
     const long blocks = (tiles * groups + 3) / 4;
-    hipLaunchKernelGGL((mix_direct_kernel<IN, OUT, COMPLEX, GRAD, NT>), dim3((unsigned)blocks), dim3(256), 0, stream, q, groups);
+    hipLaunchKernelGGL((mix_direct_kernel<IN, OUT, COMPLEX, GRAD, NT, RAGGED, FEW>), dim3((unsigned)blocks), dim3(256), 0, stream, q, groups);
     return hipGetLastError();
 }
 
@@ -61,6 +61,26 @@ hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, si
 template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const MixParams& q, hipStream_t stream)
 {
     if (q.columns == 0) return hipSuccess;
+    // Columns that do not fill a tile: the last tile ends with them, among columns of the one before it. Where those may be results by then (the residuals
+    // are in their place), and where there are no others, a kernel takes them one by one
+    const long last = q.columns % kColumns, head = q.columns - last;
+    if (last && head == 0) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, true, !GRAD>(q, stream);
+    if (last && q.residual && (q.residual == q.y || q.residual == q.z)) {
+        constexpr size_t SIZE = sizeof(typename Columns<OUT>::Value);
+        MixParams whole = q, rest = q;
+        whole.columns = head;
+        rest.columns = last;
+        auto ahead = [&](auto* p, size_t size) { return p ? decltype(p)((size_t)p + head * size) : p; };
+        rest.x = ahead(q.x, sizeof(typename Columns<IN>::Value));
+        rest.residual = ahead(q.residual, SIZE);
+        rest.y = ahead(q.y, SIZE);
+        rest.z = ahead(q.z, SIZE);
+        if (q.xscale) rest.xscale = q.xscale + head / (COMPLEX ? 2 : 1);
+        if (hipError_t e = launch_mix<IN, OUT, COMPLEX, GRAD>(whole, stream); e != hipSuccess) return e;
+        return launch_direct<IN, OUT, COMPLEX, GRAD, 1, true, !GRAD>(rest, stream);
+    }
+    if constexpr (!GRAD)        // weights that cannot be read by eight
+        if (((long)(q.rows - 1) * q.ldw + q.contraction) * (COMPLEX ? 2 : 1) < 8) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, false, true>(q, stream);
     constexpr int CHANNELS = COMPLEX ? 16 : 32;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
@@ -72,34 +92,18 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     // the lane's part of an address, up to 24 rows of the input or 12 of the results, in 32 bits
     const long widest = std::max(std::max(std::max(q.ldx, q.ldzin), q.ldr), std::max(q.ldy, q.ldz));
     const bool near = widest < (1L << 24) && tiles < (1L << 30);
-    if (near && q.columns >= kColumns && tiles * tiles16 > kFewTiles && nt * lds16 <= kResidentLds) {
+    if (near && tiles * tiles16 > kFewTiles && nt * lds16 <= kResidentLds) {
         const int groups = (tiles16 + nt - 1) / nt, fit = std::min((int)(kResidentLds / (nt * lds16)), 640 / (16 * nt));
         int chunks = (groups + fit - 1) / fit;
         while (chunks < groups && tiles * chunks < kWaves) ++chunks;
         if (GRAD && IN == kIn32) chunks = groups;       // the kernel walks 64 rows: what it made of gy and z is gone after them
         const int block_groups = (groups + chunks - 1) / chunks, block_rows = block_groups * nt * 16;
         const size_t lds = block_groups * nt * lds16 + block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
-        const long last = q.columns % kColumns;
-        if (last && q.residual && (q.residual == q.y || q.residual == q.z)) {
-            // the last tile would start among columns of the one before it, whose residuals may be results by then: it goes to the direct kernel
-            constexpr size_t SIZE = sizeof(typename Columns<OUT>::Value);
-            MixParams whole = q, rest = q;
-            whole.columns = q.columns - last;
-            rest.columns = last;
-            auto ahead = [&](auto* p, size_t size) { return p ? decltype(p)((size_t)p + whole.columns * size) : p; };
-            rest.x = ahead(q.x, sizeof(typename Columns<IN>::Value));
-            rest.residual = ahead(q.residual, SIZE);
-            rest.y = ahead(q.y, SIZE);
-            rest.z = ahead(q.z, SIZE);
-            if (q.xscale) rest.xscale = q.xscale + whole.columns / (COMPLEX ? 2 : 1);
-            if (hipError_t e = launch_mix<IN, OUT, COMPLEX, GRAD>(whole, stream); e != hipSuccess) return e;
-            return launch_direct<IN, OUT, COMPLEX, GRAD, 1>(rest, stream);
-        }
         return launch_steps<IN, OUT, COMPLEX, GRAD>(q, nt, held ? held_for(steps) : 0, block_rows, lds, stream);
     }
-    if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1>(q, stream);
-    if (tiles16 == 2 || tiles * tiles16 <= 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 2>(q, stream);
-    return launch_direct<IN, OUT, COMPLEX, GRAD, 4>(q, stream);
+    if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, false, false>(q, stream);
+    if (tiles16 == 2 || tiles * tiles16 <= 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 2, false, false>(q, stream);
+    return launch_direct<IN, OUT, COMPLEX, GRAD, 4, false, false>(q, stream);
 }
 
 }  // namespace tfno

@@ -520,8 +520,14 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
         if (s < HELD - SPARE) wave.template fetch<false>(base, ld, w, s, rows);
         else wave.template fetch<true>(base, ld, w, s, rows);
     };
-    typename Wave::Rows x[HELD ? HELD : 1];
+    typename Wave::Rows x[HELD ? HELD : 1], x0, z0;
+    auto ahead = [&](const Window& w, int s, typename Wave::Rows& x, typename Wave::Rows& z) {
+        wave.template fetch<true>(q.x, q.ldx, w, s, x);
+        if constexpr (GRAD) wave.template fetch<true>(slopes ? q.zin : q.x, slopes ? q.ldzin : q.ldx, w, s, z);
+        __builtin_amdgcn_sched_barrier(0);
+    };
     unrolled<HELD>([&](int s) { fetch(q.x, q.ldx, w, s, x[s]); });      // on their way while the operands of A are formed
+    if constexpr (HELD == 0) ahead(w, 0, x0, z0);
     {
         const int per_step = block_rows / 16 * 64, count = steps * per_step;
 #pragma unroll 4
@@ -611,16 +617,10 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
         }
     } else {
         for (; tile < tiles; tile += stride) {
-            w = window(tile);
+            const Window wn = window(tile + stride);
             for (int g = 0; g < groups; ++g) {
+                const Window wf = g < groups - 1 ? w : wn;
                 float4_v acc[NT][4] = {};
-                typename Wave::Rows x0, z0, x1, z1;
-                auto ahead = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
-                    s = s < steps ? s : steps - 1;
-                    wave.template fetch<true>(q.x, q.ldx, w, s, x);
-                    if (slopes) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
-                    __builtin_amdgcn_sched_barrier(0);
-                };
                 auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
                     if constexpr (GRAD)
                         if (slopes) wave.slope(w, s, x, z, writes && g == 0);
@@ -630,16 +630,17 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
 #pragma unroll
                     for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
                 };
-                ahead(0, x0, z0);
+                typename Wave::Rows x1, z1;
                 for (int s = 0; s < steps; s += 2) {
-                    ahead(s + 1, x1, z1);
+                    ahead(w, s + 1 < steps ? s + 1 : s, x1, z1);
                     product(s, x0, z0);
-                    if (s + 1 >= steps) break;
-                    ahead(s + 2, x0, z0);
-                    product(s + 1, x1, z1);
+                    // after the last step the first one of what follows
+                    ahead(s + 2 < steps ? w : wf, s + 2 < steps ? s + 2 : 0, x0, z0);
+                    if (s + 1 < steps) product(s + 1, x1, z1);
                 }
                 finish(g, acc);
             }
+            w = wn;
         }
     }
 }

@@ -494,8 +494,12 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
 }
 
 // Many columns: the operands of the block's rows of A stay in LDS, in the order in which lanes read them (16 bytes per lane, part, 16 rows and step), and
-// its waves walk the columns without meeting again. All steps of the input, HELD or up to `SPARE` fewer, stay in registers while the rows are walked, and
-// are asked for again for the next columns as the last rows use them up; HELD = 0: steps are read as they are needed, again for every 16 NT rows.
+// its waves walk the columns without meeting again: no barrier, and 16 NT rows of sums in registers. HELD = 0: steps of the input are read two ahead, again for
+// every 16 NT rows (out of the L2 cache), the next rows' or columns' first one during the results. HELD > 0: all steps of the input, HELD or up to `SPARE` fewer,
+// stay in registers, in 16 and 8 bits as operands, while the rows are walked.
+// Bound by memory up to about 64 channels (complex64, 64 to 64 with residual, z and gelu at 2^20 positions: 393 - 425 us, 5.1 - 5.5 TB/s, the rate of a
+// copy); then by the matrix cores, six products for one in 32 bits (complex64, 256 to 256 at 65536: 208 us, 1.0 PFLOP/s of bf16 products), and by the vector
+// instructions that form operands and activations (8 bits, 256 to 256 at 262144: 90 us, 3.7 TB/s and 0.38 PFLOP/s).
 constexpr int kWaveParts(int in) { return in == kIn32 ? 3 : 1; }
 constexpr int kResidentThreads = 512;
 // numbers of steps that there are kernels for

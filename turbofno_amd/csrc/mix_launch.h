@@ -24,7 +24,8 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t
         return e;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int chunks = (q.rows + block_rows - 1) / block_rows;
-    int threads = lds > (kResidentLds / 2) ? 512 : 256;
+    // two blocks of 256 threads on a CU where their operands fit, one of 512 otherwise (float32, 64 to 64 channels at 262144 positions: 48 us, 50 with 512)
+    const int threads = lds > (kResidentLds / 2) ? 512 : 256;
     const long most = cu_count() * (512 / threads) / chunks, want = (tiles + threads / 64 - 1) / (threads / 64);
     const long blocks = want < most ? want : most > 0 ? most : 1;
     hipLaunchKernelGGL((mix_resident_kernel<IN, OUT, COMPLEX, GRAD, NT, HELD>), dim3((unsigned)blocks, (unsigned)chunks), dim3(threads), lds, stream, q,
@@ -36,20 +37,21 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t
 // first. complex64, gelu, residual: 64 to 64 channels at 200 ... 4096 positions 7.4 ... 7.7 us, 12.2 ... 12.6 in the resident one; 128 to 128 at
 // 4096 13.2 and 14.2; bf16, 256 to 256 at 4096 11.4 and 13.7. Above, the operands are formed once for all tiles of a block.
 constexpr long kFewTiles = 1024;
-// Fewer tiles than this number of waves (of 256 CUs): the rows of A are divided too
+// Fewer tiles than this number of waves (eight on each of 256 CUs): the rows of A are divided too. bf16, 256 to 256 channels at 20000 positions: 17 us, 33 with all
+// rows in every block; complex64, 128 to 256 at 10000: 25 and 39.
 constexpr long kWaves = 2048;
 
 // steps that registers hold, and beyond how many of them the sums of 64 rows find no room beside them
-template <int IN, bool COMPLEX> constexpr int kMostSteps = IN == kIn32 && !COMPLEX ? 4 : 8;
-template <int IN, int OUT, bool COMPLEX> constexpr int kMostWideSteps = IN == kIn32 ? (COMPLEX ? 4 : 2) : OUT == kIn32 ? 4 : 8;
+template <int IN> constexpr int kMostSteps = IN == kIn32 ? 1 : 8;
+template <int IN, int OUT> constexpr int kMostWideSteps = OUT == kIn32 ? 4 : 8;
 
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int HELD = kMostSteps<IN, COMPLEX>>
+template <int IN, int OUT, bool COMPLEX, bool GRAD, int HELD = kMostSteps<IN>>
 hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, size_t lds, hipStream_t stream)
 {
     if constexpr (HELD != held_for(HELD)) return launch_steps<IN, OUT, COMPLEX, GRAD, HELD - 1>(q, nt, held, block_rows, lds, stream);
     else {
         if (held == HELD) {
-            if constexpr (HELD <= kMostWideSteps<IN, OUT, COMPLEX>)
+            if constexpr (HELD <= kMostWideSteps<IN, OUT>)
                 if (nt == 4) return launch_resident<IN, OUT, COMPLEX, GRAD, 4, HELD>(q, block_rows, lds, stream);
             return launch_resident<IN, OUT, COMPLEX, GRAD, 2, HELD>(q, block_rows, lds, stream);
         }
@@ -84,22 +86,37 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     constexpr int CHANNELS = COMPLEX ? 16 : 32;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
-    // gradients of 32-bit real rows with three or four steps are streamed in 64 rows instead of held in 32: the slopes are formed half as often
-    // (128 to 128 channels at 262144 positions, both gradients: 252 us, 264 held; 256 to 120 at 65536: 104 and 124)
-    const bool held = steps <= kMostSteps<IN, COMPLEX> && !(GRAD && IN == kIn32 && !COMPLEX && steps > 2);
-    const size_t lds16 = (size_t)(held ? held_for(steps) : steps) * kWaveParts(IN) * 1024;     // of 16 rows
-    const int nt = tiles16 <= 2 || (held && steps > kMostWideSteps<IN, OUT, COMPLEX>) ? 2 : 4;
     // the lane's part of an address, up to 24 rows of the input or 12 of the results, in 32 bits
     const long widest = std::max(std::max(std::max(q.ldx, q.ldzin), q.ldr), std::max(q.ldy, q.ldz));
     const bool near = widest < (1L << 24) && tiles < (1L << 30);
-    if (near && tiles * tiles16 > kFewTiles && nt * lds16 <= kResidentLds) {
-        const int groups = (tiles16 + nt - 1) / nt, fit = std::min((int)(kResidentLds / (nt * lds16)), 640 / (16 * nt));
+    struct Plan {
+        int nt, block_rows, groups;                     // 16 rows at a time; rows of a block, and how often it walks its columns for them
+        size_t lds16;                                   // operands of 16 rows
+    };
+    auto plan = [&](bool held) {
+        Plan p;
+        p.lds16 = (size_t)(held ? held_for(steps) : steps) * kWaveParts(IN) * 1024;
+        p.nt = tiles16 <= 2 || (held && steps > kMostWideSteps<IN, OUT>) ? 2 : 4;
+        if (p.nt * p.lds16 > kResidentLds) return p.groups = 0, p;
+        const int groups = (tiles16 + p.nt - 1) / p.nt, fit = std::min((int)(kResidentLds / (p.nt * p.lds16)), 640 / (16 * p.nt));
         int chunks = (groups + fit - 1) / fit;
         while (chunks < groups && tiles * chunks < kWaves) ++chunks;
-        if (GRAD && IN == kIn32) chunks = groups;       // the kernel walks 64 rows: what it made of gy and z is gone after them
-        const int block_groups = (groups + chunks - 1) / chunks, block_rows = block_groups * nt * 16;
-        const size_t lds = block_groups * nt * lds16 + block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
-        return launch_steps<IN, OUT, COMPLEX, GRAD>(q, nt, held ? held_for(steps) : 0, block_rows, lds, stream);
+        // 64 rows per block: walking the columns again would form the slopes again in the same wave (float32, 128 to 128 channels, both gradients at
+        // 262144 positions: 236 us, 253 with all rows in one block)
+        if (GRAD && IN == kIn32) chunks = groups;
+        p.groups = (groups + chunks - 1) / chunks;
+        p.block_rows = p.groups * p.nt * 16;
+        return p;
+    };
+    if (near && tiles * tiles16 > kFewTiles) {
+        Plan p = plan(false);
+        // Steps are held where 16- or 8-bit columns are walked more than once (bf16, 72 to 200 channels at 100003 positions: 24.3 us, streamed 27.6; 8 bits, 256
+        // to 256 at 262144: 93 and 110), and a single one. Otherwise they are streamed: the first products do not wait for the last rows, and 32-bit
+        // operands would have to be formed again all the same (complex64, 128 to 128 at 262144: 212 us, held 244; bf16, 256 to 256 at 20000: 17.4 and 20.8)
+        const bool held = steps == 1 || (IN != kIn32 && p.groups > 1 && steps <= kMostSteps<IN>);
+        if (held) p = plan(true);
+        const size_t lds = p.block_rows / 16 * p.lds16 + p.block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
+        if (p.groups) return launch_steps<IN, OUT, COMPLEX, GRAD>(q, p.nt, held ? held_for(steps) : 0, p.block_rows, lds, stream);
     }
     if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, false, false>(q, stream);
     if (tiles16 == 2 || tiles * tiles16 <= 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 2, false, false>(q, stream);

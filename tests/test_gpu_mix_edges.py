@@ -77,6 +77,27 @@ def test_channels_far_apart(kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+def test_channels_almost_as_far_apart_as_32_bits_reach(kind):
+    """24 rows of x, or 12 complex ones or rows of the results, just below 2^32 bytes apart, and sizes of the resident kernel"""
+    K, N, P, dt = 40, 64, 20003, TYPES[kind]
+    x, W, bias, residual = operands(kind, K, N, (P,), 550)
+    size = 8 if dt.is_complex else 4 if dt == torch.float32 else 2
+    ldx, ldy = ((1 << 32) - 8192) // (24 * size if not dt.is_complex else 12 * size), ((1 << 32) - 8192) // (12 * size)
+
+    def apart(t, ld):
+        return torch.empty(((t.shape[0] - 1) * ld + P,), dtype=dt, device="cuda").as_strided(t.shape, (ld, 1)).copy_(t)
+    xf, y = apart(x, ldx), apart(torch.zeros_like(residual), ldy)
+    z = torch.empty_like(residual)
+    tf.mix(xf, W, bias, residual, "silu", y=y, z=z)
+    check_forward(y, z, x, W, bias, residual, "silu")
+    del y
+    gy, gx = randn((N, P), dt, 555), apart(torch.zeros_like(x), ldx)
+    check_backward(gy, x, W, z, "silu", tf.mix_backward(gy, xf, W, z=z, activation="silu", gx=gx))
+    del xf, gx
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("K,N,P", [(8, 5, 33), (8, 5, 130), (40, 70, 20003)])
 def test_residual_in_place_at_the_last_columns(kind, K, N, P):
     x, W, bias, residual = operands(kind, K, N, (P,), 540)

@@ -86,9 +86,10 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     constexpr int CHANNELS = COMPLEX ? 16 : 32;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
-    // the lane's part of an address, up to 24 rows of the input or 12 of the results, in 32 bits
-    const long widest = std::max(std::max(std::max(q.ldx, q.ldzin), q.ldr), std::max(q.ldy, q.ldz));
-    const bool near = widest < (1L << 24) && tiles < (1L << 30);
+    // a lane's part of an address in 32 bits: up to 24 (complex: 12) rows of the input and 64 columns, up to 12 rows of the results
+    const long in_rows = (COMPLEX ? 12 : 24) * std::max(std::max(q.ldx, q.ldzin), GRAD ? q.ldz : 0), out_rows = 12 * std::max(q.ldr, std::max(q.ldy, q.ldz));
+    const bool near = std::max(in_rows * (long)sizeof(typename Columns<IN>::Value), out_rows * (long)sizeof(typename Columns<OUT>::Value)) < (1L << 32) - 4096 &&
+                      tiles < (1L << 30);
     struct Plan {
         int nt, block_rows, groups;                     // 16 rows at a time; rows of a block, and how often it walks its columns for them
         size_t lds16;                                   // operands of 16 rows

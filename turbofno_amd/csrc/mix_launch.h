@@ -90,6 +90,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     const long in_rows = (COMPLEX ? 12 : 24) * std::max(std::max(q.ldx, q.ldzin), GRAD ? q.ldz : 0), out_rows = 12 * std::max(q.ldr, std::max(q.ldy, q.ldz));
     const bool near = std::max(in_rows * (long)sizeof(typename Columns<IN>::Value), out_rows * (long)sizeof(typename Columns<OUT>::Value)) < (1L << 32) - 4096 &&
                       tiles < (1L << 30);
+    constexpr bool SHORT_OF_REGISTERS = GRAD && IN == kIn32 && !COMPLEX;      // the direct kernel of 64 rows: two steps of gy and of z
     struct Plan {
         int nt, block_rows, groups;                     // 16 rows at a time; rows of a block, and how often it walks its columns for them
         size_t lds16;                                   // operands of 16 rows
@@ -98,6 +99,9 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
         Plan p;
         p.lds16 = (size_t)(held ? held_for(steps) : steps) * kWaveParts(IN) * 1024;
         p.nt = tiles16 <= 2 || (held && steps > kMostWideSteps<IN, OUT>) ? 2 : 4;
+        // 32 rows where the operands of 64 do not fit (complex64, 256 to 256 channels at 65536 positions: 203 us, 221 in the direct kernel). Not where the
+        // slopes would be formed twice as often, as long as the direct kernel has the registers for 64 rows (the gradient there: 523 and 457; float32, 128 to 512: 231 and 382)
+        if (p.nt * p.lds16 > kResidentLds && (!GRAD || SHORT_OF_REGISTERS)) p.nt = 2;
         if (p.nt * p.lds16 > kResidentLds) return p.groups = 0, p;
         const int groups = (tiles16 + p.nt - 1) / p.nt, fit = std::min((int)(kResidentLds / (p.nt * p.lds16)), 640 / (16 * p.nt));
         int chunks = (groups + fit - 1) / fit;
@@ -120,8 +124,9 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
         if (p.groups) return launch_steps<IN, OUT, COMPLEX, GRAD>(q, p.nt, held ? held_for(steps) : 0, p.block_rows, lds, stream);
     }
     if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, false, false>(q, stream);
-    if (tiles16 == 2 || tiles * tiles16 <= 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 2, false, false>(q, stream);
-    return launch_direct<IN, OUT, COMPLEX, GRAD, 4, false, false>(q, stream);
+    if constexpr (!SHORT_OF_REGISTERS)
+        if (tiles16 > 2 && tiles * tiles16 > 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 4, false, false>(q, stream);
+    return launch_direct<IN, OUT, COMPLEX, GRAD, 2, false, false>(q, stream);
 }
 
 }  // namespace tfno

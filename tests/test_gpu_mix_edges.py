@@ -104,3 +104,18 @@ def test_residual_in_place_at_the_last_columns(kind, K, N, P):
     y = residual.clone()
     tf.mix(x, W, bias, y, "silu", y=y)
     check_forward(y, None, x, W, bias, residual, "silu")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("activation", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("K,N,P", [(200, 40, 6001), (520, 33, 4097), (140, 300, 20001)])
+def test_gradients_of_many_channels(kind, activation, K, N, P):
+    """sizes at which gz is formed by itself; rows that start anywhere and end inside a unit of 2048 columns, nothing written beside them"""
+    dt = TYPES[kind]
+    x, W = randn((K, P), dt, 560), randn((N, K), dt, 561, K ** -0.5)
+    gy, z = randn((N, P + 5), dt, 562)[:, 2:2 + P], randn((N, P + 3), dt, 563)[:, 1:1 + P]
+    gz, gx = torch.full((N, P + 7), 7.0, dtype=dt, device="cuda"), torch.full((K, P + 9), 7.0, dtype=dt, device="cuda")
+    results = tf.mix_backward(gy, x, W, z=z, activation=activation, gz=gz[:, 3:3 + P], gx=gx[:, 5:5 + P])
+    check_backward(gy, x, W, z, activation, results)
+    for t, lo in ((gz, 3), (gx, 5)):
+        assert (t[:, :lo] == 7).all() and (t[:, lo + P:] == 7).all()

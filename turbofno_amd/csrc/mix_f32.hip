@@ -4,7 +4,8 @@ namespace tfno {
 
 hipError_t launch_mix_f32(const MixParams& q, bool grad, hipStream_t stream)
 {
-    return grad ? launch_mix<kIn32, kIn32, false, true>(q, stream) : launch_mix<kIn32, kIn32, false, false>(q, stream);
+    if (!grad) return launch_mix<kIn32, kIn32, false, false, false>(q, stream);
+    return q.act == kActNone ? launch_mix<kIn32, kIn32, false, true, false>(q, stream) : launch_mix<kIn32, kIn32, false, true, true>(q, stream);
 }
 
 }  // namespace tfno

@@ -440,7 +440,7 @@ template <int N, int I = 0, typename F> __device__ __forceinline__ void unrolled
 }
 
 // Few columns: a wave for 64 columns and 16 NT rows, weights from memory
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool RAGGED, bool FEW>
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES, int NT, bool RAGGED, bool FEW>
 __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, int row_groups)
 {
     typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, true, RAGGED> Wave;
@@ -450,7 +450,6 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     const int row0 = (int)(id % row_groups) * (16 * NT);
     if (left <= 0) return;
     const Window w = { RAGGED || left >= kColumns ? column : q.columns - kColumns, RAGGED && left < kColumns ? (int)left : (int)kColumns };
-    const bool slopes = GRAD && q.act != kActNone;
     const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS, count = q.contraction * Wave::V;
     float4_v acc[NT][4] = {};
     constexpr bool AHEAD = NT == 1;                     // the weights of a step are asked for with its rows: there are registers for them
@@ -464,14 +463,13 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     auto fetch = [&](int s, Step& r) {
         s = s < steps ? s : steps - 1;
         wave.template fetch<true>(q.x, q.ldx, w, s, r.x);
-        if constexpr (GRAD) wave.template fetch<true>(slopes ? q.zin : q.x, slopes ? q.ldzin : q.ldx, w, s, r.z);
+        if constexpr (SLOPES) wave.template fetch<true>(q.zin, q.ldzin, w, s, r.z);
         if constexpr (AHEAD) fetch_a(s, 0, r.a[0]);
         __builtin_amdgcn_sched_barrier(0);              // the loads stay ahead of the products that follow
     };
     auto product = [&](int s, Step& r) {
         if constexpr (!AHEAD) unrolled<NT>([&](int t) { fetch_a(s, t, r.a[t]); });
-        if constexpr (GRAD)
-            if (slopes) wave.slope(w, s, r.x, r.z, row0 == 0);
+        if constexpr (SLOPES) wave.slope(w, s, r.x, r.z, row0 == 0);
         wave.clear(s, r.x);
         Operand<IN> b[4];
         make_operands<IN, COMPLEX, GRAD>(r.x, b);
@@ -493,6 +491,38 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); }, [&](int t) { return wave.scale_of(row0 + 16 * t + 4 * wave.kq); });
 }
 
+// gz of the gradient by itself: units of 2048 columns of a row, in turns
+template <int IN, int ACT> __device__ __forceinline__ void slope_unit(const MixParams& q, long row, long column0)
+{
+    typedef typename Columns<IN>::Value Value;
+    const Value *gy = static_cast<const Value*>(q.x) + row * q.ldx, *zin = static_cast<const Value*>(q.zin) + row * q.ldzin;
+    Value* gz = static_cast<Value*>(q.z) + row * q.ldz;
+    auto product = [&](RawOf<IN> g, RawOf<IN> z) {
+        const float4_v a = to_float<IN>(g), b = to_float<IN>(z);
+        float4_v v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = through_activation(ACT, a[i], b[i]);
+        return from_float<IN>(v);
+    };
+    if (column0 + 2048 <= q.columns) {
+        const long column = column0 + 4 * threadIdx.x;
+        const RawOf<IN> g0 = load4<IN>(gy, column), g1 = load4<IN>(gy, column + 1024), z0 = load4<IN>(zin, column), z1 = load4<IN>(zin, column + 1024);
+        store4<IN>(gz, column, product(g0, z0));
+        store4<IN>(gz, column + 1024, product(g1, z1));
+    } else
+        for (long column = column0 + 4 * threadIdx.x; column < q.columns; column += 1024)
+            store4_ragged<IN>(gz, column, q.columns, product(load4_ragged<IN>(gy, column, q.columns), load4_ragged<IN>(zin, column, q.columns)));
+}
+template <int IN> __global__ __launch_bounds__(256) void slope_kernel(const MixParams q, long units, long of_row)
+{
+    for (long u = blockIdx.x; u < units; u += gridDim.x) {
+        const long row = u / of_row, column0 = (u - row * of_row) * 2048;
+        if (q.act == kActGeluTanh) slope_unit<IN, kActGeluTanh>(q, row, column0);
+        else if (q.act == kActSilu) slope_unit<IN, kActSilu>(q, row, column0);
+        else slope_unit<IN, kActRelu>(q, row, column0);
+    }
+}
+
 // Many columns: the operands of the block's rows of A stay in LDS, in the order in which lanes read them (16 bytes per lane, part, 16 rows and step), and
 // its waves walk the columns without meeting again: no barrier, and 16 NT rows of sums in registers. HELD = 0: steps of the input are read two ahead, again for
 // every 16 NT rows (out of the L2 cache), the next rows' or columns' first one during the results. HELD > 0: all steps of the input, HELD or up to `SPARE` fewer,
@@ -504,7 +534,7 @@ constexpr int kWaveParts(int in) { return in == kIn32 ? 3 : 1; }
 constexpr int kResidentThreads = 512;
 // numbers of steps that there are kernels for
 constexpr int held_for(int steps) { return steps <= 4 ? steps : steps <= 6 ? 6 : 8; }
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD>
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES, int NT, int HELD>
 __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const MixParams q, int block_rows, int tiles)
 {
     extern __shared__ uint4_v weights[];
@@ -514,7 +544,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
     const Wave wave(q);
     const int row_first = blockIdx.y * block_rows, groups = block_rows / (16 * NT);
     const int steps = HELD ? HELD : (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS;
-    const bool slopes = GRAD && q.act != kActNone, writes = blockIdx.y == 0;
+    const bool writes = blockIdx.y == 0;
     // tiles are counted in 32 bits: 64-bit numbers are compared in vector registers. A last tile that is not whole ends with the columns; tiles beyond it are it
     auto window = [&](int tile) { return Window{ scalar(tile < tiles - 1 ? (long)tile * kColumns : q.columns - kColumns), kColumns }; };
     const int stride = gridDim.x * (blockDim.x >> 6);
@@ -527,7 +557,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
     typename Wave::Rows x[HELD ? HELD : 1], x0, z0;
     auto ahead = [&](const Window& w, int s, typename Wave::Rows& x, typename Wave::Rows& z) {
         wave.template fetch<true>(q.x, q.ldx, w, s, x);
-        if constexpr (GRAD) wave.template fetch<true>(slopes ? q.zin : q.x, slopes ? q.ldzin : q.ldx, w, s, z);
+        if constexpr (SLOPES) wave.template fetch<true>(q.zin, q.ldzin, w, s, z);
         __builtin_amdgcn_sched_barrier(0);
     };
     unrolled<HELD>([&](int s) { fetch(q.x, q.ldx, w, s, x[s]); });      // on their way while the operands of A are formed
@@ -568,17 +598,16 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
     };
     if constexpr (HELD > 0) {
         for (;;) {
-            if constexpr (GRAD)
-                if (slopes) {
-                    constexpr int AHEAD = IN == kIn32 ? (COMPLEX && HELD > 1 ? 2 : 1) : HELD < 4 ? HELD : 4;      // steps of z on their way
-                    typename Wave::Rows z[AHEAD];
-                    unrolled<AHEAD>([&](int s) { fetch(q.zin, q.ldzin, w, s, z[s]); });
-                    unrolled<HELD>([&](int s) {
-                        wave.slope(w, s, x[s], z[s % AHEAD], writes);
-                        if (s + AHEAD < HELD) fetch(q.zin, q.ldzin, w, s + AHEAD, z[s % AHEAD]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    });
-                }
+            if constexpr (SLOPES) {
+                constexpr int AHEAD = IN == kIn32 ? (COMPLEX && HELD > 1 ? 2 : 1) : HELD < 4 ? HELD : 4;      // steps of z on their way
+                typename Wave::Rows z[AHEAD];
+                unrolled<AHEAD>([&](int s) { fetch(q.zin, q.ldzin, w, s, z[s]); });
+                unrolled<HELD>([&](int s) {
+                    wave.slope(w, s, x[s], z[s % AHEAD], writes);
+                    if (s + AHEAD < HELD) fetch(q.zin, q.ldzin, w, s + AHEAD, z[s % AHEAD]);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            }
             const Window wn = window(tile + stride);
             if constexpr (IN != kIn32) {
                 // 16- and 8-bit rows: all operands at once, in the registers that the rows leave
@@ -626,8 +655,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                 const Window wf = g < groups - 1 ? w : wn;
                 float4_v acc[NT][4] = {};
                 auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
-                    if constexpr (GRAD)
-                        if (slopes) wave.slope(w, s, x, z, writes && g == 0);
+                    if constexpr (SLOPES) wave.slope(w, s, x, z, writes && g == 0);
                     wave.clear(s, x);
                     Operand<IN> b[4];
                     make_operands<IN, COMPLEX, GRAD>(x, b);

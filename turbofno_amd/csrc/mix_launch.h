@@ -6,21 +6,21 @@
 
 namespace tfno {
 
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool RAGGED, bool FEW> hipError_t launch_direct(const MixParams& q, hipStream_t stream)
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES, int NT, bool RAGGED, bool FEW> hipError_t launch_direct(const MixParams& q, hipStream_t stream)
 {
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int groups = (q.rows + 16 * NT - 1) / (16 * NT);
     const long blocks = (tiles * groups + 3) / 4;
-    hipLaunchKernelGGL((mix_direct_kernel<IN, OUT, COMPLEX, GRAD, NT, RAGGED, FEW>), dim3((unsigned)blocks), dim3(256), 0, stream, q, groups);
+    hipLaunchKernelGGL((mix_direct_kernel<IN, OUT, COMPLEX, GRAD, SLOPES, NT, RAGGED, FEW>), dim3((unsigned)blocks), dim3(256), 0, stream, q, groups);
     return hipGetLastError();
 }
 
 constexpr size_t kResidentLds = 152 << 10, kResidentBias = 8 << 10;    // operands of A; bias and scales of up to 640 complex rows
 
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t launch_resident(const MixParams& q, int block_rows, size_t lds, hipStream_t stream)
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES, int NT, int HELD> hipError_t launch_resident(const MixParams& q, int block_rows, size_t lds, hipStream_t stream)
 {
     static std::atomic<unsigned long long> served{ 0 };
-    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_resident_kernel<IN, OUT, COMPLEX, GRAD, NT, HELD>), kResidentLds + kResidentBias, served); e != hipSuccess)
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_resident_kernel<IN, OUT, COMPLEX, GRAD, SLOPES, NT, HELD>), kResidentLds + kResidentBias, served); e != hipSuccess)
         return e;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int chunks = (q.rows + block_rows - 1) / block_rows;
@@ -28,7 +28,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, int HELD> hipError_t
     const int threads = lds > (kResidentLds / 2) ? 512 : 256;
     const long most = cu_count() * (512 / threads) / chunks, want = (tiles + threads / 64 - 1) / (threads / 64);
     const long blocks = want < most ? want : most > 0 ? most : 1;
-    hipLaunchKernelGGL((mix_resident_kernel<IN, OUT, COMPLEX, GRAD, NT, HELD>), dim3((unsigned)blocks, (unsigned)chunks), dim3(threads), lds, stream, q,
+    hipLaunchKernelGGL((mix_resident_kernel<IN, OUT, COMPLEX, GRAD, SLOPES, NT, HELD>), dim3((unsigned)blocks, (unsigned)chunks), dim3(threads), lds, stream, q,
                        block_rows, (int)tiles);
     return hipGetLastError();
 }
@@ -45,28 +45,50 @@ constexpr long kWaves = 2048;
 template <int IN> constexpr int kMostSteps = IN == kIn32 ? 1 : 8;
 template <int IN, int OUT> constexpr int kMostWideSteps = OUT == kIn32 ? 4 : 8;
 
-template <int IN, int OUT, bool COMPLEX, bool GRAD, int HELD = kMostSteps<IN>>
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES, int HELD = kMostSteps<IN>>
 hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, size_t lds, hipStream_t stream)
 {
-    if constexpr (HELD != held_for(HELD)) return launch_steps<IN, OUT, COMPLEX, GRAD, HELD - 1>(q, nt, held, block_rows, lds, stream);
+    if constexpr (HELD != held_for(HELD)) return launch_steps<IN, OUT, COMPLEX, GRAD, SLOPES, HELD - 1>(q, nt, held, block_rows, lds, stream);
     else {
         if (held == HELD) {
             if constexpr (HELD <= kMostWideSteps<IN, OUT>)
-                if (nt == 4) return launch_resident<IN, OUT, COMPLEX, GRAD, 4, HELD>(q, block_rows, lds, stream);
-            return launch_resident<IN, OUT, COMPLEX, GRAD, 2, HELD>(q, block_rows, lds, stream);
+                if (nt == 4) return launch_resident<IN, OUT, COMPLEX, GRAD, SLOPES, 4, HELD>(q, block_rows, lds, stream);
+            return launch_resident<IN, OUT, COMPLEX, GRAD, SLOPES, 2, HELD>(q, block_rows, lds, stream);
         }
-        if constexpr (HELD > 0) return launch_steps<IN, OUT, COMPLEX, GRAD, HELD - 1>(q, nt, held, block_rows, lds, stream);
+        if constexpr (HELD > 0) return launch_steps<IN, OUT, COMPLEX, GRAD, SLOPES, HELD - 1>(q, nt, held, block_rows, lds, stream);
         else return hipErrorInvalidValue;
     }
 }
 
-template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const MixParams& q, hipStream_t stream)
+// From this number of blocks or waves that would form the slopes of the same columns, gz is formed by a kernel of its own and the product reads it. Both gradients, gelu:
+// complex64, 256 to 256 channels at 65536 positions 422 us, 467 in one kernel; float32, 128 to 512 at 65536 203 and 229; bf16, 128 to 1300 at 20000 107 and
+// 163, 128 to 128 at 30000 28.4 and 30.5. Two in 32 bits: complex64, 128 to 128 at 65536 135 us, 131 in one kernel.
+template <int IN> constexpr int kSlopesApart = IN == kIn32 ? 3 : 2;
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t launch_mix(const MixParams& q, hipStream_t stream);
+
+// The gradient in two kernels: gz, then the product
+template <int IN, int OUT, bool COMPLEX> hipError_t launch_slopes(const MixParams& q, hipStream_t stream)
+{
+    const long of_row = (q.columns + 2047) / 2048, units = of_row * q.contraction, most = 8l * cu_count();
+    hipLaunchKernelGGL(slope_kernel<IN>, dim3((unsigned)(units < most ? units : most)), dim3(256), 0, stream, q, units, of_row);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    MixParams rest = q;
+    rest.x = q.z;
+    rest.ldx = q.ldz;
+    rest.zin = nullptr;
+    rest.z = nullptr;
+    rest.ldz = rest.ldzin = 0;
+    rest.act = kActNone;
+    return launch_mix<IN, OUT, COMPLEX, true, false>(rest, stream);
+}
+
+template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t launch_mix(const MixParams& q, hipStream_t stream)
 {
     if (q.columns == 0) return hipSuccess;
     // Columns that do not fill a tile: the last tile ends with them, among columns of the one before it. Where those may be results by then (the residuals
     // are in their place), and where there are no others, a kernel takes them one by one
     const long last = q.columns % kColumns, head = q.columns - last;
-    if (last && head == 0) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, true, !GRAD>(q, stream);
+    if (last && head == 0) return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 1, true, !GRAD>(q, stream);
     if (last && q.residual && (q.residual == q.y || q.residual == q.z)) {
         constexpr size_t SIZE = sizeof(typename Columns<OUT>::Value);
         MixParams whole = q, rest = q;
@@ -78,11 +100,11 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
         rest.y = ahead(q.y, SIZE);
         rest.z = ahead(q.z, SIZE);
         if (q.xscale) rest.xscale = q.xscale + head / (COMPLEX ? 2 : 1);
-        if (hipError_t e = launch_mix<IN, OUT, COMPLEX, GRAD>(whole, stream); e != hipSuccess) return e;
-        return launch_direct<IN, OUT, COMPLEX, GRAD, 1, true, !GRAD>(rest, stream);
+        if (hipError_t e = launch_mix<IN, OUT, COMPLEX, GRAD, SLOPES>(whole, stream); e != hipSuccess) return e;
+        return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 1, true, !GRAD>(rest, stream);
     }
     if constexpr (!GRAD)        // weights that cannot be read by eight
-        if (((long)(q.rows - 1) * q.ldw + q.contraction) * (COMPLEX ? 2 : 1) < 8) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, false, true>(q, stream);
+        if (((long)(q.rows - 1) * q.ldw + q.contraction) * (COMPLEX ? 2 : 1) < 8) return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 1, false, true>(q, stream);
     constexpr int CHANNELS = COMPLEX ? 16 : 32;
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int tiles16 = (q.rows + 15) / 16, steps = (q.contraction + CHANNELS - 1) / CHANNELS;
@@ -90,7 +112,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
     const long in_rows = (COMPLEX ? 12 : 24) * std::max(std::max(q.ldx, q.ldzin), GRAD ? q.ldz : 0), out_rows = 12 * std::max(q.ldr, std::max(q.ldy, q.ldz));
     const bool near = std::max(in_rows * (long)sizeof(typename Columns<IN>::Value), out_rows * (long)sizeof(typename Columns<OUT>::Value)) < (1L << 32) - 4096 &&
                       tiles < (1L << 30);
-    constexpr bool SHORT_OF_REGISTERS = GRAD && IN == kIn32 && !COMPLEX;      // the direct kernel of 64 rows: two steps of gy and of z
+    constexpr bool SHORT_OF_REGISTERS = SLOPES && IN == kIn32 && !COMPLEX;      // the direct kernel of 64 rows: two steps of gy and of z
     struct Plan {
         int nt, block_rows, groups;                     // 16 rows at a time; rows of a block, and how often it walks its columns for them
         size_t lds16;                                   // operands of 16 rows
@@ -101,14 +123,14 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
         p.nt = tiles16 <= 2 || (held && steps > kMostWideSteps<IN, OUT>) ? 2 : 4;
         // 32 rows where the operands of 64 do not fit (complex64, 256 to 256 channels at 65536 positions: 203 us, 221 in the direct kernel). Not where the
         // slopes would be formed twice as often, as long as the direct kernel has the registers for 64 rows (the gradient there: 523 and 457; float32, 128 to 512: 231 and 382)
-        if (p.nt * p.lds16 > kResidentLds && (!GRAD || SHORT_OF_REGISTERS)) p.nt = 2;
+        if (p.nt * p.lds16 > kResidentLds && (!SLOPES || SHORT_OF_REGISTERS)) p.nt = 2;
         if (p.nt * p.lds16 > kResidentLds) return p.groups = 0, p;
         const int groups = (tiles16 + p.nt - 1) / p.nt, fit = std::min((int)(kResidentLds / (p.nt * p.lds16)), 640 / (16 * p.nt));
         int chunks = (groups + fit - 1) / fit;
         while (chunks < groups && tiles * chunks < kWaves) ++chunks;
         // 64 rows per block: walking the columns again would form the slopes again in the same wave (float32, 128 to 128 channels, both gradients at
         // 262144 positions: 236 us, 253 with all rows in one block)
-        if (GRAD && IN == kIn32) chunks = groups;
+        if (SLOPES && IN == kIn32) chunks = groups;
         p.groups = (groups + chunks - 1) / chunks;
         p.block_rows = p.groups * p.nt * 16;
         return p;
@@ -121,12 +143,16 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD> hipError_t launch_mix(const 
         const bool held = steps == 1 || (IN != kIn32 && p.groups > 1 && steps <= kMostSteps<IN>);
         if (held) p = plan(true);
         const size_t lds = p.block_rows / 16 * p.lds16 + p.block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
-        if (p.groups) return launch_steps<IN, OUT, COMPLEX, GRAD>(q, p.nt, held ? held_for(steps) : 0, p.block_rows, lds, stream);
+        if constexpr (SLOPES)
+            if (p.groups && (tiles16 + p.nt * p.groups - 1) / (p.nt * p.groups) >= kSlopesApart<IN>) return launch_slopes<IN, OUT, COMPLEX>(q, stream);
+        if (p.groups) return launch_steps<IN, OUT, COMPLEX, GRAD, SLOPES>(q, p.nt, held ? held_for(steps) : 0, p.block_rows, lds, stream);
     }
-    if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, 1, false, false>(q, stream);
+    if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 1, false, false>(q, stream);
+    if constexpr (SLOPES)
+        if (tiles * tiles16 > kFewTiles && tiles16 > 4 * (kSlopesApart<IN> - 1)) return launch_slopes<IN, OUT, COMPLEX>(q, stream);
     if constexpr (!SHORT_OF_REGISTERS)
-        if (tiles16 > 2 && tiles * tiles16 > 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, 4, false, false>(q, stream);
-    return launch_direct<IN, OUT, COMPLEX, GRAD, 2, false, false>(q, stream);
+        if (tiles16 > 2 && tiles * tiles16 > 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 4, false, false>(q, stream);
+    return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 2, false, false>(q, stream);
 }
 
 }  // namespace tfno

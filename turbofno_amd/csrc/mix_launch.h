@@ -53,7 +53,9 @@ hipError_t launch_steps(const MixParams& q, int nt, int held, int block_rows, si
         if (held == HELD) {
             if constexpr (HELD <= kMostWideSteps<IN, OUT>)
                 if (nt == 4) return launch_resident<IN, OUT, COMPLEX, GRAD, SLOPES, 4, HELD>(q, block_rows, lds, stream);
-            return launch_resident<IN, OUT, COMPLEX, GRAD, SLOPES, 2, HELD>(q, block_rows, lds, stream);
+            if constexpr (HELD <= 1 || HELD > kMostWideSteps<IN, OUT>)     // up to 32 rows are walked once, and more steps than one streamed
+                if (nt == 2) return launch_resident<IN, OUT, COMPLEX, GRAD, SLOPES, 2, HELD>(q, block_rows, lds, stream);
+            return hipErrorInvalidValue;
         }
         if constexpr (HELD > 0) return launch_steps<IN, OUT, COMPLEX, GRAD, SLOPES, HELD - 1>(q, nt, held, block_rows, lds, stream);
         else return hipErrorInvalidValue;
@@ -112,7 +114,6 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t laun
     const long in_rows = (COMPLEX ? 12 : 24) * std::max(std::max(q.ldx, q.ldzin), GRAD ? q.ldz : 0), out_rows = 12 * std::max(q.ldr, std::max(q.ldy, q.ldz));
     const bool near = std::max(in_rows * (long)sizeof(typename Columns<IN>::Value), out_rows * (long)sizeof(typename Columns<OUT>::Value)) < (1L << 32) - 4096 &&
                       tiles < (1L << 30);
-    constexpr bool SHORT_OF_REGISTERS = SLOPES && IN == kIn32 && !COMPLEX;      // the direct kernel of 64 rows: two steps of gy and of z
     struct Plan {
         int nt, block_rows, groups;                     // 16 rows at a time; rows of a block, and how often it walks its columns for them
         size_t lds16;                                   // operands of 16 rows
@@ -121,9 +122,9 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t laun
         Plan p;
         p.lds16 = (size_t)(held ? held_for(steps) : steps) * kWaveParts(IN) * 1024;
         p.nt = tiles16 <= 2 || (held && steps > kMostWideSteps<IN, OUT>) ? 2 : 4;
-        // 32 rows where the operands of 64 do not fit (complex64, 256 to 256 channels at 65536 positions: 203 us, 221 in the direct kernel). Not where the
-        // slopes would be formed twice as often, as long as the direct kernel has the registers for 64 rows (the gradient there: 523 and 457; float32, 128 to 512: 231 and 382)
-        if (p.nt * p.lds16 > kResidentLds && (!SLOPES || SHORT_OF_REGISTERS)) p.nt = 2;
+        // 32 rows where the operands of 64 do not fit (complex64, 256 to 256 channels with residual at 65536 positions: 203 us, 221 in the direct kernel; both
+        // gradients, float32, 64 to 512 at 65536: 141 and 173; bf16, 64 to 1300 at 30000: 115 and 148; complex64, 64 to 256 at 65536: 159 - 165 and 156)
+        if (p.nt * p.lds16 > kResidentLds) p.nt = 2;
         if (p.nt * p.lds16 > kResidentLds) return p.groups = 0, p;
         const int groups = (tiles16 + p.nt - 1) / p.nt, fit = std::min((int)(kResidentLds / (p.nt * p.lds16)), 640 / (16 * p.nt));
         int chunks = (groups + fit - 1) / fit;
@@ -150,7 +151,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t laun
     if (tiles16 == 1 || tiles * tiles16 <= 1024) return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 1, false, false>(q, stream);
     if constexpr (SLOPES)
         if (tiles * tiles16 > kFewTiles && tiles16 > 4 * (kSlopesApart<IN> - 1)) return launch_slopes<IN, OUT, COMPLEX>(q, stream);
-    if constexpr (!SHORT_OF_REGISTERS)
+    if constexpr (!(SLOPES && IN == kIn32 && !COMPLEX))     // two steps of gy and of z leave no registers for 64 rows of sums there
         if (tiles16 > 2 && tiles * tiles16 > 2048) return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 4, false, false>(q, stream);
     return launch_direct<IN, OUT, COMPLEX, GRAD, SLOPES, 2, false, false>(q, stream);
 }

@@ -61,3 +61,35 @@ def test_column_ranges_of_one_buffer(kind):
     gx, ggain = tf.rms_norm_backward(x, want[1], gain, want[2])
     tf.rms_norm_backward(bx, bz, gain, want[2], gx=by)
     assert torch.equal(by, gx) and torch.equal(bx, x)
+
+
+def test_weight_gradient_apart_from_its_operands():
+    """gW, gbias and the workspace against gz, x and one another, in fields of 6 and 4 channels of 10 float32 values"""
+    L = operators._lib()
+    need = L.turbofno_mix_weight_grad_workspace_bytes(1, 10, 6, 4)
+    gz, x, gW, gbias, ws = (BASE + (i << 20) for i in range(5))
+
+    def refused(**k):
+        o = {**dict(gz=gz, ldgz=10, x=x, ldx=10, gW=gW, gbias=gbias, ws=ws, bytes=need), **k}
+        rc = L.turbofno_mix_weight_grad(1, 10, 6, 4, o["gz"], o["ldgz"], o["x"], o["ldx"], o["gW"], o["gbias"], o["ws"], o["bytes"], None)
+        return rc == INVALID and b"overlap" in L.turbofno_last_error_string()
+    assert refused(gW=x) and refused(gW=gz + 4 * 59) and refused(gW=x - 4 * 23) and refused(gbias=gz) and refused(gbias=x + 4 * 39)
+    assert refused(ws=x) and refused(ws=gz + 4 * 59) and refused(gW=ws) and refused(gbias=gW + 4 * 23) and refused(gbias=ws + need - 4)
+    # beside them, one check further: for a workspace that is too small
+    for k in (dict(gW=x + 160), dict(gW=gz + 240), dict(gbias=gW + 96), dict(gbias=None), dict(x=gz), dict(ldx=40, gbias=x + 40), dict(gW=ws + need)):
+        assert not refused(**k, bytes=4) and b"workspace of 4 bytes" in L.turbofno_last_error_string(), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+def test_weight_gradient_refusals(kind):
+    dt = TYPES[kind]
+    gz, x = randn((6, 40), dt, 1), randn((4, 40), dt, 2)
+    with pytest.raises(tf.TurboFNOError, match="overlaps gz or x"):
+        tf.mix_weight_grad(gz, x, gW=x.flatten()[:24].view(6, 4))
+    with pytest.raises(tf.TurboFNOError, match="overlaps gz or x"):
+        tf.mix_weight_grad(gz, x, gbias=gz[0, :6])
+    want, _ = tf.mix_weight_grad(gz, x)
+    between = torch.cat([x, x], 1)      # gbias in the columns that x leaves free
+    got, gbias = tf.mix_weight_grad(gz, between[:, :40], gbias=between[0, 40:46])
+    assert torch.equal(got, want) and torch.equal(between[0, :40], x[0])

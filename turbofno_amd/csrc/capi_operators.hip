@@ -61,6 +61,8 @@ bool overlap(const void* a, long rows_a, long ld_a, size_t size_a, const void* b
     return overlap(place(a, rows_a, ld_a, size_a, P), place(b, rows_b, ld_b, size_b, P));
 }
 
+Place packed(const void* p, long bytes) { return { static_cast<const char*>(p), 1, 0, bytes }; }
+
 // a result may be an operand, element for element, and overlaps none otherwise
 bool clash(const void* out, long ldo, const void* in, long ldi, int rows, size_t size, long P)
 {
@@ -147,7 +149,14 @@ int turbofno_mix_weight_grad(int type, long P, int N, int K, const void* gz, lon
     CHECK(check_rows("gz", gz, P, N, ldgz));
     CHECK(check_rows("x", x, P, K, ldx));
     CHECK(check_there("gW", gW));
-    const size_t need = tfno::mix_weight_grad_workspace(type, P, N, K);
+    const size_t e = tfno::size_of(type), need = tfno::mix_weight_grad_workspace(type, P, N, K);
+    // blocks read gz and x while others write their sums or, without a second kernel, the results
+    const Place results[3] = { packed(gW, (long)(e * N * K)), packed(gbias, (long)(e * N)), packed(workspace, (long)need) };
+    for (int i = 0; i < 3; ++i) {
+        if (overlap(results[i], place(gz, N, ldgz, e, P)) || overlap(results[i], place(x, K, ldx, e, P)))
+            return fail(TURBOFNO_ERR_INVALID_ARG, "gW, gbias or the workspace overlaps gz or x");
+        if (overlap(results[i], results[(i + 1) % 3])) return fail(TURBOFNO_ERR_INVALID_ARG, "gW, gbias and the workspace overlap one another");
+    }
     if (!workspace || workspace_bytes < need) return fail(TURBOFNO_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, need);
     return hip_status(tfno::launch_mix_weight_grad(type, P, N, K, gz, ldgz, x, ldx, gW, gbias, workspace, (hipStream_t)stream), "mix_weight_grad launch");
 }

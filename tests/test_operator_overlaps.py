@@ -93,3 +93,41 @@ def test_weight_gradient_refusals(kind):
     between = torch.cat([x, x], 1)      # gbias in the columns that x leaves free
     got, gbias = tf.mix_weight_grad(gz, between[:, :40], gbias=between[0, 40:46])
     assert torch.equal(got, want) and torch.equal(between[0, :40], x[0])
+
+
+def test_results_apart_from_weights_scales_and_the_workspace():
+    """fields of 6 and 4 channels of 10 float32 values; the overlap is looked for last of what is checked before the launch, or before the workspace"""
+    L = operators._lib()
+    x, W, bias, r, y, z, xs, ws = (BASE + (i << 20) for i in range(8))
+
+    def says(rc, text):
+        return rc == INVALID and text in L.turbofno_last_error_string()
+
+    def mix(**k):
+        o = {**dict(x=x, W=W, bias=bias, r=r, y=y, z=z), **k}
+        return L.turbofno_mix(1, 10, 6, 4, o["x"], 10, o["W"], o["bias"], o["r"], 10, 0, o["z"], 10, o["y"], 10, None)
+    assert says(mix(W=y + 4 * 59), b"W or bias") and says(mix(bias=z - 4 * 5), b"W or bias") and says(mix(bias=y), b"W or bias") and says(mix(W=z), b"W or bias")
+
+    def mix8(**k):
+        o = {**dict(x=x, W=W, bias=bias, r=r, y=y, xs=xs, ws=ws), **k}
+        return L.turbofno_mix_8bit(1, 10, 6, 4, o["x"], 10, o["xs"], o["W"], o["ws"], o["bias"], o["r"], 10, 0, o["y"], 10, None)
+    assert all(says(mix8(**{name: y + 8}), b"a scale") for name in ("W", "bias", "xs", "ws")) and says(mix8(W=y - 23), b"a scale")
+
+    def input_grad(**k):
+        o = {**dict(gy=r, z=z, W=W, gz=y, gx=x), **k}
+        return L.turbofno_mix_input_grad(1, 10, 6, 4, o["gy"], 10, o["z"], 10, o["W"], 1, o["gz"], 10, o["gx"], 10, None)
+    assert says(input_grad(W=x), b"overlaps W") and says(input_grad(W=y + 4 * 59), b"overlaps W")
+
+    def norm(call, **k):
+        o = {**dict(x=x, r=r, gain=W, s=z, y=y, rstd=xs), **k}
+        return getattr(L, call)(1, 10, 4, o["x"], 10, o["r"], 10, o["gain"], 1e-6, o["s"], 10, o["y"], 10, o["rstd"], None)
+    for call in ("turbofno_rms_norm", "turbofno_rms_norm_8bit"):
+        assert says(norm(call, gain=y + 8), b"gain") and says(norm(call, gain=z), b"gain")
+        assert all(says(norm(call, rstd=p + 8), b"another operand") for p in (x, r, z, y, W))
+
+    def norm_grad(need=0, **k):
+        o = {**dict(gy=y, s=z, gain=W, rstd=xs, gs=r, gx=x, ggain=bias, ws=ws), **k}
+        return L.turbofno_rms_norm_backward(1, 10, 4, o["gy"], 10, o["s"], 10, o["gain"], o["rstd"], o["gs"], 10, o["gx"], 10, o["ggain"], o["ws"], need, None)
+    assert all(says(norm_grad(**{name: x + 8}), b"gx overlaps gain") for name in ("gain", "rstd", "ggain"))
+    assert all(says(norm_grad(ws=p + 8), b"the workspace overlaps") for p in (y, z, r, x, W, xs, bias))
+    assert norm_grad() == WORKSPACE and norm_grad(ggain=W) == WORKSPACE      # gain is read before ggain is written

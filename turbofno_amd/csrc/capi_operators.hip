@@ -2,6 +2,7 @@
 #include "../../include/turbofno.h"
 #include "capi_error.h"
 #include "mix_kernel.h"
+#include <initializer_list>
 
 using tfno::fail;
 using tfno::hip_status;
@@ -69,6 +70,14 @@ bool clash(const void* out, long ldo, const void* in, long ldi, int rows, size_t
     return overlap(out, rows, ldo, size, in, rows, ldi, size, P) && !(out == in && (ldo == ldi || rows == 1));
 }
 
+// a result against operands that every block may read until the end of the call
+bool among(const Place& result, std::initializer_list<Place> operands)
+{
+    for (const Place& operand : operands)
+        if (overlap(result, operand)) return true;
+    return false;
+}
+
 #define CHECK(call) if (int rc_ = (call)) return rc_
 
 }  // namespace
@@ -88,6 +97,8 @@ int turbofno_mix(int type, long P, int N, int K, const void* x, long ldx, const 
     if (overlap(x, K, ldx, e, y, N, ldy, e, P) || overlap(x, K, ldx, e, z, N, ldz, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps x");
     if (overlap(y, N, ldy, e, z, N, ldz, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "y and z overlap");
     if (clash(y, ldy, residual, ldr, N, e, P) || clash(z, ldz, residual, ldr, N, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps residual without being it");
+    const Place small[2] = { packed(W, (long)(e * N * K)), packed(bias, (long)(e * N)) };
+    if (among(place(y, N, ldy, e, P), { small[0], small[1] }) || among(place(z, N, ldz, e, P), { small[0], small[1] })) return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps W or bias");
     const int v = tfno::values_of(type);
     const tfno::MixParams q = { x, nullptr, W, bias, residual, nullptr, nullptr, y, z, P * v, ldx * v, 0, ldr * v, ldy * v, ldz * v, N, K, K, act };
     const hipStream_t st = (hipStream_t)stream;
@@ -108,6 +119,8 @@ int turbofno_mix_8bit(int type, long P, int N, int K, const void* xq, long ldx, 
     const int v = tfno::values_of(type);
     if (overlap(xq, K, ldx, v, y, N, ldy, tfno::size_of(type), P)) return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps xq");
     if (clash(y, ldy, residual, ldr, N, tfno::size_of(type), P)) return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps residual without being it");
+    if (among(place(y, N, ldy, tfno::size_of(type), P), { packed(Wq, (long)N * K * v), packed(bias, N * (long)tfno::size_of(type)), packed(xscale, 4 * P), packed(wscale, 4l * N) }))
+        return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps Wq, bias or a scale");
     const tfno::MixParams q = { xq, nullptr, Wq, bias, residual, xscale, wscale, y, nullptr, P * v, ldx * v, 0, ldr * v, ldy * v, 0, N, K, K, act };
     return hip_status(tfno::launch_mix_8bit(q, type, (hipStream_t)stream), "mix_8bit launch");
 }
@@ -128,6 +141,8 @@ int turbofno_mix_input_grad(int type, long P, int N, int K, const void* gy, long
     if (overlap(gx, K, ldgx, e, gy, N, ldgy, e, P) || (slopes && (overlap(gx, K, ldgx, e, z, N, ldz, e, P) || overlap(gx, K, ldgx, e, gz, N, ldgz, e, P) ||
                                                                   overlap(gz, N, ldgz, e, gy, N, ldgy, e, P) || overlap(gz, N, ldgz, e, z, N, ldz, e, P))))
         return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps gy, z or the other result");
+    const Place weights = packed(W, (long)(e * N * K));
+    if (overlap(place(gx, K, ldgx, e, P), weights) || (slopes && overlap(place(gz, N, ldgz, e, P), weights))) return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps W");
     const int v = tfno::values_of(type);
     const tfno::MixParams q = { gy, slopes ? z : nullptr, W, nullptr, nullptr, nullptr, nullptr, gx, slopes ? gz : nullptr, P * v, ldgy * v, ldz * v, 0, ldgx * v,
                                 ldgz * v, K, N, K, act };
@@ -180,6 +195,9 @@ static int norm_on(bool eight, int type, long P, int K, const void* x, long ldx,
     if (taken(x, ldx) || taken(residual, ldr))
         return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps an operand without being it");
     if (overlap(y, K, ldy, ey, s, K, lds, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "the results overlap");
+    const Place px = place(x, K, ldx, e, P), pr = place(residual, K, ldr, e, P), ps = place(s, K, lds, e, P), py = place(y, K, ldy, ey, P);
+    if (among(packed(gain, 4l * K), { ps, py }) || among(packed(rstd, 4 * P), { px, pr, ps, py, packed(gain, 4l * K) }))
+        return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps gain, or %s another operand", eight ? "scale" : "rstd");
     const tfno::NormParams q = { x, residual, gain, s, y, rstd, P * v, ldx * v, ldr * v, lds * v, ldy * v, K, eps };
     return hip_status(tfno::launch_rms_norm(q, type, eight, (hipStream_t)stream), eight ? "rms_norm_8bit launch" : "rms_norm launch");
 }
@@ -215,6 +233,10 @@ int turbofno_rms_norm_backward(int type, long P, int K, const void* gy, long ldg
     CHECK(check_there("ggain", ggain));
     const size_t e = tfno::size_of(type), need = tfno::rms_norm_backward_workspace(type, P, K);
     if (clash(gx, ldgx, gy, ldgy, K, e, P) || clash(gx, ldgx, s, lds, K, e, P) || clash(gx, ldgx, gs, ldgs, K, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "gx overlaps an operand without being it");
+    const Place px = place(gx, K, ldgx, e, P), pg = packed(gain, 4l * K), pr = packed(rstd, 4 * P), po = packed(ggain, 4l * K);
+    if (among(px, { pg, pr, po })) return fail(TURBOFNO_ERR_INVALID_ARG, "gx overlaps gain, rstd or ggain");
+    if (among(packed(workspace, (long)need), { place(gy, K, ldgy, e, P), place(s, K, lds, e, P), place(gs, K, ldgs, e, P), px, pg, pr, po }))
+        return fail(TURBOFNO_ERR_INVALID_ARG, "the workspace overlaps an operand");
     if (!workspace || workspace_bytes < need) return fail(TURBOFNO_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, need);
     const int v = tfno::values_of(type);
     const tfno::NormGradParams q = { gy, s, gs, gain, rstd, gx, ggain, static_cast<float*>(workspace), P * v, ldgy * v, lds * v, ldgs * v, ldgx * v, K };

@@ -131,3 +131,61 @@ def test_results_apart_from_weights_scales_and_the_workspace():
     assert all(says(norm_grad(**{name: x + 8}), b"gx overlaps gain") for name in ("gain", "rstd", "ggain"))
     assert all(says(norm_grad(ws=p + 8), b"the workspace overlaps") for p in (y, z, r, x, W, xs, bias))
     assert norm_grad() == WORKSPACE and norm_grad(ggain=W) == WORKSPACE      # gain is read before ggain is written
+
+
+def test_places_of_tensors():
+    """the rule of the binding against single elements"""
+    rng = random.Random(9)
+    outcomes = []
+    for _ in range(3000):
+        base = torch.arange(90)
+
+        def part():
+            rows, width = rng.randint(1, 5), rng.randint(1, 5)
+            pitch = rng.choice([10, rng.randint(width, 16)])
+            return base.as_strided((rows, width), (pitch, 1), rng.randint(0, 90 - (rows - 1) * pitch - width))
+        a, b = part(), part()
+        expected = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert operators._meet(a, b) == expected and operators._meet(b, a) == expected, (a, b)
+        outcomes.append(expected)
+    assert 300 < sum(outcomes) < 2700
+    assert not operators._meet(None, base) and not operators._meet(base, "x") and not operators._meet(base[:0], base)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("kind", TYPES)
+def test_backward_results_apart_from_x(kind, compiled, monkeypatch):
+    """what the second of the two products reads is not written by the first, nor what the first wrote by the second"""
+    if not compiled:
+        monkeypatch.setattr(operators.api, "_operands", None)
+    dt, C, P = TYPES[kind], 12, 50
+    gy, x, z, W = randn((C, P), dt, 1), randn((C, P), dt, 2), randn((C, P), dt, 3), randn((C, C), dt, 4)
+    gx, gW, gbias, gz = tf.mix_backward(gy, x, W, z, "silu")
+    kept = x.clone()
+    rows = torch.cat([x, x], 1)
+    for activation in ("silu", "none"):
+        with pytest.raises(ValueError, match="gx overlaps x"):
+            tf.mix_backward(gy, x, W, z, activation, gx=x)
+        with pytest.raises(ValueError, match="gx overlaps x"):
+            tf.mix_backward(gy, rows[:, :P], W, z, activation, gx=rows[:, 1:1 + P])
+        with pytest.raises(ValueError, match="gW overlaps gx"):
+            tf.mix_backward(gy, x, W, z, activation, gx=gx, gW=gx.flatten()[:C * C].view(C, C))
+        with pytest.raises(ValueError, match="gbias overlaps gx"):
+            tf.mix_backward(gy, x, W, z, activation, gx=gx, gbias=gx[3, :C])
+        with pytest.raises(ValueError, match="workspace overlaps gx"):
+            tf.mix_backward(gy, x, W, z, activation, gx=gx, workspace=torch.view_as_real(gx).view(torch.uint8) if dt.is_complex else gx.view(torch.uint8))
+    with pytest.raises(ValueError, match="gz overlaps x"):
+        tf.mix_backward(gy, x, W, z, "silu", gz=x)
+    assert torch.equal(x, kept)
+    with pytest.raises(tf.TurboFNOError, match="0 elements between channels"):
+        tf.mix_backward(gy, x[:1].expand(C, P), W, z, "silu", gx=rows[:, :P])
+    with pytest.raises(tf.TurboFNOError, match="0 elements between channels"):
+        tf.mix_backward(gy, kept[:1].expand(C, P), W, z, "silu", gx=kept)
+    # beside x in the same rows, and over operands that both products have read by then
+    rows = torch.cat([x, x], 1)
+    results = tf.mix_backward(gy, rows[:, :P], W, z, "silu", gx=rows[:, P:])
+    assert torch.equal(rows[:, P:], gx) and torch.equal(rows[:, :P], x) and torch.equal(results[1], gW)
+    own = W.clone()
+    results = tf.mix_backward(gy, x, own, z, "silu", gW=own)
+    assert torch.equal(own, gW) and torch.equal(results[0], gx) and torch.equal(results[2], gbias) and torch.equal(results[3], gz)

@@ -2,10 +2,15 @@
 #include "../../include/turbofno.h"
 #include "capi_error.h"
 #include "mix_kernel.h"
+#include "places.h"
 #include <initializer_list>
 
 using tfno::fail;
 using tfno::hip_status;
+using tfno::overlap;
+using tfno::packed;
+using tfno::Place;
+using tfno::place;
 
 namespace {
 
@@ -35,34 +40,10 @@ int check_rows(const char* name, const void* p, long P, int rows, long ld, bool 
 }
 int check_there(const char* name, const void* p) { return p ? TURBOFNO_OK : fail(TURBOFNO_ERR_INVALID_ARG, "%s is null", name); }
 
-// Memory of an operand: rows of `width` bytes, `pitch` bytes apart
-struct Place {
-    const char* at;
-    long rows, pitch, width;
-};
-Place place(const void* p, long rows, long ld, size_t size, long P) { return { static_cast<const char*>(p), rows, rows > 1 ? ld * (long)size : 0, P * (long)size }; }
-
-// Byte for byte: two column ranges of one buffer lie between one another and do not meet
-bool overlap(const Place& a, const Place& b)
-{
-    if (!a.at || !b.at || !a.width || !b.width) return false;
-    if (a.at >= b.at + (b.rows - 1) * b.pitch + b.width || b.at >= a.at + (a.rows - 1) * a.pitch + a.width) return false;
-    if (a.rows > b.rows) return overlap(b, a);
-    for (long i = 0; i < a.rows; ++i) {
-        const char* from = a.at + i * a.pitch;
-        const long before = from - b.at - b.width;      // the first row of b that ends behind `from`
-        const long j = before < 0 || b.rows == 1 ? 0 : before / b.pitch + 1;
-        const char* row = b.at + j * b.pitch;
-        if (j < b.rows && row < from + a.width && from < row + b.width) return true;
-    }
-    return false;
-}
 bool overlap(const void* a, long rows_a, long ld_a, size_t size_a, const void* b, long rows_b, long ld_b, size_t size_b, long P)
 {
     return overlap(place(a, rows_a, ld_a, size_a, P), place(b, rows_b, ld_b, size_b, P));
 }
-
-Place packed(const void* p, long bytes) { return { static_cast<const char*>(p), 1, 0, bytes }; }
 
 // a result may be an operand, element for element, and overlaps none otherwise
 bool clash(const void* out, long ldo, const void* in, long ldi, int rows, size_t size, long P)

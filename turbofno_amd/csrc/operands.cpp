@@ -7,6 +7,7 @@
 // which raise. Only plain torch.Tensor / Parameter objects are looked at, so subclasses and wrappers keep their own behaviour, and
 // nothing is kept from one call to the next.
 #include "../../include/turbofno.h"
+#include "places.h"
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 #include <climits>
@@ -365,6 +366,12 @@ PyObject* mix_backward(PyObject*, PyObject* const* args, Py_ssize_t count)
         void *gW = packed(args[10], dt, device, { N, K }), *gbias = packed(args[11], dt, device, { N });
         const long P = positions(gy);
         const Workspace ws(args[12], bytes(type, P, N, K), gy, device);
+        // neither call sees what the other one reads or writes
+        const size_t e = dt == at::kComplexFloat ? 8 : dt == at::kFloat ? 4 : 2;
+        const tfno::Place at_x = tfno::place(fx.data, K, fx.ld, e, P), at_gx = tfno::place(gx.data, K, gx.ld, e, P);
+        if (overlap(at_gx, at_x) || (slopes && overlap(tfno::place(gz.data, N, gz.ld, e, P), at_x)) || overlap(tfno::packed(gW, (long)(e * N * K)), at_gx) ||
+            overlap(tfno::packed(gbias, (long)(e * N)), at_gx) || overlap(tfno::packed(ws.data, (long)ws.bytes), at_gx))
+            throw NotHere();
         const WithoutLock unlocked;
         const int rc = input(type, P, N, K, g.data, g.ld, z.data, z.ld, W, act, slopes ? gz.data : nullptr, gz.ld, gx.data, gx.ld, stream);
         return rc ? rc : weight(type, P, N, K, gz.data, gz.ld, fx.data, fx.ld, gW, gbias, ws.data, ws.bytes, stream);

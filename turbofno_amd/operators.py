@@ -109,6 +109,31 @@ def _packed(t, name, shape, dtype, device):
     return t.data_ptr()
 
 
+def _place(t):
+    """memory of a tensor whose rows lie side by side each: address, rows, bytes from row to row, bytes of a row; None for what is no such tensor"""
+    if not isinstance(t, torch.Tensor) or not t.numel():
+        return None
+    if t.is_contiguous():
+        return t.data_ptr(), 1, 0, t.numel() * t.element_size()
+    if t.dim() < 2 or t.stride(0) <= 0 or not t[0].is_contiguous():
+        return None
+    return t.data_ptr(), t.shape[0], t.stride(0) * t.element_size(), t[0].numel() * t.element_size()
+
+
+def _meet(a, b):
+    """do two tensors share a byte"""
+    a, b = _place(a), _place(b)
+    if a is None or b is None or a[0] >= b[0] + (b[1] - 1) * b[2] + b[3] or b[0] >= a[0] + (a[1] - 1) * a[2] + a[3]:
+        return False
+    (at, rows, pitch, width), (other, others, other_pitch, other_width) = (a, b) if a[1] <= b[1] else (b, a)
+    for start in range(at, at + rows * pitch if rows > 1 else at + 1, pitch or 1):
+        before = start - other - other_width            # the first of the other's rows that ends behind `start`
+        row = 0 if before < 0 or others == 1 else before // other_pitch + 1
+        if row < others and other + row * other_pitch < start + width and start < other + row * other_pitch + other_width:
+            return True
+    return False
+
+
 def _input(x, name):
     """type, device, channels and positions of the field a call starts from"""
     if not isinstance(x, torch.Tensor):
@@ -231,13 +256,18 @@ def mix_weight_grad(gz, x, gW=None, gbias=None, workspace=None):
 
 
 def mix_backward(gy, x, W, z=None, activation="none", gz=None, gx=None, gW=None, gbias=None, workspace=None):
-    """(gx, gW, gbias, gz) from the gradient of y, and the x, W and z of mix; gz is the gradient of its residual."""
+    """(gx, gW, gbias, gz) from the gradient of y, and the x, W and z of mix; gz is the gradient of its residual. x is read after gx and gz are written:
+    they share no memory with it."""
     act = _ACTIVATIONS.get(activation, -1)
     if isinstance(gy, torch.Tensor) and isinstance(x, torch.Tensor) and isinstance(W, torch.Tensor) and gy.is_cuda:
         gz = gy if act == 0 else _result(gz, gy.shape, gy.dtype, gy.device)
         gx, gW, gbias = _result(gx, x.shape, x.dtype, x.device), _result(gW, W.shape, W.dtype, W.device), _result(gbias, gy.shape[:1], gy.dtype, gy.device)
         if _compiled("mix_backward", ("mix_input_grad", "mix_weight_grad", "mix_weight_grad_workspace_bytes"), gy, x, W, z, act, gz, gx, gW, gbias, workspace):
             return gx, gW, gbias, gz
+    for name, t in (("gx", gx), ("gz", None if act == 0 else gz)):
+        _need(not _meet(t, x), "%s overlaps x, which the gradient of W is formed from afterwards", name)
+    for name, t in (("gW", gW), ("gbias", gbias), ("workspace", workspace)):
+        _need(not _meet(t, gx), "%s overlaps gx", name)
     gx, gz = mix_input_grad(gy, W, z=z, activation=activation, gz=gz, gx=gx)
     gW, gbias = mix_weight_grad(gz, x, gW=gW, gbias=gbias, workspace=workspace)
     return gx, gW, gbias, gz

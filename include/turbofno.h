@@ -255,7 +255,8 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *   turbofno_rms_norm        s = x + residual, rstd[p] = 1 / sqrt(mean over k of |s[k][p]|^2 + eps), y[k] = gain[k] rstd s[k]; gain [K] in fp32 for every
  *                            type. residual, s (not needed without residual) and rstd may be NULL. s and y may be x or residual themselves.
  *   turbofno_rms_norm_8bit   the same with y in e4m3 and a scale per position: scale[p] = max over k of |y[k][p]| / 448 (real and imaginary parts; 1
- *                            where that is no normal number), q = y / scale: what turbofno_mix_8bit takes.
+ *                            where that is below 2^-126, and all q are zeros then; NaN where an s is infinite or NaN), q = y / scale: what
+ *                            turbofno_mix_8bit takes.
  *   turbofno_rms_norm_backward  gx = gradient of s: that of y through the norm, plus gs (what reaches s by the residual stream; may be NULL). It is
  *                            that of x and of residual. ggain [K]: gradient of gain. gx may be gy, s or gs itself.
  *   turbofno_clip_grad_norm  norm = sqrt(sum of |g|^2 over all tensors), on the device; out[i] = grads[i] min(1, max_norm / (norm + 1e-6)). Lists of

@@ -10,7 +10,7 @@
 // 16 or 64 lanes side by side make a strip of 64 or 256 columns (16: four channels per wave and access), the waves of a block take turns over the
 // channels. Sums over channels are formed per lane, then over the lanes and waves that share a column through LDS, in fp32. Where the channels do
 // not fit into registers the strip is read a second time. Measured, with residual: complex64, 64 channels, 2^20 positions 405 us (5.3 TB/s), its gradient
-// 426 us (5.0 TB/s); bf16 to 8 bits, 256 channels, 262144 positions 96 us (4.9 TB/s); a large copy reaches 5.15 TB/s.
+// 426 us (5.0 TB/s); bf16 to 8 bits, 256 channels, 262144 positions 97 us (4.8 TB/s); a large copy reaches 5.15 TB/s.
 #include "columns.h"
 #include <algorithm>
 
@@ -149,16 +149,23 @@ __device__ __forceinline__ void norm_strip(const NormParams& q, float4_v* shared
             if (strip.has(r)) add(r, value(r));
     sum = strip.template over_channels<true>(per_position<COMPLEX>(sum), shared, sum4);
     if constexpr (EIGHT) most = strip.template over_channels<true>(largest_per_position<COMPLEX>(most), shared + kThreads, larger4);
-    float4_v rstd, factor;
+    float4_v rstd, factor, lift = { 1.f, 1.f, 1.f, 1.f };
 #pragma unroll
     for (int i = 0; i < 4; ++i) factor[i] = rstd[i] = __builtin_amdgcn_rsqf(sum[i] / (float)q.K + q.eps);
     if constexpr (EIGHT)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            // y / scale = s gain (448 / max |s gain|), which is at most 448 and a few roundings: e4m3 takes up to 464 to 448
-            const float f = 448.f / most[i];
-            factor[i] = f > 0x1p120f ? 0x1p120f : f;
-            rstd[i] = most[i] == 0.f ? 1.f : rstd[i] / factor[i];
+            // y / scale = s gain (448 / max |s gain|), which is at most 448 and a few roundings: e4m3 takes up to 464 to 448. The product s gain comes first: 448 / max
+            // alone times a gain may be infinite. Where max is small, both are lifted so that 448 / max is finite
+            if (most[i] < 0x1p-96f) lift[i] = 0x1p64f;
+            factor[i] = 448.f / (most[i] * lift[i]);
+            rstd[i] /= factor[i];
+            if (most[i] < 0x1p-96f) rstd[i] *= 0x1p-64f;
+            // nothing but zeros, or no normal number for a scale: a scale of 1, which leaves zeros of what is below 2^-117
+            if (most[i] == 0.f || rstd[i] < 0x1p-126f) {
+                rstd[i] = 1.f;
+                factor[i] = 0.f;
+            }
         }
     if (strip.group() == 0 && q.rstd)
 #pragma unroll
@@ -166,12 +173,12 @@ __device__ __forceinline__ void norm_strip(const NormParams& q, float4_v* shared
             if (FULL || i < lane_there) q.rstd[(column + i) / PARTS] = rstd[i];
     auto store_sum = [&](int r, float4_v v) { strip.template write<IN, FULL>(q.s, q.lds, column0, there, r, from_float<IN>(v)); };
     auto finish = [&](int r, float4_v v) {
-        v *= factor * gain(r);
         if constexpr (EIGHT) {
+            v = v * gain(r) * lift * factor;
             int bytes = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
             bytes = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], bytes, true);
             strip.template write<kIn8, FULL>(q.y, q.ldy, column0, there, r, (unsigned)bytes);
-        } else strip.template write<IN, FULL>(q.y, q.ldy, column0, there, r, from_float<IN>(v));
+        } else strip.template write<IN, FULL>(q.y, q.ldy, column0, there, r, from_float<IN>(v * (factor * gain(r))));
     };
     auto both = [&](int r, float4_v v) {                // v is there before either result is written: they may take its operands' place
         if (q.s) store_sum(r, v);

@@ -260,7 +260,8 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *   turbofno_rms_norm_backward  gx = gradient of s: that of y through the norm, plus gs (what reaches s by the residual stream; may be NULL). It is
  *                            that of x and of residual. ggain [K]: gradient of gain. gx may be gy, s or gs itself.
  *   turbofno_clip_grad_norm  norm = sqrt(sum of |g|^2 over all tensors), on the device; out[i] = grads[i] min(1, max_norm / (norm + 1e-6)). Lists of
- *                            `count` tensors, on the host, of sizes[i] elements; out[i] may be grads[i], which is left alone when nothing is scaled. The
+ *                            `count` tensors, on the host, of sizes[i] elements; out[i] may be grads[i], which is left alone when nothing is scaled; apart from
+ *                            that the results overlap neither one another nor a gradient (a tensor that is in the list twice would be scaled twice). The
  *                            sum is formed in 64 bits. An infinite or NaN value makes norm the same, and every result follows the formula.
  *                            Workspace: as queried, 8-byte aligned.
  */

@@ -1,5 +1,6 @@
 """Which operands of the operators around the layer may share memory: every result is apart from what the call reads or writes, except in the places
 that the header names. Refusals are checked without a GPU, on addresses that are never looked at."""
+import ctypes
 import random
 
 import pytest
@@ -189,3 +190,50 @@ def test_backward_results_apart_from_x(kind, compiled, monkeypatch):
     own = W.clone()
     results = tf.mix_backward(gy, x, own, z, "silu", gW=own)
     assert torch.equal(own, gW) and torch.equal(results[0], gx) and torch.equal(results[2], gbias) and torch.equal(results[3], gz)
+
+
+def test_clipped_tensors_that_meet():
+    """lists of one to five tensors against single bytes: refused for their memory, or, one check further, for the missing workspace"""
+    L, rng = operators._lib(), random.Random(11)
+    bytes_of = {0: 8, 1: 4, 2: 2}
+    outcomes = []
+    for round_ in range(6000):
+        n = rng.randint(1, 5)
+        kinds, sizes = [rng.randint(0, 2) for _ in range(n)], [rng.choice([0, 1, 2, 3, 5]) for _ in range(n)]
+        where = lambda: BASE + 2 * rng.randint(0, 200)  # noqa: E731
+        grads = [where() for _ in range(n)]
+        out = [g if rng.random() < 0.7 else where() for g in grads]
+        norm = BASE + 1000 if rng.random() < 0.9 else where()
+        rc = L.turbofno_clip_grad_norm(n, (ctypes.c_void_p * n)(*grads), (ctypes.c_void_p * n)(*out), (ctypes.c_long * n)(*sizes), (ctypes.c_int * n)(*kinds),
+                                       1.0, norm, None, 0, None)
+        covered = lambda at, i: set(range(at, at + sizes[i] * bytes_of[kinds[i]]))  # noqa: E731
+        at_norm = set(range(norm, norm + 4))
+        meet = any(covered(out[i], i) & covered(out[j], j) for i in range(n) for j in range(i))
+        meet |= any(covered(out[i], i) & covered(grads[j], j) for i in range(n) for j in range(n) if i != j or out[i] != grads[j])
+        meet |= any((covered(out[i], i) | covered(grads[i], i)) & at_norm for i in range(n))
+        assert rc == (INVALID if meet else WORKSPACE), (grads, out, sizes, kinds, norm, L.turbofno_last_error_string())
+        outcomes.append(rc)
+    assert 1000 < outcomes.count(INVALID) < 5000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [3, 150])
+def test_clip_refuses_shared_memory(count):
+    flat = randn((count * 100,), torch.float32, 1)
+    grads = [flat[i * 100:(i + 1) * 100] for i in range(count)]
+    kept = flat.clone()
+    for again in (grads[1], flat[250:260], flat[:7], flat[99:101]):
+        with pytest.raises(tf.TurboFNOError, match="overlap"):
+            tf.clip_grad_norm(grads + [again], 0.1)
+        with pytest.raises(tf.TurboFNOError, match="overlap"):
+            tf.clip_grad_norm(grads + [again], 0.1, out=grads + [torch.empty_like(again)])
+    with pytest.raises(tf.TurboFNOError, match="overlaps the norm"):
+        tf.clip_grad_norm(grads, 0.1, norm=flat[5])
+    assert torch.equal(flat, kept)
+    # parts of one buffer, and a gradient that is read twice, are taken
+    out = torch.empty_like(flat)
+    norm = tf.clip_grad_norm(grads + [grads[0]], 0.1, out=[out[i * 100:(i + 1) * 100] for i in range(count)] + [torch.empty(100, device="cuda")])
+    exact = (flat.double().square().sum() + grads[0].double().square().sum()).sqrt()
+    assert abs(norm.item() - exact.item()) <= 2.0 ** -22 * exact.item()
+    tf.clip_grad_norm(list(reversed(grads)), 0.1)
+    assert not torch.equal(flat, kept)

@@ -3,7 +3,10 @@
 #include "capi_error.h"
 #include "mix_kernel.h"
 #include "places.h"
+#include <algorithm>
 #include <initializer_list>
+#include <memory>
+#include <new>
 
 using tfno::fail;
 using tfno::hip_status;
@@ -57,6 +60,39 @@ bool among(const Place& result, std::initializer_list<Place> operands)
     for (const Place& operand : operands)
         if (overlap(result, operand)) return true;
     return false;
+}
+
+// Where the results of the clipping lie: apart from one another, from every gradient but their own, and from the norm and the workspace
+struct Span {
+    const char *from, *to;
+    int of;
+};
+int check_clip_places(Span* spans, int count, const void* const* grads, void* const* out, const long* sizes, const int* types, const Place& norm, const Place& workspace)
+{
+    auto span = [&](const void* p, int i) { return Span{ static_cast<const char*>(p), static_cast<const char*>(p) + sizes[i] * (long)tfno::size_of(types[i]), i }; };
+    auto before = [](const Span& a, const Span& b) { return a.from < b.from; };
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+        if (!sizes[i]) continue;
+        const Span o = span(out[i], i), g = span(grads[i], i);
+        for (const Place* p : { &norm, &workspace })
+            if (p->at && ((o.from < p->at + p->width && p->at < o.to) || (g.from < p->at + p->width && p->at < g.to)))
+                return fail(TURBOFNO_ERR_INVALID_ARG, "tensor %d overlaps the norm or the workspace", i);
+        spans[n++] = o;
+    }
+    if (!std::is_sorted(spans, spans + n, before)) std::sort(spans, spans + n, before);
+    for (int k = 1; k < n; ++k)
+        if (spans[k].from < spans[k - 1].to) {
+            const int a = spans[k - 1].of, b = spans[k].of;
+            return fail(TURBOFNO_ERR_INVALID_ARG, "results %d and %d overlap: each would be scaled for both", a < b ? a : b, a < b ? b : a);
+        }
+    for (int i = 0; i < count; ++i) {
+        if (!sizes[i] || out[i] == grads[i]) continue;
+        const Span g = span(grads[i], i);
+        const Span* o = std::lower_bound(spans, spans + n, g, [](const Span& a, const Span& b) { return a.to <= b.from; });
+        if (o < spans + n && o->from < g.to) return fail(TURBOFNO_ERR_INVALID_ARG, "result %d overlaps gradient %d", o->of, i);
+    }
+    return TURBOFNO_OK;
 }
 
 #define CHECK(call) if (int rc_ = (call)) return rc_
@@ -239,6 +275,12 @@ int turbofno_clip_grad_norm(int count, const void* const* grads, void* const* ou
         if (sizes[i] && (!grads[i] || !out[i])) return fail(TURBOFNO_ERR_INVALID_ARG, "tensor %d is null", i);
     }
     const size_t need = tfno::clip_workspace(count);
+    Span few[128];
+    const std::unique_ptr<Span[]> many(count > 128 ? new (std::nothrow) Span[count] : nullptr);
+    if (count > 128 && !many) return fail(TURBOFNO_ERR_INVALID_ARG, "no host memory for the places of %d tensors", count);
+    const Place at_norm = packed(norm, sizeof(float)), at_workspace = packed(workspace, (long)need);
+    if (overlap(at_norm, at_workspace)) return fail(TURBOFNO_ERR_INVALID_ARG, "norm overlaps the workspace");
+    CHECK(check_clip_places(count > 128 ? many.get() : few, count, grads, out, sizes, types, at_norm, at_workspace));
     if (!workspace || workspace_bytes < need) return fail(TURBOFNO_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, need);
     return hip_status(tfno::launch_clip(count, grads, out, sizes, types, max_norm, norm, workspace, (hipStream_t)stream), "clip_grad_norm launch");
 }

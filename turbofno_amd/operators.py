@@ -349,7 +349,8 @@ def rms_norm_backward(gy, s, gain, rstd, gs=None, gx=None, ggain=None, workspace
 
 def clip_grad_norm(grads, max_norm, out=None, norm=None, workspace=None):
     """The norm over all values of the tensors in `grads` (complex64, float32 and bfloat16, contiguous, in any mixture), as a float32 tensor of no
-    dimensions on the GPU; each is scaled by min(1, max_norm / (norm + 1e-6)), into the tensor of the same place in `out`, or in place."""
+    dimensions on the GPU; each is scaled by min(1, max_norm / (norm + 1e-6)), into the tensor of the same place in `out`, or in place. A gradient that
+    several parameters share is given once: results that overlap are refused."""
     grads = list(grads)
     out = grads if out is None else list(out)
     _need(len(out) == len(grads), "out has %d tensors, grads %d", len(out), len(grads))

@@ -21,7 +21,7 @@ static_assert(TURBOFNO_C64 == tfno::kC64 && TURBOFNO_F32 == tfno::kF32 && TURBOF
 static_assert(TURBOFNO_ACT_NONE == tfno::kActNone && TURBOFNO_ACT_RELU == tfno::kActRelu && TURBOFNO_ACT_SILU == tfno::kActSilu &&
               TURBOFNO_ACT_GELU_TANH == tfno::kActGeluTanh, "activations");
 
-constexpr long kMaxPositions = 1L << 36;                // two real values each and a launch of a block per 64 fit every index
+constexpr long kMaxPositions = 1L << 36;                // 2^37 real columns: strips of 64, and bytes, fit every index
 
 int check_sizes(int type, long P, int N, int K, int act)
 {

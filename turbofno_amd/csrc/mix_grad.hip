@@ -291,7 +291,7 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ sums, int splits, long count, long weights, int type, void* gW, void* gbias)
 {
     __shared__ float part[4][64];
-    const long e = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const long e = block_index() * 64 + (threadIdx.x & 63);
     const int quarter = threadIdx.x >> 6;
     float sum = 0.f;
     if (e < count) {
@@ -362,7 +362,7 @@ hipError_t launch_mix_weight_grad(int type, long P, int N, int K, const void* gz
     const hipError_t e = type == kC64 ? launch_tiles<kIn32, true>(g.t, q, stream) : type == kF32 ? launch_tiles<kIn32, false>(g.t, q, stream) : launch_tiles<kIn16, false>(g.t, q, stream);
     if (e != hipSuccess || (g.t == 2 && g.splits == 1)) return e;
     const long weights = (long)N * K * v, count = weights + (long)N * v;
-    hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)((count + 63) / 64)), dim3(256), 0, stream, q.sums, q.splits, count, weights, type, gW, gbias);
+    hipLaunchKernelGGL(add_parts_kernel, grid_of((count + 63) / 64), dim3(256), 0, stream, q.sums, q.splits, count, weights, type, gW, gbias);
     return hipGetLastError();
 }
 

@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
 {
     typedef MixWave<IN, OUT, COMPLEX, GRAD, NT, true, RAGGED> Wave;
     const Wave wave(q);
-    const long id = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long id = block_index() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long column = id / row_groups * kColumns, left = q.columns - column;
     const int row0 = (int)(id % row_groups) * (16 * NT);
     if (left <= 0) return;

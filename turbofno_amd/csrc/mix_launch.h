@@ -11,7 +11,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES, int NT, bool RA
     const long tiles = (q.columns + kColumns - 1) / kColumns;
     const int groups = (q.rows + 16 * NT - 1) / (16 * NT);
     const long blocks = (tiles * groups + 3) / 4;
-    hipLaunchKernelGGL((mix_direct_kernel<IN, OUT, COMPLEX, GRAD, SLOPES, NT, RAGGED, FEW>), dim3((unsigned)blocks), dim3(256), 0, stream, q, groups);
+    hipLaunchKernelGGL((mix_direct_kernel<IN, OUT, COMPLEX, GRAD, SLOPES, NT, RAGGED, FEW>), grid_of(blocks), dim3(256), 0, stream, q, groups);
     return hipGetLastError();
 }
 

@@ -196,11 +196,12 @@ __device__ __forceinline__ void norm_strip(const NormParams& q, float4_v* shared
 template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD> __global__ __launch_bounds__(kThreads, IN == kIn16 ? 4 : 2) void norm_kernel(const NormParams q)
 {
     typedef Strip<LANES> S;
+    const long column0 = block_index() * S::COLUMNS;
+    if (column0 >= q.columns) return;
     __shared__ float4_v shared[(EIGHT ? 2 : 1) * kThreads];
     __shared__ float gains[HELD ? HELD * S::GROUPS : 1];
     if constexpr (HELD > 0)
         for (int k = threadIdx.x; k < HELD * S::GROUPS; k += kThreads) gains[k] = q.gain[k < q.K ? k : q.K - 1];
-    const long column0 = (long)blockIdx.x * S::COLUMNS;
     if (column0 + S::COLUMNS <= q.columns) norm_strip<IN, COMPLEX, EIGHT, LANES, HELD, true>(q, shared, gains, column0, S::COLUMNS);
     else norm_strip<IN, COMPLEX, EIGHT, LANES, HELD, false>(q, shared, gains, column0, (int)(q.columns - column0));
 }
@@ -290,14 +291,15 @@ __device__ __forceinline__ void norm_grad_long_strip(const NormGradParams& q, fl
             if (FULL || i < lane_there) sum = __builtin_fmaf(d[i], rstd[i], sum);
 #pragma unroll
         for (int e = 1; e < LANES; e *= 2) sum += __shfl_xor(sum, e, LANES);
-        if (strip.lane == 0) q.sums[(long)blockIdx.x * q.K + strip.channel(r)] = sum;
+        if (strip.lane == 0) q.sums[block_index() * q.K + strip.channel(r)] = sum;
     }
 }
 template <int IN, bool COMPLEX, int LANES> __global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const NormGradParams q)
 {
     __shared__ float4_v shared[kThreads];
     constexpr int COLUMNS = Strip<LANES>::COLUMNS;
-    const long column0 = (long)blockIdx.x * COLUMNS;
+    const long column0 = block_index() * COLUMNS;
+    if (column0 >= q.columns) return;
     if (column0 + COLUMNS <= q.columns) norm_grad_long_strip<IN, COMPLEX, LANES, true>(q, shared, column0, COLUMNS);
     else norm_grad_long_strip<IN, COMPLEX, LANES, false>(q, shared, column0, (int)(q.columns - column0));
 }
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(256) void add_gain_kernel(const float* __restrict__
 
 template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD> hipError_t launch_norm_as(const NormParams& q, hipStream_t stream)
 {
-    hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, LANES, HELD>), dim3((unsigned)((q.columns + 4 * LANES - 1) / (4 * LANES))), dim3(kThreads), 0, stream, q);
+    hipLaunchKernelGGL((norm_kernel<IN, COMPLEX, EIGHT, LANES, HELD>), grid_of((q.columns + 4 * LANES - 1) / (4 * LANES)), dim3(kThreads), 0, stream, q);
     return hipGetLastError();
 }
 template <int IN, bool COMPLEX, bool EIGHT> hipError_t launch_norm(const NormParams& q, hipStream_t stream)
@@ -358,7 +360,7 @@ template <int IN, bool COMPLEX> hipError_t launch_grad(const NormGradParams& q, 
     const long strips = grad_strips(q.K, q.columns), wide = (q.columns + 255) / 256;
     const bool far = std::max(std::max(q.ldgy, q.lds), std::max(q.ldgs, q.ldgx)) >= kFar;
     const long blocks = far && q.K > kGradHeldChannels ? wide : grad_blocks(q.K, q.columns);
-    const dim3 grid((unsigned)blocks);
+    const dim3 grid = grid_of(blocks);                  // one row of them where they are persistent
 #define TFNO_NORM_GRAD(LANES, HELD, STRIPS) hipLaunchKernelGGL((norm_grad_kernel<IN, COMPLEX, LANES, HELD>), grid, dim3(kThreads), 0, stream, q, STRIPS)
     if (blocks) {
         if (q.K > kGradHeldChannels) {

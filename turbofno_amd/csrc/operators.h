@@ -11,6 +11,12 @@ enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGeluTanh = 3 };
 inline int values_of(int type) { return type == kC64 ? 2 : 1; }         // real values of an element
 inline size_t size_of(int type) { return type == kC64 ? 8 : type == kF32 ? 4 : 2; }
 
+// A grid of any number of blocks: a dimension of a launch holds fewer than 2^32 threads, so from 2^22 blocks (of up to 512) on there are several rows of
+// them, whose last blocks may have nothing to do
+constexpr long kGridRow = 1L << 22;
+inline dim3 grid_of(long blocks) { return blocks <= kGridRow ? dim3((unsigned)blocks) : dim3((unsigned)kGridRow, (unsigned)((blocks + kGridRow - 1) / kGridRow)); }
+__device__ __forceinline__ long block_index() { return blockIdx.y * kGridRow + blockIdx.x; }
+
 typedef unsigned uint2_v __attribute__((ext_vector_type(2)));
 
 struct MixParams;

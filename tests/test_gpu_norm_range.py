@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import turbofno_amd as tf
-from operators_reference import EPS32, TYPES, randn, wide
+from operators_reference import EPS32, TYPES, randn, rounding, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -12,8 +12,9 @@ SIZES = [(3, 70), (40, 90), (200, 75), (600, 66), (30, 140003), (100, 140003), (
 GAINS = [1.0, 256.0, -256.0, 1e4, -1e4, 1e-3, 0.0, 1e9]
 
 
-def check_8bit(x, gain, eps=1e-6):
-    """q and scale against the definition in 64 bits: scale = max |y| / 448, or 1 where that is below the normal numbers"""
+def check_8bit(x, gain, eps=1e-6, root=0.0):
+    """q and scale against the definition in 64 bits: scale = max |y| / 448, or 1 where that is below the normal numbers. root: what
+    the root of the mean is off by beside its roundings"""
     K = x.shape[0]
     q, scale, _ = tf.rms_norm_8bit(x, gain, eps=eps)
     S = wide(x)
@@ -25,7 +26,7 @@ def check_8bit(x, gain, eps=1e-6):
     assert not ((most / 448 / 2.0 ** -126 - 1).abs() < 0.01).any()          # which of the two it is does not hang on a rounding
     # the largest s gain is known to half of the smallest number, 2^-149, the rest is a sum of K squares and a few roundings
     largest = (S * wide(gain)[:, None, None]).abs().amax(dim=(0, 2))
-    noise = (K + 24) * EPS32 + 2.0 ** -149 / largest.clamp_min(2.0 ** -149)
+    noise = (K + 24) * EPS32 + 2.0 ** -149 / largest.clamp_min(2.0 ** -149) + root
     assert ((wide(scale) - exact).abs() <= noise * exact).all(), ((wide(scale) - exact).abs() / exact).max()
     want = parts / exact[None, :, None]
     got = q.cpu().double().reshape(want.shape)
@@ -61,3 +62,24 @@ def test_8bit_position_of_zeros_through_the_product():
     Wq, bias = randn((N, K), torch.float32, 2).to(torch.float8_e4m3fn), randn((N,), torch.bfloat16, 3)
     y = tf.mix_8bit(q, scale, Wq, torch.ones(N, device="cuda"), bias=bias)
     assert torch.equal(y[:, 17], bias) and torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,P", [(3, 70), (40, 90), (600, 66), (100, 140003)])
+def test_small_positions_without_eps(kind, K, P):
+    """means of squares down to the smallest numbers: 2^-149 / mean of themselves is what they may be off by"""
+    dt = TYPES[kind]
+    x, gain = randn((K, P), dt, 4), 1 + 0.2 * randn((K,), torch.float32, 5)
+    for i, size in enumerate((1e-10, 1e-17, 1e-18, 1e-19, 3e-20, 1e-20)):
+        x[:, i] = x[:, i] * size
+        x[:, P - 1 - 2 * i] = x[:, P - 1 - 2 * i] * size
+    y, s, rstd = tf.rms_norm(x, gain, eps=0.0)
+    S = wide(x)
+    mean = (S.abs() ** 2).mean(0)
+    R = 1 / torch.sqrt(mean)
+    # of a mean of K squares, each of which and the mean itself may be rounded to a multiple of 2^-149 (real and imaginary parts: twice); half of it in the root
+    noise = (K + 16) * EPS32 + 3 * 2.0 ** -149 / mean
+    assert ((wide(rstd) - R).abs() <= noise * R).all(), ((wide(rstd) - R).abs() / R / noise).max()
+    Y = S * R * wide(gain)[:, None]
+    assert ((wide(y) - Y).abs() <= (noise + 1.01 * rounding(dt)) * Y.abs()).all()
+    check_8bit(x, gain, eps=0.0, root=3 * 2.0 ** -149 / mean)

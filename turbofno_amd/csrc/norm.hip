@@ -101,6 +101,14 @@ template <int PARTS> __device__ __forceinline__ float4_v per_column(const float*
     return v;
 }
 
+// 1 / sqrt(v). The instruction takes numbers below 2^-126 for zeros
+__device__ __forceinline__ float reciprocal_root(float v)
+{
+    const bool small = v < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p48f : v);
+    return small ? r * 0x1p24f : r;
+}
+
 // HELD: channels per lane kept in registers; 0: read again. At most 16: 32 lanes side by side for 256 channels, 16 for 512 (bf16 to 8 bits, 256 channels at 262144
 // positions: 97 us, with 64 lanes and so 32 channels in a lane, which spill, 467; float32 210 and 219)
 template <int IN, bool COMPLEX, bool EIGHT, int LANES, int HELD, bool FULL>
@@ -151,7 +159,7 @@ __device__ __forceinline__ void norm_strip(const NormParams& q, float4_v* shared
     if constexpr (EIGHT) most = strip.template over_channels<true>(largest_per_position<COMPLEX>(most), shared + kThreads, larger4);
     float4_v rstd, factor, lift = { 1.f, 1.f, 1.f, 1.f };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) factor[i] = rstd[i] = __builtin_amdgcn_rsqf(sum[i] / (float)q.K + q.eps);
+    for (int i = 0; i < 4; ++i) factor[i] = rstd[i] = reciprocal_root(sum[i] / (float)q.K + q.eps);
     if constexpr (EIGHT)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -243,7 +243,7 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *
  *   turbofno_mix             z = W x + bias + residual, y = act(z): x[K][P] -> y[N][P]. bias [N], residual [N][P] and z [N][P] may be NULL; z is the
  *                            pre-activation that the gradient needs. residual may be y or z itself. 32-bit products are formed as those of the
- *                            layer (see "Precision"), sums that come out infinite or NaN again in fp32; parts of operands below 2^-133 are lost.
+ *                            layer: fp32 over the whole range of floats, infinities and NaN included (see "Precision").
  *   turbofno_mix_8bit        the same from 8-bit operands (e4m3, complex values as (re, im) pairs): x = xscale[p] xq[k][p], W = wscale[n] Wq[n][k];
  *                            type is that of bias, residual and y, ldx counts elements (pairs where they are complex).
  *   turbofno_mix_input_grad  gz = gy act'(z) (re and im apart), gx[k] = sum_n conj(W[n][k]) gz[n]. gz is the gradient of residual, and what

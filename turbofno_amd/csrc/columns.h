@@ -106,6 +106,21 @@ template <int IN> __device__ __forceinline__ void near_store4(ScalarAddress base
     else if constexpr (IN == kIn16) *(TFNO_GLOBAL uint2_any*)(base + offset) = v;
     else *(TFNO_GLOBAL uint_any*)(base + offset) = v;
 }
+// Is one of the values below the range of the split (bf16_split.h), but not zero, in any lane: uniform. One minimum per two values; zeros are told
+// apart where there are any
+template <int COUNT> __device__ __forceinline__ bool below_split_range(const float4_v (&v)[COUNT])
+{
+    float low = 1.f;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) low = smaller(smaller(low, v[j][0], v[j][1]), v[j][2], v[j][3]);
+    if (__builtin_expect(!any_lane(low < kSplitSmallest), 1)) return false;
+    unsigned bits = ~0u;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) bits = lower(lower(bits, float2{ v[j][0], v[j][1] }), float2{ v[j][2], v[j][3] });
+    return any_lane(bits < kSplitLow);
+}
+__device__ __forceinline__ float4_v mfma_fp32(float a, float b, float4_v c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
 __device__ __forceinline__ float value_of(float v) { return v; }
 __device__ __forceinline__ float value_of(unsigned short v) { return __builtin_bit_cast(float, (unsigned)v << 16); }
 

@@ -14,8 +14,10 @@
 //   complex   two positions, four channels (re, im) of each, twice: (re, -im) for the real part of the product and (im, re) for the imaginary
 //             part, against the one operand (re, im) of A; conjugated weights take (re, im) and (im, -re).
 // The input goes from memory to the matrix cores without passing LDS, and is read once where 16 NT rows are all of them.
-// 32-bit operands are split into three bf16 parts each, six products (bf16_split.h); sums that are not finite are formed again in fp32, so that
-// infinities and the top of the range behave as in fp32. 16-bit operands are exact on the matrix cores; 8-bit ones are widened to bf16, which holds
+// 32-bit operands are split into three bf16 parts each, six products (bf16_split.h); sums that are not finite, and all sums of a wave that met operands below
+// the range of the split, are formed again in fp32, so that the whole range of floats behaves as in fp32. Looking for small operands costs 0.3 - 1 % where memory
+// bounds the product (complex64, 64 to 64 channels at 2^20 positions with residual, z and gelu: 410.4 us without, 411.7 with), 1.5 - 4 % where the matrix cores do (256 to 256 at
+// 65536: 223 and 231), 5 - 17 % in the direct kernel with 64 rows. 16-bit operands are exact on the matrix cores; 8-bit ones are widened to bf16, which holds
 // them exactly: the matrix instructions for 8-bit operands keep fewer bits of their sums (off by 3e-5 of the result with 8 channels). Sums are fp32
 // throughout, results are rounded once; the gradient's product takes gz as it is returned, in 16 bits rounded to them.
 #pragma once
@@ -221,26 +223,11 @@ template <int IN> __device__ __forceinline__ void multiply(const Operand<IN>& a,
     }
 }
 
-// One element of the product in fp32, channel by channel: for sums that the split left without a value. `column` is a real column.
-template <bool COMPLEX, bool GRAD> __device__ __forceinline__ float product_fp32(const MixParams& q, int row, long column)
+// of weights that were fetched (those of other entries among them: at worst a product in fp32 that need not be)
+__device__ __forceinline__ bool below_split_range(const RawWeights<kIn32>& r)
 {
-    const float *W = static_cast<const float*>(q.W), *x = static_cast<const float*>(q.x), *z = static_cast<const float*>(q.zin);
-    auto value = [&](int k, long c) {
-        const float v = x[k * q.ldx + c];
-        if constexpr (GRAD) return q.act == kActNone ? v : through_activation(q.act, v, z[k * q.ldzin + c]);
-        else return v;
-    };
-    float sum = 0.f;
-    for (int k = 0; k < q.contraction; ++k) {
-        const long w = GRAD ? (long)k * q.ldw + row : (long)row * q.ldw + k;
-        if constexpr (COMPLEX) {
-            const bool imag = column & 1;
-            const float wr = W[2 * w], wi = GRAD ? -W[2 * w + 1] : W[2 * w + 1], xr = value(k, column & ~1L), xi = value(k, column | 1L);
-            sum = __builtin_fmaf(wr, imag ? xi : xr, sum);
-            sum = __builtin_fmaf(imag ? wi : -wi, imag ? xr : xi, sum);
-        } else sum = __builtin_fmaf(W[w], value(k, column), sum);
-    }
-    return sum;
+    const float4_v v[2] = { { r.w[0], r.w[1], r.w[2], r.w[3] }, { r.w[4], r.w[5], r.w[6], r.w[7] } };
+    return below_split_range(v);
 }
 
 // Columns of a wave: column0 ... column0 + 63, of which `there` exist
@@ -321,36 +308,61 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR, bool RAGGE
             if (writes && (whole || first + lane_row + j < q.contraction)) write<IN>(q.z, q.ldz, first + j, lane_row, w, x[j]);
         }
     }
-    // sums that are not finite, again in fp32
-    __device__ __forceinline__ void mend(const Window& w, int row0, float4_v (&acc)[NT][4]) const
+    // Sums that the split left without a value, again in fp32, and all of them where an operand was below the range of the split: four channels
+    // per matrix instruction, one in each quarter of the wave, out of memory
+    __device__ __forceinline__ void mend(const Window& w, int row0, bool small, float4_v (&acc)[NT][4]) const
     {
         float high = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int b = 0; b < 4; ++b) high = larger(high, acc[t][b]);
-        if (__builtin_expect(!any_lane(not_finite(high, 0.f)), 1)) return;
-        unsigned long long wrong = 0;                   // a bit for each of the lane's sums
+        if (__builtin_expect(!small && !any_lane(not_finite(high, 0.f)), 1)) return;
 #pragma unroll
-        for (int e = 0; e < 16 * NT; ++e)
-            if (not_finite(__builtin_fabsf(acc[e / 16][e / 4 % 4][e % 4]), 0.f)) wrong |= 1ull << e;
+        for (int t = 0; t < NT; ++t) {
+            const int row = row0 + 16 * t + c < q.rows ? row0 + 16 * t + c : q.rows - 1;
+            float4_v sum[4] = {};
 #pragma unroll 1
-        for (int e = 0; e < 16 * NT; ++e) {
-            const bool here = wrong >> e & 1;
-            if (!any_lane(here)) continue;
-            const int row = row0 + 16 * (e / 16) + 4 * kq + e % 4, column = 4 * c + e / 4 % 4;
-            const float v = here && row < q.rows ? product_fp32<COMPLEX, GRAD>(q, row, w.column0 + (column < w.there ? column : w.there - 1)) : 0.f;
+            for (int first = 0; first < q.contraction; first += 4) {
+                const int k = first + kq < q.contraction ? first + kq : q.contraction - 1;
+                float4_v v = here(q.x, q.ldx, k, w);
+                if constexpr (GRAD)
+                    if (q.act != kActNone) {
+                        const float4_v z = here(q.zin, q.ldzin, k, w);
 #pragma unroll
-            for (int f = 0; f < 16 * NT; ++f)
-                if (here && f == e) acc[f / 16][f / 4 % 4][f % 4] = v;
+                        for (int b = 0; b < 4; ++b) v[b] = through_activation(q.act, v[b], z[b]);
+                    }
+                const float* at = static_cast<const float*>(q.W) + (GRAD ? (long)k * q.ldw + row : (long)row * q.ldw + k) * V;
+                float re = at[0], im = COMPLEX ? (GRAD ? -at[V - 1] : at[V - 1]) : 0.f;
+                if (first + kq >= q.contraction) {
+                    v = zero4<kIn32>();
+                    re = im = 0.f;
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b) sum[b] = mfma_fp32(re, v[b], sum[b]);
+                if constexpr (COMPLEX)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) sum[b] = mfma_fp32(b & 1 ? im : -im, v[b ^ 1], sum[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][b][i] = small || not_finite(__builtin_fabsf(acc[t][b][i]), 0.f) ? sum[b][i] : acc[t][b][i];
         }
     }
+    // the lane's four columns of a row
+    __device__ __forceinline__ float4_v here(const void* base, long ld, int row, const Window& w) const
+    {
+        const float* p = static_cast<const float*>(base) + row * ld + w.column0;
+        return RAGGED ? load4_ragged<kIn32>(p, 4 * c, w.there) : load4<kIn32>(p, 4 * c);
+    }
     // results of rows row0 + 16 t + 4 kq + i: acc[t][b][i] belongs to column 4 c + b
+    // small: an operand was below the range of the split
     // bias(t): the bias of the lane's four rows of 16 rows t, real and imaginary parts apart; row_scale(t): their scales, of 8-bit operands
     template <typename Bias, typename Scale>
-    __device__ __forceinline__ void finish(const Window& w, int row0, float4_v (&acc)[NT][4], Bias bias, Scale row_scale) const
+    __device__ __forceinline__ void finish(const Window& w, int row0, bool small, float4_v (&acc)[NT][4], Bias bias, Scale row_scale) const
     {
-        if constexpr (IN == kIn32) mend(w, row0, acc);
+        if constexpr (IN == kIn32) mend(w, row0, small, acc);
         RawOf<OUT> residual[GRAD ? 1 : NT][4];          // all loads first
         float4_v xs = { 1.f, 1.f, 1.f, 1.f };
         if constexpr (!GRAD) {
@@ -452,6 +464,7 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     const Window w = { RAGGED || left >= kColumns ? column : q.columns - kColumns, RAGGED && left < kColumns ? (int)left : (int)kColumns };
     const int steps = (q.contraction + Wave::CHANNELS - 1) / Wave::CHANNELS, count = q.contraction * Wave::V;
     float4_v acc[NT][4] = {};
+    bool small = false;
     constexpr bool AHEAD = NT == 1;                     // the weights of a step are asked for with its rows: there are registers for them
     struct Step {
         typename Wave::Rows x, z;
@@ -470,12 +483,14 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
     auto product = [&](int s, Step& r) {
         if constexpr (!AHEAD) unrolled<NT>([&](int t) { fetch_a(s, t, r.a[t]); });
         if constexpr (SLOPES) wave.slope(w, s, r.x, r.z, row0 == 0);
+        if constexpr (IN == kIn32) small |= below_split_range(r.x);
         wave.clear(s, r.x);
         Operand<IN> b[4];
         make_operands<IN, COMPLEX, GRAD>(r.x, b);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             Operand<IN> a;
+            if constexpr (IN == kIn32) small |= below_split_range(r.a[t]);
             form_weights<IN, COMPLEX, GRAD, FEW>(r.a[t], row0 + 16 * t + wave.c, q.rows, 32 * s + 8 * wave.kq, count, q.ldw, a);
             multiply<IN>(a, b, acc[t]);
         }
@@ -488,7 +503,7 @@ __global__ __launch_bounds__(256, 2) void mix_direct_kernel(const MixParams q, i
         fetch(s + 2, s0);
         product(s + 1, s1);
     }
-    wave.finish(w, row0, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); }, [&](int t) { return wave.scale_of(row0 + 16 * t + 4 * wave.kq); });
+    wave.finish(w, row0, small, acc, [&](int t) { return wave.bias_of(row0 + 16 * t + 4 * wave.kq); }, [&](int t) { return wave.scale_of(row0 + 16 * t + 4 * wave.kq); });
 }
 
 // gz of the gradient by itself: units of 2048 columns of a row, in turns
@@ -562,6 +577,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
     };
     unrolled<HELD>([&](int s) { fetch(q.x, q.ldx, w, s, x[s]); });      // on their way while the operands of A are formed
     if constexpr (HELD == 0) ahead(w, 0, x0, z0);
+    unsigned low = ~0u;                                 // of the weights, as lower() counts it
     {
         const int per_step = block_rows / 16 * 64, count = steps * per_step;
 #pragma unroll 4
@@ -570,6 +586,9 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
             RawWeights<IN> raw;
             Operand<IN> a;
             fetch_weights<IN, COMPLEX, GRAD, false>(q.W, row, q.rows, entry, q.contraction * Wave::V, q.ldw, raw);
+            if constexpr (IN == kIn32)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) low = lower(low, float2{ raw.w[j], raw.w[j + 1] });
             form_weights<IN, COMPLEX, GRAD, false>(raw, row, q.rows, entry, q.contraction * Wave::V, q.ldw, a);
             uint4_v* to = weights + (long)(e / 64) * (64 * PARTS) + l;
             if constexpr (IN == kIn32) { to[0] = a.h; to[64] = a.m; to[128] = a.l; }
@@ -583,8 +602,19 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
     float4_v* scales = reinterpret_cast<float4_v*>(biases + block_rows / 4);
     if constexpr (IN == kIn8)
         for (int e = threadIdx.x; e < block_rows / 4; e += blockDim.x) scales[e] = wave.scale_of(row_first + 4 * e);
+    unsigned* lows = reinterpret_cast<unsigned*>(scales);       // 32-bit operands have no scales: a word for each wave
+    if constexpr (IN == kIn32) {
+        const bool found = any_lane(low < kSplitLow);
+        if (wave.lane == 0) lows[threadIdx.x >> 6] = found;
+    }
     __syncthreads();
     if (tile >= tiles) return;
+    bool small_weights = false;
+    if constexpr (IN == kIn32) {
+        unsigned any = 0;
+        for (unsigned i = 0; i < blockDim.x >> 6; ++i) any |= lows[i];
+        small_weights = __builtin_amdgcn_readfirstlane(any);
+    }
 
     auto weight = [&](int s, int t16) {                 // operand of step s, 16 rows t16
         const uint4_v* from = weights + (long)(s * (block_rows / 16) + t16) * (64 * PARTS) + wave.lane;
@@ -593,8 +623,8 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
         else a.v = from[0];
         return a;
     };
-    auto finish = [&](int g, float4_v (&acc)[NT][4]) {
-        wave.finish(w, row_first + g * (16 * NT), acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; }, [&](int t) { return scales[(g * NT + t) * 4 + wave.kq]; });
+    auto finish = [&](int g, bool small, float4_v (&acc)[NT][4]) {
+        wave.finish(w, row_first + g * (16 * NT), small, acc, [&](int t) { return biases[(g * NT + t) * 4 + wave.kq]; }, [&](int t) { return scales[(g * NT + t) * 4 + wave.kq]; });
     };
     if constexpr (HELD > 0) {
         for (;;) {
@@ -623,7 +653,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                         for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b[s], acc[t]);
                         __builtin_amdgcn_sched_barrier(0);
                     });
-                    finish(g, acc);
+                    finish(g, false, acc);
                 }
                 unrolled<HELD>([&](int s) { fetch(q.x, q.ldx, wn, s, x[s]); });
             } else
@@ -632,7 +662,9 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                     // last one again). Without a branch: loads whose results meet others where branches join are waited for there
                     const Window wf = g < groups - 1 ? w : wn;
                     float4_v acc[NT][4] = {};
+                    bool small = small_weights;
                     unrolled<HELD>([&](int s) {
+                        small |= below_split_range(x[s]);
                         if (s >= HELD - SPARE) wave.clear(s, x[s]);
                         Operand<IN> b[4];
                         make_operands<IN, COMPLEX, GRAD>(x[s], b);
@@ -642,7 +674,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                         for (int t = 0; t < NT; ++t) multiply<IN>(weight(s, g * NT + t), b, acc[t]);
                         __builtin_amdgcn_sched_barrier(0);
                     });
-                    finish(g, acc);
+                    finish(g, small, acc);
                 }
             tile += stride;
             if (tile >= tiles) return;
@@ -654,8 +686,10 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
             for (int g = 0; g < groups; ++g) {
                 const Window wf = g < groups - 1 ? w : wn;
                 float4_v acc[NT][4] = {};
+                bool small = small_weights;
                 auto product = [&](int s, typename Wave::Rows& x, typename Wave::Rows& z) {
                     if constexpr (SLOPES) wave.slope(w, s, x, z, writes && g == 0);
+                    if constexpr (IN == kIn32) small |= below_split_range(x);
                     wave.clear(s, x);
                     Operand<IN> b[4];
                     make_operands<IN, COMPLEX, GRAD>(x, b);
@@ -670,7 +704,7 @@ __global__ __launch_bounds__(kResidentThreads, 2) void mix_resident_kernel(const
                     ahead(s + 2 < steps ? w : wf, s + 2 < steps ? s + 2 : 0, x0, z0);
                     if (s + 1 < steps) product(s + 1, x1, z1);
                 }
-                finish(g, acc);
+                finish(g, small, acc);
             }
             w = wn;
         }

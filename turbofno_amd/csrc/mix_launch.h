@@ -143,7 +143,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t laun
         // operands would have to be formed again all the same (complex64, 128 to 128 at 262144: 212 us, held 244; bf16, 256 to 256 at 20000: 17.4 and 20.8)
         const bool held = steps == 1 || (IN != kIn32 && p.groups > 1 && steps <= kMostSteps<IN>);
         if (held) p = plan(true);
-        const size_t lds = p.block_rows / 16 * p.lds16 + p.block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0));
+        const size_t lds = p.block_rows / 16 * p.lds16 + p.block_rows * ((COMPLEX ? 8 : 4) + (IN == kIn8 ? 4 : 0)) + (IN == kIn32 ? 32 : 0);
         if constexpr (SLOPES)
             if (p.groups && (tiles16 + p.nt * p.groups - 1) / (p.nt * p.groups) >= kSlopesApart<IN>) return launch_slopes<IN, OUT, COMPLEX>(q, stream);
         if (p.groups) return launch_steps<IN, OUT, COMPLEX, GRAD, SLOPES>(q, p.nt, held ? held_for(steps) : 0, p.block_rows, lds, stream);

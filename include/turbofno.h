@@ -251,7 +251,7 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *                            from gz as it was rounded.
  *   turbofno_mix_weight_grad gW[n][k] = sum_p gz[n][p] conj(x[k][p]), gbias[n] = sum_p gz[n][p] (may be NULL), in the type of the fields. On truncated
  *                            spectra (turbofno_fft_stride_DY, turbofno_fft2d_trunc) gW is also the gradient of the spectral layer's own weights.
- *                            The sums do not depend on anything but the operands and sizes. Workspace: as queried, 4-byte aligned.
+ *                            32-bit operands as in turbofno_mix. The sums do not depend on anything but the operands and sizes. Workspace: as queried, 4-byte aligned.
  *   turbofno_rms_norm        s = x + residual, rstd[p] = 1 / sqrt(mean over k of |s[k][p]|^2 + eps), y[k] = gain[k] rstd s[k]; gain [K] in fp32 for every
  *                            type. residual, s (not needed without residual) and rstd may be NULL. s and y may be x or residual themselves.
  *   turbofno_rms_norm_8bit   the same with y in e4m3 and a scale per position: scale[p] = max over k of |y[k][p]| / 448 (real and imaginary parts; 1

@@ -95,3 +95,76 @@ def test_a_permutation_returns_what_it_was_given(kind, K, P):
     W = torch.eye(K, dtype=dt, device="cuda")[order].contiguous()
     assert torch.equal(tf.mix(x, W), x[order])
     assert torch.equal(tf.mix_input_grad(x[order], W)[0], x)
+
+
+# channels of x and of gz, real columns (complex: half): fewer than a step, one tile of 32 x 32 and more, tiles of 64 x 64, and those with less than a step
+WEIGHT_SIZES = [(5, 3, 20), (40, 70, 1001), (20, 30, 200), (64, 64, 140003), (70, 130, 140000), (4128, 4100, 20)]
+
+
+def weight_gradient(gz, x):
+    """gz x^H in 64 bits, real and imaginary parts apart: what is not finite is as the formula has it"""
+    G, X = wide(gz), wide(x)
+    if not G.is_complex():
+        return G @ X.T
+    return torch.complex(G.real @ X.real.T + G.imag @ X.imag.T, G.imag @ X.real.T - G.real @ X.imag.T)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("K,N,P", WEIGHT_SIZES)
+def test_weight_gradient(kind, K, N, P):
+    dt = TYPES[kind]
+    parts = 2 if dt.is_complex else 1
+    P //= parts
+    gz, x = randn((N, P), dt, 8), randn((K, P), dt, 9)
+    for scale in SCALES if N < 1000 else SCALES[1:2]:
+        for which in (gz, x):
+            kept = which.clone()
+            which[::3] *= scale
+            gW, gbias = tf.mix_weight_grad(gz, x)
+            G, XH = wide(gz), wide(x).mH
+            terms = parts * min(P, 4096)
+            within(gW, weight_gradient(gz, x), product_bound(G, XH, terms) + P * parts * 2.0 ** -149 * 6, "gW %g" % scale)
+            within(gbias, G.sum(1), (terms + 4) * EPS32 * G.abs().sum(1), "gbias %g" % scale)
+            which.copy_(kept)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("K,N,P", WEIGHT_SIZES[:-1])
+def test_weight_gradient_picks_single_values(kind, K, N, P):
+    """x with one 1 per channel: every value of gz by itself, whatever stands beside it"""
+    dt = TYPES[kind]
+    P //= 2 if dt.is_complex else 1
+    gz, where = any_magnitude((N, P), dt, 10), torch.randint(0, P, (K,), generator=torch.Generator().manual_seed(11)).cuda()
+    where[0] = P - 1
+    x = torch.zeros((K, P), dtype=dt, device="cuda")
+    x[torch.arange(K, device="cuda"), where] = 1
+    gW, _ = tf.mix_weight_grad(gz, x)
+    assert torch.equal(gW, gz[:, where])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("K,N,P", WEIGHT_SIZES[:-1])
+def test_weight_gradient_not_finite_and_at_the_top(kind, K, N, P):
+    """infinities and NaN reach the sums that they take part in, the largest floats are numbers"""
+    dt = TYPES[kind]
+    P //= 2 if dt.is_complex else 1
+    gz, x = randn((N, P), dt, 12), randn((K, P), dt, 13)
+    top = torch.finfo(torch.float32).max
+    real = lambda t: torch.view_as_real(t)[..., 0] if t.is_complex() else t  # noqa: E731
+    real(gz)[0, P - 1] = float("inf")
+    real(x)[1, 0] = float("-inf")
+    real(x)[2, P // 2] = float("nan")
+    x[:, P // 3] *= 0.125
+    real(gz)[1, P // 3] = top
+    gW, _ = tf.mix_weight_grad(gz, x)
+    want, got = weight_gradient(gz, x), wide(gW)
+    as_parts = lambda t: torch.view_as_real(t) if t.is_complex() else t  # noqa: E731
+    want, got = as_parts(want), as_parts(got)
+    beyond = want.abs() > top
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    finite = torch.isfinite(want) & ~beyond
+    G, X = wide(gz).nan_to_num(0, 0, 0), wide(x).nan_to_num(0, 0, 0)
+    bound = product_bound(G, X.mH, (2 if dt.is_complex else 1) * min(P, 4096))
+    bound = bound[..., None] if dt.is_complex else bound
+    assert ((got - want).abs() <= bound.expand_as(want))[finite].all() and finite.sum() > 0.5 * finite.numel() * (K - 2) / K * (N - 1) / N
+    assert not beyond[torch.isfinite(want)].any()

@@ -12,7 +12,8 @@
 // same order: results do not change from call to call.
 // Bound by the issue of one wave per SIMD in complex64, whose sums take half of its 512 registers (64 x 64 channels, 2^20 positions: 295 - 330 us, 3.3 - 3.6 TB/s;
 // matrix cores busy 32 % of the time, vector instructions 32 %, waits for memory 5 %), by loads on their way in the others (float32 152 us, 3.5 TB/s; bf16 90 us, 3.0 TB/s).
-// An infinite operand, or one above the largest bf16 number (3.3895e38), makes the sums it takes part in infinite or NaN.
+// Sums of a wave with operands that the split does not hold (below 2^-110, above the largest bf16 number 3.3895e38, infinite or NaN) are formed again in fp32. Looking
+// for them costs 1 - 2.5 % (complex64, 64 x 64 channels, 2^20 positions: 272.4 us without, 275.7 with; with half of x zeros 269 and 278).
 #include "columns.h"
 #include "kernels.h"
 
@@ -144,6 +145,31 @@ template <int T, int V, int ACC> __device__ __forceinline__ void multiply(const 
         for (int i = 0; i < V; ++i) c[t][first + i] = mfma_bf16(a[t], b[i], c[t][first + i]);
 }
 
+// The same of one row of 16 each with the fp32 matrix instructions, from the values themselves: one position of each quarter of the wave per instruction
+template <int V> __device__ __forceinline__ void multiply_fp32(const Eight<kIn32>& g, const Eight<kIn32>& x, float4_v (&c)[V])
+{
+    auto value = [](const Eight<kIn32>& e, int i) { return i < 4 ? e.lo[i % 4] : e.hi[i % 4]; };
+#pragma unroll
+    for (int j = 0; j < 8; j += V) {
+        c[0] = mfma_fp32(value(g, j), value(x, j), c[0]);
+        if constexpr (V == 2) {
+            c[1] = mfma_fp32(value(g, j + 1), value(x, j), c[1]);
+            c[0] = mfma_fp32(value(g, j + 1), value(x, j + 1), c[0]);
+            c[1] = mfma_fp32(-value(g, j), value(x, j + 1), c[1]);
+        }
+    }
+}
+template <int T> __device__ __forceinline__ bool rows_below_split_range(const Eight<kIn32> (&g)[T], const Eight<kIn32> (&x)[T])
+{
+    float4_v v[4 * T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        v[4 * t] = g[t].lo; v[4 * t + 1] = g[t].hi;
+        v[4 * t + 2] = x[t].lo; v[4 * t + 3] = x[t].hi;
+    }
+    return below_split_range(v);
+}
+
 // SHORT: rows of fewer than a step's values
 template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const GradParams q)
 {
@@ -188,7 +214,9 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
     };
     // operands of gz together, of x one row of 16 after another: all of both would not fit into the registers beside the sums and the rows on their way
     // (complex64, 64 to 64 channels, 2^20 positions: 408 -> 330 us)
+    bool lost = false;                                  // a value was below the range of the split
     auto product = [&](const Rows& r) {
+        if constexpr (IN == kIn32) lost |= rows_below_split_range(r.g, r.x);
         Op a[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -235,7 +263,8 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
     }
     // the rest of the columns: a step that ends with them, less what the one before it has had
     const int rest = (int)(q.columns - steps * kStep);
-    if (rest && steps % stride / 2 * 2 == first) {
+    const bool takes_rest = rest && steps % stride / 2 * 2 == first;
+    if (takes_rest) {
         Rows r;
         if constexpr (SHORT) {
             const int there = rest > LANE * kq ? rest - LANE * kq : 1, back = rest > LANE * kq ? 0 : LANE * kq;
@@ -253,6 +282,47 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
     }
 
     flush();
+    // Infinities and the top of the range leave the split without a value, small numbers lose their low parts there: then all sums of the wave again, in fp32, those
+    // of 16 x 16 channels after those of others, which takes no registers from the loop above
+    if constexpr (IN == kIn32) {
+        float high = 0.f;
+        asm volatile("" ::: "memory");                  // read again: kept in registers, the totals would spill those of the loop
+#pragma unroll 8
+        for (int t = 0; t < ACC; ++t) high = larger(high, total[t * 64]);
+        if (__builtin_expect(lost || any_lane(not_finite(high, 0.f)), 0))
+#pragma unroll 1
+            for (int pair = 0; pair < T * T; ++pair) {
+                const int n = n0 + 16 * (pair / T) + c, k = k0 + 16 * (pair % T) + c;
+                const Value *gn = static_cast<const Value*>(q.g) + (n < q.N ? n : q.N - 1) * q.ldg, *xk = static_cast<const Value*>(q.x) + (k < q.K ? k : q.K - 1) * q.ldx;
+                float4_v part[V] = {}, sum[V] = {};
+                auto add = [&] {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        sum[i] += part[i];
+                        part[i] = float4_v{};
+                    }
+                };
+                int n_steps = 0;
+#pragma unroll 1
+                for (long s = first; s < steps; s = s % 2 ? s - 1 + stride : s + 1) {
+                    multiply_fp32(load8<IN>(gn + s * kStep + LANE * kq), load8<IN>(xk + s * kStep + LANE * kq), part);
+                    if (++n_steps % kRun == 0) add();
+                }
+                if (takes_rest) {                       // value by value: those that the lane has of the last columns
+                    auto last = [&](const Value* row) {
+                        auto at = [&](int i) {
+                            const long column = steps * kStep + LANE * kq + place<IN>(i);
+                            return column < q.columns ? row[column] : 0.f;
+                        };
+                        return Eight<IN>{ { at(0), at(1), at(2), at(3) }, { at(4), at(5), at(6), at(7) } };
+                    };
+                    multiply_fp32(last(gn), last(xk), part);
+                }
+                add();
+#pragma unroll
+                for (int i = 0; i < V; ++i) total[(pair * V + i) * 64] = sum[i];
+            }
+    }
     __syncthreads();
     // to the workspace; the sums of all positions to the results
     const long weights = (long)q.N * q.K * V;

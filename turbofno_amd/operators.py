@@ -186,7 +186,7 @@ def mix_8bit(xq, xscale, Wq, wscale, bias=None, residual=None, activation="none"
     """mix from 8-bit operands: x = xscale[position] xq, W = wscale[n] Wq, all of float8_e4m3fn with float32 scales; xq and xscale as
     rms_norm_8bit gives them. The result has the type of `y`, `residual` or `dtype`, whichever is there (bfloat16 if none is). Complex
     operands are (re, im) pairs along a last dimension of two: xq[K][...][2], Wq[N][K][2]."""
-    if getattr(y, "is_cuda", False) and _compiled("mix_8bit", ("mix_8bit",), xq, xscale, Wq, wscale, bias, residual, _ACTIVATIONS.get(activation, -1), y):
+    if getattr(y, "is_cuda", False) and dtype in (None, y.dtype) and _compiled("mix_8bit", ("mix_8bit",), xq, xscale, Wq, wscale, bias, residual, _ACTIVATIONS.get(activation, -1), y):
         return y
     if dtype is None:
         dtype = next((t.dtype for t in (y, residual) if isinstance(t, torch.Tensor)), torch.bfloat16)

@@ -243,15 +243,17 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *
  *   turbofno_mix             z = W x + bias + residual, y = act(z): x[K][P] -> y[N][P]. bias [N], residual [N][P] and z [N][P] may be NULL; z is the
  *                            pre-activation that the gradient needs. residual may be y or z itself. 32-bit products are formed as those of the
- *                            layer: fp32 over the whole range of floats, infinities and NaN included (see "Precision").
+ *                            layer: fp32 over the whole range of floats, infinities and NaN included (see "Precision"; with such operands a part of the
+ *                            product takes three to six times as long).
  *   turbofno_mix_8bit        the same from 8-bit operands (e4m3, complex values as (re, im) pairs): x = xscale[p] xq[k][p], W = wscale[n] Wq[n][k];
  *                            type is that of bias, residual and y, ldx counts elements (pairs where they are complex).
  *   turbofno_mix_input_grad  gz = gy act'(z) (re and im apart), gx[k] = sum_n conj(W[n][k]) gz[n]. gz is the gradient of residual, and what
  *                            turbofno_mix_weight_grad takes. With TURBOFNO_ACT_NONE gz is gy: z and gz are not used and may be NULL. For bf16, gx is formed
- *                            from gz as it was rounded.
+ *                            from gz as it was rounded, and so are gW and gbias of turbofno_mix_weight_grad.
  *   turbofno_mix_weight_grad gW[n][k] = sum_p gz[n][p] conj(x[k][p]), gbias[n] = sum_p gz[n][p] (may be NULL), in the type of the fields. On truncated
  *                            spectra (turbofno_fft_stride_DY, turbofno_fft2d_trunc) gW is also the gradient of the spectral layer's own weights.
- *                            32-bit operands as in turbofno_mix. The sums do not depend on anything but the operands and sizes. Workspace: as queried, 4-byte aligned.
+ *                            32-bit operands as in turbofno_mix. The sums do not depend on anything but the operands and sizes. Workspace: as
+ *                            queried, 4-byte aligned.
  *   turbofno_rms_norm        s = x + residual, rstd[p] = 1 / sqrt(mean over k of |s[k][p]|^2 + eps), y[k] = gain[k] rstd s[k]; gain [K] in fp32 for every
  *                            type. residual, s (not needed without residual) and rstd may be NULL. s and y may be x or residual themselves.
  *   turbofno_rms_norm_8bit   the same with y in e4m3 and a scale per position: scale[p] = max over k of |y[k][p]| / 448 (real and imaginary parts; 1

@@ -7,7 +7,8 @@
 // 64 bits, which costs nothing beside the memory traffic: no overflow, and the same order in every call. The work is cut into units of 4096 values of one tensor that
 // the blocks take turns over; the second kernel walks them backwards, because the last ones read are the ones that the Infinity Cache still holds,
 // and stores past the caches (100 million fp32 values: 232 -> 199 us, 4.0 TB/s of what is read and written once: 68 us for the squares, 5.9 TB/s, and
-// 132 us for reading again and scaling, 6.1 TB/s). Small lists are two launches: 60 tensors of 250000 values 12.7 us, 0.7 of them the check on the host that no two results overlap.
+// 132 us for reading again and scaling, 6.1 TB/s). Small lists are two launches: 60 tensors of 250000 values 12.7 us, 0.7 of them
+// the check on the host that no two results overlap.
 // Where nothing is to be scaled and the results are the gradients themselves, the second kernel writes nothing.
 #include "columns.h"
 #include "kernels.h"

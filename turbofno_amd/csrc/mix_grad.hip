@@ -293,7 +293,8 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
 #pragma unroll 1
             for (int pair = 0; pair < T * T; ++pair) {
                 const int n = n0 + 16 * (pair / T) + c, k = k0 + 16 * (pair % T) + c;
-                const Value *gn = static_cast<const Value*>(q.g) + (n < q.N ? n : q.N - 1) * q.ldg, *xk = static_cast<const Value*>(q.x) + (k < q.K ? k : q.K - 1) * q.ldx;
+                const Value* gn = static_cast<const Value*>(q.g) + (n < q.N ? n : q.N - 1) * q.ldg;
+                const Value* xk = static_cast<const Value*>(q.x) + (k < q.K ? k : q.K - 1) * q.ldx;
                 float4_v part[V] = {}, sum[V] = {};
                 auto add = [&] {
 #pragma unroll

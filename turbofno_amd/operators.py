@@ -4,6 +4,10 @@ clipping.
 Fields are channel outermost like the layer's, x[K][positions...]: any trailing dimensions, contiguous among themselves, with any distance
 between channels (a slice of a larger batch of channels is taken as it is). Types: complex64, float32, bfloat16. Results are
 allocated where they are not passed. Every call is asynchronous on torch's current stream.
+
+Nothing is recorded for autograd, as with the layer: a result is cut off from the graph, also where an operand requires a gradient. The gradients are calls
+of their own (mix_backward, rms_norm_backward, mix_weight_grad), to be made by a training step like examples/fourier_block.py or by the backward of an
+autograd function.
 """
 import ctypes
 
@@ -161,7 +165,8 @@ def _workspace(t, need, device):
 
 def mix(x, W, bias=None, residual=None, activation="none", y=None, z=None):
     """z = W x + bias + residual, y = activation(z): x[K][...], W[N][K] -> y[N][...]. `z`, where passed, receives the pre-activation that
-    mix_backward takes. `residual` may be `y` or `z` itself. Activations: none, relu, silu, gelu_tanh; on real and imaginary parts."""
+    mix_backward takes. `residual` may be `y` or `z` itself. Activations: none, relu, silu, gelu_tanh; on real and imaginary parts. Not recorded for
+    autograd: the gradients are mix_backward's."""
     if y is None and isinstance(x, torch.Tensor) and isinstance(W, torch.Tensor) and x.is_cuda and x.dim() and W.dim():
         y = torch.empty(W.shape[:1] + x.shape[1:], dtype=x.dtype, device=x.device)
     if getattr(y, "is_cuda", False) and _compiled("mix", ("mix",), x, W, bias, residual, _ACTIVATIONS.get(activation, -1), y, z):
@@ -214,7 +219,8 @@ def mix_8bit(xq, xscale, Wq, wscale, bias=None, residual=None, activation="none"
 
 
 def mix_input_grad(gy, W, z=None, activation="none", gz=None, gx=None):
-    """(gx, gz): gz = gy activation'(z), the gradient of the residual, and gx = W^H gz. Without an activation gz is gy itself."""
+    """(gx, gz): gz = gy activation'(z), the gradient of the residual, and gx = W^H gz. Without an activation gz is gy itself. In bfloat16 gx is formed from
+    gz as it is returned, rounded to bfloat16."""
     kind, device, N, P = _input(gy, "gy")
     act = _activation(activation)
     _need(isinstance(W, torch.Tensor) and W.dim() == 2 and W.shape[0] == N and W.shape[1] > 0, "W must be [%d][K], one row per channel of gy", N)
@@ -257,7 +263,7 @@ def mix_weight_grad(gz, x, gW=None, gbias=None, workspace=None):
 
 def mix_backward(gy, x, W, z=None, activation="none", gz=None, gx=None, gW=None, gbias=None, workspace=None):
     """(gx, gW, gbias, gz) from the gradient of y, and the x, W and z of mix; gz is the gradient of its residual. x is read after gx and gz are written:
-    they share no memory with it."""
+    they share no memory with it. In bfloat16 gx, gW and gbias are formed from gz as it is returned, rounded to bfloat16."""
     act = _ACTIVATIONS.get(activation, -1)
     if isinstance(gy, torch.Tensor) and isinstance(x, torch.Tensor) and isinstance(W, torch.Tensor) and gy.is_cuda:
         gz = gy if act == 0 else _result(gz, gy.shape, gy.dtype, gy.device)
@@ -308,7 +314,8 @@ def _norm(x, gain, residual, eps, y, scale, s, rstd, eight):
 
 def rms_norm(x, gain, residual=None, eps=1e-6, y=None, s=None, rstd=None):
     """s = x + residual, rstd = 1 / sqrt(mean over channels of |s|^2 + eps), y = gain rstd s: x[K][...], gain[K] in float32 -> (y, s, rstd).
-    Without a residual s is x itself. `s` and `y` may be `x` or `residual` themselves; rstd has the shape of the positions."""
+    Without a residual s is x itself. `s` and `y` may be `x` or `residual` themselves; rstd has the shape of the positions. Not recorded for autograd: the
+    gradients are rms_norm_backward's."""
     y, rstd, s = _norm(x, gain, residual, eps, y, None, s, rstd, False)
     return y, s, rstd
 

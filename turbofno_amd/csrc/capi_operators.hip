@@ -89,6 +89,7 @@ int check_clip_places(Span* spans, int count, const void* const* grads, void* co
     for (int i = 0; i < count; ++i) {
         if (!sizes[i] || out[i] == grads[i]) continue;
         const Span g = span(grads[i], i);
+        if (g.to <= spans[0].from || g.from >= spans[n - 1].to) continue;       // beside all of them, as a list of its own mostly is
         const Span* o = std::lower_bound(spans, spans + n, g, [](const Span& a, const Span& b) { return a.to <= b.from; });
         if (o < spans + n && o->from < g.to) return fail(TURBOFNO_ERR_INVALID_ARG, "result %d overlaps gradient %d", o->of, i);
     }

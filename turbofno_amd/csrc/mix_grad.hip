@@ -87,17 +87,19 @@ template <int IN> __device__ __forceinline__ void keep(Eight<IN>& e, int from, i
 #pragma unroll
         for (int j = 0; j < 4; ++j) e.v[j] &= (in(2 * j) ? 0xffffu : 0u) | (in(2 * j + 1) ? 0xffff0000u : 0u);
 }
-__device__ __forceinline__ void operand(const Eight<kIn32>& e, SplitOperand& o)
+// sign: 0, or the sign bit where the operand is negated
+__device__ __forceinline__ void operand(const Eight<kIn32>& e, SplitOperand& o, unsigned sign = 0)
 {
-    const float v[8] = { e.lo[0], e.lo[1], e.lo[2], e.lo[3], e.hi[0], e.hi[1], e.hi[2], e.hi[3] };
+    auto value = [&](float v) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) ^ sign); };
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        const float a = j < 2 ? e.lo[2 * j % 4] : e.hi[2 * j % 4], b = j < 2 ? e.lo[2 * j % 4 + 1] : e.hi[2 * j % 4 + 1];
         unsigned h, m, l;
-        split_bf16_pair(v[2 * j], v[2 * j + 1], h, m, l);
+        split_bf16_pair(value(a), value(b), h, m, l);
         o.h[j] = h; o.m[j] = m; o.l[j] = l;
     }
 }
-__device__ __forceinline__ void operand(const Eight<kIn16>& e, uint4_v& o) { o = e.v; }
+__device__ __forceinline__ void operand(const Eight<kIn16>& e, uint4_v& o, unsigned = 0) { o = e.v; }
 __device__ __forceinline__ uint4_v imaginary(uint4_v v)         // (re, im) -> (-im, re)
 {
 #pragma unroll
@@ -214,6 +216,9 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
     };
     // operands of gz together, of x one row of 16 after another: all of both would not fit into the registers beside the sums and the rows on their way
     // (complex64, 64 to 64 channels, 2^20 positions: 408 -> 330 us)
+    // What a matrix instruction drops from a sum that it returns has one sign whatever the sum's own, and adds up over many steps. Every other wave forms the negative of
+    // its sums, so that it cancels: error of the gradient 3.7e-7, 1.7e-6 without (complex64, 2^20 positions), 4.1e-7 and 4.8e-6 (float32, 2^24), 4.4e-7 and 1.35e-5 (2^27)
+    const unsigned sign = IN == kIn32 && (__builtin_amdgcn_readfirstlane(wave) & 1) ? 0x80000000u : 0u;
     bool lost = false;                                  // a value was below the range of the split
     auto product = [&](const Rows& r) {
         if constexpr (IN == kIn32) lost |= rows_below_split_range(r.g, r.x);
@@ -226,13 +231,13 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             Op b[V];
-            operand(r.x[t], b[0]);
+            operand(r.x[t], b[0], sign);
             if constexpr (COMPLEX) b[1] = imaginary(b[0]);
             multiply(a, b, acc, V * t);
         }
     };
     // The sums of kRun steps are added to totals in LDS: each of the six instructions of a step rounds the sum that it adds to, and a sum over a wave's whole
-    // part would be rounded at its full size each time (2^20 positions, complex: error 3.5e-6 of the gradient)
+    // part would be rounded at its full size each time (complex, 2^20 and 2^23 positions: error 7.0e-7 and 1.9e-6 of the gradient, 3.7e-7 and 3.9e-7 with runs)
     float4_v* total = totals + wave * (ACC * 64) + lane;
     int run = 0;
     bool begun = false;
@@ -321,7 +326,7 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
                 }
                 add();
 #pragma unroll
-                for (int i = 0; i < V; ++i) total[(pair * V + i) * 64] = sum[i];
+                for (int i = 0; i < V; ++i) total[(pair * V + i) * 64] = sign ? -sum[i] : sum[i];
             }
     }
     __syncthreads();
@@ -333,7 +338,8 @@ template <int IN, bool COMPLEX, int T, bool SHORT> __global__ __launch_bounds__(
         else out[at] = sum;
     };
     for (int e = threadIdx.x; e < ACC * 64; e += 256) {
-        const float4_v sum = (totals[e] + totals[ACC * 64 + e]) + (totals[2 * ACC * 64 + e] + totals[3 * ACC * 64 + e]);
+        const float4_v w0 = totals[e], w1 = totals[ACC * 64 + e], w2 = totals[2 * ACC * 64 + e], w3 = totals[3 * ACC * 64 + e];
+        const float4_v sum = IN == kIn32 ? (w0 - w1) + (w2 - w3) : (w0 + w1) + (w2 + w3);
         const int l = e % 64, t = e / 64, n = n0 + 16 * (t / (T * V)) + 4 * (l / 16), k = k0 + 16 * (t % (T * V) / V) + l % 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import turbofno_amd as tf
-from operators_reference import EPS32, TYPES, product_bound, randn, slope, wide, within
+from operators_reference import EPS32, TYPES, product_bound, randn, rounding, slope, wide, within
 
 pytestmark = pytest.mark.gpu
 KINDS = ["f32", "c64"]
@@ -168,3 +168,27 @@ def test_weight_gradient_not_finite_and_at_the_top(kind, K, N, P):
     bound = bound[..., None] if dt.is_complex else bound
     assert ((got - want).abs() <= bound.expand_as(want))[finite].all() and finite.sum() > 0.5 * finite.numel() * (K - 2) / K * (N - 1) / N
     assert not beyond[torch.isfinite(want)].any()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,N,P", [(40, 20, 100), (100, 72, 140003)])
+def test_8bit_scales_of_any_size(kind, K, N, P):
+    """scales of positions down to the smallest normal number, as rms_norm_8bit gives them, and up to 1e30, with scales of weights around 1e-3"""
+    dt = TYPES[kind]
+    pair = (2,) if dt.is_complex else ()
+    P //= 2 if pair else 1
+    xq = (randn((K, P) + pair, torch.float32, 20) * 100).to(torch.float8_e4m3fn)
+    Wq = (randn((N, K) + pair, torch.float32, 21) * 100).to(torch.float8_e4m3fn)
+    ws = 1e-3 * (0.5 + torch.rand(N, generator=torch.Generator().manual_seed(22))).cuda()
+    xs = torch.ones(P, device="cuda")
+    idx, _ = picked(P)
+    xs[idx] = (2.0 ** (torch.rand(len(idx), generator=torch.Generator().manual_seed(23)) * 226 - 126)).cuda()
+    y = tf.mix_8bit(xq, xs, Wq, ws, dtype=dt)
+    X, V = xq[:, idx].cpu().double(), Wq.cpu().double()
+    if pair:
+        X, V = torch.view_as_complex(X.contiguous()), torch.view_as_complex(V)
+    X, V = X * wide(xs[idx]), V * wide(ws)[:, None]
+    Z = V @ X
+    bound = product_bound(V, X, K * (2 if pair else 1)) + 3 * EPS32 * Z.abs()
+    smallest = 2.0 ** -133 if dt == torch.bfloat16 else 2.0 ** -149         # of the type, for results that are no normal numbers
+    within(y[:, idx], Z, bound + 1.01 * rounding(dt) * (Z.abs() + bound) + 2 * smallest, "y")

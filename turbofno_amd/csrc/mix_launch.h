@@ -139,7 +139,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, bool SLOPES> hipError_t laun
     if (near && tiles * tiles16 > kFewTiles) {
         Plan p = plan(false);
         // Steps are held where 16- or 8-bit columns are walked more than once (bf16, 72 to 200 channels at 100003 positions: 24.3 us, streamed 27.6; 8 bits, 256
-        // to 256 at 262144: 93 and 110), and a single one. Otherwise they are streamed: the first products do not wait for the last rows, and 32-bit
+        // to 256 at 262144: 81 and 105), and a single one. Otherwise they are streamed: the first products do not wait for the last rows, and 32-bit
         // operands would have to be formed again all the same (complex64, 128 to 128 at 262144: 212 us, held 244; bf16, 256 to 256 at 20000: 17.4 and 20.8)
         const bool held = steps == 1 || (IN != kIn32 && p.groups > 1 && steps <= kMostSteps<IN>);
         if (held) p = plan(true);

@@ -83,3 +83,22 @@ def test_small_positions_without_eps(kind, K, P):
     Y = S * R * wide(gain)[:, None]
     assert ((wide(y) - Y).abs() <= (noise + 1.01 * rounding(dt)) * Y.abs()).all()
     check_8bit(x, gain, eps=0.0, root=3 * 2.0 ** -149 / mean)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,P", [(3, 70), (40, 90), (300, 66), (100, 140003), (200, 70001)])
+def test_gradient_of_small_positions_without_eps(kind, K, P):
+    """rstd up to 1e19, whose cube is no float: the gradient is, wherever it is one"""
+    dt = TYPES[kind]
+    s, gy, gain = randn((K, P), dt, 6), randn((K, P), dt, 7), 1 + 0.2 * randn((K,), torch.float32, 8)
+    for i, size in enumerate((1e-10, 1e-13, 1e-15, 1e-18, 1e-19)):
+        s[:, i] = s[:, i] * size
+        s[:, P - 1 - 2 * i] = s[:, P - 1 - 2 * i] * size
+    rstd = (1 / torch.sqrt((s.to(torch.complex128 if dt.is_complex else torch.float64).abs() ** 2).mean(0))).float()
+    gx, ggain = tf.rms_norm_backward(gy, s, gain, rstd)
+    S, G, g, R = wide(s), wide(gy), wide(gain)[:, None], wide(rstd)
+    along, size = (S.conj() * G).real, S.abs() * G.abs()
+    E = R * g * G - R ** 3 * (g * along).mean(0) * S
+    mags = R * (g * G).abs() + R ** 3 * (g.abs() * size).mean(0) * S.abs()
+    assert ((wide(gx) - E).abs() <= (K + 16) * EPS32 * mags + 1.01 * rounding(dt) * (E.abs() + (K + 16) * EPS32 * mags)).all()
+    assert ((wide(ggain) - (along * R).sum(1)).abs() <= (min(P, 2048) + 16) * EPS32 * (size * R).sum(1)).all()

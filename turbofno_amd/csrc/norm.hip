@@ -238,12 +238,12 @@ __device__ __forceinline__ void norm_grad_strip(const NormGradParams& q, float4_
                 if (FULL || i < lane_there) ggain[r] = __builtin_fmaf(d[i], rstd[i], ggain[r]);
         }
     along = strip.template over_channels<false>(per_position<COMPLEX>(along), shared, sum4);
-    const float4_v shrink = along * rstd * rstd * rstd * (1.f / (float)q.K);
+    const float4_v shrink = along * rstd * rstd * (1.f / (float)q.K);        // times s rstd: the cube of rstd may be infinite
 #pragma unroll
     for (int r = 0; r < HELD; ++r)
         if (strip.has(r)) {
             if constexpr (IN == kIn16) asm volatile("" : "+v"(gy[r]), "+v"(s[r]));       // widened again, not held in twice the registers
-            float4_v v = to_float<IN>(gy[r]) * (rstd * gain(r)) - to_float<IN>(s[r]) * shrink;
+            float4_v v = to_float<IN>(gy[r]) * (rstd * gain(r)) - to_float<IN>(s[r]) * rstd * shrink;
             if (q.gs) v += to_float<IN>(strip.template read<IN, FULL>(q.gs, q.ldgs, column0, there, r));
             strip.template write<IN, FULL>(q.gx, q.ldgx, column0, there, r, from_float<IN>(v));
         }
@@ -285,11 +285,11 @@ __device__ __forceinline__ void norm_grad_long_strip(const NormGradParams& q, fl
     for (int r = 0; r < rounds; ++r)
         if (strip.has(r)) along += value(q.gy, q.ldgy, r) * value(q.s, q.lds, r) * q.gain[strip.channel(r)];
     along = strip.template over_channels<false>(per_position<COMPLEX>(along), shared, sum4);
-    const float4_v shrink = along * rstd * rstd * rstd * (1.f / (float)q.K);
+    const float4_v shrink = along * rstd * rstd * (1.f / (float)q.K);
     for (int r = 0; r < rounds; ++r) {
         if (!strip.has(r)) continue;                    // the lanes of a group together
         const float4_v gy = value(q.gy, q.ldgy, r), s = value(q.s, q.lds, r);
-        float4_v v = gy * (rstd * q.gain[strip.channel(r)]) - s * shrink;
+        float4_v v = gy * (rstd * q.gain[strip.channel(r)]) - s * rstd * shrink;
         if (q.gs) v += value(q.gs, q.ldgs, r);
         strip.template write<IN, FULL>(q.gx, q.ldgx, column0, there, r, from_float<IN>(v));
         const float4_v d = gy * s;

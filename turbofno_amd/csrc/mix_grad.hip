@@ -10,8 +10,8 @@
 // real values side by side, then those as many steps further as all blocks take together. So the blocks move through the rows as one window: with a contiguous part for each
 // block they all would stand at the same offset of their parts, on the same few memory channels. The blocks' sums go to the workspace and are added in a second kernel, always in the
 // same order: results do not change from call to call.
-// Bound by the issue of one wave per SIMD in complex64, whose sums take half of its 512 registers (64 x 64 channels, 2^20 positions: 295 - 330 us, 3.3 - 3.6 TB/s;
-// matrix cores busy 32 % of the time, vector instructions 32 %, waits for memory 5 %), by loads on their way in the others (float32 152 us, 3.5 TB/s; bf16 90 us, 3.0 TB/s).
+// Bound by the issue of one wave per SIMD in complex64, whose sums take half of its 512 registers (64 x 64 channels, 2^20 positions: 275 - 330 us, 3.3 - 3.9 TB/s;
+// matrix cores busy 32 % of the time, vector instructions 32 %, waits for memory 5 %), by loads on their way in the others (float32 139 - 154 us, 3.5 - 3.9 TB/s; bf16 75 - 90 us, 3.0 - 3.6 TB/s).
 // Sums of a wave with operands that the split does not hold (below 2^-110, above the largest bf16 number 3.3895e38, infinite or NaN) are formed again in fp32. Looking
 // for them costs 1 - 2.5 % (complex64, 64 x 64 channels, 2^20 positions: 272.4 us without, 275.7 with; with half of x zeros 269 and 278).
 #include "columns.h"

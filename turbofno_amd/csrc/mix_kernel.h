@@ -543,8 +543,8 @@ template <int IN> __global__ __launch_bounds__(256) void slope_kernel(const MixP
 // its waves walk the columns without meeting again: no barrier, and 16 NT rows of sums in registers. HELD = 0: steps of the input are read two ahead, again for
 // every 16 NT rows (out of the L2 cache), the next rows' or columns' first one during the results. HELD > 0: all steps of the input, HELD or up to `SPARE` fewer,
 // stay in registers, in 16 and 8 bits as operands, while the rows are walked.
-// Bound by memory up to about 64 channels (complex64, 64 to 64 with residual, z and gelu at 2^20 positions: 393 - 425 us, 5.1 - 5.5 TB/s, the rate of a
-// copy); then by the matrix cores, six products for one in 32 bits (complex64, 256 to 256 with residual at 65536: 203 us, 1.0 PFLOP/s of bf16 products), and by the vector
+// Bound by memory up to about 64 channels (complex64, 64 to 64 with residual, z and gelu at 2^20 positions: 404 - 427 us, 5.0 - 5.3 TB/s, the rate of a
+// copy); then by the matrix cores, six products for one in 32 bits (complex64, 256 to 256 with residual at 65536: 206 us, 1.0 PFLOP/s of bf16 products), and by the vector
 // instructions that form operands and activations (8 bits, 256 to 256 at 262144: 86 us, 3.9 TB/s and 0.40 PFLOP/s).
 constexpr int kWaveParts(int in) { return in == kIn32 ? 3 : 1; }
 constexpr int kResidentThreads = 512;

@@ -192,3 +192,23 @@ def test_8bit_scales_of_any_size(kind, K, N, P):
     bound = product_bound(V, X, K * (2 if pair else 1)) + 3 * EPS32 * Z.abs()
     smallest = 2.0 ** -133 if dt == torch.bfloat16 else 2.0 ** -149         # of the type, for results that are no normal numbers
     within(y[:, idx], Z, bound + 1.01 * rounding(dt) * (Z.abs() + bound) + 2 * smallest, "y")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("K,N,P", SIZES[2:])
+def test_small_values_beside_a_nan(kind, K, N, P):
+    """a column that is not a number, or infinite, beside one below the range of the split, which keeps fp32 precision, as the ordinary ones beside them do"""
+    dt, (K, P) = TYPES[kind], sized(kind, K, P)
+    x, W = randn((K, P), dt, 30), randn((N, K), dt, 31, K ** -0.5)
+    idx, _ = picked(P)
+    x[:, idx[0::4]] *= 1e-35
+    x[:, idx[1::8]] = float("nan")
+    x[:, idx[5::8]] = float("inf")
+    rest = torch.tensor([i for i in range(len(idx)) if i % 4 != 1], device="cuda")
+    terms = K * (2 if dt.is_complex else 1)
+    for got in (tf.mix(x, W), tf.mix_input_grad(x, W.mH.contiguous())[0]):
+        got = got[:, idx]
+        X, V = wide(x[:, idx[rest]]), wide(W)
+        within(got[:, rest], V @ X, product_bound(V, X, terms) + tiny(terms, V), "beside")
+        touched = got[:, 1::8]
+        assert torch.isnan(torch.view_as_real(touched.contiguous())).any(-1).all() if dt.is_complex else torch.isnan(touched).all()

@@ -319,6 +319,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR, bool RAGGE
 #pragma unroll
             for (int b = 0; b < 4; ++b) high = larger(high, acc[t][b]);
         if (__builtin_expect(!small && !any_lane(not_finite(high, 0.f)), 1)) return;
+        unsigned low = ~0u;                             // small numbers again: a NaN among the values of a lane hides them from a minimum
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int row = row0 + 16 * t + c < q.rows ? row0 + 16 * t + c : q.rows - 1;
@@ -339,12 +340,14 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR, bool RAGGE
                     v = zero4<kIn32>();
                     re = im = 0.f;
                 }
+                low = lower(lower(lower(low, float2{ v[0], v[1] }), float2{ v[2], v[3] }), float2{ re, im });
 #pragma unroll
                 for (int b = 0; b < 4; ++b) sum[b] = mfma_fp32(re, v[b], sum[b]);
                 if constexpr (COMPLEX)
 #pragma unroll
                     for (int b = 0; b < 4; ++b) sum[b] = mfma_fp32(b & 1 ? im : -im, v[b ^ 1], sum[b]);
             }
+            small = small || any_lane(low < kSplitLow);
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll

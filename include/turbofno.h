@@ -266,6 +266,28 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *                            that the results overlap neither one another nor a gradient (a tensor that is in the list twice would be scaled twice). The
  *                            sum is formed in 64 bits. An infinite or NaN value makes norm the same, and every result follows the formula.
  *                            Workspace: as queried, 8-byte aligned.
+ *
+ * Training with dropout and a layer norm, and 8 bits with a scale for each block of 128 channels (the last block may hold fewer):
+ *
+ *   turbofno_dropout         y = residual + dropout(x) (residual may be NULL): dropout(x) is x / (1 - drop) where the element is kept and 0 elsewhere, whatever x
+ *                            is there; 0 <= drop < 1. No mask is stored: the element of channel k at position p is kept where word p % 4 of
+ *                            Philox 4x32-10 (Salmon, Moraes, Dror, Shaw 2011) with key = seed and counter = (low 32 bits of p / 4, k + 2^16 (p / 4 >> 32),
+ *                            offset) is at least the whole number nearest to drop 2^32; a complex element is kept or dropped as a whole. `rng`: two 64-bit
+ *                            numbers on the GPU, seed and offset, which are read when the kernel runs, so that a captured graph takes what stands there at
+ *                            each replay. Each use in a model and each step takes an offset (or a seed) of its own. The gradient of x is the same call on the
+ *                            gradient of y, with the same rng, that of residual is the gradient of y. y may be x or residual itself.
+ *   turbofno_layer_norm      s = residual + dropout(x), mean[p] = mean over k of s[k][p], rstd[p] = 1 / sqrt(mean over k of |s - mean|^2 + eps),
+ *                            y[k] = gain[k] rstd (s[k] - mean) + bias[k]. gain [K] in fp32, bias [K] and mean [P] in fp32 or, for complex fields, complex64.
+ *                            residual, bias, s, mean and rstd may be NULL; so may rng where drop = 0. s and y may be x or residual themselves.
+ *   turbofno_layer_norm_8bit the same without dropout and with y in e4m3, as turbofno_quantise_8bit writes it.
+ *   turbofno_layer_norm_backward  gr = gradient of s and of residual: that of y through the norm, plus gs (what reaches s by the residual stream; may be
+ *                            NULL); gx = dropout(gr), the gradient of x, with the drop and rng of turbofno_layer_norm. Without dropout gx is gr itself, and gr is
+ *                            not used and may be NULL. ggain [K], gbias [K] (in the type of bias; may be NULL). gx and gr may be gy, s or gs themselves, but do
+ *                            not overlap. The sums do not depend on anything but the operands and sizes. Workspace: as queried, 4-byte aligned.
+ *   turbofno_quantise_8bit   scale[b][p] = max over the channels k of block b of |x[k][p]| / 448 (real and imaginary parts; 1 where that is below 2^-126, and
+ *                            all q of the block are zeros then; NaN where an x of it is infinite or NaN), q = x / scale in e4m3: scale [ceil(K / 128)][P].
+ *   turbofno_mix_8bit_blocks turbofno_mix_8bit with x = xscale[k / 128][p] xq[k][p] and W = wscale[n / 128][k / 128] Wq[n][k]: xscale [ceil(K / 128)][P],
+ *                            wscale [ceil(N / 128)][ceil(K / 128)].
  */
 #define TURBOFNO_C64  0
 #define TURBOFNO_F32  1
@@ -296,6 +318,20 @@ int turbofno_rms_norm_backward(int type, long P, int K, const void* gy, long ldg
 size_t turbofno_clip_grad_norm_workspace_bytes(int count);
 int turbofno_clip_grad_norm(int count, const void* const* grads, void* const* out, const long* sizes, const int* types, float max_norm,
                             float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+int turbofno_dropout(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, double drop, const void* rng, void* y, long ldy,
+                     void* stream);
+int turbofno_layer_norm(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, const void* bias, float eps,
+                        double drop, const void* rng, void* s, long lds, void* y, long ldy, void* mean, float* rstd, void* stream);
+int turbofno_layer_norm_8bit(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, const void* bias, float eps,
+                             void* s, long lds, void* q, long ldq, float* scale, void* stream);
+size_t turbofno_layer_norm_backward_workspace_bytes(int type, long P, int K);
+int turbofno_layer_norm_backward(int type, long P, int K, const void* gy, long ldgy, const void* s, long lds, const float* gain, const void* mean,
+                                 const float* rstd, const void* gs, long ldgs, double drop, const void* rng, void* gr, long ldgr, void* gx, long ldgx,
+                                 float* ggain, void* gbias, void* workspace, size_t workspace_bytes, void* stream);
+int turbofno_quantise_8bit(int type, long P, int K, const void* x, long ldx, void* q, long ldq, float* scale, void* stream);
+int turbofno_mix_8bit_blocks(int type, long P, int N, int K, const void* xq, long ldx, const float* xscale, const void* Wq, const float* wscale,
+                             const void* bias, const void* residual, long ldr, int act, void* y, long ldy, void* stream);
 
 /* Explanation of the last non-zero return value on this thread ("" if none). Never NULL. */
 const char* turbofno_last_error_string(void);

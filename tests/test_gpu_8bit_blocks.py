@@ -1,0 +1,176 @@
+"""Fields in 8 bits with a scale for each position and block of 128 channels, and products of them, against 64-bit evaluations."""
+import pytest
+import torch
+
+import turbofno_amd as tf
+from layer_norm_reference import Product, check_eight, per_channel, quantised_weights, rounded, wide, within
+from operators_reference import EPS32, TYPES, act, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def field(kind, K, places, seed, spread=True):
+    dt = TYPES[kind]
+    x = randn((K,) + places, torch.complex64 if dt.is_complex else torch.float32, seed)
+    if spread:
+        x = x * torch.exp(0.7 * randn((K,) + (1,) * len(places), torch.float32, seed + 1))
+    return x.to(dt)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,places", [(1, (1,)), (4, (3,)), (127, (65,)), (128, (256,)), (129, (7, 19)), (300, (257,)), (1000, (33,)), (20, (70001,)), (260, (66000,))])
+def test_quantise(kind, K, places):
+    x = field(kind, K, places, 1)
+    q, scale = tf.quantise_8bit(x)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape + ((2,) if x.is_complex() else ()) and scale.shape == (-(-K // 128),) + places
+    X = wide(x).flatten(1)
+    check_eight(q, scale, X, torch.zeros(X.shape, dtype=torch.float64, device=X.device), "quantise_8bit")
+    # the nearest of the type's numbers, except where the factor's rounding may tip a tie
+    parts = torch.view_as_real(X) if X.is_complex() else X[..., None]
+    near = (parts / per_channel(scale.double().flatten(1), K)[..., None]).clamp(-448, 448).float().to(torch.float8_e4m3fn).double()
+    assert (near != q.double().reshape(near.shape)).double().mean() <= 1e-3 or near.numel() < 2000
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_quantise_ends(kind):
+    dt = TYPES[kind]
+    x = torch.zeros((200, 70), dtype=dt, device="cuda")
+    x[7, 1], x[150, 1] = -3.0, 1e-3
+    x[:, 2] = 1e-38
+    x[5, 3], x[140, 3] = float("nan"), 1.0
+    x[6, 65], x[7, 65] = float("inf"), 1.0
+    q, scale = tf.quantise_8bit(x)
+    v = q.float().reshape(200, 70, -1)
+    assert (scale[:, 0] == 1).all() and (v[:, 0] == 0).all()
+    assert v[7, 1, 0] == -448 and v[150, 1, 0] == 448 and (v[:7, 1] == 0).all() and (v[151:, 1] == 0).all()
+    assert (scale[:, 2] == 1).all() and (v[:, 2] == 0).all()
+    assert torch.isnan(scale[0, [3, 65]]).all() and torch.isnan(v[:128, [3, 65]]).all()
+    assert scale[1, 3] == torch.tensor(1.0) / 448 and scale[1, 65] == 1 and v[140, 3, 0] == 448       # the other block is its own
+    wide_x, bytes_ = torch.full((200, 79), 7.0, dtype=dt, device="cuda"), torch.zeros((200, 76) + v.shape[2:] if dt.is_complex else (200, 76), dtype=torch.float8_e4m3fn, device="cuda")
+    for shift in range(1, 5):
+        wide_x[:, shift:shift + 70] = x
+        tf.quantise_8bit(wide_x[:, shift:shift + 70], q=bytes_[:, shift:shift + 70])
+        raw = bytes_.view(torch.uint8)
+        assert torch.equal(raw[:, shift:shift + 70], q.view(torch.uint8)) and (raw[:, :shift] == 0).all() and (raw[:, shift + 70:] == 0).all()
+        bytes_.view(torch.uint8).zero_()
+        wide_x.fill_(7.0)
+    assert tf.quantise_8bit(x[:, :0])[1].shape == (2, 0)
+
+
+def product_operands(kind, K, N, places, seed=0, residual=True, bias=True):
+    dt, pair = TYPES[kind], (2,) if TYPES[kind].is_complex else ()
+    xq, xscale = tf.quantise_8bit(field(kind, K, places, seed))
+    Wq, wscale = quantised_weights(randn((N, K) + pair, torch.float32, seed + 3, K ** -0.5))
+    return xq, xscale, Wq, wscale, randn((N,), dt, seed + 4) if bias else None, randn((N,) + places, dt, seed + 5) if residual else None
+
+
+def check_product(kind, operands, activation, got):
+    """K + 12 roundings of sums of magnitudes, as products in 32 bits are allowed; the activation's slope is at most 1.13"""
+    E = Product(*operands)
+    terms = operands[0].shape[0] * (2 if TYPES[kind].is_complex else 1)
+    bound = (terms + 12) * EPS32 * E.sizes + 4 * EPS32 * E.more
+    if TYPES[kind] == torch.bfloat16:
+        bound = bound + SUMS_8BIT * E.sizes
+    bound = 1.13 * bound + (2.0 ** -20 * E.z.abs() if activation != "none" else 0)
+    Y = act(activation, E.z)
+    within(got.flatten(1), Y, rounded(Y, bound, TYPES[kind]), "y")
+
+
+# what the matrix instructions for 8-bit operands may drop from a sum, of the sum of its terms' magnitudes; used where the result is bf16 only (half a step 2^-8)
+SUMS_8BIT = 2.0 ** -13
+
+SHAPES = [(1, 1, (1,)), (3, 5, (7,)), (16, 16, (64,)), (40, 33, (65,)), (127, 17, (130,)), (128, 128, (256,)), (129, 130, (3, 43)), (200, 136, (301,)), (256, 64, (1000,)),
+          (300, 260, (16,)), (520, 200, (1,)), (1100, 70, (4,)), (64, 700, (200,)), (384, 256, (2049,)), (513, 1025, (515,))]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,N,places", SHAPES)
+def test_product(kind, K, N, places):
+    operands = product_operands(kind, K, N, places)
+    y = tf.mix_8bit_blocks(*operands, activation="gelu_tanh", dtype=TYPES[kind])
+    assert y.shape == (N,) + places and y.dtype == TYPES[kind]
+    check_product(kind, operands, "gelu_tanh", y)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,N,P", [(140, 90, 77), (260, 300, 5000), (60, 20, 3), (1300, 150, 40)])
+def test_product_epilogues_and_places(kind, K, N, P):
+    """with and without bias and residual, every activation; the residual replaced; rows that start anywhere and neighbours that stay"""
+    dt = TYPES[kind]
+    for activation in ("none", "relu", "silu", "gelu_tanh"):
+        for residual, bias in ((True, False), (False, True), (False, False)):
+            operands = product_operands(kind, K, N, (P,), 10, residual, bias)
+            check_product(kind, operands, activation, tf.mix_8bit_blocks(*operands, activation=activation, dtype=dt))
+    operands = product_operands(kind, K, N, (P,), 20)
+    y = tf.mix_8bit_blocks(*operands, activation="silu")
+    place = operands[5].clone()
+    assert tf.mix_8bit_blocks(*operands[:5], residual=place, activation="silu", y=place) is place and torch.equal(place, y)
+    xq, pair = operands[0], (2,) if dt.is_complex else ()
+    for shift in range(1, 5):
+        apart = torch.full((K, P + 7) + pair, 448.0, device="cuda").to(torch.float8_e4m3fn)
+        apart[:, shift:shift + P] = xq
+        out = torch.full((N, P + 9), 7.0, dtype=dt, device="cuda")
+        rows = torch.full((N, P + 5), 7.0, dtype=dt, device="cuda")
+        rows[:, 2:2 + P] = operands[5]
+        tf.mix_8bit_blocks(apart[:, shift:shift + P], *operands[1:5], residual=rows[:, 2:2 + P], activation="silu", y=out[:, shift:shift + P])
+        assert torch.equal(out[:, shift:shift + P], y) and (out[:, :shift] == 7).all() and (out[:, shift + P:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,N,P", [(200, 40, 70), (200, 200, 6000), (300, 260, 9)])
+def test_product_ends(kind, K, N, P):
+    """NaN operands stay in their position or row; scales whose product is no normal number; no positions"""
+    dt = TYPES[kind]
+    xq, xscale, Wq, wscale, _, _ = product_operands(kind, K, N, (P,), 30)
+    y = tf.mix_8bit_blocks(xq, xscale, Wq, wscale, dtype=dt)
+    bad = xq.clone()
+    bad.view(torch.uint8)[K - 1, P - 1] = 0x7F
+    z = tf.mix_8bit_blocks(bad, xscale, Wq, wscale, dtype=dt)
+    is_nan = torch.isnan(torch.view_as_real(z).sum(-1) if dt.is_complex else z)
+    assert is_nan[:, P - 1].all() and not is_nan[:, :P - 1].any() and torch.equal(z[:, :P - 1], y[:, :P - 1])
+    bad = Wq.clone()
+    bad.view(torch.uint8)[N - 1, 0] = 0xFF
+    z = tf.mix_8bit_blocks(xq, xscale, bad, wscale, dtype=dt)
+    is_nan = torch.isnan(torch.view_as_real(z).sum(-1) if dt.is_complex else z)
+    assert is_nan[N - 1].all() and not is_nan[:N - 1].any()
+    small_x, small_w = xscale * 2.0 ** -70, wscale * 2.0 ** -70
+    z = tf.mix_8bit_blocks(xq, small_x, Wq, small_w, dtype=torch.complex64 if dt.is_complex else torch.float32)
+    E = Product(xq, small_x, Wq, small_w)
+    off = (K * 2 + 12) * EPS32 * E.sizes + 2.0 ** -148
+    within(z, E.z, off, "small scales")
+    z = tf.mix_8bit_blocks(xq, xscale * 2.0 ** -60, Wq, wscale * 2.0 ** 60, dtype=dt)
+    assert torch.equal(z, y)
+    assert tf.mix_8bit_blocks(xq[:, :0], xscale[:, :0].contiguous(), Wq, wscale, dtype=dt).shape == (N, 0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_norm_product_and_quantise_together(kind):
+    """serving a feed-forward part: norm into 8 bits, wide product with activation, its result into 8 bits, product back onto the residual stream; then in a graph"""
+    dt, K, H, P = TYPES[kind], 192, 520, 333
+    pair = (2,) if dt.is_complex else ()
+    wide_type = torch.complex64 if dt.is_complex else torch.float32
+    x, r = randn((K, P), dt, 1), randn((K, P), dt, 2)
+    gain, bias = 1 + 0.1 * randn((K,), torch.float32, 3), 0.1 * randn((K,), wide_type, 4)
+    W1, s1 = quantised_weights(randn((H, K) + pair, torch.float32, 5, K ** -0.5))
+    W2, s2 = quantised_weights(randn((K, H) + pair, torch.float32, 6, H ** -0.5))
+    b1, b2 = randn((H,), dt, 7), randn((K,), dt, 8)
+
+    def serve(x, r):
+        q, scale, s = tf.layer_norm_8bit(x, gain, bias, r)
+        v = tf.mix_8bit_blocks(q, scale, W1, s1, bias=b1, activation="gelu_tanh", dtype=dt)
+        vq, vs = tf.quantise_8bit(v)
+        return tf.mix_8bit_blocks(vq, vs, W2, s2, bias=b2, residual=s), (q, scale, s, v, vq, vs)
+    y, (q, scale, s, v, vq, vs) = serve(x, r)
+    check_product(kind, (q, scale, W1, s1, b1, None), "gelu_tanh", v)
+    check_product(kind, (vq, vs, W2, s2, b2, s), "none", y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, _ = serve(x, r)
+    for i in range(3):
+        x.copy_(randn((K, P), dt, 20 + i))
+        want, _ = serve(x, r)
+        torch.cuda.synchronize()
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want), i

@@ -34,12 +34,19 @@ from .api import (  # noqa: F401
 )
 from .operators import (  # noqa: F401
     clip_grad_norm,
+    dropout,
+    layer_norm,
+    layer_norm_8bit,
+    layer_norm_backward,
+    layer_norm_backward_workspace_bytes,
     mix,
     mix_8bit,
+    mix_8bit_blocks,
     mix_backward,
     mix_input_grad,
     mix_weight_grad,
     mix_weight_grad_workspace_bytes,
+    quantise_8bit,
     rms_norm,
     rms_norm_8bit,
     rms_norm_backward,

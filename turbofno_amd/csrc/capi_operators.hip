@@ -4,6 +4,7 @@
 #include "mix_kernel.h"
 #include "places.h"
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <memory>
 #include <new>
@@ -284,6 +285,156 @@ int turbofno_clip_grad_norm(int count, const void* const* grads, void* const* ou
     CHECK(check_clip_places(count > 128 ? many.get() : few, count, grads, out, sizes, types, at_norm, at_workspace));
     if (!workspace || workspace_bytes < need) return fail(TURBOFNO_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, need);
     return hip_status(tfno::launch_clip(count, grads, out, sizes, types, max_norm, norm, workspace, (hipStream_t)stream), "clip_grad_norm launch");
+}
+
+// ---- layer norm, dropout, 8 bits with scales by blocks ----
+
+// elements whose word is below the threshold are dropped, the others lifted; without dropout rng is null
+static int drop_of(double drop, const void* rng, tfno::Drop& d)
+{
+    if (!(drop >= 0. && drop < 1.)) return fail(TURBOFNO_ERR_INVALID_ARG, "drop=%g: 0 <= drop < 1 is taken", drop);
+    if (drop > 0.) CHECK(check_there("rng", rng));
+    const double words = std::nearbyint(drop * 4294967296.);
+    d = { drop > 0. ? static_cast<const unsigned*>(rng) : nullptr, words < 4294967295. ? (unsigned)words : 0xffffffffu, (float)(1. / (1. - drop)) };
+    return TURBOFNO_OK;
+}
+constexpr long kRngBytes = 16;
+static long scale_blocks(int channels) { return (channels + tfno::kScaleBlock - 1) / tfno::kScaleBlock; }
+
+static int layer_norm_on(bool eight, int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, const void* bias, float eps,
+                         double drop, const void* rng, void* s, long lds, void* y, long ldy, void* mean, float* rstd, void* stream)
+{
+    CHECK(check_sizes(type, P, 1, K, TURBOFNO_ACT_NONE));
+    CHECK(check_rows("x", x, P, K, ldx));
+    CHECK(check_rows("residual", residual, P, K, ldr, true));
+    CHECK(check_there("gain", gain));
+    CHECK(check_rows("s", s, P, K, lds, true));
+    CHECK(check_rows(eight ? "q" : "y", y, P, K, ldy));
+    if (eight && P) CHECK(check_there("scale", rstd));
+    if (!(eps >= 0.f)) return fail(TURBOFNO_ERR_INVALID_ARG, "eps=%g must not be negative", (double)eps);
+    tfno::Drop d;
+    CHECK(drop_of(drop, rng, d));
+    const int v = tfno::values_of(type);
+    const size_t e = tfno::size_of(type), ey = eight ? (size_t)v : e;
+    auto taken = [&](const void* in, long ldi) {
+        return clash(s, lds, in, ldi, K, e, P) || (eight ? overlap(y, K, ldy, ey, in, K, ldi, e, P) : clash(y, ldy, in, ldi, K, e, P));
+    };
+    if (taken(x, ldx) || taken(residual, ldr)) return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps an operand without being it");
+    if (overlap(y, K, ldy, ey, s, K, lds, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "the results overlap");
+    const Place px = place(x, K, ldx, e, P), pr = place(residual, K, ldr, e, P), ps = place(s, K, lds, e, P), py = place(y, K, ldy, ey, P);
+    const Place pg = packed(gain, 4l * K), pb = packed(bias, 4l * v * K), pd = packed(d.rng, kRngBytes);
+    const Place pm = packed(mean, 4 * P * v), pt = packed(rstd, 4 * P * (eight ? scale_blocks(K) : 1));
+    for (const Place& p : { pg, pb, pd })
+        if (among(p, { ps, py })) return fail(TURBOFNO_ERR_INVALID_ARG, "a result overlaps gain, bias or rng");
+    if (among(pm, { px, pr, ps, py, pg, pb, pd, pt }) || among(pt, { px, pr, ps, py, pg, pb, pd }))
+        return fail(TURBOFNO_ERR_INVALID_ARG, "%s overlaps another operand", eight ? "scale" : "mean or rstd");
+    const tfno::LayerNormParams q = { x, residual, gain, static_cast<const float*>(bias), s, y, static_cast<float*>(mean), rstd, P * v, P, ldx * v, ldr * v, lds * v, ldy * v, K, eps, d };
+    return hip_status(tfno::launch_layer_norm(q, type, eight, (hipStream_t)stream), eight ? "layer_norm_8bit launch" : "layer_norm launch");
+}
+
+int turbofno_layer_norm(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, const void* bias, float eps, double drop,
+                        const void* rng, void* s, long lds, void* y, long ldy, void* mean, float* rstd, void* stream)
+{
+    return layer_norm_on(false, type, P, K, x, ldx, residual, ldr, gain, bias, eps, drop, rng, s, lds, y, ldy, mean, rstd, stream);
+}
+
+int turbofno_layer_norm_8bit(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, const float* gain, const void* bias, float eps, void* s,
+                             long lds, void* q, long ldq, float* scale, void* stream)
+{
+    return layer_norm_on(true, type, P, K, x, ldx, residual, ldr, gain, bias, eps, 0., nullptr, s, lds, q, ldq, nullptr, scale, stream);
+}
+
+size_t turbofno_layer_norm_backward_workspace_bytes(int type, long P, int K)
+{
+    if (check_sizes(type, P, 1, K, TURBOFNO_ACT_NONE)) return 0;
+    return tfno::layer_norm_backward_workspace(type, P, K);
+}
+
+int turbofno_layer_norm_backward(int type, long P, int K, const void* gy, long ldgy, const void* s, long lds, const float* gain, const void* mean, const float* rstd,
+                                 const void* gs, long ldgs, double drop, const void* rng, void* gr, long ldgr, void* gx, long ldgx, float* ggain, void* gbias,
+                                 void* workspace, size_t workspace_bytes, void* stream)
+{
+    CHECK(check_sizes(type, P, 1, K, TURBOFNO_ACT_NONE));
+    CHECK(check_rows("gy", gy, P, K, ldgy));
+    CHECK(check_rows("s", s, P, K, lds));
+    CHECK(check_there("gain", gain));
+    if (P) CHECK(check_there("mean", mean));
+    if (P) CHECK(check_there("rstd", rstd));
+    CHECK(check_rows("gs", gs, P, K, ldgs, true));
+    tfno::Drop d;
+    CHECK(drop_of(drop, rng, d));
+    if (!d.rng) gr = nullptr;                           // gx is it
+    CHECK(check_rows("gr", gr, P, K, ldgr, !d.rng));
+    CHECK(check_rows("gx", gx, P, K, ldgx));
+    CHECK(check_there("ggain", ggain));
+    const int v = tfno::values_of(type);
+    const size_t e = tfno::size_of(type), need = tfno::layer_norm_backward_workspace(type, P, K);
+    auto taken = [&](const void* out, long ldo) { return clash(out, ldo, gy, ldgy, K, e, P) || clash(out, ldo, s, lds, K, e, P) || clash(out, ldo, gs, ldgs, K, e, P); };
+    if (taken(gx, ldgx) || taken(gr, ldgr)) return fail(TURBOFNO_ERR_INVALID_ARG, "gx or gr overlaps an operand without being it");
+    const Place px = place(gx, K, ldgx, e, P), pr = place(gr, K, ldgr, e, P), pw = packed(workspace, (long)need);
+    if (overlap(px, pr)) return fail(TURBOFNO_ERR_INVALID_ARG, "gx and gr overlap");
+    const Place py = place(gy, K, ldgy, e, P), ps = place(s, K, lds, e, P), pgs = place(gs, K, ldgs, e, P), pg = packed(gain, 4l * K), pm = packed(mean, 4 * P * v),
+                pt = packed(rstd, 4 * P), pd = packed(d.rng, kRngBytes), pog = packed(ggain, 4l * K), pob = packed(gbias, 4l * v * K);
+    if (among(px, { pg, pm, pt, pd, pog, pob }) || among(pr, { pg, pm, pt, pd, pog, pob }))
+        return fail(TURBOFNO_ERR_INVALID_ARG, "gx or gr overlaps gain, mean, rstd, rng, ggain or gbias");
+    if (overlap(pog, pob)) return fail(TURBOFNO_ERR_INVALID_ARG, "ggain and gbias overlap");
+    if (among(pw, { py, ps, pgs, px, pr, pg, pm, pt, pd, pog, pob })) return fail(TURBOFNO_ERR_INVALID_ARG, "the workspace overlaps an operand");
+    if (!workspace || workspace_bytes < need) return fail(TURBOFNO_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, need);
+    const tfno::LayerNormGradParams q = { gy, s, gs, gain, static_cast<const float*>(mean), rstd, gr, gx, ggain, static_cast<float*>(gbias), static_cast<float*>(workspace),
+                                          P * v, ldgy * v, lds * v, ldgs * v, ldgr * v, ldgx * v, K, d };
+    return hip_status(tfno::launch_layer_norm_backward(q, type, (hipStream_t)stream), "layer_norm_backward launch");
+}
+
+int turbofno_dropout(int type, long P, int K, const void* x, long ldx, const void* residual, long ldr, double drop, const void* rng, void* y, long ldy, void* stream)
+{
+    CHECK(check_sizes(type, P, 1, K, TURBOFNO_ACT_NONE));
+    CHECK(check_rows("x", x, P, K, ldx));
+    CHECK(check_rows("residual", residual, P, K, ldr, true));
+    CHECK(check_rows("y", y, P, K, ldy));
+    CHECK(check_there("rng", rng));
+    tfno::Drop d;
+    CHECK(drop_of(drop, rng, d));
+    d.rng = static_cast<const unsigned*>(rng);          // drop = 0 keeps all
+    const int v = tfno::values_of(type);
+    const size_t e = tfno::size_of(type);
+    if (clash(y, ldy, x, ldx, K, e, P) || clash(y, ldy, residual, ldr, K, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps an operand without being it");
+    if (overlap(place(y, K, ldy, e, P), packed(rng, kRngBytes))) return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps rng");
+    const tfno::DropoutParams q = { x, residual, y, P * v, ldx * v, ldr * v, ldy * v, K, d };
+    return hip_status(tfno::launch_dropout(q, type, (hipStream_t)stream), "dropout launch");
+}
+
+int turbofno_quantise_8bit(int type, long P, int K, const void* x, long ldx, void* q, long ldq, float* scale, void* stream)
+{
+    CHECK(check_sizes(type, P, 1, K, TURBOFNO_ACT_NONE));
+    CHECK(check_rows("x", x, P, K, ldx));
+    CHECK(check_rows("q", q, P, K, ldq));
+    if (P) CHECK(check_there("scale", scale));
+    const int v = tfno::values_of(type);
+    const Place px = place(x, K, ldx, tfno::size_of(type), P), pq = place(q, K, ldq, v, P), ps = packed(scale, 4 * P * scale_blocks(K));
+    if (overlap(px, pq) || overlap(px, ps) || overlap(pq, ps)) return fail(TURBOFNO_ERR_INVALID_ARG, "x, q and scale overlap");
+    const tfno::QuantiseParams p = { x, q, scale, P * v, P, ldx * v, ldq * v, K };
+    return hip_status(tfno::launch_quantise_8bit(p, type, (hipStream_t)stream), "quantise_8bit launch");
+}
+
+int turbofno_mix_8bit_blocks(int type, long P, int N, int K, const void* xq, long ldx, const float* xscale, const void* Wq, const float* wscale, const void* bias,
+                             const void* residual, long ldr, int act, void* y, long ldy, void* stream)
+{
+    CHECK(check_sizes(type, P, N, K, act));
+    CHECK(check_rows("xq", xq, P, K, ldx));
+    CHECK(check_there("Wq", Wq));
+    CHECK(check_there("wscale", wscale));
+    if (P) CHECK(check_there("xscale", xscale));
+    CHECK(check_rows("residual", residual, P, N, ldr, true));
+    CHECK(check_rows("y", y, P, N, ldy));
+    const int v = tfno::values_of(type);
+    const size_t e = tfno::size_of(type);
+    if (overlap(xq, K, ldx, v, y, N, ldy, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps xq");
+    if (clash(y, ldy, residual, ldr, N, e, P)) return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps residual without being it");
+    if (among(place(y, N, ldy, e, P), { packed(Wq, (long)N * K * v), packed(bias, N * (long)e), packed(xscale, 4 * P * scale_blocks(K)),
+                                        packed(wscale, 4 * scale_blocks(N) * scale_blocks(K)) }))
+        return fail(TURBOFNO_ERR_INVALID_ARG, "y overlaps Wq, bias or a scale");
+    const tfno::MixBlocksParams q = { xq, Wq, bias, residual, xscale, wscale, y, P * v, P, ldx * v, ldr * v, ldy * v, N, K, act };
+    return hip_status(tfno::launch_mix_8bit_blocks(q, type, (hipStream_t)stream), "mix_8bit_blocks launch");
 }
 
 }  // extern "C"

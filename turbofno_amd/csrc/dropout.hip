@@ -1,0 +1,74 @@
+// Dropout with the residual's addition (turbofno_dropout): y = residual + keep x / (1 - drop), the mask from a counter-based generator (philox.h) and never
+// stored; the gradient is the same call on the gradient of y.
+#include "philox.h"
+#include "operators.h"
+
+namespace tfno {
+
+namespace {
+
+// A thread has four real columns of four channels, which lie side by side in the wave's turns; 2^log_lanes threads side by side in a row
+constexpr int kDropRows = 4;
+template <int IN, bool COMPLEX> __global__ __launch_bounds__(256) void dropout_kernel(const DropoutParams q, int log_lanes, long tiles)
+{
+    typedef typename Columns<IN>::Value Value;
+    const long id = block_index(), part = id / tiles;
+    const int lane = threadIdx.x & ((1 << log_lanes) - 1), row0 = (int)part * ((256 >> log_lanes) * kDropRows) + (int)(threadIdx.x >> log_lanes);
+    const long column = ((id - part * tiles) << (log_lanes + 2)) + 4 * lane;
+    const int step = 256 >> log_lanes;
+    if (part * (step * kDropRows) >= q.K) return;
+    const Keep<COMPLEX> keep(q.drop, column);
+    auto row = [&](int u) { const int k = row0 + u * step; return k < q.K ? k : q.K - 1; };
+    const bool whole = column + 4 <= q.columns;
+    RawOf<IN> x[kDropRows], r[kDropRows];
+    if (whole) {
+#pragma unroll
+        for (int u = 0; u < kDropRows; ++u) x[u] = load4<IN>(static_cast<const Value*>(q.x) + row(u) * q.ldx, column);
+        if (q.residual)
+#pragma unroll
+            for (int u = 0; u < kDropRows; ++u) r[u] = load4<IN>(static_cast<const Value*>(q.residual) + row(u) * q.ldr, column);
+    } else if (column < q.columns) {
+#pragma unroll
+        for (int u = 0; u < kDropRows; ++u) {
+            x[u] = load4_ragged<IN>(static_cast<const Value*>(q.x) + row(u) * q.ldx, column, q.columns);
+            if (q.residual) r[u] = load4_ragged<IN>(static_cast<const Value*>(q.residual) + row(u) * q.ldr, column, q.columns);
+        }
+    }
+    unsigned bits[kDropRows];
+#pragma unroll
+    for (int u = 0; u < kDropRows; u += 2) keep.pair(row(u), row(u + 1), bits[u], bits[u + 1]);
+    if (column >= q.columns) return;
+#pragma unroll
+    for (int u = 0; u < kDropRows; ++u) {
+        if (row0 + u * step >= q.K) break;
+        float4_v v = Keep<COMPLEX>::apply(to_float<IN>(x[u]), bits[u], q.drop.lift);
+        if (q.residual) v += to_float<IN>(r[u]);
+        Value* y = static_cast<Value*>(q.y) + row(u) * q.ldy;
+        if (whole) store4<IN>(y, column, from_float<IN>(v));
+        else store4_ragged<IN>(y, column, q.columns, from_float<IN>(v));
+    }
+}
+
+template <int IN, bool COMPLEX> hipError_t launch(const DropoutParams& q, hipStream_t stream)
+{
+    int log_lanes = 2;                                  // threads side by side: rows of few positions share a block
+    while (log_lanes < 8 && (4l << log_lanes) < q.columns) ++log_lanes;
+    const long tiles = (q.columns + (4l << log_lanes) - 1) >> (log_lanes + 2);
+    const int rows = (256 >> log_lanes) * kDropRows;
+    hipLaunchKernelGGL((dropout_kernel<IN, COMPLEX>), grid_of(tiles * ((q.K + rows - 1) / rows)), dim3(256), 0, stream, q, log_lanes, tiles);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_dropout(const DropoutParams& q, int type, hipStream_t stream)
+{
+    if (q.columns == 0) return hipSuccess;
+    switch (type) {
+    case kC64: return launch<kIn32, true>(q, stream);
+    case kF32: return launch<kIn32, false>(q, stream);
+    default: return launch<kIn16, false>(q, stream);
+    }
+}
+
+}  // namespace tfno

@@ -165,6 +165,13 @@ using NormGrad = decltype(&turbofno_rms_norm_backward);
 using NormGradBytes = decltype(&turbofno_rms_norm_backward_workspace_bytes);
 using Clip = decltype(&turbofno_clip_grad_norm);
 using ClipBytes = decltype(&turbofno_clip_grad_norm_workspace_bytes);
+using Dropout = decltype(&turbofno_dropout);
+using LayerNorm = decltype(&turbofno_layer_norm);
+using LayerNorm8bit = decltype(&turbofno_layer_norm_8bit);
+using LayerNormGrad = decltype(&turbofno_layer_norm_backward);
+using LayerNormGradBytes = decltype(&turbofno_layer_norm_backward_workspace_bytes);
+using Quantise = decltype(&turbofno_quantise_8bit);
+using Mix8bitBlocks = decltype(&turbofno_mix_8bit_blocks);
 
 struct NotHere { };                                     // an operand for Python to judge
 
@@ -268,6 +275,33 @@ float real_value(PyObject* o)
     const double v = PyFloat_AsDouble(o);
     if (PyErr_Occurred()) throw NotHere();
     return (float)v;
+}
+double double_value(PyObject* o)
+{
+    const double v = PyFloat_AsDouble(o);
+    if (PyErr_Occurred()) throw NotHere();
+    return v;
+}
+// seed and offset; none without dropout
+const void* seed_and_offset(PyObject* o, int device) { return packed(o, at::kLong, device, { 2 }, true); }
+// the 32-bit type of values that accompany a field
+at::ScalarType wide(at::ScalarType dt) { return dt == at::kComplexFloat ? dt : at::kFloat; }
+// one value per position of `like`, of a type
+void* at_positions(PyObject* o, at::ScalarType type, int device, const at::Tensor& like)
+{
+    const at::Tensor& t = on_gpu(o, type, device);
+    if (!t.is_contiguous() || t.sizes() != like.sizes().slice(1)) throw NotHere();
+    return t.data_ptr();
+}
+// one float per block of 128 channels and position of `like`
+float* block_scales(PyObject* o, int device, int K, const at::Tensor& like, bool like_pairs = false)
+{
+    const at::Tensor& t = on_gpu(o, at::kFloat, device);
+    const int64_t dims = like.dim() - (like_pairs ? 1 : 0);
+    if (!t.is_contiguous() || t.dim() != dims || t.size(0) != (K + 127) / 128) throw NotHere();
+    for (int64_t i = 1; i < dims; ++i)
+        if (t.size(i) != like.size(i)) throw NotHere();
+    return static_cast<float*>(t.data_ptr());
 }
 // the caller's workspace, or memory that is free again, in the order of the stream, when the call returns
 struct Workspace {
@@ -422,6 +456,143 @@ PyObject* rms_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t count)
     });
 }
 
+// dropout(function, x, residual, drop, rng, y, device, stream)
+PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 8, [&] {
+        const auto call = function<Dropout>(args[0]);
+        const int device = small(args[6]);
+        void* stream = stream_of(args[7]);
+        const at::Tensor& x = first_operand(args[1], device);
+        const at::ScalarType dt = x.scalar_type();
+        const int type = type_of(x), K = channels(x.size(0));
+        const Field fx = field(args[1], dt, device, K, x), r = field(args[2], dt, device, K, x, false, false, true), y = field(args[5], dt, device, K, x);
+        const double drop = double_value(args[3]);
+        const void* rng = seed_and_offset(args[4], device);
+        const long P = positions(x);
+        const WithoutLock unlocked;
+        return call(type, P, K, fx.data, fx.ld, r.data, r.ld, drop, rng, y.data, y.ld, stream);
+    });
+}
+
+// layer_norm(function, x, gain, bias, residual, eps, drop, rng, s, y, mean, rstd, device, stream)
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 14, [&] {
+        const auto call = function<LayerNorm>(args[0]);
+        const int device = small(args[12]);
+        void* stream = stream_of(args[13]);
+        const at::Tensor& x = first_operand(args[1], device);
+        const at::ScalarType dt = x.scalar_type();
+        const int type = type_of(x), K = channels(x.size(0));
+        const float* gain = static_cast<float*>(packed(args[2], at::kFloat, device, { K }));
+        const void* bias = packed(args[3], wide(dt), device, { K }, true);
+        const float eps = real_value(args[5]);
+        const double drop = double_value(args[6]);
+        const void* rng = seed_and_offset(args[7], device);
+        const Field fx = field(args[1], dt, device, K, x), r = field(args[4], dt, device, K, x, false, false, true), s = field(args[8], dt, device, K, x, false, false, true);
+        const Field y = field(args[9], dt, device, K, x);
+        void* mean = at_positions(args[10], wide(dt), device, x);
+        float* rstd = static_cast<float*>(at_positions(args[11], at::kFloat, device, x));
+        const long P = positions(x);
+        const WithoutLock unlocked;
+        return call(type, P, K, fx.data, fx.ld, r.data, r.ld, gain, bias, eps, drop, rng, s.data, s.ld, y.data, y.ld, mean, rstd, stream);
+    });
+}
+
+// layer_norm_8bit(function, x, gain, bias, residual, eps, s, q, scale, device, stream)
+PyObject* layer_norm_8bit(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 11, [&] {
+        const auto call = function<LayerNorm8bit>(args[0]);
+        const int device = small(args[9]);
+        void* stream = stream_of(args[10]);
+        const at::Tensor& x = first_operand(args[1], device);
+        const at::ScalarType dt = x.scalar_type();
+        const int type = type_of(x), K = channels(x.size(0));
+        const float* gain = static_cast<float*>(packed(args[2], at::kFloat, device, { K }));
+        const void* bias = packed(args[3], wide(dt), device, { K }, true);
+        const float eps = real_value(args[5]);
+        const Field fx = field(args[1], dt, device, K, x), r = field(args[4], dt, device, K, x, false, false, true), s = field(args[6], dt, device, K, x, false, false, true);
+        const Field q = field(args[7], at::kFloat8_e4m3fn, device, K, x, type == TURBOFNO_C64);
+        float* scale = block_scales(args[8], device, K, x);
+        const long P = positions(x);
+        const WithoutLock unlocked;
+        return call(type, P, K, fx.data, fx.ld, r.data, r.ld, gain, bias, eps, s.data, s.ld, q.data, q.ld, scale, stream);
+    });
+}
+
+// layer_norm_backward(function, workspace_bytes, gy, s, gain, mean, rstd, gs, drop, rng, gx, gr, ggain, gbias, workspace, device, stream); gr: None without dropout
+PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 17, [&] {
+        const auto call = function<LayerNormGrad>(args[0]);
+        const auto bytes = function<LayerNormGradBytes>(args[1]);
+        const int device = small(args[15]);
+        void* stream = stream_of(args[16]);
+        const at::Tensor& gy = first_operand(args[2], device);
+        const at::ScalarType dt = gy.scalar_type();
+        const int type = type_of(gy), K = channels(gy.size(0));
+        const Field g = field(args[2], dt, device, K, gy), s = field(args[3], dt, device, K, gy), gs = field(args[7], dt, device, K, gy, false, false, true);
+        const float* gain = static_cast<float*>(packed(args[4], at::kFloat, device, { K }));
+        const void* mean = at_positions(args[5], wide(dt), device, gy);
+        const float* rstd = static_cast<float*>(at_positions(args[6], at::kFloat, device, gy));
+        const double drop = double_value(args[8]);
+        const void* rng = seed_and_offset(args[9], device);
+        const Field gx = field(args[10], dt, device, K, gy), gr = field(args[11], dt, device, K, gy, false, false, true);
+        float* ggain = static_cast<float*>(packed(args[12], at::kFloat, device, { K }));
+        void* gbias = packed(args[13], wide(dt), device, { K });
+        const long P = positions(gy);
+        const Workspace ws(args[14], bytes(type, P, K), gy, device);
+        const WithoutLock unlocked;
+        return call(type, P, K, g.data, g.ld, s.data, s.ld, gain, mean, rstd, gs.data, gs.ld, drop, rng, gr.data, gr.ld, gx.data, gx.ld, ggain, gbias, ws.data, ws.bytes,
+                    stream);
+    });
+}
+
+// quantise_8bit(function, x, q, scale, device, stream)
+PyObject* quantise_8bit(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 6, [&] {
+        const auto call = function<Quantise>(args[0]);
+        const int device = small(args[4]);
+        void* stream = stream_of(args[5]);
+        const at::Tensor& x = first_operand(args[1], device);
+        const int type = type_of(x), K = channels(x.size(0));
+        const Field fx = field(args[1], x.scalar_type(), device, K, x), q = field(args[2], at::kFloat8_e4m3fn, device, K, x, type == TURBOFNO_C64);
+        float* scale = block_scales(args[3], device, K, x);
+        const long P = positions(x);
+        const WithoutLock unlocked;
+        return call(type, P, K, fx.data, fx.ld, q.data, q.ld, scale, stream);
+    });
+}
+
+// mix_8bit_blocks(function, xq, xscale, Wq, wscale, bias, residual, activation, y, device, stream)
+PyObject* mix_8bit_blocks(PyObject*, PyObject* const* args, Py_ssize_t count)
+{
+    return judged(count == 11, [&] {
+        const auto call = function<Mix8bitBlocks>(args[0]);
+        const int device = small(args[9]), act = small(args[7]);
+        void* stream = stream_of(args[10]);
+        const at::Tensor& x = first_operand(args[1], device);
+        if (x.scalar_type() != at::kFloat8_e4m3fn || !THPVariable_CheckExact(args[8]) || !THPVariable_CheckExact(args[3])) throw NotHere();
+        const at::Tensor& out = THPVariable_Unpack(args[8]);
+        if (THPVariable_Unpack(args[3]).dim() < 2) throw NotHere();
+        const int type = type_of(out), K = channels(x.size(0)), N = channels(THPVariable_Unpack(args[3]).size(0));
+        const bool pairs = type == TURBOFNO_C64;
+        const at::ScalarType dt = out.scalar_type();
+        if (pairs && (x.dim() < 3 || x.size(x.dim() - 1) != 2)) throw NotHere();
+        const void* W = pairs ? packed(args[3], at::kFloat8_e4m3fn, device, { N, K, 2 }) : packed(args[3], at::kFloat8_e4m3fn, device, { N, K });
+        const float *xs = block_scales(args[2], device, K, x, pairs), *ws = static_cast<float*>(packed(args[4], at::kFloat, device, { (N + 127) / 128, (K + 127) / 128 }));
+        const void* bias = packed(args[5], dt, device, { N }, true);
+        const Field r = field(args[6], dt, device, N, x, false, pairs, true), y = field(args[8], dt, device, N, x, false, pairs);
+        const long P = positions(x, pairs), ld = spread(x, pairs ? 2 : 1);
+        const void* xq = x.data_ptr();
+        const WithoutLock unlocked;
+        return call(type, P, N, K, xq, ld, xs, W, ws, bias, r.data, r.ld, act, y.data, y.ld, stream);
+    });
+}
+
 // clip_grad_norm(function, workspace_bytes, list of gradients, list of results, max_norm, norm, workspace, device, stream)
 PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t count)
 {
@@ -466,6 +637,12 @@ PyMethodDef methods[] = {
     TFNO_METHOD(mix_backward, "turbofno_mix_input_grad and turbofno_mix_weight_grad on checked tensors, or -1"),
     TFNO_METHOD(rms_norm, "turbofno_rms_norm or turbofno_rms_norm_8bit on checked tensors, or -1"),
     TFNO_METHOD(rms_norm_backward, "turbofno_rms_norm_backward on checked tensors, or -1"),
+    TFNO_METHOD(dropout, "turbofno_dropout on checked tensors, or -1"),
+    TFNO_METHOD(layer_norm, "turbofno_layer_norm on checked tensors, or -1"),
+    TFNO_METHOD(layer_norm_8bit, "turbofno_layer_norm_8bit on checked tensors, or -1"),
+    TFNO_METHOD(layer_norm_backward, "turbofno_layer_norm_backward on checked tensors, or -1"),
+    TFNO_METHOD(quantise_8bit, "turbofno_quantise_8bit on checked tensors, or -1"),
+    TFNO_METHOD(mix_8bit_blocks, "turbofno_mix_8bit_blocks on checked tensors, or -1"),
     TFNO_METHOD(clip_grad_norm, "turbofno_clip_grad_norm on lists of checked tensors, or -1"),
     { nullptr, nullptr, 0, nullptr },
 };

@@ -53,6 +53,67 @@ struct NormGradParams {
 size_t rms_norm_backward_workspace(int type, long P, int K);
 hipError_t launch_rms_norm_backward(const NormGradParams& q, int type, hipStream_t stream);
 
+// Layer norm over channels, strides in real values. bias: K values, pairs where the fields are complex, or null. 8 bits: y is q, rstd the scales of blocks of 128
+// channels, which are `positions` apart; mean is not used. drop.rng: null without dropout.
+struct Drop {
+    const unsigned* rng;                                // seed and offset, low words first
+    unsigned threshold;                                 // elements whose word is below it are dropped
+    float lift;                                         // 1 / (1 - drop)
+};
+struct LayerNormParams {
+    const void *x, *residual;
+    const float *gain, *bias;
+    void *s, *y;
+    float *mean, *rstd;
+    long columns, positions, ldx, ldr, lds, ldy;
+    int K;
+    float eps;
+    Drop drop;
+};
+hipError_t launch_layer_norm(const LayerNormParams& q, int type, bool eight_bits, hipStream_t stream);
+struct LayerNormGradParams {
+    const void *gy, *s, *gs;
+    const float *gain, *mean, *rstd;
+    void *gr, *gx;                                      // gradients of s and, with dropout, of x; without, gr is null
+    float *ggain, *gbias, *sums;                        // gbias: null, or K values or pairs
+    long columns, ldgy, lds, ldgs, ldgr, ldgx;
+    int K;
+    Drop drop;
+};
+size_t layer_norm_backward_workspace(int type, long P, int K);
+hipError_t launch_layer_norm_backward(const LayerNormGradParams& q, int type, hipStream_t stream);
+
+// y = residual + dropout(x), strides in real values
+struct DropoutParams {
+    const void *x, *residual;
+    void* y;
+    long columns, ldx, ldr, ldy;
+    int K;
+    Drop drop;
+};
+hipError_t launch_dropout(const DropoutParams& q, int type, hipStream_t stream);
+
+// A field in 8 bits with a scale per position and block of 128 channels, strides in real values
+constexpr int kScaleBlock = 128;                        // channels of a scale
+struct QuantiseParams {
+    const void* x;
+    void* q;
+    float* scale;
+    long columns, positions, ldx, ldq;
+    int K;
+};
+hipError_t launch_quantise_8bit(const QuantiseParams& q, int type, hipStream_t stream);
+
+// Channel product of 8-bit operands with scales by blocks of 128 channels, strides in real values; type of the result
+struct MixBlocksParams {
+    const void *x, *W, *bias, *residual;
+    const float *xscale, *wscale;                       // [K / 128][positions], [N / 128][K / 128]
+    void* y;
+    long columns, positions, ldx, ldr, ldy;
+    int rows, contraction, act;
+};
+hipError_t launch_mix_8bit_blocks(const MixBlocksParams& q, int type, hipStream_t stream);
+
 // Norm over many tensors and clipping. sizes in elements; `out` may name the gradients themselves.
 size_t clip_workspace(int count);
 hipError_t launch_clip(int count, const void* const* grads, void* const* out, const long* sizes, const int* types, float max_norm, float* norm, void* workspace,

@@ -1,12 +1,12 @@
-"""Binding of the operators around the spectral layer (include/turbofno.h): channel product with epilogue, root-mean-square norm, gradient
-clipping.
+"""Binding of the operators around the spectral layer (include/turbofno.h): channel product with epilogue, root-mean-square norm and layer norm, dropout, fields
+in 8 bits, gradient clipping.
 
 Fields are channel outermost like the layer's, x[K][positions...]: any trailing dimensions, contiguous among themselves, with any distance
 between channels (a slice of a larger batch of channels is taken as it is). Types: complex64, float32, bfloat16. Results are
 allocated where they are not passed. Every call is asynchronous on torch's current stream.
 
 Nothing is recorded for autograd, as with the layer: a result is cut off from the graph, also where an operand requires a gradient. The gradients are calls
-of their own (mix_backward, rms_norm_backward, mix_weight_grad), to be made by a training step like examples/fourier_block.py or by the backward of an
+of their own (mix_backward, rms_norm_backward, layer_norm_backward, mix_weight_grad; dropout is its own), to be made by a training step like examples/fourier_block.py or by the backward of an
 autograd function.
 """
 import ctypes
@@ -37,14 +37,24 @@ def _lib():
         L.turbofno_rms_norm_backward_workspace_bytes.argtypes = [i, l, i]
         L.turbofno_rms_norm_backward.argtypes = [i, l, i, vp, l, vp, l, vp, vp, vp, l, vp, l, vp, vp, sz, vp]
         L.turbofno_clip_grad_norm_workspace_bytes.argtypes = [i]
+        d = ctypes.c_double
+        L.turbofno_dropout.argtypes = [i, l, i, vp, l, vp, l, d, vp, vp, l, vp]
+        L.turbofno_layer_norm.argtypes = [i, l, i, vp, l, vp, l, vp, vp, f, d, vp, vp, l, vp, l, vp, vp, vp]
+        L.turbofno_layer_norm_8bit.argtypes = [i, l, i, vp, l, vp, l, vp, vp, f, vp, l, vp, l, vp, vp]
+        L.turbofno_layer_norm_backward_workspace_bytes.argtypes = [i, l, i]
+        L.turbofno_layer_norm_backward.argtypes = [i, l, i, vp, l, vp, l, vp, vp, vp, vp, l, d, vp, vp, l, vp, l, vp, vp, vp, sz, vp]
+        L.turbofno_quantise_8bit.argtypes = [i, l, i, vp, l, vp, l, vp, vp]
+        L.turbofno_mix_8bit_blocks.argtypes = [i, l, i, i, vp, l, vp, vp, vp, vp, vp, l, i, vp, l, vp]
         L.turbofno_clip_grad_norm.argtypes = [i, vp, vp, vp, vp, f, vp, vp, sz, vp]
         for name in ("turbofno_mix", "turbofno_mix_8bit", "turbofno_mix_input_grad", "turbofno_mix_weight_grad", "turbofno_rms_norm",
-                     "turbofno_rms_norm_8bit", "turbofno_rms_norm_backward", "turbofno_clip_grad_norm"):
+                     "turbofno_rms_norm_8bit", "turbofno_rms_norm_backward", "turbofno_clip_grad_norm", "turbofno_dropout", "turbofno_layer_norm",
+                     "turbofno_layer_norm_8bit", "turbofno_layer_norm_backward", "turbofno_quantise_8bit", "turbofno_mix_8bit_blocks"):
             getattr(L, name).restype = i
-        for name in ("mix_weight_grad", "rms_norm_backward", "clip_grad_norm"):
+        for name in ("mix_weight_grad", "rms_norm_backward", "layer_norm_backward", "clip_grad_norm"):
             getattr(L, "turbofno_%s_workspace_bytes" % name).restype = sz
         for name in ("mix", "mix_8bit", "mix_input_grad", "mix_weight_grad", "mix_weight_grad_workspace_bytes", "rms_norm", "rms_norm_8bit",
-                     "rms_norm_backward", "rms_norm_backward_workspace_bytes", "clip_grad_norm", "clip_grad_norm_workspace_bytes"):
+                     "rms_norm_backward", "rms_norm_backward_workspace_bytes", "clip_grad_norm", "clip_grad_norm_workspace_bytes", "dropout", "layer_norm",
+                     "layer_norm_8bit", "layer_norm_backward", "layer_norm_backward_workspace_bytes", "quantise_8bit", "mix_8bit_blocks"):
             _AT[name] = ctypes.cast(getattr(L, "turbofno_" + name), vp).value
         _LIB = L
     return _LIB
@@ -353,6 +363,191 @@ def rms_norm_backward(gy, s, gain, rstd, gs=None, gx=None, ggain=None, workspace
                                              workspace.numel(), _stream()))
     return gx, ggain
 
+
+_BLOCK = 128                            # channels of a scale
+
+
+def _blocks(channels):
+    return -(-channels // _BLOCK)
+
+
+def _wide(dtype):
+    """the 32-bit type of values that accompany a field"""
+    return torch.complex64 if dtype.is_complex else torch.float32
+
+
+def _rng(rng, device):
+    return _packed(rng, "rng", (2,), torch.int64, device)
+
+
+def dropout(x, drop, rng, residual=None, y=None):
+    """y = residual + dropout(x): x / (1 - drop) where the element is kept, 0 elsewhere. `rng`: int64 GPU tensor (seed, offset), read when the kernel runs (in a
+    captured graph, at each replay); no mask is stored, the same rng gives the same one. Every use in a model and every step takes an offset of its own. The
+    gradient of x is dropout(gy, drop, rng), that of residual is gy. `y` may be `x` or `residual` itself. The elements that are kept depend on rng, drop, the
+    channel and the position, on nothing else: include/turbofno.h has the generator."""
+    if y is None and isinstance(x, torch.Tensor) and x.is_cuda:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if getattr(y, "is_cuda", False) and _compiled("dropout", ("dropout",), x, residual, drop, rng, y):
+        return y
+    kind, device, K, P = _input(x, "x")
+    px, ldx = _field(x, "x", x.shape, x.dtype, device)
+    pr, ldr = _field(residual, "residual", x.shape, x.dtype, device)
+    y = _result(y, x.shape, x.dtype, device)
+    py, ldy = _field(y, "y", x.shape, x.dtype, device)
+    pd = _rng(rng, device)
+    _current(device)
+    _check(_lib().turbofno_dropout(kind, P, K, px, ldx, pr, ldr, float(drop), pd, py, ldy, _stream()))
+    return y
+
+
+def layer_norm(x, gain, bias=None, residual=None, eps=1e-6, drop=0.0, rng=None, y=None, s=None, mean=None, rstd=None):
+    """s = residual + dropout(x), mean over channels of s, rstd = 1 / sqrt(mean over channels of |s - mean|^2 + eps), y = gain rstd (s - mean) + bias: x[K][...],
+    gain[K] in float32, bias[K] in float32, complex64 for complex fields -> (y, s, mean, rstd). Without residual and dropout s is x itself. `s` and `y` may be `x` or
+    `residual` themselves; mean (of the type of bias) and rstd have the shape of the positions. drop, rng: as dropout takes them. Not recorded for autograd:
+    the gradients are layer_norm_backward's."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() >= 2:
+        y, mean = _result(y, x.shape, x.dtype, x.device), _result(mean, x.shape[1:], _wide(x.dtype), x.device)
+        rstd = _result(rstd, x.shape[1:], torch.float32, x.device)
+        if residual is not None or drop:
+            s = _result(s, x.shape, x.dtype, x.device)
+        if _compiled("layer_norm", ("layer_norm",), x, gain, bias, residual, eps, drop, rng, s, y, mean, rstd):
+            return y, x if s is None else s, mean, rstd
+    kind, device, K, P = _input(x, "x")
+    dtype, places = x.dtype, tuple(x.shape[1:])
+    px, ldx = _field(x, "x", x.shape, dtype, device)
+    pr, ldr = _field(residual, "residual", x.shape, dtype, device)
+    if not isinstance(gain, torch.Tensor):
+        raise TypeError("gain must be a float32 tensor on the GPU")
+    pg, pb = _packed(gain, "gain", (K,), torch.float32, device), _packed(bias, "bias", (K,), _wide(dtype), device)
+    pd = _rng(rng, device)
+    if residual is not None or drop:
+        s = _result(s, x.shape, dtype, device)
+    y, mean, rstd = _result(y, x.shape, dtype, device), _result(mean, places, _wide(dtype), device), _result(rstd, places, torch.float32, device)
+    ps, lds = _field(s, "s", x.shape, dtype, device)
+    py, ldy = _field(y, "y", x.shape, dtype, device)
+    pm, pt = _packed(mean, "mean", places, _wide(dtype), device), _packed(rstd, "rstd", places, torch.float32, device)
+    _current(device)
+    _check(_lib().turbofno_layer_norm(kind, P, K, px, ldx, pr, ldr, pg, pb, float(eps), float(drop), pd, ps, lds, py, ldy, pm, pt, _stream()))
+    return y, x if s is None else s, mean, rstd
+
+
+def _eight_results(x, q, scale):
+    """the 8-bit field and scales of a field, where they are not passed"""
+    q = _result(q, tuple(x.shape) + ((2,) if x.dtype.is_complex else ()), torch.float8_e4m3fn, x.device)
+    return q, _result(scale, (_blocks(x.shape[0]),) + tuple(x.shape[1:]), torch.float32, x.device)
+
+
+def _eight_fields(x, q, scale, device):
+    pair = (2,) if x.dtype.is_complex else ()
+    pq, _ = _field(q, "q", tuple(x.shape) + pair, torch.float8_e4m3fn, device)
+    return pq, _spread(q, "q", 2 if pair else 1), _packed(scale, "scale", (_blocks(x.shape[0]),) + tuple(x.shape[1:]), torch.float32, device)
+
+
+def layer_norm_8bit(x, gain, bias=None, residual=None, eps=1e-6, q=None, scale=None, s=None):
+    """layer_norm without dropout and with its result as quantise_8bit gives it: (q, scale, s)."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() >= 2:
+        q, scale = _eight_results(x, q, scale)
+        if residual is not None:
+            s = _result(s, x.shape, x.dtype, x.device)
+        if _compiled("layer_norm_8bit", ("layer_norm_8bit",), x, gain, bias, residual, eps, s, q, scale):
+            return q, scale, x if s is None else s
+    kind, device, K, P = _input(x, "x")
+    dtype = x.dtype
+    px, ldx = _field(x, "x", x.shape, dtype, device)
+    pr, ldr = _field(residual, "residual", x.shape, dtype, device)
+    if not isinstance(gain, torch.Tensor):
+        raise TypeError("gain must be a float32 tensor on the GPU")
+    pg, pb = _packed(gain, "gain", (K,), torch.float32, device), _packed(bias, "bias", (K,), _wide(dtype), device)
+    if residual is not None:
+        s = _result(s, x.shape, dtype, device)
+    ps, lds = _field(s, "s", x.shape, dtype, device)
+    q, scale = _eight_results(x, q, scale)
+    pq, ldq, pc = _eight_fields(x, q, scale, device)
+    _current(device)
+    _check(_lib().turbofno_layer_norm_8bit(kind, P, K, px, ldx, pr, ldr, pg, pb, float(eps), ps, lds, pq, ldq, pc, _stream()))
+    return q, scale, x if s is None else s
+
+
+def layer_norm_backward_workspace_bytes(K, P, dtype):
+    return int(_lib().turbofno_layer_norm_backward_workspace_bytes(_type(dtype, "the operand"), P, K))
+
+
+def layer_norm_backward(gy, s, gain, mean, rstd, gs=None, drop=0.0, rng=None, gx=None, gr=None, ggain=None, gbias=None, workspace=None):
+    """(gx, gr, ggain, gbias) from the gradient of y, the s, mean and rstd of layer_norm, and gs, what reaches s by the residual stream. gr is the gradient of s and of
+    residual, gx = dropout(gr) that of x, with the drop and rng of layer_norm; without dropout gr is gx itself, and what is passed for it is not used. gx
+    and gr may be gy, s or gs themselves. gbias has the type of bias."""
+    if isinstance(gy, torch.Tensor) and gy.is_cuda and gy.dim() >= 2:
+        gx, gr = _result(gx, gy.shape, gy.dtype, gy.device), _result(gr, gy.shape, gy.dtype, gy.device) if drop else None
+        ggain, gbias = _result(ggain, gy.shape[:1], torch.float32, gy.device), _result(gbias, gy.shape[:1], _wide(gy.dtype), gy.device)
+        if _compiled("layer_norm_backward", ("layer_norm_backward", "layer_norm_backward_workspace_bytes"), gy, s, gain, mean, rstd, gs, drop, rng, gx, gr, ggain,
+                     gbias, workspace):
+            return gx, gr if drop else gx, ggain, gbias
+    kind, device, K, P = _input(gy, "gy")
+    dtype, places = gy.dtype, tuple(gy.shape[1:])
+    if not all(isinstance(t, torch.Tensor) for t in (s, gain, mean, rstd)):
+        raise TypeError("s, gain, mean and rstd must be tensors")
+    py, ldy = _field(gy, "gy", gy.shape, dtype, device)
+    ps, lds = _field(s, "s", gy.shape, dtype, device)
+    pgs, ldgs = _field(gs, "gs", gy.shape, dtype, device)
+    gx, gr = _result(gx, gy.shape, dtype, device), _result(gr, gy.shape, dtype, device) if drop else None
+    px, ldx = _field(gx, "gx", gy.shape, dtype, device)
+    pr, ldr = _field(gr, "gr", gy.shape, dtype, device)
+    pg, pm, pt = _packed(gain, "gain", (K,), torch.float32, device), _packed(mean, "mean", places, _wide(dtype), device), _packed(rstd, "rstd", places, torch.float32, device)
+    pd = _rng(rng, device)
+    ggain, gbias = _result(ggain, (K,), torch.float32, device), _result(gbias, (K,), _wide(dtype), device)
+    po, pb = _packed(ggain, "ggain", (K,), torch.float32, device), _packed(gbias, "gbias", (K,), _wide(dtype), device)
+    workspace = _workspace(workspace, _lib().turbofno_layer_norm_backward_workspace_bytes(kind, P, K), device)
+    _current(device)
+    _check(_lib().turbofno_layer_norm_backward(kind, P, K, py, ldy, ps, lds, pg, pm, pt, pgs, ldgs, float(drop), pd, pr, ldr, px, ldx, po, pb, workspace.data_ptr(),
+                                               workspace.numel(), _stream()))
+    return gx, gr if drop else gx, ggain, gbias
+
+
+def quantise_8bit(x, q=None, scale=None):
+    """x in float8_e4m3fn with a float32 scale for each position and block of 128 channels, its largest magnitude over 448: (q, scale), what mix_8bit_blocks takes.
+    scale has the shape [ceil(K / 128)][positions...]; q has a last dimension of two, (re, im), for complex fields."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() >= 2:
+        q, scale = _eight_results(x, q, scale)
+        if _compiled("quantise_8bit", ("quantise_8bit",), x, q, scale):
+            return q, scale
+    kind, device, K, P = _input(x, "x")
+    px, ldx = _field(x, "x", x.shape, x.dtype, device)
+    q, scale = _eight_results(x, q, scale)
+    pq, ldq, pc = _eight_fields(x, q, scale, device)
+    _current(device)
+    _check(_lib().turbofno_quantise_8bit(kind, P, K, px, ldx, pq, ldq, pc, _stream()))
+    return q, scale
+
+
+def mix_8bit_blocks(xq, xscale, Wq, wscale, bias=None, residual=None, activation="none", y=None, dtype=None):
+    """mix from 8-bit operands with a scale for each block of 128 channels: x = xscale[k / 128][position] xq, W = wscale[n / 128][k / 128] Wq, all of float8_e4m3fn
+    with float32 scales; xq and xscale as quantise_8bit and layer_norm_8bit give them. For the rest like mix_8bit."""
+    if getattr(y, "is_cuda", False) and dtype in (None, y.dtype) and _compiled("mix_8bit_blocks", ("mix_8bit_blocks",), xq, xscale, Wq, wscale, bias, residual,
+                                                                               _ACTIVATIONS.get(activation, -1), y):
+        return y
+    if dtype is None:
+        dtype = next((t.dtype for t in (y, residual) if isinstance(t, torch.Tensor)), torch.bfloat16)
+    kind = _type(dtype, "the result")
+    act = _activation(activation)
+    tail = (2,) if dtype == torch.complex64 else ()
+    if not isinstance(xq, torch.Tensor) or not isinstance(Wq, torch.Tensor):
+        raise TypeError("xq and Wq must be tensors")
+    _need(xq.dim() >= 2 + len(tail) and xq.shape[0] > 0 and (not tail or xq.shape[-1] == 2), "xq must be [K][positions...]%s", "[2]" if tail else "")
+    K, device = xq.shape[0], xq.device
+    _need(Wq.dim() == 2 + len(tail) and Wq.shape[0] > 0 and tuple(Wq.shape[1:]) == (K,) + tail, "Wq must be [N][%d]%s", K, "[2]" if tail else "")
+    N, places = Wq.shape[0], tuple(xq.shape[1:-1] if tail else xq.shape[1:])
+    P = xq.numel() // (K * (2 if tail else 1))
+    f8 = torch.float8_e4m3fn
+    _on_gpu(xq, "xq", f8, device)
+    ldx = _spread(xq, "xq", 2 if tail else 1)
+    y = _result(y, (N,) + places, dtype, device)
+    pr, ldr = _field(residual, "residual", (N,) + places, dtype, device)
+    py, ldy = _field(y, "y", (N,) + places, dtype, device)
+    pxs, pW = _packed(xscale, "xscale", (_blocks(K),) + places, torch.float32, device), _packed(Wq, "Wq", Wq.shape, f8, device)
+    pws, pb = _packed(wscale, "wscale", (_blocks(N), _blocks(K)), torch.float32, device), _packed(bias, "bias", (N,), dtype, device)
+    _current(device)
+    _check(_lib().turbofno_mix_8bit_blocks(kind, P, N, K, xq.data_ptr(), ldx, pxs, pW, pws, pb, pr, ldr, act, py, ldy, _stream()))
+    return y
 
 def clip_grad_norm(grads, max_norm, out=None, norm=None, workspace=None):
     """The norm over all values of the tensors in `grads` (complex64, float32 and bfloat16, contiguous, in any mixture), as a float32 tensor of no

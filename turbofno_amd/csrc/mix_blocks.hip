@@ -12,6 +12,7 @@
 // The sum of a step is multiplied by both scales and added to the total, in fp32.
 #include "kernels.h"
 #include "mix_kernel.h"
+#include <algorithm>
 
 namespace tfno {
 
@@ -28,7 +29,7 @@ template <bool COMPLEX> struct RawStep {
     unsigned row[2][kRowsOfHalf<COMPLEX>];              // four columns of the lane's channels
     float4_v scale;                                     // of the columns
 };
-// Columns of a wave, from column0 on, of which `there` exist, at least one. CAREFUL: fewer than 64 may exist, channels may lie any distance apart
+// 64 columns of a wave, from column0 on. CAREFUL: only `there` of them may exist, at least one, and channels may lie any distance apart
 template <bool COMPLEX, bool CAREFUL> struct Input {
     static constexpr int V = COMPLEX ? 2 : 1, HALF = kRowsOfHalf<COMPLEX>;
     const MixBlocksParams& q;
@@ -50,12 +51,7 @@ template <bool COMPLEX, bool CAREFUL> struct Input {
                     // a word that would end behind the last value of all starts earlier and is shifted; what it holds beyond its row's end is not used
                     const long row = k + kq * HALF < q.contraction ? k + kq * HALF : q.contraction - 1;
                     const long at = row * q.ldx + column0 + (4 * c < there ? 4 * c : 0), last = (q.contraction - 1) * q.ldx + q.columns - 4;
-                    const unsigned char* x = static_cast<const unsigned char*>(q.x);
-                    if (last < 0) {                             // fewer than four values
-                        unsigned v = 0;
-                        for (int i = 0; i < 4; ++i) v |= at + i < last + 4 ? (unsigned)x[at + i] << 8 * i : 0u;
-                        raw.row[h][j] = v;
-                    } else raw.row[h][j] = *reinterpret_cast<const uint_any*>(x + (at < last ? at : last)) >> (at > last ? 8 * (int)(at - last) : 0);
+                    raw.row[h][j] = *reinterpret_cast<const uint_any*>(static_cast<const unsigned char*>(q.x) + (at < last ? at : last)) >> (at > last ? 8 * (int)(at - last) : 0);
                 } else if constexpr (GUARD) {
                     const int common = k < q.contraction ? k : q.contraction - 1;
                     raw.row[h][j] = near_load4<kIn8>(scalar(q.x, common * q.ldx + column0), fresh(k + kq * HALF < q.contraction ? quarter : 4 * c));
@@ -173,26 +169,19 @@ __device__ __forceinline__ void add_scaled_apart(float4_v x, float w, const floa
 
 // ---- the weights: 16 bytes of a row ----
 
-// Bytes e ... e + 15 of a row of `count`, from memory; where they would end behind the last weight, earlier ones, and mend_weights() has to follow. `few`: there are
-// fewer than 16 weights
-__device__ __forceinline__ uint4_v fetch_weights(const void* W, int row, int rows, int count, int e, bool few)
+// Bytes e ... e + 15 of a row of `count`, from memory; where they would end behind the last weight, earlier ones, and mend_weights() has to follow
+__device__ __forceinline__ uint4_v fetch_weights(const void* W, int row, int rows, int count, int e)
 {
     const unsigned char* w = static_cast<const unsigned char*>(W);
     const long at = (long)(row < rows ? row : rows - 1) * count + e, last = (long)rows * count - 16;
-    if (few) {
-        uint4_v v = {};
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i / 4] |= at + i < last + 16 ? (unsigned)w[at + i] << i % 4 * 8 : 0u;
-        return v;
-    }
     return *reinterpret_cast<const uint4_any*>(w + (at < last ? at : last));
 }
 // zeros for bytes from `count` on
-__device__ __forceinline__ uint4_v mend_weights(uint4_v v, int row, int rows, int count, int e, bool few)
+__device__ __forceinline__ uint4_v mend_weights(uint4_v v, int row, int rows, int count, int e)
 {
     if (e + 16 <= count) return v;
     const long at = (long)(row < rows ? row : rows - 1) * count + e, last = (long)rows * count - 16;
-    const int by = few || at <= last ? 0 : at - last < 16 ? (int)(at - last) : 15;
+    const int by = at <= last ? 0 : at - last < 16 ? (int)(at - last) : 15;
 #pragma unroll
     for (int words = 1; words < 4; words *= 2)
 #pragma unroll
@@ -218,57 +207,111 @@ template <int ACT, int ROWS> __device__ __forceinline__ void activate_rows(float
 #pragma unroll
         for (int b = 0; b < 4; ++b) v[i][b] = activate(ACT, v[i][b]);
 }
-// ROWS rows row0 + i, four columns each from `column` on, of which those of lower numbers than `from` and those beyond the last are left alone: bias, residual,
-// activation. All loads first
-template <int OUT, bool COMPLEX, int ROWS>
-__device__ __forceinline__ void put_rows(const MixBlocksParams& q, long column, long from, int row0, float4_v (&v)[ROWS])
-{
+// Rows row0 + lane_row + i and four columns each, column0 + 4 c ..., of a lane: columns before `from` and beyond the last, and rows beyond the last, are left alone.
+// WHOLE: there are none of them in the wave; then an address is a uniform part and one of 32 bits
+template <int OUT, bool COMPLEX, int ROWS> struct Results {
     typedef typename Columns<OUT>::Value Value;
-    constexpr int V = COMPLEX ? 2 : 1;
-    if (column >= q.columns || column + 4 <= from) return;
-    const bool whole = column >= from && column + 4 <= q.columns;
-    auto at = [&](int i) { return (long)(row0 + i < q.rows ? row0 + i : q.rows - 1); };
-    RawOf<OUT> residual[ROWS];
-    if (q.residual)
+    static constexpr int V = COMPLEX ? 2 : 1;
+    const MixBlocksParams& q;
+    const long column0, from;
+    const int c, lane_row;
+    __device__ __forceinline__ unsigned offset(long ld) const { return fresh(((unsigned)lane_row * (unsigned)ld + 4 * c) * (unsigned)sizeof(Value)); }
+    __device__ __forceinline__ long row_at(int row) const { return row + lane_row < q.rows ? row + lane_row : q.rows - 1; }
+    template <bool WHOLE> __device__ __forceinline__ void fetch(int row0, RawOf<OUT> (&residual)[ROWS]) const
+    {
+        if constexpr (WHOLE) {
+            const unsigned at = offset(q.ldr);
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            const Value* p = static_cast<const Value*>(q.residual) + at(i) * q.ldr;
-            residual[i] = whole ? load4<OUT>(p, column) : load4_ragged<OUT>(p, column, q.columns);
-        }
-    if (q.bias)
+            for (int i = 0; i < ROWS; ++i) residual[i] = near_load4<OUT>(scalar(q.residual, ((row0 + i) * q.ldr + column0) * (long)sizeof(Value)), at);
+        } else
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            const Value* p = static_cast<const Value*>(q.bias) + at(i) * V;
-            const float re = value_of(p[0]), im = value_of(p[V - 1]);
-            v[i] += (float4_v){ re, im, re, im };
-        }
-    if (q.residual)
+            for (int i = 0; i < ROWS; ++i) residual[i] = load4_ragged<OUT>(static_cast<const Value*>(q.residual) + row_at(row0 + i) * q.ldr, column0 + 4 * c, q.columns);
+    }
+    __device__ __forceinline__ void finish(float4_v (&v)[ROWS], const float* bias, const RawOf<OUT> (&residual)[ROWS]) const
+    {
+        if (q.bias)
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) v[i] += to_float<OUT>(residual[i]);
-    if (q.act == kActGeluTanh) activate_rows<kActGeluTanh>(v);
-    else if (q.act == kActSilu) activate_rows<kActSilu>(v);
-    else if (q.act == kActRelu) activate_rows<kActRelu>(v);
+            for (int i = 0; i < ROWS; ++i) {
+                const float re = bias[i * V], im = bias[i * V + V - 1];
+                v[i] += (float4_v){ re, im, re, im };
+            }
+        if (q.residual)
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        if (row0 + i >= q.rows) break;
-        Value* p = static_cast<Value*>(q.y) + at(i) * q.ldy;
-        const RawOf<OUT> raw = from_float<OUT>(v[i]);
-        if (whole) store4<OUT>(p, column, raw);
-        else
+            for (int i = 0; i < ROWS; ++i) v[i] += to_float<OUT>(residual[i]);
+        if (q.act == kActGeluTanh) activate_rows<kActGeluTanh>(v);
+        else if (q.act == kActSilu) activate_rows<kActSilu>(v);
+        else if (q.act == kActRelu) activate_rows<kActRelu>(v);
+    }
+    template <bool WHOLE> __device__ __forceinline__ void store(int row0, const float4_v (&v)[ROWS]) const
+    {
+        if constexpr (WHOLE) {
+            const unsigned at = offset(q.ldy);
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (column + b >= from && column + b < q.columns) {
-                    if constexpr (OUT == kIn32) p[column + b] = raw[b];
-                    else p[column + b] = (unsigned short)(b & 1 ? raw[b / 2] >> 16 : raw[b / 2]);
+            for (int i = 0; i < ROWS; ++i) near_store4<OUT>(scalar(q.y, ((row0 + i) * q.ldy + column0) * (long)sizeof(Value)), at, from_float<OUT>(v[i]));
+        } else
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                if (row0 + lane_row + i >= q.rows) break;
+                Value* p = static_cast<Value*>(q.y) + (row0 + lane_row + i) * q.ldy;
+                const RawOf<OUT> raw = from_float<OUT>(v[i]);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const long column = column0 + 4 * c + b;
+                    if (column < from || column >= q.columns) continue;
+                    if constexpr (OUT == kIn32) p[column] = raw[b];
+                    else p[column] = (unsigned short)(b & 1 ? raw[b / 2] >> 16 : raw[b / 2]);
                 }
+            }
+    }
+    __device__ __forceinline__ float bias_at(int row, int part) const { return value_of(static_cast<const Value*>(q.bias)[(long)(row < q.rows ? row : q.rows - 1) * V + part]); }
+};
+__device__ __forceinline__ float4_v row_of(const float4_v (&total)[4], int i) { return (float4_v){ total[0][i], total[1][i], total[2][i], total[3][i] }; }
+
+// ---- one value of the product, in plain fp32 ----
+template <bool COMPLEX> __device__ __forceinline__ float plain_sum(const MixBlocksParams& q, long row, long column)
+{
+    constexpr int V = COMPLEX ? 2 : 1;
+    const int part = (int)(column % V), blocks = (q.contraction + kScaleBlock - 1) / kScaleBlock;
+    const unsigned char *W = static_cast<const unsigned char*>(q.W) + row * q.contraction * V, *x = static_cast<const unsigned char*>(q.x) + column - part;
+    auto value = [](unsigned char v) { return __builtin_amdgcn_cvt_f32_fp8((int)v, 0); };
+    float total = 0.f;
+#pragma unroll 1
+    for (int b = 0; b < blocks; ++b) {
+        float sum = 0.f;
+#pragma unroll 1
+        for (int k = b * kScaleBlock; k < (b + 1) * kScaleBlock && k < q.contraction; ++k) {
+            sum = __builtin_fmaf(value(W[k * V]), value(x[k * q.ldx + part]), sum);
+            if constexpr (COMPLEX) sum = __builtin_fmaf(part ? value(W[k * V + 1]) : -value(W[k * V + 1]), value(x[k * q.ldx + 1 - part]), sum);
+        }
+        const float xs = q.xscale[b * q.positions + column / V], ws = q.wscale[row / kScaleBlock * blocks + b];
+        total = __builtin_fmaf(sum * (xs > ws ? xs : ws), xs > ws ? ws : xs, total);
+    }
+    return total;
+}
+// the results of a wave whose scales may not be multiplied first: rows row0 + 16 t + i of the lane, value by value
+template <int OUT, bool COMPLEX> __device__ __forceinline__ void put_plain(const MixBlocksParams& q, const Results<OUT, COMPLEX, 4>& results, int row0, int tiles16, const float* biases)
+{
+#pragma unroll 1
+    for (int t = 0; t < tiles16 && row0 + 16 * t < q.rows; ++t) {
+        float4_v v[4];
+        RawOf<OUT> residual[4];
+        if (q.residual) results.template fetch<false>(row0 + 16 * t, residual);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const long column = results.column0 + 4 * results.c + b;
+                v[i][b] = plain_sum<COMPLEX>(q, results.row_at(row0 + 16 * t + i), column < q.columns ? column : q.columns - 1);
+            }
+        results.finish(v, biases + (16 * t + results.lane_row) * (COMPLEX ? 2 : 1), residual);
+        results.template store<false>(row0 + 16 * t, v);
     }
 }
-__device__ __forceinline__ float4_v row_of(const float4_v (&total)[4], int i) { return (float4_v){ total[0][i], total[1][i], total[2][i], total[3][i] }; }
 
 // ---- 16 rows of one wave, steps wave, wave + waves ...: weights straight from memory ----
 
 template <int OUT, bool COMPLEX, bool CAREFUL>
-__device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<COMPLEX, CAREFUL>& in, int row0, int first, int stride, bool few, float4_v (&total)[4])
+__device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<COMPLEX, CAREFUL>& in, int row0, int first, int stride, float4_v (&total)[4])
 {
     const int count = q.contraction * (COMPLEX ? 2 : 1), steps = (count + kStep - 1) / kStep;
     const int blocks = (q.contraction + kScaleBlock - 1) / kScaleBlock;
@@ -278,14 +321,14 @@ __device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<
     auto ask = [&](int s) {
         in.template fetch<true>(s, raw);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) w[h] = fetch_weights(q.W, row0 + in.c, q.rows, count, s * kStep + 64 * h + 16 * in.kq, CAREFUL && few);
+        for (int h = 0; h < 2; ++h) w[h] = fetch_weights(q.W, row0 + in.c, q.rows, count, s * kStep + 64 * h + 16 * in.kq);
     };
     if (first < steps) ask(first);
     for (int s = first; s < steps; s += stride) {
         in.clear(s, raw);
         if ((s + 1) * kStep > count)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) w[h] = mend_weights(w[h], row0 + in.c, q.rows, count, s * kStep + 64 * h + 16 * in.kq, CAREFUL && few);
+            for (int h = 0; h < 2; ++h) w[h] = mend_weights(w[h], row0 + in.c, q.rows, count, s * kStep + 64 * h + 16 * in.kq);
         const float4_v scale = raw.scale;
         const float ws = wscale[s / (COMPLEX ? 2 : 1)];
         bool out = false;
@@ -311,7 +354,9 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
 {
     constexpr bool EXACT = OUT == kIn32;
     constexpr int CHUNKS = NT * 128, PHASES = NT == 8 ? 2 : 1, EACH = CHUNKS / 256 / PHASES;        // 16 bytes each; asked for at once by a thread
+    constexpr int V = COMPLEX ? 2 : 1;
     __shared__ uint4_v weights[2 * CHUNKS];
+    __shared__ float biases[16 * NT * V];
     const long id = block_index();
     // Blocks go to the eight XCDs in turns: with many columns those of the same columns follow one another on one XCD, whose L2 cache then holds them
     const long slot = by_xcd ? id / 8 : id, column_tile = by_xcd ? slot / row_tiles * 8 + id % 8 : slot / row_tiles;
@@ -326,30 +371,33 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     auto chunk = [&](int i) { return (int)threadIdx.x + 256 * i; };
     auto chunk_row = [&](int e) { return e / 128 * 16 + (e & 15); };
     auto chunk_entry = [&](int e) { return (e >> 6 & 1) * 64 + (e >> 4 & 3) * 16; };
-    auto ask = [&](int s, int phase, auto guard) {
+    auto ask = [&](int s, int phase, auto guard, uint4_v (&w)[EACH]) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int e = chunk(phase * EACH + i), row = row0 + chunk_row(e) < q.rows ? chunk_row(e) : q.rows - 1 - row0;
-            if constexpr (decltype(guard)::value) w[i] = fetch_weights(q.W, row0 + row, q.rows, count, s * kStep + chunk_entry(e), false);
+            if constexpr (decltype(guard)::value) w[i] = fetch_weights(q.W, row0 + row, q.rows, count, s * kStep + chunk_entry(e));
             else w[i] = *reinterpret_cast<const TFNO_GLOBAL uint4_any*>(scalar(q.W, (long)row0 * count + s * kStep) + fresh((unsigned)row * (unsigned)count + chunk_entry(e)));
         }
     };
-    auto keep = [&](int s, int phase, auto guard) {
+    auto keep = [&](int s, int phase, auto guard, uint4_v (&w)[EACH]) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int e = chunk(phase * EACH + i);
-            if constexpr (decltype(guard)::value) w[i] = mend_weights(w[i], row0 + chunk_row(e), q.rows, count, s * kStep + chunk_entry(e), false);
+            if constexpr (decltype(guard)::value) w[i] = mend_weights(w[i], row0 + chunk_row(e), q.rows, count, s * kStep + chunk_entry(e));
             weights[(s & 1) * CHUNKS + e] = w[i];
         }
     };
     RawStep<COMPLEX> raw;
+    const Results<OUT, COMPLEX, 4> results = { q, in.column0, from, in.c, 4 * in.kq };
     auto begin = [&](auto guard) {
         in.template fetch<decltype(guard)::value>(0, raw);
+        uint4_v first[PHASES][EACH];
 #pragma unroll
-        for (int p = 0; p < PHASES; ++p) {
-            ask(0, p, guard);
-            keep(0, p, guard);
-        }
+        for (int p = 0; p < PHASES; ++p) ask(0, p, guard, first[p]);
+        if (q.bias)
+            for (int e = threadIdx.x; e < 16 * NT * V; e += 256) biases[e] = results.bias_at(row0 + e / V, e % V);
+#pragma unroll
+        for (int p = 0; p < PHASES; ++p) keep(0, p, guard, first[p]);
     };
     float4_v total[NT][4] = {};
     bool out = false;
@@ -361,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
         ops.make(raw);
         if constexpr (NEXT) {
             in.template fetch<GUARD>(s + 1, raw);
-            ask(s + 1, 0, guard);
+            ask(s + 1, 0, guard, w);
         }
         __builtin_amdgcn_sched_barrier(0);              // the loads stay ahead of the products
         const uint4_v* from_lds = weights + (s & 1) * CHUNKS + lane;
@@ -387,14 +435,14 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
                 }
                 add_scaled(joint, (i - 1) % 2 * 2, part[(i - 1) % 2], total[(i - 1) / 2]);
                 if (NEXT && PHASES == 2 && i == NT) {
-                    keep(s + 1, 0, guard);
-                    ask(s + 1, 1, guard);
+                    keep(s + 1, 0, guard, w);
+                    ask(s + 1, 1, guard, w);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         if constexpr (NEXT) {
-            keep(s + 1, PHASES - 1, guard);
+            keep(s + 1, PHASES - 1, guard, w);
             __syncthreads();
         }
     };
@@ -408,38 +456,253 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     }
     body(steps - 1, std::false_type(), std::false_type());
     if (from >= q.columns) return;
-    const long column = in.column0 + 4 * in.c;
-    if (__builtin_expect(any_lane(out), 0)) {           // scales that may not be multiplied first: the sums once more, 16 rows at a time
-#pragma unroll 1
-        for (int row = row0; row < row0 + 16 * NT && row < q.rows; row += 16) {
-            float4_v sums[4] = {}, v[4];
-            sum_steps<OUT, COMPLEX, false>(q, in, row, 0, 1, false, sums);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = row_of(sums, i);
-            put_rows<OUT, COMPLEX, 4>(q, column, from, row + 4 * in.kq, v);
-        }
+    if (__builtin_expect(any_lane(out), 0)) {
+        put_plain<OUT, COMPLEX>(q, results, row0, NT, biases);
         return;
     }
+    // 32 rows at a time, always from the same registers, which the next rows' sums are moved to: unrolled, the code would not stay in the instruction cache
+    auto put = [&](auto whole_wave) {
+        constexpr bool WHOLE = decltype(whole_wave)::value;
+#pragma unroll 1
+        for (int t = 0; t < NT; t += 2) {
+            const int row = row0 + 16 * t;
+            if (!WHOLE && row >= q.rows) break;
+            RawOf<OUT> residual[2][4];
+            if (q.residual)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (row0 + 16 * t >= q.rows) break;
-        float4_v v[4];
+                for (int u = 0; u < 2; ++u) results.template fetch<WHOLE>(row + 16 * u, residual[u]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = row_of(total[t], i);
-        put_rows<OUT, COMPLEX, 4>(q, column, from, row0 + 16 * t + 4 * in.kq, v);
+            for (int u = 0; u < 2; ++u) {
+                float4_v v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = row_of(total[u], i);
+                results.finish(v, biases + (16 * (t + u) + 4 * in.kq) * V, residual[u]);
+                results.template store<WHOLE>(row + 16 * u, v);
+            }
+#pragma unroll
+            for (int u = 0; u + 2 < NT; ++u)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) total[u][b] = total[u + 2][b];
+        }
+    };
+    if (from + kColumns <= q.columns && row0 + 16 * NT <= q.rows) put(std::true_type());
+    else put(std::false_type());
+}
+
+// ---- many rows and columns: waves RG deep and CG side by side share 16 NT RG rows of W and 64 CG columns of x ----
+
+// Both pass LDS in two buffers: a step's values are on their way from memory, 16 bytes a load, during the products of the step before, and written when those are done.
+// W lies there in the order in which lanes read it. x lies there as in memory, 16 columns of a row together; ds_read_b64_tr_b8 hands a lane eight rows of one column.
+// The places of a row's 16-byte pieces are exchanged by its number, so that a read of 32 rows takes all banks. A lane's column of 16 is c here, not 4 c ... 4 c + 3: the results
+// pass LDS once more on their way out.
+template <int OUT, int NT, int RG, int CG, int BUFFERS> struct Staged {
+    static constexpr int THREADS = 64 * RG * CG, ROWS = 16 * NT * RG, COLUMNS = 64 * CG, PIECES = COLUMNS / 16;
+    static constexpr int X_EACH = kStep * PIECES / THREADS, W_EACH = ROWS * 8 / THREADS, X_ROWS = THREADS / PIECES;      // 16-byte pieces of a thread; rows of x at a time
+    static constexpr int X_BYTES = kStep * COLUMNS, W_BYTES = ROWS * kStep;
+    static_assert(X_BYTES >= RG * CG * 4096, "the results' way out");
+    static constexpr size_t LDS = BUFFERS * (X_BYTES + W_BYTES + COLUMNS * 4) + ROWS * 4;
+    // what a row's pieces are exchanged by
+    static __device__ __forceinline__ int place_of(int row) { return PIECES == 16 ? (row & 7) | (row >> 1 & 8) : (row & 7) ^ (row >> 4 & 1); }
+    static_assert(PIECES == 8 || PIECES == 16, "columns of a block");
+};
+typedef int int2_v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ int2_v read_transposed(const unsigned char* lds)
+{
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_v*)lds);
+}
+template <int OUT, int NT, int RG, int CG, int BUFFERS, int WAVES>
+__global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES) void mix_blocks_staged_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
+{
+    typedef Staged<OUT, NT, RG, CG, BUFFERS> S;
+    constexpr bool EXACT = OUT == kIn32;
+    extern __shared__ uint4_v staged[];
+    unsigned char* const bytes = reinterpret_cast<unsigned char*>(staged);
+    unsigned char* const xs = bytes;                    // two buffers each
+    unsigned char* const ws = bytes + BUFFERS * S::X_BYTES;
+    float* const scales = reinterpret_cast<float*>(ws + BUFFERS * S::W_BYTES);
+    float* const biases = scales + BUFFERS * S::COLUMNS;
+    const long id = block_index();
+    const long slot = by_xcd ? id / 8 : id, column_tile = by_xcd ? slot / row_tiles * 8 + id % 8 : slot / row_tiles;
+    if (column_tile >= column_tiles) return;
+    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
+    const int wr = wave / CG, wc = wave % CG, wave_row = row0 + wr * 16 * NT;
+    const long from = column_tile * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);      // the last tile ends with the columns
+    const int count = q.contraction, steps = (count + kStep - 1) / kStep, whole = count / kStep;
+    const float* wscale = q.wscale + (long)(wave_row / kScaleBlock) * ((q.contraction + kScaleBlock - 1) / kScaleBlock);
+    const int x_row = tid / S::PIECES, x_piece = tid % S::PIECES;
+
+    uint4_v x[S::X_EACH], w[S::W_EACH];
+    float scale = 0.f;
+    // pieces of W: eight side by side make 128 bytes of a row
+    auto w_row = [&](int e) { return e / 8; };
+    auto w_entry = [&](int e) { return e % 8 * 16; };
+    // piece j of the thread, of x and then of W, and at last the scale
+    auto ask = [&](int s, int j, auto guard) {
+        constexpr bool GUARD = decltype(guard)::value;
+        if (j < S::X_EACH) {
+            const int k = s * kStep + j * S::X_ROWS;
+            if constexpr (GUARD) {
+                const long row = k + x_row < q.contraction ? k + x_row : q.contraction - 1;
+                x[j] = *reinterpret_cast<const uint4_any*>(static_cast<const unsigned char*>(q.x) + row * q.ldx + column0 + 16 * x_piece);
+            } else x[j] = *reinterpret_cast<const TFNO_GLOBAL uint4_any*>(scalar(q.x, k * q.ldx + column0) + fresh((unsigned)x_row * (unsigned)q.ldx + 16 * x_piece));
+        } else if (j < S::X_EACH + S::W_EACH) {
+            const int e = tid + S::THREADS * (j - S::X_EACH), row = row0 + w_row(e) < q.rows ? w_row(e) : q.rows - 1 - row0;
+            if constexpr (GUARD) w[j - S::X_EACH] = fetch_weights(q.W, row0 + row, q.rows, count, s * kStep + w_entry(e));
+            else w[j - S::X_EACH] = *reinterpret_cast<const TFNO_GLOBAL uint4_any*>(scalar(q.W, (long)row0 * count + s * kStep) + fresh((unsigned)row * (unsigned)count + w_entry(e)));
+        } else scale = q.xscale[s * q.positions + column0 + tid % S::COLUMNS];
+    };
+    constexpr int PIECES = S::X_EACH + S::W_EACH + 1;
+    auto keep = [&](int s, auto guard) {
+        constexpr bool GUARD = decltype(guard)::value;
+        unsigned char* const to = xs + (BUFFERS == 2 ? s & 1 : 0) * S::X_BYTES;
+#pragma unroll
+        for (int i = 0; i < S::X_EACH; ++i) {
+            const int row = i * S::X_ROWS + x_row;
+            if (GUARD && s * kStep + row >= q.contraction) x[i] = (uint4_v){ 0u, 0u, 0u, 0u };
+            *reinterpret_cast<uint4_v*>(to + row * S::COLUMNS + (x_piece ^ S::place_of(row)) * 16) = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < S::W_EACH; ++i) {
+            const int e = tid + S::THREADS * i, row = w_row(e), p = e % 8;
+            if constexpr (GUARD) w[i] = mend_weights(w[i], row0 + row, q.rows, count, s * kStep + w_entry(e));
+            reinterpret_cast<uint4_v*>(ws + (BUFFERS == 2 ? s & 1 : 0) * S::W_BYTES)[row / 16 * 128 + p * 16 + ((row & 15) ^ p)] = w[i];
+        }
+        scales[(BUFFERS == 2 ? s & 1 : 0) * S::COLUMNS + tid % S::COLUMNS] = scale;        // by all threads, without a branch: more than one of them write the same
+    };
+    auto begin = [&](auto guard) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) ask(0, j, guard);
+        keep(0, guard);
+    };
+    if (whole) begin(std::false_type());
+    else begin(std::true_type());
+    if (q.bias)
+        for (int e = tid; e < S::ROWS; e += S::THREADS)
+            biases[e] = value_of(static_cast<const typename Columns<OUT>::Value*>(q.bias)[row0 + e < q.rows ? row0 + e : q.rows - 1]);
+    __syncthreads();
+
+    float4_v total[NT][4] = {};
+    bool out = false;
+    // a lane reads one half of a row's piece: lanes 2 j and 2 j + 1 row j of eight
+    const int piece = wc * 4 ^ S::place_of(16 * kq + (c >> 1));
+    const unsigned char* const x_from = xs + (16 * kq + (c >> 1)) * S::COLUMNS + 8 * (c & 1);
+    const uint4_v* const w_from = reinterpret_cast<const uint4_v*>(ws) + wr * NT * 128 + kq * 16;
+    auto body = [&](int s, auto next, auto guard) {
+        constexpr bool NEXT = decltype(next)::value;
+        const unsigned char* const here = x_from + (BUFFERS == 2 ? s & 1 : 0) * S::X_BYTES;
+        const uint4_v *const lower = w_from + (BUFFERS == 2 ? s & 1 : 0) * (S::W_BYTES / 16) + (c ^ kq), *const upper = w_from + (BUFFERS == 2 ? s & 1 : 0) * (S::W_BYTES / 16) + 64 + (c ^ (4 + kq));
+        float4_v joint;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) joint[b] = scales[(BUFFERS == 2 ? s & 1 : 0) * S::COLUMNS + wc * 64 + 16 * b + c];
+        joint = joint_scale(joint, wscale[s], out);
+        Operands<false, EXACT> ops;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int2_v v = read_transposed(here + (piece ^ b) * 16 + (u / 2 * 64 + u % 2 * 8) * S::COLUMNS);
+                if constexpr (EXACT) {
+                    const uint2_v lo = widen((unsigned)v[0]), hi = widen((unsigned)v[1]);
+                    ops.b[u][b].v = (uint4_v){ lo[0], lo[1], hi[0], hi[1] };
+                } else { ops.b[b][2 * u] = v[0]; ops.b[b][2 * u + 1] = v[1]; }
+            }
+        // the loads of the next step among the products: all at once, they would keep the waves from their products
+        constexpr int TURNS = EXACT ? NT : 2 * NT;
+        auto ask_some = [&](int turn) {
+            if constexpr (NEXT)
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j)
+                    if (j * TURNS / PIECES == turn) ask(s + 1, j, guard);
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const uint4_v a[2] = { lower[t * 128], upper[t * 128] };
+                float4_v part[4];
+                ask_some(t);
+                ops.product(a, 0, part);
+                add_scaled(joint, 0, part, total[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            // two columns' products at a time; they are added while the next two are formed
+            float4_v part[2][2];
+            uint4_v a[2] = { lower[0], upper[0] };
+            ops.product(a, 0, part[0]);
+#pragma unroll
+            for (int i = 1; i <= 2 * NT; ++i) {
+                ask_some(i - 1);
+                if (i < 2 * NT) {
+                    if (i % 2 == 0) { a[0] = lower[i / 2 * 128]; a[1] = upper[i / 2 * 128]; }
+                    ops.product(a, i % 2 * 2, part[i % 2]);
+                }
+                add_scaled(joint, (i - 1) % 2 * 2, part[(i - 1) % 2], total[(i - 1) / 2]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if constexpr (NEXT) {
+            if constexpr (BUFFERS == 1) __syncthreads();
+            keep(s + 1, guard);
+            __syncthreads();
+        }
+    };
+    for (int s = 0; s < whole - 1; ++s) body(s, std::true_type(), std::false_type());
+    if (whole && whole < steps) body(whole - 1, std::true_type(), std::true_type());
+    body(steps - 1, std::false_type(), std::false_type());
+
+    if constexpr (BUFFERS == 1) __syncthreads();        // the results' way out is free
+    const long wave_column = scalar(column0 + wc * 64);
+    const Results<OUT, false, 4> results = { q, wave_column, from, c, 4 * kq };
+    if (__builtin_expect(any_lane(out), 0)) {
+        put_plain<OUT, false>(q, results, wave_row, NT, biases + wr * 16 * NT);
+        return;
     }
+    // 16 rows of 64 columns of the wave, through the buffer that the last step did not read; columns exchanged by kq, for the banks
+    float* const way = reinterpret_cast<float*>(xs + (BUFFERS == 2 ? steps & 1 : 0) * S::X_BYTES) + wave * 1024;
+    auto put = [&](auto whole_wave) {
+        constexpr bool WHOLE = decltype(whole_wave)::value;
+#pragma unroll 1
+        for (int t = 0; t < NT; t += 2) {
+            const int row = wave_row + 16 * t;
+            if (!WHOLE && row >= q.rows) break;
+            RawOf<OUT> residual[2][4];
+            if (q.residual)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) results.template fetch<WHOLE>(row + 16 * u, residual[u]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float4_v v[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) way[(4 * kq + i) * 64 + (b ^ kq) * 16 + c] = total[u][b][i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float4_v*>(way + (4 * kq + i) * 64 + (c / 4 ^ kq) * 16 + c % 4 * 4);
+                results.finish(v, biases + wr * 16 * NT + 16 * (t + u) + 4 * kq, residual[u]);
+                results.template store<WHOLE>(row + 16 * u, v);
+            }
+#pragma unroll
+            for (int u = 0; u + 2 < NT; ++u)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) total[u][b] = total[u + 2][b];
+        }
+    };
+    if (wave_column >= from && wave_row + 16 * NT <= q.rows) put(std::true_type());
+    else put(std::false_type());
 }
 
 // ---- few columns: the waves of a block share 64 columns and 16 rows, and the steps are divided among them ----
 
 constexpr int kSplitWaves = 8;
 template <int OUT, bool COMPLEX, bool CAREFUL>
-__device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, long column0, int row0, bool few)
+__device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, long from, int row0)
 {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const long column0 = CAREFUL || from + kColumns <= q.columns ? from : q.columns - kColumns;
     const Input<COMPLEX, CAREFUL> in(q, column0);
     float4_v total[4] = {};
-    sum_steps<OUT, COMPLEX, CAREFUL>(q, in, row0, wave, kSplitWaves, few, total);
+    sum_steps<OUT, COMPLEX, CAREFUL>(q, in, row0, wave, kSplitWaves, total);
     // joined in a fixed order: wave i takes the rows 4 kq + i
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[(wave * 4 + i) * 64 + lane] = row_of(total, i);
@@ -448,42 +711,79 @@ __device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, 
     float4_v v[1] = { sums[wave * 64 + lane] };
 #pragma unroll
     for (int u = 1; u < kSplitWaves; ++u) v[0] += sums[(u * 4 + wave) * 64 + lane];
-    put_rows<OUT, COMPLEX, 1>(q, in.column0 + 4 * in.c, 0, row0 + 4 * in.kq + wave, v);
+    const int row = row0 + 4 * in.kq + wave;
+    if (row >= q.rows || column0 + 4 * in.c >= q.columns) return;
+    const Results<OUT, COMPLEX, 1> results = { q, column0, from, in.c, 4 * in.kq + wave };
+    float bias[COMPLEX ? 2 : 1];
+    if (q.bias)
+#pragma unroll
+        for (int i = 0; i < (COMPLEX ? 2 : 1); ++i) bias[i] = results.bias_at(row, i);
+    RawOf<OUT> residual[1];
+    if (q.residual) results.template fetch<false>(row0, residual);
+    results.finish(v, bias, residual);
+    results.template store<false>(row0, v);
 }
-template <int OUT, bool COMPLEX> __global__ __launch_bounds__(64 * kSplitWaves, 2) void mix_blocks_split_kernel(const MixBlocksParams q, int row_tiles, bool careful, bool few)
+template <int OUT, bool COMPLEX> __global__ __launch_bounds__(64 * kSplitWaves, 2) void mix_blocks_split_kernel(const MixBlocksParams q, int row_tiles, bool careful)
 {
     __shared__ float4_v sums[kSplitWaves * 4 * 64];
     const long id = block_index(), column0 = id / row_tiles * kColumns;
     if (column0 >= q.columns) return;
     const int row0 = (int)(id % row_tiles) * 16;
-    if (careful || column0 + kColumns > q.columns) split<OUT, COMPLEX, true>(q, sums, column0, row0, few);
-    else split<OUT, COMPLEX, false>(q, sums, column0, row0, few);
+    if (careful) split<OUT, COMPLEX, true>(q, sums, column0, row0);
+    else split<OUT, COMPLEX, false>(q, sums, column0, row0);
 }
 
-template <int OUT, bool COMPLEX, int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t stream)
+template <int OUT, int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t stream)
 {
     const long column_tiles = (q.columns + 4 * kColumns - 1) / (4 * kColumns);
     const int row_tiles = (q.rows + 16 * NT - 1) / (16 * NT);
     const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_tile_kernel<OUT, COMPLEX, NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(256), 0, stream, q, row_tiles,
+    hipLaunchKernelGGL((mix_blocks_tile_kernel<OUT, true, NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(256), 0, stream, q, row_tiles,
                        column_tiles, by_xcd);
     return hipGetLastError();
 }
-template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, hipStream_t stream)
+template <int OUT, int NT, int RG, int CG, int BUFFERS, int WAVES> hipError_t launch_staged(const MixBlocksParams& q, hipStream_t stream)
 {
-    // a lane's part of an address in 32 bits, 48 rows of the input (complex: 24); weights that cannot be read by 16
-    const bool few = (long)q.rows * q.contraction * (COMPLEX ? 2 : 1) < 16, careful = few || 48 * q.ldx >= (1L << 32) - 4096;
+    typedef Staged<OUT, NT, RG, CG, BUFFERS> S;
+    static std::atomic<unsigned long long> served{ 0 };
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, BUFFERS, WAVES>), S::LDS, served); e != hipSuccess) return e;
+    const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
+    const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
+    const bool by_xcd = column_tiles >= 64;
+    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, BUFFERS, WAVES>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(S::THREADS), S::LDS, stream, q,
+                       row_tiles, column_tiles, by_xcd);
+    return hipGetLastError();
+}
+// Up to this number of real values the contraction is one step or less than half of one: the product with scales per position and row has kernels for it, whose scales
+// are those of one block. bf16, 64 to 64 channels at 2^20 positions 54 us (here 59 - 70), 16 to 16 at 10^6 16 us (40); 128 to 128 at 262144 29 us (26)
+constexpr int kOneBlock = 64;
+// Blocks of 64 columns and 16 rows up to which their waves divide the steps: bf16, 1024 to 1024 channels at 256 positions 7.2 us (tiles 8.1), at 512 12.9 (8.3)
+constexpr long kSplitBlocks = 256;
+// Tiles of 128 rows from which they are enough for the GPU: bf16, 1024 to 1024 at 8192 positions 18.8 us (with 64 rows 21.9), at 4096 14.9 (14.2), at 2048 12.6 (10.6)
+constexpr long kWholeTiles = 384;
+template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int type, hipStream_t stream)
+{
+    if (q.contraction * (COMPLEX ? 2 : 1) <= kOneBlock) {
+        const MixParams p = { q.x, nullptr, q.W, q.bias, q.residual, q.xscale, q.wscale, q.y, nullptr, q.columns, q.ldx, 0, q.ldr, q.ldy, 0, q.rows, q.contraction, q.contraction, q.act,
+                              kScaleShift };
+        return launch_mix_8bit(p, type, stream);
+    }
+    // a lane's part of an address in 32 bits, 48 rows of the input (complex: 24) and 12 of the results
+    const bool near = 48 * q.ldx < (1L << 32) - 4096 && 12 * std::max(q.ldr, q.ldy) * (long)sizeof(typename Columns<OUT>::Value) < (1L << 32) - 4096;
     const int tiles16 = (q.rows + 15) / 16;
-    const long wide = (q.columns + 4 * kColumns - 1) / (4 * kColumns);
-    if (careful || q.columns < kColumns || wide * ((tiles16 + 1) / 2) < 256) {
-        const long columns = (q.columns + kColumns - 1) / kColumns;
-        hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX>), grid_of(columns * tiles16), dim3(64 * kSplitWaves), 0, stream, q, tiles16, careful, few);
+    const long columns = (q.columns + kColumns - 1) / kColumns;
+    if (!near || q.columns < 2 * kColumns || columns * tiles16 <= kSplitBlocks) {
+        hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX>), grid_of(columns * tiles16), dim3(64 * kSplitWaves), 0, stream, q, tiles16, !near || q.columns < kColumns);
         return hipGetLastError();
     }
-    if constexpr (OUT != kIn32)
-        if (tiles16 > 4 && wide * ((tiles16 + 7) / 8) >= 256) return launch_tiles<OUT, COMPLEX, 8>(q, stream);
-    if (tiles16 > 2 && wide * ((tiles16 + 3) / 4) >= 256) return launch_tiles<OUT, COMPLEX, 4>(q, stream);
-    return launch_tiles<OUT, COMPLEX, 2>(q, stream);
+    if constexpr (COMPLEX) {
+        const long wide = (columns + 3) / 4;
+        if (tiles16 > 2 && wide * ((tiles16 + 3) / 4) >= 256) return launch_tiles<OUT, 4>(q, stream);
+        return launch_tiles<OUT, 2>(q, stream);
+    } else {
+        if ((columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 2>(q, stream);
+        return launch_staged<OUT, 2, 2, 2, OUT == kIn32 ? 2 : 1, OUT == kIn32 ? 3 : 4>(q, stream);
+    }
 }
 
 }  // namespace
@@ -492,9 +792,9 @@ hipError_t launch_mix_8bit_blocks(const MixBlocksParams& q, int type, hipStream_
 {
     if (q.columns == 0) return hipSuccess;
     switch (type) {
-    case kC64: return launch<kIn32, true>(q, stream);
-    case kF32: return launch<kIn32, false>(q, stream);
-    default: return launch<kIn16, false>(q, stream);
+    case kC64: return launch<kIn32, true>(q, type, stream);
+    case kF32: return launch<kIn32, false>(q, type, stream);
+    default: return launch<kIn16, false>(q, type, stream);
     }
 }
 

@@ -36,6 +36,7 @@ struct MixParams {
     long columns, ldx, ldzin, ldr, ldy, ldz;            // in real values of their tensors
     int rows, contraction, ldw;                         // channels of the result, channels of the input, channels in a row of W
     int act;
+    int scale_rows = 0;                                 // rows of a wscale: 2^scale_rows
 };
 
 // ---- activations ----
@@ -423,7 +424,7 @@ template <int IN, int OUT, bool COMPLEX, bool GRAD, int NT, bool FAR, bool RAGGE
     {
         float4_v v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = q.wscale[first + i < q.rows ? first + i : q.rows - 1];
+        for (int i = 0; i < 4; ++i) v[i] = q.wscale[(first + i < q.rows ? first + i : q.rows - 1) >> q.scale_rows];
         return v;
     }
     template <int ACT> static __device__ __forceinline__ void act_rows(float4_v (&v)[4])

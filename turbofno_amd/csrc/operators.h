@@ -94,7 +94,7 @@ struct DropoutParams {
 hipError_t launch_dropout(const DropoutParams& q, int type, hipStream_t stream);
 
 // A field in 8 bits with a scale per position and block of 128 channels, strides in real values
-constexpr int kScaleBlock = 128;                        // channels of a scale
+constexpr int kScaleShift = 7, kScaleBlock = 1 << kScaleShift;         // channels of a scale
 struct QuantiseParams {
     const void* x;
     void* q;

@@ -26,11 +26,17 @@ template <int LANES, int COUNT, typename F> __device__ __forceinline__ void over
         for (int c = 0; c < COUNT; ++c) shared[(c * WAVES + wave) * LANES + lane] = v[c];
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < COUNT; ++c) {
-        v[c] = shared[c * WAVES * LANES + lane];
+    for (int c = 0; c < COUNT; ++c) v[c] = shared[c * WAVES * LANES + lane];
+    auto add = [&](int w) {
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) v[c] = join(v[c], shared[(c * WAVES + w) * LANES + lane]);
-    }
+        for (int c = 0; c < COUNT; ++c) v[c] = join(v[c], shared[(c * WAVES + w) * LANES + lane]);
+    };
+    if constexpr (COUNT <= 2) {
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) add(w);
+    } else                                              // few registers at a time
+#pragma unroll 1
+        for (int w = 1; w < WAVES; ++w) add(w);
 }
 // largest magnitudes per position, of COUNT blocks of channels
 template <bool COMPLEX, int LANES, int COUNT> __device__ __forceinline__ void block_maxima(float4_v (&most)[COUNT], float4_v* shared)

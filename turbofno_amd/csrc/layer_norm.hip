@@ -42,11 +42,17 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
     auto fetch = [&](int first, auto& v) {
         constexpr int COUNT = sizeof(v) / sizeof(v[0]);
         RawOf<IN> x[COUNT], residual[COUNT];            // all loads first: channels beyond the last read another one
+        if constexpr (!FULL)
 #pragma unroll
-        for (int r = 0; r < COUNT; ++r) x[r] = strip.template read<IN, FULL>(q.x, q.ldx, column0, there, first + r);
-        if (q.residual)
+            for (int r = 0; r < COUNT; ++r) x[r] = residual[r] = zero4<IN>();
+        for_lane<FULL>(lane_there, [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-            for (int r = 0; r < COUNT; ++r) residual[r] = strip.template read<IN, FULL>(q.residual, q.ldr, column0, there, first + r);
+            for (int r = 0; r < COUNT; ++r) x[r] = strip.template read<IN, WHOLE>(q.x, q.ldx, column0, there, first + r);
+            if (q.residual)
+#pragma unroll
+                for (int r = 0; r < COUNT; ++r) residual[r] = strip.template read<IN, WHOLE>(q.residual, q.ldr, column0, there, first + r);
+        });
         unsigned bits[COUNT];
         if constexpr (DROP) {
             __builtin_amdgcn_sched_barrier(0);
@@ -122,8 +128,8 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
                 if (strip.has(first + r)) {
-                    if (q.s) strip.template write<IN, FULL>(q.s, q.lds, column0, there, first + r, from_float<IN>(four(v[r])));
-                    strip.template write<IN, FULL>(q.y, q.ldy, column0, there, first + r, from_float<IN>(result(first + r, four(v[r]))));
+                    if (q.s) write_row<IN, FULL>(strip, q.s, q.lds, column0, there, first + r, from_float<IN>(four(v[r])));
+                    write_row<IN, FULL>(strip, q.y, q.ldy, column0, there, first + r, from_float<IN>(result(first + r, four(v[r]))));
                 }
         };
         if constexpr (HELD > 0) finish(0, held);
@@ -141,7 +147,7 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
 #pragma unroll
             for (int r = 0; r < COUNT_ROWS; ++r)
                 if (strip.has(first + r)) {
-                    if (q.s) strip.template write<IN, FULL>(q.s, q.lds, column0, there, first + r, from_float<IN>(four(v[r])));
+                    if (q.s) write_row<IN, FULL>(strip, q.s, q.lds, column0, there, first + r, from_float<IN>(four(v[r])));
                     const float4_v y = result(first + r, four(v[r]));
                     most[r / OF_BLOCK] = larger4(most[r / OF_BLOCK], magnitude(y));
 #pragma unroll
@@ -155,7 +161,7 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
                 const float4_v factor = write_scales<COMPLEX, FULL>(q.rstd + (block + c) * q.positions, column, lane_there, strip.group() == 0, most[c]);
 #pragma unroll
                 for (int r = c * OF_BLOCK; r < (c + 1) * OF_BLOCK && r < COUNT_ROWS; ++r)
-                    if (strip.has(first + r)) strip.template write<kIn8, FULL>(q.y, q.ldy, column0, there, first + r, eight_bits(four(v[r]), factor));
+                    if (strip.has(first + r)) write_row<kIn8, FULL>(strip, q.y, q.ldy, column0, there, first + r, eight_bits(four(v[r]), factor));
             }
         };
         if constexpr (HELD > 0) finish(0, held);
@@ -171,7 +177,7 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
 // areas of LDS for joins: the mean's, the squares' (two values where channels are read again), and the maxima of blocks of 128 channels
 template <bool EIGHT, int LANES, int HELD> constexpr int kAreas = (HELD ? 2 : 3) + (!EIGHT ? 0 : HELD ? (HELD * (kThreads / LANES) + kScaleBlock - 1) / kScaleBlock : 2);
 template <int IN, bool COMPLEX, bool DROP, bool EIGHT, int LANES, int HELD>
-__global__ __launch_bounds__(kThreads, IN == kIn16 && HELD < 16 ? 4 : 2) void layer_norm_kernel(const LayerNormParams q)
+__global__ __launch_bounds__(kThreads, (IN == kIn16 && HELD < 16 && !(EIGHT && LANES < 16) ? 4 : 2)) void layer_norm_kernel(const LayerNormParams q)
 {
     typedef Strip<LANES> S;
     const long column0 = block_index() * S::COLUMNS;
@@ -189,21 +195,33 @@ template <int IN, bool COMPLEX, bool DROP, bool EIGHT, int LANES, int HELD> hipE
     hipLaunchKernelGGL((layer_norm_kernel<IN, COMPLEX, DROP, EIGHT, LANES, HELD>), grid_of((q.columns + 4 * LANES - 1) / (4 * LANES)), dim3(kThreads), 0, stream, q);
     return hipGetLastError();
 }
+// Lanes side by side and channels held: wide strips read long pieces of a row, narrow ones give the GPU more blocks, and hold more channels
 template <int IN, bool COMPLEX, bool DROP, bool EIGHT> hipError_t launch(const LayerNormParams& q, hipStream_t stream)
 {
-    // a lane's part of an address, up to three channels, in 32 bits; with 64 lanes side by side it has no channel in it
-    const bool far = std::max(std::max(q.ldx, q.ldr), std::max(q.lds, q.ldy)) >= kFar;
-    if (q.columns < kFewColumns && !far) {
+    if (far_apart(std::max(std::max(q.ldx, q.ldr), std::max(q.lds, q.ldy)))) {         // with 64 lanes side by side a lane's part of an address has no channel in it
+        if (q.K <= 32) return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 4>(q, stream);
+        if (q.K <= 64) return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 8>(q, stream);
+        return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 0>(q, stream);
+    }
+    if (q.K <= 64 && q.columns >= kFewColumns) return q.K <= 32 ? launch_as<IN, COMPLEX, DROP, EIGHT, 64, 4>(q, stream) : launch_as<IN, COMPLEX, DROP, EIGHT, 64, 8>(q, stream);
+    if (q.K <= 256 && q.columns < kFewColumns / (q.K <= 64 ? 1 : 2)) {
         if (q.K <= 64) return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 2>(q, stream);
         if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 4>(q, stream);
-        if (q.K <= 256) return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 8>(q, stream);
+        return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 8>(q, stream);
     }
-    if (q.K <= 32) return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 4>(q, stream);
-    if (q.K <= 64) return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 8>(q, stream);
-    if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 16>(q, stream);
-    if (far) return launch_as<IN, COMPLEX, DROP, EIGHT, 64, 0>(q, stream);
+    // bf16, 128 channels at 262144 columns 60 us, 65 with 64 lanes; float32, 256 at 65536 53 us, 58 with 16
+    if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, EIGHT, 32, 8>(q, stream);
     if (q.K <= 256) return launch_as<IN, COMPLEX, DROP, EIGHT, 32, 16>(q, stream);
-    if (q.K <= 512) return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 16>(q, stream);
+    // float32, 512 channels at 4000 columns 8.7 us, 11.2 with 16 lanes; at 16000 24.1 and 23.0
+    if (q.K <= 512) return q.columns < kNarrowColumns ? launch_as<IN, COMPLEX, DROP, EIGHT, 8, 8>(q, stream) : launch_as<IN, COMPLEX, DROP, EIGHT, 16, 16>(q, stream);
+    // bf16, 1024 channels, strips read once with 4 or 8 lanes, and twice with 16: at 1000 columns 10.3, 11.3 and 25 us, at 4000 18, 13 and 27, at 16000 60, 42 and 38;
+    // float32 at 16000 86, 64 and 75 us, at 32000 178, 127 and 158
+    if (q.K <= 1024) {
+        if (q.columns <= 1024) return launch_as<IN, COMPLEX, DROP, EIGHT, 4, 8>(q, stream);
+        if (q.columns < kNarrowColumns || (IN == kIn32 && !EIGHT)) return launch_as<IN, COMPLEX, DROP, EIGHT, 8, 16>(q, stream);
+    }
+    // bf16, 2048 channels at 1000 columns 16 us, 50 with 16 lanes; at 16000 157 and 87
+    if (q.columns < kNarrowColumns) return q.K <= 2048 ? launch_as<IN, COMPLEX, DROP, EIGHT, 4, 16>(q, stream) : launch_as<IN, COMPLEX, DROP, EIGHT, 4, 0>(q, stream);
     return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 0>(q, stream);
 }
 template <int IN, bool COMPLEX> hipError_t launch(const LayerNormParams& q, bool eight, hipStream_t stream)

@@ -61,10 +61,10 @@ __device__ __forceinline__ void write_gradients(const LayerNormGradParams& q, co
     float4_v v = f.rstd * (g - f.level - h * f.slope);
     if (q.gs) v += to_float<IN>(gs);
     if constexpr (DROP) {
-        strip.template write<IN, FULL>(q.gr, q.ldgr, column0, there, r, from_float<IN>(v));
+        write_row<IN, FULL>(strip, q.gr, q.ldgr, column0, there, r, from_float<IN>(v));
         v = Keep<COMPLEX>::apply(v, bits, q.drop.lift);
     }
-    strip.template write<IN, FULL>(q.gx, q.ldgx, column0, there, r, from_float<IN>(v));
+    write_row<IN, FULL>(strip, q.gx, q.ldgx, column0, there, r, from_float<IN>(v));
 }
 
 template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD, bool FULL>
@@ -73,12 +73,17 @@ __device__ __forceinline__ void layer_norm_grad_strip(const LayerNormGradParams&
     const Strip<LANES> strip(q.K);
     auto gain = [&](int r) { return gains[r * strip.GROUPS + strip.group()]; };
     RawOf<IN> gy[HELD], s[HELD], gs[HELD];
-#pragma unroll
-    for (int r = 0; r < HELD; ++r) {
-        gy[r] = strip.template read<IN, FULL>(q.gy, q.ldgy, column0, there, r);
-        s[r] = strip.template read<IN, FULL>(q.s, q.lds, column0, there, r);
-    }
     const int lane_there = there - 4 * strip.lane;
+    if constexpr (!FULL)
+#pragma unroll
+        for (int r = 0; r < HELD; ++r) gy[r] = s[r] = gs[r] = zero4<IN>();
+    for_lane<FULL>(lane_there, [&](auto whole) {
+#pragma unroll
+        for (int r = 0; r < HELD; ++r) {
+            gy[r] = strip.template read<IN, decltype(whole)::value>(q.gy, q.ldgy, column0, there, r);
+            s[r] = strip.template read<IN, decltype(whole)::value>(q.s, q.lds, column0, there, r);
+        }
+    });
     const long column = column0 + 4 * strip.lane;
     Shares f;
     read_shares<COMPLEX, FULL>(q, column, lane_there, f);
@@ -99,8 +104,10 @@ __device__ __forceinline__ void layer_norm_grad_strip(const LayerNormGradParams&
             sums[r].template add<FULL>(v, h, lane_there);
         }
     if (q.gs)
+        for_lane<FULL>(lane_there, [&](auto whole) {
 #pragma unroll
-        for (int r = 0; r < HELD; ++r) gs[r] = strip.template read<IN, FULL>(q.gs, q.ldgs, column0, there, r);
+            for (int r = 0; r < HELD; ++r) gs[r] = strip.template read<IN, decltype(whole)::value>(q.gs, q.ldgs, column0, there, r);
+        });
     join_shares<COMPLEX, LANES>(joint, shared, q.K, f);
 #pragma unroll
     for (int r = 0; r < HELD; ++r)
@@ -153,11 +160,16 @@ __device__ __forceinline__ void layer_norm_grad_long_strip(const LayerNormGradPa
     float4_v joint[2] = {};
     for (int r0 = 0; r0 < rounds; r0 += kChunk) {
         RawOf<IN> gy[kChunk], s[kChunk];
+        if constexpr (!FULL)
 #pragma unroll
-        for (int r = 0; r < kChunk; ++r) {
-            gy[r] = strip.template read<IN, FULL>(q.gy, q.ldgy, column0, there, r0 + r);
-            s[r] = strip.template read<IN, FULL>(q.s, q.lds, column0, there, r0 + r);
-        }
+            for (int r = 0; r < kChunk; ++r) gy[r] = s[r] = zero4<IN>();
+        for_lane<FULL>(lane_there, [&](auto whole) {
+#pragma unroll
+            for (int r = 0; r < kChunk; ++r) {
+                gy[r] = strip.template read<IN, decltype(whole)::value>(q.gy, q.ldgy, column0, there, r0 + r);
+                s[r] = strip.template read<IN, decltype(whole)::value>(q.s, q.lds, column0, there, r0 + r);
+            }
+        });
 #pragma unroll
         for (int r = 0; r < kChunk; ++r)
             if (strip.has(r0 + r)) {
@@ -172,14 +184,17 @@ __device__ __forceinline__ void layer_norm_grad_long_strip(const LayerNormGradPa
     for (int r0 = 0; r0 < rounds; r0 += PART) {
         RawOf<IN> gy[PART], s[PART], gs[PART];
         unsigned bits[PART] = {};
+        if constexpr (!FULL)
 #pragma unroll
-        for (int r = 0; r < PART; ++r) {
-            gy[r] = strip.template read<IN, FULL>(q.gy, q.ldgy, column0, there, r0 + r);
-            s[r] = strip.template read<IN, FULL>(q.s, q.lds, column0, there, r0 + r);
-        }
-        if (q.gs)
+            for (int r = 0; r < PART; ++r) gy[r] = s[r] = gs[r] = zero4<IN>();
+        for_lane<FULL>(lane_there, [&](auto whole) {
 #pragma unroll
-            for (int r = 0; r < PART; ++r) gs[r] = strip.template read<IN, FULL>(q.gs, q.ldgs, column0, there, r0 + r);
+            for (int r = 0; r < PART; ++r) {
+                gy[r] = strip.template read<IN, decltype(whole)::value>(q.gy, q.ldgy, column0, there, r0 + r);
+                s[r] = strip.template read<IN, decltype(whole)::value>(q.s, q.lds, column0, there, r0 + r);
+                if (q.gs) gs[r] = strip.template read<IN, decltype(whole)::value>(q.gs, q.ldgs, column0, there, r0 + r);
+            }
+        });
         if constexpr (DROP)
 #pragma unroll
             for (int r = 0; r < PART; r += 2) keep.pair(strip.channel(r0 + r), strip.channel(r0 + r + 1), bits[r], bits[r + 1]);
@@ -218,14 +233,17 @@ template <int IN, bool COMPLEX, bool DROP, int LANES> __global__ __launch_bounds
 }
 
 // The blocks' sums, 16 values per block, always in the same order; those of the bias may not be asked for
-__global__ __launch_bounds__(256) void add_sums_kernel(const float* __restrict__ sums, long blocks, int K, int count, float* __restrict__ ggain, float* __restrict__ gbias)
+__global__ __launch_bounds__(1024) void add_sums_kernel(const float* __restrict__ sums, long blocks, int K, int count, float* __restrict__ ggain, float* __restrict__ gbias)
 {
     __shared__ float part[16][17];
     const int c = threadIdx.x % 16, r = threadIdx.x / 16, value = blockIdx.x * 16 + c;
     float v = 0.f;
     if (value < count)
-        for (long b = r; b < blocks; b += 16) v += sums[b * count + value];
-    part[r][c] = v;
+#pragma unroll 8
+        for (long b = r; b < blocks; b += 64) v += sums[b * count + value];
+    v += __shfl_xor(v, 16, 64);                         // four rows of a wave
+    v += __shfl_xor(v, 32, 64);
+    if (threadIdx.x % 64 < 16) part[r / 4][c] = v;
     __syncthreads();
     if (r || value >= count) return;
 #pragma unroll
@@ -234,39 +252,41 @@ __global__ __launch_bounds__(256) void add_sums_kernel(const float* __restrict__
     else if (gbias) gbias[value - K] = v;
 }
 
-
-constexpr int kGradHeldChannels = 256;                  // 8 per lane, 32 side by side
 constexpr long kGradBlocks = 512;                       // persistent blocks
 
-// lanes side by side: by the channels that registers hold, fewer where wide strips would leave most of the GPU idle
-int grad_lanes(int K, long columns) { return columns < kFewColumns ? 16 : K <= 64 ? 64 : K <= 128 ? 32 : 16; }
-long grad_strips(int K, long columns) { return (columns + 4 * grad_lanes(K, columns) - 1) / (4 * grad_lanes(K, columns)); }
-long grad_blocks(int K, long columns) { return std::min(grad_strips(K, columns), kGradBlocks); }
-
-template <int IN, bool COMPLEX, bool DROP> hipError_t launch_grad(const LayerNormGradParams& q, hipStream_t stream)
+// Lanes side by side and channels held per lane (0: read twice). The workspace is for as many blocks as there are strips of the narrowest kind
+template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD> hipError_t launch_as(const LayerNormGradParams& q, hipStream_t stream)
 {
-    const bool far = std::max(std::max(q.ldgy, q.lds), std::max(std::max(q.ldgs, q.ldgr), q.ldgx)) >= kFar;
-    const long wide = (q.columns + 255) / 256, strips = far ? wide : grad_strips(q.K, q.columns), blocks = std::min(strips, grad_blocks(q.K, q.columns));
-    const dim3 grid((unsigned)blocks);
-#define TFNO_GRAD(LANES, HELD) hipLaunchKernelGGL((layer_norm_grad_kernel<IN, COMPLEX, DROP, LANES, HELD>), grid, dim3(kThreads), 0, stream, q, strips)
+    const long strips = (q.columns + 4 * LANES - 1) / (4 * LANES), blocks = std::min(strips, kGradBlocks);
     if (blocks) {
-        if (far) {
-            if (q.K <= 64) TFNO_GRAD(64, 8);
-            else hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, 64>), grid, dim3(kThreads), 0, stream, q, strips);
-        } else if (q.K > kGradHeldChannels) hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, 16>), grid, dim3(kThreads), 0, stream, q, strips);
-        else if (grad_lanes(q.K, q.columns) == 64) {
-            if (q.K <= 32) TFNO_GRAD(64, 4);
-            else TFNO_GRAD(64, 8);
-        } else if (grad_lanes(q.K, q.columns) == 32) TFNO_GRAD(32, 8);
-        else if (q.K <= 64) TFNO_GRAD(16, 2);
-        else if (q.K <= 128) TFNO_GRAD(16, 4);
-        else TFNO_GRAD(16, 8);
+        if constexpr (HELD > 0) hipLaunchKernelGGL((layer_norm_grad_kernel<IN, COMPLEX, DROP, LANES, HELD>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, strips);
+        else hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, LANES>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, strips);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
-#undef TFNO_GRAD
     const int count = q.K * (COMPLEX ? 3 : 2);
-    hipLaunchKernelGGL(add_sums_kernel, dim3((unsigned)((count + 15) / 16)), dim3(256), 0, stream, q.sums, blocks, q.K, count, q.ggain, q.gbias);
+    hipLaunchKernelGGL(add_sums_kernel, dim3((unsigned)((count + 15) / 16)), dim3(1024), 0, stream, q.sums, blocks, q.K, count, q.ggain, q.gbias);
     return hipGetLastError();
+}
+template <int IN, bool COMPLEX, bool DROP> hipError_t launch_grad(const LayerNormGradParams& q, hipStream_t stream)
+{
+    if (far_apart(std::max(std::max(q.ldgy, q.lds), std::max(std::max(q.ldgs, q.ldgr), q.ldgx))))      // with 64 lanes side by side a lane's part of an address has no channel in it
+        return q.K <= 64 ? launch_as<IN, COMPLEX, DROP, 64, 8>(q, stream) : launch_as<IN, COMPLEX, DROP, 64, 0>(q, stream);
+    if (q.K <= 64 && q.columns >= kFewColumns) return q.K <= 32 ? launch_as<IN, COMPLEX, DROP, 64, 4>(q, stream) : launch_as<IN, COMPLEX, DROP, 64, 8>(q, stream);
+    if (q.K <= 64) return launch_as<IN, COMPLEX, DROP, 16, 2>(q, stream);
+    // bf16, 128 channels at 262144 columns 84 us, 90 with 32 lanes
+    if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, 16, 4>(q, stream);
+    if (q.K <= 256) return launch_as<IN, COMPLEX, DROP, 16, 8>(q, stream);
+    const bool few = q.columns < kNarrowColumns;
+    // bf16, 512 channels at 65536 columns 99 us (8 lanes 131, read twice 132), 300 at 4000 18.6 us (8 lanes 12.3); 32 bits spill with 16 channels
+    if (q.K <= 512) {
+        if constexpr (IN == kIn16)
+            if (!few) return launch_as<IN, COMPLEX, DROP, 16, 16>(q, stream);
+        return launch_as<IN, COMPLEX, DROP, 8, 8>(q, stream);
+    }
+    // float32, 1024 channels at 4000 columns 28.6 us, 53 where the strip is read twice, at 16384 113 and 100; bf16, 2048 at 2000 44 and 95
+    if (q.K <= 1024 && few) return launch_as<IN, COMPLEX, DROP, 4, 8>(q, stream);
+    if (q.K <= 2048 && q.columns < kNarrowColumns / 2) return launch_as<IN, COMPLEX, DROP, 2, 8>(q, stream);
+    return few ? launch_as<IN, COMPLEX, DROP, 4, 0>(q, stream) : launch_as<IN, COMPLEX, DROP, 16, 0>(q, stream);
 }
 template <int IN, bool COMPLEX> hipError_t launch_grad(const LayerNormGradParams& q, hipStream_t stream)
 {
@@ -277,7 +297,7 @@ template <int IN, bool COMPLEX> hipError_t launch_grad(const LayerNormGradParams
 
 size_t layer_norm_backward_workspace(int type, long P, int K)
 {
-    const long blocks = grad_blocks(K, P * values_of(type));
+    const long blocks = std::min((P * values_of(type) + 7) / 8, kGradBlocks);          // strips of 8 columns are the narrowest
     return (size_t)(blocks ? blocks : 1) * K * (1 + values_of(type)) * sizeof(float);
 }
 

@@ -29,8 +29,10 @@ template <bool COMPLEX> struct RawStep {
     unsigned row[2][kRowsOfHalf<COMPLEX>];              // four columns of the lane's channels
     float4_v scale;                                     // of the columns
 };
-// 64 columns of a wave, from column0 on. CAREFUL: only `there` of them may exist, at least one, and channels may lie any distance apart
-template <bool COMPLEX, bool CAREFUL> struct Input {
+// 64 columns of a wave, from column0 on. kWindow: all of them exist; otherwise `there` of them, at least one, and a word that would end behind the last value of all starts
+// earlier and is shifted (what it holds beyond its row's end is not used): kNarrow by 32-bit offsets from the first value, kFar whatever lies between the channels
+enum { kWindow = 0, kNarrow = 1, kFar64 = 2 };
+template <bool COMPLEX, int MODE> struct Input {
     static constexpr int V = COMPLEX ? 2 : 1, HALF = kRowsOfHalf<COMPLEX>;
     const MixBlocksParams& q;
     const int c, kq, there;
@@ -41,24 +43,27 @@ template <bool COMPLEX, bool CAREFUL> struct Input {
     template <bool GUARD> __device__ __forceinline__ void fetch(int step, RawStep<COMPLEX>& raw) const
     {
         const int first = step * (kStep / V);
-        const unsigned quarter = fresh((unsigned)(kq * HALF) * (unsigned)q.ldx + 4 * c);
+        const unsigned quarter = fresh((unsigned)(kq * HALF) * (unsigned)q.ldx + (MODE == kWindow || 4 * c < there ? 4 * c : 0));
+        const unsigned end = MODE == kNarrow ? (unsigned)((q.contraction - 1) * q.ldx + q.columns - 4) : 0;     // of the last word
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < HALF; ++j) {
                 const int k = first + h * 4 * HALF + j;         // the first quarter's
-                if constexpr (CAREFUL) {
-                    // a word that would end behind the last value of all starts earlier and is shifted; what it holds beyond its row's end is not used
+                if constexpr (MODE == kFar64) {
                     const long row = k + kq * HALF < q.contraction ? k + kq * HALF : q.contraction - 1;
                     const long at = row * q.ldx + column0 + (4 * c < there ? 4 * c : 0), last = (q.contraction - 1) * q.ldx + q.columns - 4;
                     raw.row[h][j] = *reinterpret_cast<const uint_any*>(static_cast<const unsigned char*>(q.x) + (at < last ? at : last)) >> (at > last ? 8 * (int)(at - last) : 0);
+                } else if constexpr (MODE == kNarrow) {
+                    const unsigned at = quarter + (unsigned)k * (unsigned)q.ldx, by = at < end ? at : end;      // rows beyond the last: the last word, any shift
+                    raw.row[h][j] = near_load4<kIn8>(scalar(q.x, 0), by) >> (8 * (at - by) & 31);
                 } else if constexpr (GUARD) {
                     const int common = k < q.contraction ? k : q.contraction - 1;
                     raw.row[h][j] = near_load4<kIn8>(scalar(q.x, common * q.ldx + column0), fresh(k + kq * HALF < q.contraction ? quarter : 4 * c));
                 } else raw.row[h][j] = near_load4<kIn8>(scalar(q.x, k * q.ldx + column0), quarter);
             }
         const long scales = step / V * q.positions;
-        if constexpr (CAREFUL)
+        if constexpr (MODE != kWindow)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const long column = column0 + 4 * c + i;
@@ -310,8 +315,8 @@ template <int OUT, bool COMPLEX> __device__ __forceinline__ void put_plain(const
 
 // ---- 16 rows of one wave, steps wave, wave + waves ...: weights straight from memory ----
 
-template <int OUT, bool COMPLEX, bool CAREFUL>
-__device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<COMPLEX, CAREFUL>& in, int row0, int first, int stride, float4_v (&total)[4])
+template <int OUT, bool COMPLEX, int MODE>
+__device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<COMPLEX, MODE>& in, int row0, int first, int stride, float4_v (&total)[4])
 {
     const int count = q.contraction * (COMPLEX ? 2 : 1), steps = (count + kStep - 1) / kStep;
     const int blocks = (q.contraction + kScaleBlock - 1) / kScaleBlock;
@@ -363,7 +368,7 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     if (column_tile >= column_tiles) return;
     const int row0 = (int)(slot % row_tiles) * (16 * NT), lane = threadIdx.x & 63;
     const long from = column_tile * (4 * kColumns) + (long)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kColumns;
-    const Input<COMPLEX, false> in(q, scalar(from + kColumns <= q.columns ? from : q.columns - kColumns));
+    const Input<COMPLEX, kWindow> in(q, scalar(from + kColumns <= q.columns ? from : q.columns - kColumns));
     const int count = q.contraction * (COMPLEX ? 2 : 1), steps = (count + kStep - 1) / kStep;
     const float* wscale = q.wscale + (long)(row0 / kScaleBlock) * ((q.contraction + kScaleBlock - 1) / kScaleBlock);
     const int whole = count / kStep;                    // steps of 128 values
@@ -695,15 +700,24 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
 // ---- few columns: the waves of a block share 64 columns and 16 rows, and the steps are divided among them ----
 
 constexpr int kSplitWaves = 8;
-template <int OUT, bool COMPLEX, bool CAREFUL>
+template <int OUT, bool COMPLEX, int MODE>
 __device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, long from, int row0)
 {
+    constexpr int V = COMPLEX ? 2 : 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const long column0 = CAREFUL || from + kColumns <= q.columns ? from : q.columns - kColumns;
-    const Input<COMPLEX, CAREFUL> in(q, column0);
+    const long column0 = MODE != kWindow || from + kColumns <= q.columns ? from : q.columns - kColumns;
+    const Input<COMPLEX, MODE> in(q, column0);
+    // what wave i < 4 finishes in the end, the rows 4 kq + i: asked for ahead of the products
+    const Results<OUT, COMPLEX, 1> results = { q, column0, from, in.c, 4 * in.kq + (wave & 3) };
+    float bias[V];
+    RawOf<OUT> residual[1];
+    if (q.bias)
+#pragma unroll
+        for (int i = 0; i < V; ++i) bias[i] = results.bias_at(row0 + results.lane_row, i);
+    if (q.residual && column0 + 4 * in.c < q.columns) results.template fetch<false>(row0, residual);
     float4_v total[4] = {};
-    sum_steps<OUT, COMPLEX, CAREFUL>(q, in, row0, wave, kSplitWaves, total);
-    // joined in a fixed order: wave i takes the rows 4 kq + i
+    sum_steps<OUT, COMPLEX, MODE>(q, in, row0, wave, kSplitWaves, total);
+    // joined in a fixed order
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[(wave * 4 + i) * 64 + lane] = row_of(total, i);
     __syncthreads();
@@ -711,26 +725,15 @@ __device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, 
     float4_v v[1] = { sums[wave * 64 + lane] };
 #pragma unroll
     for (int u = 1; u < kSplitWaves; ++u) v[0] += sums[(u * 4 + wave) * 64 + lane];
-    const int row = row0 + 4 * in.kq + wave;
-    if (row >= q.rows || column0 + 4 * in.c >= q.columns) return;
-    const Results<OUT, COMPLEX, 1> results = { q, column0, from, in.c, 4 * in.kq + wave };
-    float bias[COMPLEX ? 2 : 1];
-    if (q.bias)
-#pragma unroll
-        for (int i = 0; i < (COMPLEX ? 2 : 1); ++i) bias[i] = results.bias_at(row, i);
-    RawOf<OUT> residual[1];
-    if (q.residual) results.template fetch<false>(row0, residual);
+    if (row0 + results.lane_row >= q.rows || column0 + 4 * in.c >= q.columns) return;
     results.finish(v, bias, residual);
     results.template store<false>(row0, v);
 }
-template <int OUT, bool COMPLEX> __global__ __launch_bounds__(64 * kSplitWaves, 2) void mix_blocks_split_kernel(const MixBlocksParams q, int row_tiles, bool careful)
+template <int OUT, bool COMPLEX, int MODE> __global__ __launch_bounds__(64 * kSplitWaves, 2) void mix_blocks_split_kernel(const MixBlocksParams q, int row_tiles)
 {
     __shared__ float4_v sums[kSplitWaves * 4 * 64];
     const long id = block_index(), column0 = id / row_tiles * kColumns;
-    if (column0 >= q.columns) return;
-    const int row0 = (int)(id % row_tiles) * 16;
-    if (careful) split<OUT, COMPLEX, true>(q, sums, column0, row0);
-    else split<OUT, COMPLEX, false>(q, sums, column0, row0);
+    if (column0 < q.columns) split<OUT, COMPLEX, MODE>(q, sums, column0, (int)(id % row_tiles) * 16);
 }
 
 template <int OUT, int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t stream)
@@ -773,7 +776,10 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
     const int tiles16 = (q.rows + 15) / 16;
     const long columns = (q.columns + kColumns - 1) / kColumns;
     if (!near || q.columns < 2 * kColumns || columns * tiles16 <= kSplitBlocks) {
-        hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX>), grid_of(columns * tiles16), dim3(64 * kSplitWaves), 0, stream, q, tiles16, !near || q.columns < kColumns);
+        const dim3 grid = grid_of(columns * tiles16), block(64 * kSplitWaves);
+        if (near && q.columns >= kColumns) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kWindow>), grid, block, 0, stream, q, tiles16);
+        else if (near && (q.contraction + kStep) * q.ldx < (1L << 31)) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kNarrow>), grid, block, 0, stream, q, tiles16);
+        else hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kFar64>), grid, block, 0, stream, q, tiles16);
         return hipGetLastError();
     }
     if constexpr (COMPLEX) {

@@ -71,6 +71,8 @@ struct LayerNormParams {
     Drop drop;
 };
 hipError_t launch_layer_norm(const LayerNormParams& q, int type, bool eight_bits, hipStream_t stream);
+hipError_t launch_layer_norm_dropout(const LayerNormParams& q, int type, hipStream_t stream);
+hipError_t launch_layer_norm_8bit(const LayerNormParams& q, int type, hipStream_t stream);
 struct LayerNormGradParams {
     const void *gy, *s, *gs;
     const float *gain, *mean, *rstd;

@@ -99,3 +99,44 @@ def test_one_block_of_channels_is_the_product_with_scales_per_position(kind):
         y = tf.mix_8bit_blocks(xq, xscale, Wq, wscale, bias, residual, activation="gelu_tanh")
         same = tf.mix_8bit(xq, xscale[0], Wq, wscale[:, 0].repeat_interleave(128)[:N].contiguous(), bias, residual, activation="gelu_tanh")
         assert torch.equal(y, same)
+
+
+@pytest.mark.parametrize("kind,K,N,P", CASES)
+def test_scales_of_zero_and_none(kind, K, N, P):
+    """a scale of zero takes its block out, infinite and NaN ones make their position or rows so, and nothing beside them"""
+    xq, xscale, Wq, wscale, _, residual = product_operands(kind, K, N, (P,), 50, bias=False)
+    xscale, wscale = xscale.clone(), wscale.clone()
+    xscale[:, 0] = 0
+    wscale[:, 0] = 0
+    if P > 2:
+        xscale[0, P // 2], xscale[0, P - 1] = float("nan"), float("inf")
+    operands = (xq, xscale, Wq, wscale, None, residual)
+    y = tf.mix_8bit_blocks(*operands)
+    part = torch.view_as_real(y).sum(-1) if y.is_complex() else y
+    if P > 2:
+        assert not torch.isfinite(part[:, [P // 2, P - 1]]).any()
+    kept = [p for p in range(P) if p not in ((P // 2, P - 1) if P > 2 else ())]
+    assert torch.isfinite(part[:, kept]).all() and torch.equal(y[:, 0], residual[:, 0])
+    if K <= 128:
+        assert torch.equal(y[:128][:, kept], residual[:128][:, kept])
+    few = (xq[:, kept], xscale[:, kept], Wq, wscale, None, residual[:, kept])
+    check(kind, few, "none", y[:, kept], K * (2 if kind == "c64" else 1))
+
+
+def test_on_two_streams_at_once():
+    """calls of several kernels beside one another on two streams, each the result that it gives alone"""
+    shapes = [("bf16", 256, 1030, 5637), ("f32", 512, 200, 200), ("c64", 100, 500, 4100), ("bf16", 900, 60, 63)]
+    operands = [product_operands(kind, K, N, (P,), 60) for kind, K, N, P in shapes]
+    want = [tf.mix_8bit_blocks(*o, activation="silu") for o in operands]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i, side in enumerate(sides):
+        side.wait_stream(torch.cuda.current_stream())
+    for turn in range(3):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                for n in range(len(operands)):
+                    o = operands[(n + i) % len(operands)]
+                    got.append(((n + i) % len(operands), tf.mix_8bit_blocks(*o, activation="silu")))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[n]) for n, y in got)

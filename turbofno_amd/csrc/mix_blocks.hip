@@ -147,13 +147,16 @@ template <bool COMPLEX> struct Operands<COMPLEX, true> {
     }
 };
 
-// total += part x w, both scales of a step: by their product, an ordinary number (`out`: it is none in some lane), or the larger one first
+// Both scales of a step in one number. `out`: in some lane it is no ordinary number though both scales are finite and none is zero, and they have to be multiplied one after
+// the other, the larger one first. A scale of zero, infinite or NaN makes of a sum what it would have made alone.
 __device__ __forceinline__ float4_v joint_scale(float4_v x, float w, bool& out)
 {
-    x *= w;
+    constexpr int kFiniteNotZero = 0x198;               // classes of numbers: normal and subnormal ones of both signs
+    const float4_v joint = x * w;
+    const bool counts = __builtin_amdgcn_classf(w, kFiniteNotZero);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out |= !(x[i] >= 0x1p-126f && x[i] <= 0x1p127f);
-    return x;
+    for (int i = 0; i < 4; ++i) out |= counts & !(joint[i] >= 0x1p-126f && joint[i] <= 0x1p127f) & __builtin_amdgcn_classf(x[i], kFiniteNotZero);
+    return joint;
 }
 template <int COUNT> __device__ __forceinline__ void add_scaled(float4_v joint, int first, const float4_v (&part)[COUNT], float4_v (&total)[4])
 {
@@ -162,6 +165,7 @@ template <int COUNT> __device__ __forceinline__ void add_scaled(float4_v joint, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) total[first + b][i] = __builtin_fmaf(part[b][i], joint[first + b], total[first + b][i]);
 }
+// total += part x w, the larger scale first
 __device__ __forceinline__ void add_scaled_apart(float4_v x, float w, const float4_v (&part)[4], float4_v (&total)[4])
 {
 #pragma unroll

@@ -147,16 +147,29 @@ template <bool COMPLEX> struct Operands<COMPLEX, true> {
     }
 };
 
-// Both scales of a step in one number. `out`: in some lane it is no ordinary number though both scales are finite and none is zero, and they have to be multiplied one after
-// the other, the larger one first. A scale of zero, infinite or NaN makes of a sum what it would have made alone.
+// a scale of the weights, read past the vector unit: one for the wave, and its wait holds up no other load
+__device__ __forceinline__ float common_scale(const float* p) { return *reinterpret_cast<const __attribute__((address_space(4))) float*>(scalar(reinterpret_cast<long>(p))); }
+// Both scales of a step in one number. `out`: in some lane it is no positive normal number, and the scales may have to be multiplied one after the other, the larger one first
 __device__ __forceinline__ float4_v joint_scale(float4_v x, float w, bool& out)
 {
-    constexpr int kFiniteNotZero = 0x198;               // classes of numbers: normal and subnormal ones of both signs
-    const float4_v joint = x * w;
-    const bool counts = __builtin_amdgcn_classf(w, kFiniteNotZero);
+    x *= w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out |= counts & !(joint[i] >= 0x1p-126f && joint[i] <= 0x1p127f) & __builtin_amdgcn_classf(x[i], kFiniteNotZero);
-    return joint;
+    for (int i = 0; i < 4; ++i) out |= !__builtin_amdgcn_classf(x[i], 0x100);
+    return x;
+}
+// Whether they do, in some step of a wave's 64 columns: both are finite and not zero. A scale of zero, infinite or NaN makes of the sum what it would have made alone.
+template <bool COMPLEX> __device__ __forceinline__ bool scales_apart(const MixBlocksParams& q, const float* wscale, long column0)
+{
+    constexpr int kFiniteNotZero = 0x198;
+    const long column = column0 + (threadIdx.x & 63), last = q.columns - 1;
+    const int blocks = (q.contraction + kScaleBlock - 1) / kScaleBlock;
+    bool apart = false;
+#pragma unroll 1
+    for (int b = 0; b < blocks; ++b) {
+        const float x = q.xscale[b * q.positions + (column < last ? column : last) / (COMPLEX ? 2 : 1)], w = wscale[b];
+        apart |= __builtin_amdgcn_classf(x, kFiniteNotZero) & __builtin_amdgcn_classf(w, kFiniteNotZero) & !__builtin_amdgcn_classf(x * w, 0x100);
+    }
+    return any_lane(apart);
 }
 template <int COUNT> __device__ __forceinline__ void add_scaled(float4_v joint, int first, const float4_v (&part)[COUNT], float4_v (&total)[4])
 {
@@ -339,7 +352,7 @@ __device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<
 #pragma unroll
             for (int h = 0; h < 2; ++h) w[h] = mend_weights(w[h], row0 + in.c, q.rows, count, s * kStep + 64 * h + 16 * in.kq);
         const float4_v scale = raw.scale;
-        const float ws = wscale[s / (COMPLEX ? 2 : 1)];
+        const float ws = common_scale(wscale + s / (COMPLEX ? 2 : 1));
         bool out = false;
         const float4_v joint = joint_scale(scale, ws, out);
         Operands<COMPLEX, OUT == kIn32> ops;
@@ -410,10 +423,12 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     };
     float4_v total[NT][4] = {};
     bool out = false;
+    float weight_scale = common_scale(wscale);
     // step s; NEXT: the one after it is asked for, GUARD: which is the last one and not whole
     auto body = [&](int s, auto next, auto guard) {
         constexpr bool NEXT = decltype(next)::value, GUARD = decltype(guard)::value;
-        const float4_v joint = joint_scale(raw.scale, wscale[s / (COMPLEX ? 2 : 1)], out);
+        const float4_v joint = joint_scale(raw.scale, weight_scale, out);
+        if constexpr (NEXT) weight_scale = common_scale(wscale + (s + 1) / V);
         Operands<COMPLEX, EXACT> ops;
         ops.make(raw);
         if constexpr (NEXT) {
@@ -465,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     }
     body(steps - 1, std::false_type(), std::false_type());
     if (from >= q.columns) return;
-    if (__builtin_expect(any_lane(out), 0)) {
+    if (__builtin_expect(any_lane(out), 0) && scales_apart<COMPLEX>(q, wscale, in.column0)) {
         put_plain<OUT, COMPLEX>(q, results, row0, NT, biases);
         return;
     }
@@ -518,6 +533,47 @@ typedef int int2_v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int2_v read_transposed(const unsigned char* lds)
 {
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_v*)lds);
+}
+// What a wave makes of its sums, 16 rows of 64 columns at a time through 4 KB of LDS of its own (`way`; columns exchanged by kq, for the banks); `biases`: of its rows
+template <int OUT, int NT>
+__device__ __forceinline__ void put_staged(const MixBlocksParams& q, bool out, const float* wscale, float4_v (&total)[NT][4], float* way, const float* biases, int wave_row, long wave_column, long from)
+{
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    const Results<OUT, false, 4> results = { q, wave_column, from, c, 4 * kq };
+    if (__builtin_expect(any_lane(out), 0) && scales_apart<false>(q, wscale, wave_column)) {
+        put_plain<OUT, false>(q, results, wave_row, NT, biases);
+        return;
+    }
+    auto put = [&](auto whole_wave) {
+        constexpr bool WHOLE = decltype(whole_wave)::value;
+#pragma unroll 1
+        for (int t = 0; t < NT; t += 2) {
+            const int row = wave_row + 16 * t;
+            if (!WHOLE && row >= q.rows) break;
+            RawOf<OUT> residual[2][4];
+            if (q.residual)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) results.template fetch<WHOLE>(row + 16 * u, residual[u]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float4_v v[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) way[(4 * kq + i) * 64 + (b ^ kq) * 16 + c] = total[u][b][i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float4_v*>(way + (4 * kq + i) * 64 + (c / 4 ^ kq) * 16 + c % 4 * 4);
+                results.finish(v, biases + 16 * (t + u) + 4 * kq, residual[u]);
+                results.template store<WHOLE>(row + 16 * u, v);
+            }
+#pragma unroll
+            for (int u = 0; u + 2 < NT; ++u)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) total[u][b] = total[u + 2][b];
+        }
+    };
+    if (wave_column >= from && wave_row + 16 * NT <= q.rows) put(std::true_type());
+    else put(std::false_type());
 }
 template <int OUT, int NT, int RG, int CG, int BUFFERS, int WAVES>
 __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES) void mix_blocks_staged_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
@@ -592,6 +648,7 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
 
     float4_v total[NT][4] = {};
     bool out = false;
+    float weight_scale = common_scale(wscale);
     // a lane reads one half of a row's piece: lanes 2 j and 2 j + 1 row j of eight
     const int piece = wc * 4 ^ S::place_of(16 * kq + (c >> 1));
     const unsigned char* const x_from = xs + (16 * kq + (c >> 1)) * S::COLUMNS + 8 * (c & 1);
@@ -603,7 +660,8 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
         float4_v joint;
 #pragma unroll
         for (int b = 0; b < 4; ++b) joint[b] = scales[(BUFFERS == 2 ? s & 1 : 0) * S::COLUMNS + wc * 64 + 16 * b + c];
-        joint = joint_scale(joint, wscale[s], out);
+        joint = joint_scale(joint, weight_scale, out);
+        if constexpr (NEXT) weight_scale = common_scale(wscale + s + 1);
         Operands<false, EXACT> ops;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
@@ -660,45 +718,147 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
     if (whole && whole < steps) body(whole - 1, std::true_type(), std::true_type());
     body(steps - 1, std::false_type(), std::false_type());
 
-    if constexpr (BUFFERS == 1) __syncthreads();        // the results' way out is free
-    const long wave_column = scalar(column0 + wc * 64);
-    const Results<OUT, false, 4> results = { q, wave_column, from, c, 4 * kq };
-    if (__builtin_expect(any_lane(out), 0)) {
-        put_plain<OUT, false>(q, results, wave_row, NT, biases + wr * 16 * NT);
-        return;
+    if constexpr (BUFFERS == 1) __syncthreads();        // the results' way out is free: the buffer that the last step did not read
+    put_staged<OUT, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs + (BUFFERS == 2 ? steps & 1 : 0) * S::X_BYTES) + wave * 1024, biases + wr * 16 * NT, wave_row,
+                        scalar(column0 + wc * 64), from);
+}
+
+// Memory -> LDS, 16 bytes (one word) per lane, of all lanes one after the other from `to` on, which is uniform. Nothing that the compiler knows of is loaded, so that it has no
+// wait of its own for it: arrived() below waits, ahead of a barrier
+__device__ __forceinline__ unsigned place_in_lds(const void* p) { return (unsigned)(unsigned long)(__attribute__((address_space(3))) const char*)p; }
+__device__ __forceinline__ void direct_to_lds(ScalarAddress base, unsigned offset, unsigned to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
+}
+__device__ __forceinline__ void direct_word_to_lds(ScalarAddress base, unsigned offset, unsigned to)
+{
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" : : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
+}
+// The same where whole steps and 16-byte pieces are all there is, for bf16 results: memory is read into LDS directly, past the registers. The registers that this leaves hold the
+// operands of x of the next step, read while the products of this one are formed: x is asked for two steps ahead, W one.
+template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_blocks_direct_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
+{
+    typedef Staged<kIn16, NT, 2, 2, 2> S;
+    extern __shared__ uint4_v staged[];
+    unsigned char* const bytes = reinterpret_cast<unsigned char*>(staged);
+    unsigned char *const xs = bytes, *const ws = bytes + 2 * S::X_BYTES;
+    float* const scales = reinterpret_cast<float*>(ws + 2 * S::W_BYTES);
+    float* const biases = scales + 2 * S::COLUMNS;
+    const long id = block_index();
+    const long slot = by_xcd ? id / 8 : id, column_tile = by_xcd ? slot / row_tiles * 8 + id % 8 : slot / row_tiles;
+    if (column_tile >= column_tiles) return;
+    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
+    const int wr = wave / 2, wc = wave % 2, wave_row = row0 + wr * 16 * NT;
+    const long from = column_tile * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);
+    const int count = q.contraction, steps = count / kStep;
+    const float* wscale = q.wscale + (long)(row0 / kScaleBlock) * steps;
+    const unsigned x_offset = (unsigned)(lane / 8) * (unsigned)q.ldx + 16 * ((lane % 8) ^ S::place_of(8 * wave + lane / 8));
+    constexpr int X_CALLS = S::X_BYTES / 4096, W_CALLS = S::W_BYTES / 4096;
+    unsigned w_offset[W_CALLS];
+#pragma unroll
+    for (int j = 0; j < W_CALLS; ++j) {
+        const int u = (4 * j + wave) * 64 + lane, p = u / 16 % 8, row = u / 128 * 16 + ((u & 15) ^ p);
+        w_offset[j] = (unsigned)(row0 + row < q.rows ? row : q.rows - 1 - row0) * (unsigned)count + 16 * p;
     }
-    // 16 rows of 64 columns of the wave, through the buffer that the last step did not read; columns exchanged by kq, for the banks
-    float* const way = reinterpret_cast<float*>(xs + (BUFFERS == 2 ? steps & 1 : 0) * S::X_BYTES) + wave * 1024;
-    auto put = [&](auto whole_wave) {
-        constexpr bool WHOLE = decltype(whole_wave)::value;
-#pragma unroll 1
-        for (int t = 0; t < NT; t += 2) {
-            const int row = wave_row + 16 * t;
-            if (!WHOLE && row >= q.rows) break;
-            RawOf<OUT> residual[2][4];
-            if (q.residual)
+    long x_at = scalar(wave * 8 * q.ldx + column0);     // of the step that is asked for next
+    const long x_part = scalar(32 * q.ldx);
+    auto ask_x = [&](int s, int j) {
+        direct_to_lds(scalar(q.x, x_at), x_offset, place_in_lds(xs) + (s & 1) * S::X_BYTES + (4 * j + wave) * 1024);
+        x_at += x_part;
+    };
+    auto ask_w = [&](int s, int j) {
+        direct_to_lds(scalar(q.W, (long)row0 * count + s * kStep), w_offset[j], place_in_lds(ws) + (s & 1) * S::W_BYTES + (4 * j + wave) * 1024);
+    };
+    auto ask_scales = [&](int s) {                      // by two waves each half of them
+        direct_word_to_lds(scalar(q.xscale, 4 * (s * q.positions + column0 + wc * 64)), 4 * lane, place_in_lds(scales) + ((s & 1) * S::COLUMNS + wc * 64) * 4);
+    };
+    // all but the last LATER of the wave's loads have arrived, and those of the others
+    auto arrived = [&](auto later) {
+        asm volatile("s_waitcnt vmcnt(%0)" : : "n"(decltype(later)::value) : "memory");
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    };
+    constexpr std::integral_constant<int, 0> none;
+    if (q.bias)
+        for (int e = tid; e < S::ROWS; e += S::THREADS) biases[e] = value_of(static_cast<const unsigned short*>(q.bias)[row0 + e < q.rows ? row0 + e : q.rows - 1]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) results.template fetch<WHOLE>(row + 16 * u, residual[u]);
+    for (int j = 0; j < X_CALLS; ++j) ask_x(0, j);
+    ask_scales(0);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float4_v v[4];
+    for (int j = 0; j < W_CALLS; ++j) ask_w(0, j);
+    if (steps > 1) {
+#pragma unroll
+        for (int j = 0; j < X_CALLS; ++j) ask_x(1, j);
+        ask_scales(1);
+    }
+    const int piece = wc * 4 ^ S::place_of(16 * kq + (c >> 1));
+    const unsigned char* const x_from = xs + (16 * kq + (c >> 1)) * S::COLUMNS + 8 * (c & 1);
+    const uint4_v* const w_from = reinterpret_cast<const uint4_v*>(ws) + wr * NT * 128 + kq * 16;
+    int8_v next[4];
+    float4_v next_scale;
+    float weight_scale = common_scale(wscale);
+    auto read_x = [&](int s, int b) {                   // 16 columns
+        const unsigned char* const here = x_from + (s & 1) * S::X_BYTES;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int2_v v = read_transposed(here + (piece ^ b) * 16 + (u / 2 * 64 + u % 2 * 8) * S::COLUMNS);
+            next[b][2 * u] = v[0];
+            next[b][2 * u + 1] = v[1];
+        }
+        next_scale[b] = scales[(s & 1) * S::COLUMNS + wc * 64 + 16 * b + c];
+    };
+    if (steps > 1) arrived(std::integral_constant<int, X_CALLS + 1>());
+    else arrived(none);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) read_x(0, b);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    float4_v total[NT][4] = {};
+    bool out = false;
+    // LEFT: steps after this one, 2 for more
+    auto body = [&](int s, auto left) {
+        constexpr int LEFT = decltype(left)::value;
+        Operands<false, false> ops;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) ops.b[b] = next[b];
+        const float4_v joint = joint_scale(next_scale, weight_scale, out);
+        const uint4_v *const lower = w_from + (s & 1) * (S::W_BYTES / 16) + (c ^ kq), *const upper = w_from + (s & 1) * (S::W_BYTES / 16) + 64 + (c ^ (4 + kq));
+        constexpr int CALLS = X_CALLS + W_CALLS + 1;
+        auto ask_some = [&](int turn) {
+#pragma unroll
+            for (int j = 0; j < CALLS; ++j)
+                if (j * (NT - 1) / CALLS == turn) {
+                    if (j < W_CALLS) { if constexpr (LEFT >= 1) ask_w(s + 1, j); }
+                    else if (j < W_CALLS + X_CALLS) { if constexpr (LEFT >= 2) ask_x(s + 2, j - W_CALLS); }
+                    else if constexpr (LEFT >= 2) ask_scales(s + 2);
+                }
+        };
+        float4_v part[2][2];
+        uint4_v a[2][2] = { { lower[0], upper[0] } };
+        if constexpr (LEFT >= 1) weight_scale = common_scale(wscale + s + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        ops.product(a[0], 0, part[0]);
+#pragma unroll
+        for (int i = 1; i <= 2 * NT; ++i) {
+            if (i % 2 && i / 2 + 1 < NT) { a[(i / 2 + 1) % 2][0] = lower[(i / 2 + 1) * 128]; a[(i / 2 + 1) % 2][1] = upper[(i / 2 + 1) * 128]; }
+            ask_some(i - 1);
+            if (i < 2 * NT) ops.product(a[i / 2 % 2], i % 2 * 2, part[i % 2]);
+            add_scaled(joint, (i - 1) % 2 * 2, part[(i - 1) % 2], total[(i - 1) / 2]);
+            if (LEFT >= 1 && i == NT) arrived(std::integral_constant<int, LEFT == 2 ? CALLS : W_CALLS>());
+            if constexpr (LEFT >= 1)
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) way[(4 * kq + i) * 64 + (b ^ kq) * 16 + c] = total[u][b][i];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float4_v*>(way + (4 * kq + i) * 64 + (c / 4 ^ kq) * 16 + c % 4 * 4);
-                results.finish(v, biases + wr * 16 * NT + 16 * (t + u) + 4 * kq, residual[u]);
-                results.template store<WHOLE>(row + 16 * u, v);
-            }
-#pragma unroll
-            for (int u = 0; u + 2 < NT; ++u)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) total[u][b] = total[u + 2][b];
+                    if (i == NT + 1 + b * NT / 4) read_x(s + 1, b);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (LEFT >= 1) arrived(std::integral_constant<int, LEFT == 2 ? X_CALLS + 1 : 0>());
     };
-    if (wave_column >= from && wave_row + 16 * NT <= q.rows) put(std::true_type());
-    else put(std::false_type());
+    int s = 0;
+    for (; s < steps - 2; ++s) body(s, std::integral_constant<int, 2>());
+    if (s == steps - 2) body(s++, std::integral_constant<int, 1>());
+    body(s, std::integral_constant<int, 0>());
+    put_staged<kIn16, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs) + wave * 1024, biases + wr * 16 * NT, wave_row, scalar(column0 + wc * 64), from);
 }
 
 // ---- few columns: the waves of a block share 64 columns and 16 rows, and the steps are divided among them ----
@@ -761,6 +921,18 @@ template <int OUT, int NT, int RG, int CG, int BUFFERS, int WAVES> hipError_t la
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }
+template <int NT> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t stream)
+{
+    typedef Staged<kIn16, NT, 2, 2, 2> S;
+    static std::atomic<unsigned long long> served{ 0 };
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_direct_kernel<NT>), S::LDS, served); e != hipSuccess) return e;
+    const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
+    const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
+    const bool by_xcd = column_tiles >= 64;
+    hipLaunchKernelGGL((mix_blocks_direct_kernel<NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(S::THREADS), S::LDS, stream, q,
+                       row_tiles, column_tiles, by_xcd);
+    return hipGetLastError();
+}
 // Up to this number of real values the contraction is one step or less than half of one: the product with scales per position and row has kernels for it, whose scales
 // are those of one block. bf16, 64 to 64 channels at 2^20 positions 54 us (here 59 - 70), 16 to 16 at 10^6 16 us (40); 128 to 128 at 262144 29 us (26)
 constexpr int kOneBlock = 64;
@@ -791,7 +963,10 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
         if (tiles16 > 2 && wide * ((tiles16 + 3) / 4) >= 256) return launch_tiles<OUT, 4>(q, stream);
         return launch_tiles<OUT, 2>(q, stream);
     } else {
-        if ((columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 2>(q, stream);
+        const bool whole_tiles = (columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles;
+        if constexpr (OUT == kIn16)
+            if (q.contraction % kStep == 0 && ((q.ldx | q.columns | (long)q.x | (long)q.W) & 15) == 0) return whole_tiles ? launch_direct<4>(q, stream) : launch_direct<2>(q, stream);
+        if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 2>(q, stream);
         return launch_staged<OUT, 2, 2, 2, OUT == kIn32 ? 2 : 1, OUT == kIn32 ? 3 : 4>(q, stream);
     }
 }

@@ -16,7 +16,9 @@ SHAPES = {
     "f32": [(256, 1030, 5637), (300, 1030, 5637), (100, 1030, 5637), (128, 256, 2049), (200, 70, 3000), (70, 513, 1030), (512, 200, 200), (1300, 40, 100), (900, 60, 63), (390, 300, 3), (65, 17, 1)],
     "c64": [(64, 500, 4100), (100, 500, 4100), (40, 500, 4100), (128, 200, 2049), (70, 30, 9000), (33, 200, 2049), (256, 100, 60), (300, 40, 32), (450, 60, 31), (100, 300, 2), (33, 9, 1)],
 }
-SHAPES["bf16"] = SHAPES["f32"]
+# whole steps and pieces of 16 columns: read into LDS directly, tiles of 128 rows from three steps on, tiles of 64 rows for one and two steps and for fewer columns
+SHAPES["bf16"] = SHAPES["f32"] + [(384, 1030, 8208), (640, 520, 16400), (1024, 392, 16384), (512, 1030, 8064), (128, 1030, 8208), (256, 520, 16400), (384, 300, 1040), (640, 77, 3008),
+                                  (896, 650, 528)]
 CASES = [(kind,) + shape for kind in TYPES for shape in SHAPES[kind]]
 
 
@@ -42,6 +44,10 @@ def test_each_kernel(kind, K, N, P):
     tf.mix_8bit_blocks(*operands[:5], residual=place, activation="silu", y=place)
     assert torch.equal(place, y)
     xq, pair = operands[0], (2,) if kind == "c64" else ()
+    if P % 16 == 0:                                     # channels a multiple of 16 bytes apart, as in the field itself
+        apart = torch.full((K, P + 48) + pair, 448.0, device="cuda").to(torch.float8_e4m3fn)
+        apart[:, 32:32 + P] = xq
+        assert torch.equal(tf.mix_8bit_blocks(apart[:, 32:32 + P], *operands[1:], activation="silu"), y)
     apart = torch.full((K, P + 5) + pair, 448.0, device="cuda").to(torch.float8_e4m3fn)
     apart[:, 3:3 + P] = xq
     out = torch.full((N, P + 9), 7.0, dtype=y.dtype, device="cuda")

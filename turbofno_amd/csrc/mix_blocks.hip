@@ -936,9 +936,9 @@ template <int NT> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t
 // Up to this number of real values the contraction is one step or less than half of one: the product with scales per position and row has kernels for it, whose scales
 // are those of one block. bf16, 64 to 64 channels at 2^20 positions 54 us (here 59 - 70), 16 to 16 at 10^6 16 us (40); 128 to 128 at 262144 29 us (26)
 constexpr int kOneBlock = 64;
-// Blocks of 64 columns and 16 rows up to which their waves divide the steps: bf16, 1024 to 1024 channels at 256 positions 7.2 us (tiles 8.1), at 512 12.9 (8.3)
+// Blocks of 64 columns and 16 rows up to which their waves divide the steps: bf16, 1024 to 1024 channels at 256 positions 6.7 us (tiles 7.5), at 512 11 (7.7)
 constexpr long kSplitBlocks = 256;
-// Tiles of 128 rows from which they are enough for the GPU: bf16, 1024 to 1024 at 8192 positions 18.8 us (with 64 rows 21.9), at 4096 14.9 (14.2), at 2048 12.6 (10.6)
+// Tiles of 128 rows from which they are enough for the GPU: bf16, 1024 to 1024 at 8192 positions 18.7 us (with 64 rows 21.6), at 4096 13.6 (12.8), at 2048 11.2 (8.5)
 constexpr long kWholeTiles = 384;
 template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int type, hipStream_t stream)
 {
@@ -964,8 +964,9 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
         return launch_tiles<OUT, 2>(q, stream);
     } else {
         const bool whole_tiles = (columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles;
-        if constexpr (OUT == kIn16)
-            if (q.contraction % kStep == 0 && ((q.ldx | q.columns | (long)q.x | (long)q.W) & 15) == 0) return whole_tiles ? launch_direct<4>(q, stream) : launch_direct<2>(q, stream);
+        if constexpr (OUT == kIn16)                     // one or two steps: 128 to 128 channels at 262144 positions 24.0 us with 64 rows, 26.1 with 128; 512 to 512 at 16384 14.6 and 12.7
+            if (q.contraction % kStep == 0 && ((q.ldx | q.columns | (long)q.x | (long)q.W) & 15) == 0)
+                return whole_tiles && q.contraction > 2 * kStep ? launch_direct<4>(q, stream) : launch_direct<2>(q, stream);
         if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 2>(q, stream);
         return launch_staged<OUT, 2, 2, 2, OUT == kIn32 ? 2 : 1, OUT == kIn32 ? 3 : 4>(q, stream);
     }

@@ -113,3 +113,28 @@ def test_on_two_streams_at_once(kind):
     torch.cuda.synchronize()
     for i, result in got:
         assert all(torch.equal(a, b) for a, b in zip(result, want[i]))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K", [20, 50, 130])
+def test_dropout_of_channels_far_apart(kind, K):
+    """channels 2^25 values apart and more, where a lane's offset in a narrow strip would pass 32 bits"""
+    dt, P = TYPES[kind], 300
+    step = (1 << 25) + 13
+    x, gain, bias, gs = operands(kind, K, (P,), 90)
+    far = torch.empty((K - 1) * step + P, dtype=dt, device="cuda").as_strided((K, P), (step, 1))
+    far.copy_(x)
+    y, s, mean, rstd = tf.layer_norm(far, gain, bias, gs, drop=0.3, rng=rng_of())
+    E = Forward(x, gain, bias, gs, drop=0.3, rng=SEED)
+    within(s, E.s, rounded(E.s, E.s_off, dt), "s")
+    within(y, E.y, rounded(E.y, E.y_off, dt), "y")
+    gy = randn((K, P), dt, 91)
+    far.copy_(s)
+    gx, gr, ggain, gbias = tf.layer_norm_backward(gy, far, gain, mean, rstd, gs=gs, drop=0.3, rng=rng_of(), gx=far)
+    E = Backward(gy, s, gain, mean, rstd, gs, 0.3, SEED)
+    within(gr, E.gr, rounded(E.gr, E.gr_off, dt), "gr")
+    within(gx, E.gx, rounded(E.gx, E.gx_off, dt), "gx")
+    within(ggain, E.ggain, E.ggain_off, "ggain")
+    within(gbias, E.gbias, E.gbias_off, "gbias")
+    del far, gx
+    torch.cuda.empty_cache()

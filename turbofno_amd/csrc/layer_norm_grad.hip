@@ -5,6 +5,10 @@
 //
 // Strips of positions with all of their channels, as in the norm; the blocks are persistent and hold their sums over positions in registers, a second kernel adds
 // them up in a fixed order. Where the channels do not fit into registers the strip is read twice and the sums lie in the workspace.
+//
+// complex64, 64 channels at 2^20 positions with residual stream and dropout 528 us, 5.1 TB/s: the stream, and 5 us of the second kernel. bf16 takes as long per value for half the
+// bytes, 256 channels at 131072 55 us, 3.7 TB/s. 200 channels at 30011 positions, bf16, 21.6 us: 469 strips are one round, in which loads, sums, joins and stores follow one another
+// (16.0 us at 30016, where rows start at whole words), and 4 us of the second kernel.
 #include "layer_norm.h"
 
 namespace tfno {

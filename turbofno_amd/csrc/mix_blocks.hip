@@ -2,14 +2,24 @@
 //
 //   z[n][p] = sum_b xscale[b][p] wscale[n / 128][b] (sum over the channels k of block b of Wq[n][k] xq[k][p]) + bias[n] + residual[n][p],   y = act(z)
 //
-// As in the other channel products a complex row of P positions is a row of 2 P real columns, a wave takes 64 columns, a lane four consecutive ones,
-// 4 c ... 4 c + 3 with c = lane % 16, of the input, the residual and the result. A step holds 128 real values of the contraction, one block of channels (complex: half
-// of one). A quarter kq of the wave has the values 16 kq ... 16 kq + 15 of each half of a step, in this order in the operands of both sides: the lane reads whole
-// rows of x, four columns each, and transposes them in its own registers; x passes no LDS.
+// As in the other channel products a complex row of P positions is a row of 2 P real columns, and a wave takes 64 columns. A step holds 128 real values of the contraction,
+// one block of channels (complex: half of one). A quarter kq of the wave has the values 16 kq ... 16 kq + 15 of each half of a step, in this order in the operands of both
+// sides. The sum of a step is multiplied by both scales and added to the total, in fp32.
 //   bf16 result    one matrix instruction takes a step of 16 rows and columns, 128 products of 8-bit operands. It drops what lies more than about 2^-19 below the
 //                  largest product: at most 2^-12 of the sum of magnitudes together, 1e-5 of a typical sum (the result's rounding: 2^-9 of it).
 //   fp32 result    the operands are widened to bf16, which holds them exactly, and take four matrix instructions whose sums are fp32.
-// The sum of a step is multiplied by both scales and added to the total, in fp32.
+// Kernels, from many columns to few:
+//   direct         bf16, whole steps and 16-byte pieces: tiles of 128 or 64 rows and 128 columns, x and W read into LDS past the registers and ahead of time, x taken from
+//                  there by transposing reads. 1024 to 1024 channels at 65536 positions with GELU 134 us, 1.03 PFLOP/s; without it 127, of which 26 are the result's stores at
+//                  a copy's rate; each further 1024 channels 78 us, 1.8 PFLOP/s. There waves wait for data 34 % of their time, for their turn to issue 34 %; matrix
+//                  instructions take 28 % of the cycles, vector instructions (16 multiply-adds of totals for each 4 of the former) 29 %, LDS 17 %.
+//   staged         the same through registers: any strides, ends of steps and fp32 results. 1024 to 1024 at 65536 with W one byte on 120 us where direct takes 110 (inputs
+//                  in the caches); float32 176
+//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 28.5 us, 2.7 TB/s of 77.6 MB:
+//                  118 x 3 tiles, less than two rounds
+//   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 7.0 us, of which an empty launch
+//                  after launch takes 3; 4.2 MB of weights
+// Up to 64 real values of the contraction the kernels of the product with one scale per row are ahead, and take this one's scales.
 #include "kernels.h"
 #include "mix_kernel.h"
 #include <algorithm>
@@ -22,7 +32,7 @@ typedef int int8_v __attribute__((ext_vector_type(8)));
 typedef uint4_v uint4_any __attribute__((aligned(1)));
 constexpr int kStep = 128;                              // real values of a step
 
-// ---- the input ----
+// ---- the input of the tile and split kernels: a lane has four consecutive columns, 4 c ... 4 c + 3 with c = lane % 16, and transposes them ----
 
 template <bool COMPLEX> constexpr int kRowsOfHalf = COMPLEX ? 8 : 16;
 template <bool COMPLEX> struct RawStep {
@@ -366,17 +376,16 @@ __device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<
     }
 }
 
-// ---- many columns: four waves side by side share 16 NT rows of W ----
+// ---- many columns, complex: four waves side by side share 16 NT rows of W ----
 
 // The weights of a step pass LDS, in the order in which lanes read them: 16 bytes per lane, half and 16 rows. Two buffers: a step's are written while those of the
 // step before are read, after they were asked for ahead of its products, like the rows of x of the next step. A wave whose 64 columns are not all there takes the last
 // 64 and leaves those that it shares with others alone; one that has none goes along for its part of the weights.
-template <int OUT, bool COMPLEX, int NT>
+template <int NT>
 __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
 {
-    constexpr bool EXACT = OUT == kIn32;
-    constexpr int CHUNKS = NT * 128, PHASES = NT == 8 ? 2 : 1, EACH = CHUNKS / 256 / PHASES;        // 16 bytes each; asked for at once by a thread
-    constexpr int V = COMPLEX ? 2 : 1;
+    constexpr int CHUNKS = NT * 128, EACH = CHUNKS / 256;       // 16 bytes each; of a thread
+    constexpr int V = 2;
     __shared__ uint4_v weights[2 * CHUNKS];
     __shared__ float biases[16 * NT * V];
     const long id = block_index();
@@ -385,41 +394,38 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     if (column_tile >= column_tiles) return;
     const int row0 = (int)(slot % row_tiles) * (16 * NT), lane = threadIdx.x & 63;
     const long from = column_tile * (4 * kColumns) + (long)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kColumns;
-    const Input<COMPLEX, kWindow> in(q, scalar(from + kColumns <= q.columns ? from : q.columns - kColumns));
-    const int count = q.contraction * (COMPLEX ? 2 : 1), steps = (count + kStep - 1) / kStep;
+    const Input<true, kWindow> in(q, scalar(from + kColumns <= q.columns ? from : q.columns - kColumns));
+    const int count = q.contraction * V, steps = (count + kStep - 1) / kStep;
     const float* wscale = q.wscale + (long)(row0 / kScaleBlock) * ((q.contraction + kScaleBlock - 1) / kScaleBlock);
     const int whole = count / kStep;                    // steps of 128 values
     uint4_v w[EACH];
     auto chunk = [&](int i) { return (int)threadIdx.x + 256 * i; };
     auto chunk_row = [&](int e) { return e / 128 * 16 + (e & 15); };
     auto chunk_entry = [&](int e) { return (e >> 6 & 1) * 64 + (e >> 4 & 3) * 16; };
-    auto ask = [&](int s, int phase, auto guard, uint4_v (&w)[EACH]) {
+    auto ask = [&](int s, auto guard, uint4_v (&w)[EACH]) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int e = chunk(phase * EACH + i), row = row0 + chunk_row(e) < q.rows ? chunk_row(e) : q.rows - 1 - row0;
+            const int e = chunk(i), row = row0 + chunk_row(e) < q.rows ? chunk_row(e) : q.rows - 1 - row0;
             if constexpr (decltype(guard)::value) w[i] = fetch_weights(q.W, row0 + row, q.rows, count, s * kStep + chunk_entry(e));
             else w[i] = *reinterpret_cast<const TFNO_GLOBAL uint4_any*>(scalar(q.W, (long)row0 * count + s * kStep) + fresh((unsigned)row * (unsigned)count + chunk_entry(e)));
         }
     };
-    auto keep = [&](int s, int phase, auto guard, uint4_v (&w)[EACH]) {
+    auto keep = [&](int s, auto guard, uint4_v (&w)[EACH]) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int e = chunk(phase * EACH + i);
+            const int e = chunk(i);
             if constexpr (decltype(guard)::value) w[i] = mend_weights(w[i], row0 + chunk_row(e), q.rows, count, s * kStep + chunk_entry(e));
             weights[(s & 1) * CHUNKS + e] = w[i];
         }
     };
-    RawStep<COMPLEX> raw;
-    const Results<OUT, COMPLEX, 4> results = { q, in.column0, from, in.c, 4 * in.kq };
+    RawStep<true> raw;
+    const Results<kIn32, true, 4> results = { q, in.column0, from, in.c, 4 * in.kq };
     auto begin = [&](auto guard) {
         in.template fetch<decltype(guard)::value>(0, raw);
-        uint4_v first[PHASES][EACH];
-#pragma unroll
-        for (int p = 0; p < PHASES; ++p) ask(0, p, guard, first[p]);
+        ask(0, guard, w);
         if (q.bias)
             for (int e = threadIdx.x; e < 16 * NT * V; e += 256) biases[e] = results.bias_at(row0 + e / V, e % V);
-#pragma unroll
-        for (int p = 0; p < PHASES; ++p) keep(0, p, guard, first[p]);
+        keep(0, guard, w);
     };
     float4_v total[NT][4] = {};
     bool out = false;
@@ -429,44 +435,24 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
         constexpr bool NEXT = decltype(next)::value, GUARD = decltype(guard)::value;
         const float4_v joint = joint_scale(raw.scale, weight_scale, out);
         if constexpr (NEXT) weight_scale = common_scale(wscale + (s + 1) / V);
-        Operands<COMPLEX, EXACT> ops;
+        Operands<true, true> ops;
         ops.make(raw);
         if constexpr (NEXT) {
             in.template fetch<GUARD>(s + 1, raw);
-            ask(s + 1, 0, guard, w);
+            ask(s + 1, guard, w);
         }
         __builtin_amdgcn_sched_barrier(0);              // the loads stay ahead of the products
         const uint4_v* from_lds = weights + (s & 1) * CHUNKS + lane;
-        if constexpr (EXACT) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint4_v a[2] = { from_lds[t * 128], from_lds[t * 128 + 64] };
-                float4_v part[4];
-                ops.product(a, 0, part);
-                add_scaled(joint, 0, part, total[t]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-            // two columns' products at a time; they are added while the next two are formed
-            float4_v part[2][2];
-            uint4_v a[2] = { from_lds[0], from_lds[64] };
-            ops.product(a, 0, part[0]);
-#pragma unroll
-            for (int i = 1; i <= 2 * NT; ++i) {
-                if (i < 2 * NT) {
-                    if (i % 2 == 0) { a[0] = from_lds[i / 2 * 128]; a[1] = from_lds[i / 2 * 128 + 64]; }
-                    ops.product(a, i % 2 * 2, part[i % 2]);
-                }
-                add_scaled(joint, (i - 1) % 2 * 2, part[(i - 1) % 2], total[(i - 1) / 2]);
-                if (NEXT && PHASES == 2 && i == NT) {
-                    keep(s + 1, 0, guard, w);
-                    ask(s + 1, 1, guard, w);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int t = 0; t < NT; ++t) {
+            const uint4_v a[2] = { from_lds[t * 128], from_lds[t * 128 + 64] };
+            float4_v part[4];
+            ops.product(a, 0, part);
+            add_scaled(joint, 0, part, total[t]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (NEXT) {
-            keep(s + 1, PHASES - 1, guard, w);
+            keep(s + 1, guard, w);
             __syncthreads();
         }
     };
@@ -480,8 +466,8 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     }
     body(steps - 1, std::false_type(), std::false_type());
     if (from >= q.columns) return;
-    if (__builtin_expect(any_lane(out), 0) && scales_apart<COMPLEX>(q, wscale, in.column0)) {
-        put_plain<OUT, COMPLEX>(q, results, row0, NT, biases);
+    if (__builtin_expect(any_lane(out), 0) && scales_apart<true>(q, wscale, in.column0)) {
+        put_plain<kIn32, true>(q, results, row0, NT, biases);
         return;
     }
     // 32 rows at a time, always from the same registers, which the next rows' sums are moved to: unrolled, the code would not stay in the instruction cache
@@ -491,7 +477,7 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
         for (int t = 0; t < NT; t += 2) {
             const int row = row0 + 16 * t;
             if (!WHOLE && row >= q.rows) break;
-            RawOf<OUT> residual[2][4];
+            RawOf<kIn32> residual[2][4];
             if (q.residual)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) results.template fetch<WHOLE>(row + 16 * u, residual[u]);
@@ -513,9 +499,9 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     else put(std::false_type());
 }
 
-// ---- many rows and columns: waves RG deep and CG side by side share 16 NT RG rows of W and 64 CG columns of x ----
+// ---- many columns, real: waves RG deep and CG side by side share 16 NT RG rows of W and 64 CG columns of x ----
 
-// Both pass LDS in two buffers: a step's values are on their way from memory, 16 bytes a load, during the products of the step before, and written when those are done.
+// Both pass LDS in BUFFERS buffers: a step's values are on their way from memory, 16 bytes a load, during the products of the step before, and written when those are done.
 // W lies there in the order in which lanes read it. x lies there as in memory, 16 columns of a row together; ds_read_b64_tr_b8 hands a lane eight rows of one column.
 // The places of a row's 16-byte pieces are exchanged by its number, so that a read of 32 rows takes all banks. A lane's column of 16 is c here, not 4 c ... 4 c + 3: the results
 // pass LDS once more on their way out.
@@ -723,8 +709,8 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
                         scalar(column0 + wc * 64), from);
 }
 
-// Memory -> LDS, 16 bytes (one word) per lane, of all lanes one after the other from `to` on, which is uniform. Nothing that the compiler knows of is loaded, so that it has no
-// wait of its own for it: arrived() below waits, ahead of a barrier
+// Memory -> LDS, 16 bytes (one word) per lane, of all lanes one after the other from `to` on, which is uniform. No register is loaded. The compiler's form of it waits for all loads
+// ahead of each transposing read (149 us instead of 135); here arrived() waits, ahead of the barrier behind which the values are read
 __device__ __forceinline__ unsigned place_in_lds(const void* p) { return (unsigned)(unsigned long)(__attribute__((address_space(3))) const char*)p; }
 __device__ __forceinline__ void direct_to_lds(ScalarAddress base, unsigned offset, unsigned to)
 {
@@ -735,7 +721,9 @@ __device__ __forceinline__ void direct_word_to_lds(ScalarAddress base, unsigned 
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" : : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
 }
 // The same where whole steps and 16-byte pieces are all there is, for bf16 results: memory is read into LDS directly, past the registers. The registers that this leaves hold the
-// operands of x of the next step, read while the products of this one are formed: x is asked for two steps ahead, W one.
+// operands of x of the next step, read in the second half of this one. So a buffer of x is free again a step earlier than one of W: x is asked for two steps ahead, W one.
+// Loads arrive in their order, and the loop has no others: in the middle of a step those of the step before have, at its end those of W too. Each wait is followed by a barrier,
+// for the other waves' loads; the last step ends with none on the way.
 template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_blocks_direct_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
 {
     typedef Staged<kIn16, NT, 2, 2, 2> S;
@@ -772,7 +760,7 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
     auto ask_scales = [&](int s) {                      // by two waves each half of them
         direct_word_to_lds(scalar(q.xscale, 4 * (s * q.positions + column0 + wc * 64)), 4 * lane, place_in_lds(scales) + ((s & 1) * S::COLUMNS + wc * 64) * 4);
     };
-    // all but the last LATER of the wave's loads have arrived, and those of the others
+    // all but the last `later` of each wave's loads have arrived
     auto arrived = [&](auto later) {
         asm volatile("s_waitcnt vmcnt(%0)" : : "n"(decltype(later)::value) : "memory");
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -900,12 +888,12 @@ template <int OUT, bool COMPLEX, int MODE> __global__ __launch_bounds__(64 * kSp
     if (column0 < q.columns) split<OUT, COMPLEX, MODE>(q, sums, column0, (int)(id % row_tiles) * 16);
 }
 
-template <int OUT, int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t stream)
+template <int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t stream)
 {
     const long column_tiles = (q.columns + 4 * kColumns - 1) / (4 * kColumns);
     const int row_tiles = (q.rows + 16 * NT - 1) / (16 * NT);
     const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_tile_kernel<OUT, true, NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(256), 0, stream, q, row_tiles,
+    hipLaunchKernelGGL((mix_blocks_tile_kernel<NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(256), 0, stream, q, row_tiles,
                        column_tiles, by_xcd);
     return hipGetLastError();
 }
@@ -960,8 +948,8 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
     }
     if constexpr (COMPLEX) {
         const long wide = (columns + 3) / 4;
-        if (tiles16 > 2 && wide * ((tiles16 + 3) / 4) >= 256) return launch_tiles<OUT, 4>(q, stream);
-        return launch_tiles<OUT, 2>(q, stream);
+        if (tiles16 > 2 && wide * ((tiles16 + 3) / 4) >= 256) return launch_tiles<4>(q, stream);
+        return launch_tiles<2>(q, stream);
     } else {
         const bool whole_tiles = (columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles;
         if constexpr (OUT == kIn16)                     // one or two steps: 128 to 128 channels at 262144 positions 24.0 us with 64 rows, 26.1 with 128; 512 to 512 at 16384 14.6 and 12.7

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 # channels and real columns: 32, 64, 128, 256, 512, 1024 and 2048 channels are held by one kernel or another; 2^17, 2^16, 8192, 4096 and 1024 columns part them; persistent
 # blocks take several strips from 2^15 on
 SIZES = [(20, 131080), (50, 131072), (50, 200003), (40, 1001), (100, 5002), (200, 6016), (100, 70001), (200, 65536), (400, 4004), (400, 9002), (400, 40007), (700, 1000), (700, 4002),
-         (700, 9007), (1500, 3000), (1500, 5008), (2500, 902), (2500, 9008), (2100, 33001)]
+         (700, 9007), (1500, 3000), (1500, 5008), (2500, 902), (2500, 9008), (2500, 5003), (2100, 33001)]
 CASES = [(kind, K, columns) for kind in TYPES for K, columns in SIZES]
 
 

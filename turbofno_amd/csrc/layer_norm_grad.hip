@@ -7,8 +7,8 @@
 // them up in a fixed order. Where the channels do not fit into registers the strip is read twice and the sums lie in the workspace.
 //
 // complex64, 64 channels at 2^20 positions with residual stream and dropout 528 us, 5.1 TB/s: the stream, and 5 us of the second kernel. bf16 takes as long per value for half the
-// bytes, 256 channels at 131072 55 us, 3.7 TB/s. 200 channels at 30011 positions, bf16, 21.6 us: 469 strips are one round, in which loads, sums, joins and stores follow one another
-// (16.0 us at 30016, where rows start at whole words), and 4 us of the second kernel.
+// bytes, 256 channels at 131072 55 us, 3.7 TB/s. 200 channels at 30011 positions, bf16, 19.3 us: 469 strips are one round, in which loads, sums, joins and stores follow one another
+// (16.0 us at 30016, where rows start at whole cache lines), and 4 us of the second kernel.
 #include "layer_norm.h"
 
 namespace tfno {
@@ -128,7 +128,7 @@ template <bool COMPLEX> __device__ __forceinline__ void put_sums(float* sums, in
     for (int i = 0; i < (COMPLEX ? 2 : 1); ++i) sums[K + (COMPLEX ? 2 : 1) * k + i] = v.bias[i];
 }
 // Persistent over strips, so that the sums of the channels stay in registers
-template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD> __global__ __launch_bounds__(kThreads, 2) void layer_norm_grad_kernel(const LayerNormGradParams q, long strips)
+template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD> __global__ __launch_bounds__(kThreads, 2) void layer_norm_grad_kernel(const LayerNormGradParams q, const StripTurns turns)
 {
     // two buffers: a strip's sums are read while the next strip's are written by the waves that are ahead, never two strips ahead
     __shared__ float4_v shared[2][2 * (kThreads / 64) * LANES];
@@ -137,7 +137,8 @@ template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD> __global__ __lau
     __syncthreads();
     ChannelSums<COMPLEX> sums[HELD];
     int turn = 0;
-    for (long b = blockIdx.x; b < strips; b += gridDim.x, turn ^= 1) {
+    const long last = turns.last(blockIdx.x);
+    for (long b = turns.first(blockIdx.x); b < last; b += turns.step, turn ^= 1) {
         const long column0 = b * Strip<LANES>::COLUMNS;
         if (column0 + Strip<LANES>::COLUMNS <= q.columns)
             layer_norm_grad_strip<IN, COMPLEX, DROP, LANES, HELD, true>(q, shared[turn], gains, column0, Strip<LANES>::COLUMNS, sums);
@@ -222,15 +223,18 @@ __device__ __forceinline__ void layer_norm_grad_long_strip(const LayerNormGradPa
         }
     }
 }
-template <int IN, bool COMPLEX, bool DROP, int LANES> __global__ __launch_bounds__(kThreads, 2) void layer_norm_grad_long_kernel(const LayerNormGradParams q, long strips)
+template <int IN, bool COMPLEX, bool DROP, int LANES> __global__ __launch_bounds__(kThreads, 2) void layer_norm_grad_long_kernel(const LayerNormGradParams q, const StripTurns turns)
 {
     __shared__ float4_v shared[2][2 * (kThreads / 64) * LANES];
     constexpr int COLUMNS = Strip<LANES>::COLUMNS;
     float* to = q.sums + (long)blockIdx.x * q.K * (COMPLEX ? 3 : 2);
     int turn = 0;
-    for (long b = blockIdx.x; b < strips; b += gridDim.x, turn ^= 1) {
+    const long start = turns.first(blockIdx.x), last = turns.last(blockIdx.x);
+    if (start >= last)                                  // no strip: its sums are added up all the same
+        for (int k = threadIdx.x; k < q.K * (COMPLEX ? 3 : 2); k += kThreads) to[k] = 0.f;
+    for (long b = start; b < last; b += turns.step, turn ^= 1) {
         const long column0 = b * COLUMNS;
-        const bool first = b == blockIdx.x;
+        const bool first = b == start;
         if (column0 + COLUMNS <= q.columns) layer_norm_grad_long_strip<IN, COMPLEX, DROP, LANES, true>(q, shared[turn], column0, COLUMNS, to, first);
         else layer_norm_grad_long_strip<IN, COMPLEX, DROP, LANES, false>(q, shared[turn], column0, (int)(q.columns - column0), to, first);
     }
@@ -261,10 +265,12 @@ constexpr long kGradBlocks = 512;                       // persistent blocks
 // Lanes side by side and channels held per lane (0: read twice). The workspace is for as many blocks as there are strips of the narrowest kind
 template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD> hipError_t launch_as(const LayerNormGradParams& q, hipStream_t stream)
 {
-    const long strips = (q.columns + 4 * LANES - 1) / (4 * LANES), blocks = std::min(strips, kGradBlocks);
+    const long strips = (q.columns + 4 * LANES - 1) / (4 * LANES);
+    const StripTurns turns(strips, LANES >= 4 && run_together(q.columns, IN, strips), kGradBlocks);
+    const long blocks = turns.blocks();
     if (blocks) {
-        if constexpr (HELD > 0) hipLaunchKernelGGL((layer_norm_grad_kernel<IN, COMPLEX, DROP, LANES, HELD>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, strips);
-        else hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, LANES>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, strips);
+        if constexpr (HELD > 0) hipLaunchKernelGGL((layer_norm_grad_kernel<IN, COMPLEX, DROP, LANES, HELD>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, turns);
+        else hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, LANES>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, turns);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     const int count = q.K * (COMPLEX ? 3 : 2);

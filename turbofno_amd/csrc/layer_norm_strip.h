@@ -180,10 +180,10 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
 // areas of LDS for joins: the mean's, the squares' (two values where channels are read again), and the maxima of blocks of 128 channels
 template <bool EIGHT, int LANES, int HELD> constexpr int kAreas = (HELD ? 2 : 3) + (!EIGHT ? 0 : HELD ? (HELD * (kThreads / LANES) + kScaleBlock - 1) / kScaleBlock : 2);
 template <int IN, bool COMPLEX, bool DROP, bool EIGHT, int LANES, int HELD>
-__global__ __launch_bounds__(kThreads, (IN == kIn16 && HELD < 16 && !(EIGHT && LANES < 16) ? 4 : 2)) void layer_norm_kernel(const LayerNormParams q)
+__global__ __launch_bounds__(kThreads, (IN == kIn16 && HELD < 16 && !(EIGHT && LANES < 16) ? 4 : 2)) void layer_norm_kernel(const LayerNormParams q, long run)
 {
     typedef Strip<LANES> S;
-    const long column0 = block_index() * S::COLUMNS;
+    const long id = block_index(), column0 = (run ? id % 8 * run + id / 8 : id) * S::COLUMNS;
     if (column0 >= q.columns) return;
     __shared__ float4_v shared[kAreas<EIGHT, LANES, HELD> * (kThreads / 64) * LANES];
     __shared__ Affine<COMPLEX> affines[HELD ? HELD * S::GROUPS : 1];
@@ -195,7 +195,8 @@ __global__ __launch_bounds__(kThreads, (IN == kIn16 && HELD < 16 && !(EIGHT && L
 
 template <int IN, bool COMPLEX, bool DROP, bool EIGHT, int LANES, int HELD> hipError_t launch_as(const LayerNormParams& q, hipStream_t stream)
 {
-    hipLaunchKernelGGL((layer_norm_kernel<IN, COMPLEX, DROP, EIGHT, LANES, HELD>), grid_of((q.columns + 4 * LANES - 1) / (4 * LANES)), dim3(kThreads), 0, stream, q);
+    const long strips = (q.columns + 4 * LANES - 1) / (4 * LANES), run = run_together(q.columns, IN, strips) ? (strips + 7) / 8 : 0;
+    hipLaunchKernelGGL((layer_norm_kernel<IN, COMPLEX, DROP, EIGHT, LANES, HELD>), grid_of(run ? 8 * run : strips), dim3(kThreads), 0, stream, q, run);
     return hipGetLastError();
 }
 // Lanes side by side and channels held: wide strips read long pieces of a row, narrow ones give the GPU more blocks, and hold more channels

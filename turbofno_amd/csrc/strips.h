@@ -8,6 +8,10 @@ namespace tfno {
 constexpr int kThreads = 512;
 constexpr long kFar = 1L << 28;                         // real values between channels
 
+// Whether strips that lie side by side go to one XCD: where rows do not start at whole cache lines of 128 bytes, so that neighbours share lines, which the XCD's L2 cache then
+// fetches once. bf16, layer norm of 300 channels at 65551 positions 57 us, 73 with strips dealt out to the XCDs in turns; its gradient, 128 channels at 200003 76 and 97 us; where
+// rows start at whole lines the turns are ahead: complex64, 64 channels at 2^20 408 us and 422
+inline bool run_together(long columns, int type, long strips) { return strips >= 64 && columns * (type == kIn16 ? 2 : 4) % 128; }
 // columns a lane adds up belong to one position each (real) or two and two (complex)
 template <bool COMPLEX> __device__ __forceinline__ float4_v per_position(float4_v v)
 {

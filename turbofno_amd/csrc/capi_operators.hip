@@ -378,8 +378,9 @@ int turbofno_layer_norm_backward(int type, long P, int K, const void* gy, long l
     if (among(px, { pg, pm, pt, pd, pog, pob }) || among(pr, { pg, pm, pt, pd, pog, pob }))
         return fail(TURBOFNO_ERR_INVALID_ARG, "gx or gr overlaps gain, mean, rstd, rng, ggain or gbias");
     if (overlap(pog, pob)) return fail(TURBOFNO_ERR_INVALID_ARG, "ggain and gbias overlap");
-    if (among(pw, { py, ps, pgs, px, pr, pg, pm, pt, pd, pog, pob })) return fail(TURBOFNO_ERR_INVALID_ARG, "the workspace overlaps an operand");
+    // first: how far a workspace that is too small would reach says nothing
     if (!workspace || workspace_bytes < need) return fail(TURBOFNO_ERR_WORKSPACE, "workspace of %zu bytes, %zu are needed", workspace ? workspace_bytes : (size_t)0, need);
+    if (among(pw, { py, ps, pgs, px, pr, pg, pm, pt, pd, pog, pob })) return fail(TURBOFNO_ERR_INVALID_ARG, "the workspace overlaps an operand");
     const tfno::LayerNormGradParams q = { gy, s, gs, gain, static_cast<const float*>(mean), rstd, gr, gx, ggain, static_cast<float*>(gbias), static_cast<float*>(workspace),
                                           P * v, ldgy * v, lds * v, ldgs * v, ldgr * v, ldgx * v, K, d };
     return hip_status(tfno::launch_layer_norm_backward(q, type, (hipStream_t)stream), "layer_norm_backward launch");

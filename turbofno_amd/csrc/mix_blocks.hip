@@ -15,8 +15,8 @@
 //                  instructions take 28 % of the cycles, vector instructions (16 multiply-adds of totals for each 4 of the former) 29 %, LDS 17 %.
 //   staged         the same through registers: any strides, ends of steps and fp32 results. 1024 to 1024 at 65536 with W one byte on 120 us where direct takes 110 (inputs
 //                  in the caches); float32 176
-//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 28.5 us, 2.7 TB/s of 77.6 MB:
-//                  118 x 3 tiles, less than two rounds
+//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 27.7 us, 2.8 TB/s of 77.6 MB:
+//                  235 x 3 tiles, less than two rounds
 //   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 7.0 us, of which an empty launch
 //                  after launch takes 3; 4.2 MB of weights
 // Up to 64 real values of the contraction the kernels of the product with one scale per row are ahead, and take this one's scales.
@@ -506,16 +506,16 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
 
 // ---- many columns, real: waves RG deep and CG side by side share 16 NT RG rows of W and 64 CG columns of x ----
 
-// Both pass LDS in BUFFERS buffers: a step's values are on their way from memory, 16 bytes a load, during the products of the step before, and written when those are done.
+// Both pass LDS in two buffers: a step's values are on their way from memory, 16 bytes a load, during the products of the step before, and written when those are done.
 // W lies there in the order in which lanes read it. x lies there as in memory, 16 columns of a row together; ds_read_b64_tr_b8 hands a lane eight rows of one column.
 // The places of a row's 16-byte pieces are exchanged by its number, so that a read of 32 rows takes all banks. A lane's column of 16 is c here, not 4 c ... 4 c + 3: the results
 // pass LDS once more on their way out.
-template <int OUT, int NT, int RG, int CG, int BUFFERS> struct Staged {
+template <int OUT, int NT, int RG, int CG> struct Staged {
     static constexpr int THREADS = 64 * RG * CG, ROWS = 16 * NT * RG, COLUMNS = 64 * CG, PIECES = COLUMNS / 16;
     static constexpr int X_EACH = kStep * PIECES / THREADS, W_EACH = ROWS * 8 / THREADS, X_ROWS = THREADS / PIECES;      // 16-byte pieces of a thread; rows of x at a time
     static constexpr int X_BYTES = kStep * COLUMNS, W_BYTES = ROWS * kStep;
     static_assert(X_BYTES >= RG * CG * 4096, "the results' way out");
-    static constexpr size_t LDS = BUFFERS * (X_BYTES + W_BYTES + COLUMNS * 4) + ROWS * 4;
+    static constexpr size_t LDS = 2 * (X_BYTES + W_BYTES + COLUMNS * 4) + ROWS * 4;
     // what a row's pieces are exchanged by
     static __device__ __forceinline__ int place_of(int row) { return PIECES == 16 ? (row & 7) | (row >> 1 & 8) : (row & 7) ^ (row >> 4 & 1); }
     static_assert(PIECES == 8 || PIECES == 16, "columns of a block");
@@ -566,17 +566,17 @@ __device__ __forceinline__ void put_staged(const MixBlocksParams& q, bool out, c
     if (wave_column >= from && wave_row + 16 * NT <= q.rows) put(std::true_type());
     else put(std::false_type());
 }
-template <int OUT, int NT, int RG, int CG, int BUFFERS, int WAVES>
-__global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES) void mix_blocks_staged_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
+template <int OUT, int NT, int RG, int CG, int WAVES>
+__global__ __launch_bounds__((Staged<OUT, NT, RG, CG>::THREADS), WAVES) void mix_blocks_staged_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
 {
-    typedef Staged<OUT, NT, RG, CG, BUFFERS> S;
+    typedef Staged<OUT, NT, RG, CG> S;
     constexpr bool EXACT = OUT == kIn32;
     extern __shared__ uint4_v staged[];
     unsigned char* const bytes = reinterpret_cast<unsigned char*>(staged);
     unsigned char* const xs = bytes;                    // two buffers each
-    unsigned char* const ws = bytes + BUFFERS * S::X_BYTES;
-    float* const scales = reinterpret_cast<float*>(ws + BUFFERS * S::W_BYTES);
-    float* const biases = scales + BUFFERS * S::COLUMNS;
+    unsigned char* const ws = bytes + 2 * S::X_BYTES;
+    float* const scales = reinterpret_cast<float*>(ws + 2 * S::W_BYTES);
+    float* const biases = scales + 2 * S::COLUMNS;
     const long id = block_index();
     const long slot = by_xcd ? id / 8 : id, column_tile = column_tile_of<OUT == kIn32>(id, slot / row_tiles, column_tiles, by_xcd);
     if (column_tile >= column_tiles) return;
@@ -610,7 +610,7 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
     constexpr int PIECES = S::X_EACH + S::W_EACH + 1;
     auto keep = [&](int s, auto guard) {
         constexpr bool GUARD = decltype(guard)::value;
-        unsigned char* const to = xs + (BUFFERS == 2 ? s & 1 : 0) * S::X_BYTES;
+        unsigned char* const to = xs + (s & 1) * S::X_BYTES;
 #pragma unroll
         for (int i = 0; i < S::X_EACH; ++i) {
             const int row = i * S::X_ROWS + x_row;
@@ -621,9 +621,9 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
         for (int i = 0; i < S::W_EACH; ++i) {
             const int e = tid + S::THREADS * i, row = w_row(e), p = e % 8;
             if constexpr (GUARD) w[i] = mend_weights(w[i], row0 + row, q.rows, count, s * kStep + w_entry(e));
-            reinterpret_cast<uint4_v*>(ws + (BUFFERS == 2 ? s & 1 : 0) * S::W_BYTES)[row / 16 * 128 + p * 16 + ((row & 15) ^ p)] = w[i];
+            reinterpret_cast<uint4_v*>(ws + (s & 1) * S::W_BYTES)[row / 16 * 128 + p * 16 + ((row & 15) ^ p)] = w[i];
         }
-        scales[(BUFFERS == 2 ? s & 1 : 0) * S::COLUMNS + tid % S::COLUMNS] = scale;        // by all threads, without a branch: more than one of them write the same
+        scales[(s & 1) * S::COLUMNS + tid % S::COLUMNS] = scale;        // by all threads, without a branch: more than one of them write the same
     };
     auto begin = [&](auto guard) {
 #pragma unroll
@@ -646,11 +646,11 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
     const uint4_v* const w_from = reinterpret_cast<const uint4_v*>(ws) + wr * NT * 128 + kq * 16;
     auto body = [&](int s, auto next, auto guard) {
         constexpr bool NEXT = decltype(next)::value;
-        const unsigned char* const here = x_from + (BUFFERS == 2 ? s & 1 : 0) * S::X_BYTES;
-        const uint4_v *const lower = w_from + (BUFFERS == 2 ? s & 1 : 0) * (S::W_BYTES / 16) + (c ^ kq), *const upper = w_from + (BUFFERS == 2 ? s & 1 : 0) * (S::W_BYTES / 16) + 64 + (c ^ (4 + kq));
+        const unsigned char* const here = x_from + (s & 1) * S::X_BYTES;
+        const uint4_v *const lower = w_from + (s & 1) * (S::W_BYTES / 16) + (c ^ kq), *const upper = w_from + (s & 1) * (S::W_BYTES / 16) + 64 + (c ^ (4 + kq));
         float4_v joint;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) joint[b] = scales[(BUFFERS == 2 ? s & 1 : 0) * S::COLUMNS + wc * 64 + 16 * b + c];
+        for (int b = 0; b < 4; ++b) joint[b] = scales[(s & 1) * S::COLUMNS + wc * 64 + 16 * b + c];
         joint = joint_scale(joint, weight_scale, out);
         if constexpr (NEXT) weight_scale = common_scale(wscale + s + 1);
         Operands<false, EXACT> ops;
@@ -700,7 +700,6 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
             }
         }
         if constexpr (NEXT) {
-            if constexpr (BUFFERS == 1) __syncthreads();
             keep(s + 1, guard);
             __syncthreads();
         }
@@ -709,8 +708,8 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG, BUFFERS>::THREADS), WAVES)
     if (whole && whole < steps) body(whole - 1, std::true_type(), std::true_type());
     body(steps - 1, std::false_type(), std::false_type());
 
-    if constexpr (BUFFERS == 1) __syncthreads();        // the results' way out is free: the buffer that the last step did not read
-    put_staged<OUT, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs + (BUFFERS == 2 ? steps & 1 : 0) * S::X_BYTES) + wave * 1024, biases + wr * 16 * NT, wave_row,
+    // the results' way out: the buffer that the last step did not read
+    put_staged<OUT, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs + (steps & 1) * S::X_BYTES) + wave * 1024, biases + wr * 16 * NT, wave_row,
                         scalar(column0 + wc * 64), from);
 }
 
@@ -731,7 +730,7 @@ __device__ __forceinline__ void direct_word_to_lds(ScalarAddress base, unsigned 
 // for the other waves' loads; the last step ends with none on the way.
 template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_blocks_direct_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
 {
-    typedef Staged<kIn16, NT, 2, 2, 2> S;
+    typedef Staged<kIn16, NT, 2, 2> S;
     extern __shared__ uint4_v staged[];
     unsigned char* const bytes = reinterpret_cast<unsigned char*>(staged);
     unsigned char *const xs = bytes, *const ws = bytes + 2 * S::X_BYTES;
@@ -902,21 +901,21 @@ template <int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t 
                        column_tiles, by_xcd);
     return hipGetLastError();
 }
-template <int OUT, int NT, int RG, int CG, int BUFFERS, int WAVES> hipError_t launch_staged(const MixBlocksParams& q, hipStream_t stream)
+template <int OUT, int NT, int RG, int CG, int WAVES> hipError_t launch_staged(const MixBlocksParams& q, hipStream_t stream)
 {
-    typedef Staged<OUT, NT, RG, CG, BUFFERS> S;
+    typedef Staged<OUT, NT, RG, CG> S;
     static std::atomic<unsigned long long> served{ 0 };
-    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, BUFFERS, WAVES>), S::LDS, served); e != hipSuccess) return e;
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES>), S::LDS, served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
     const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
     const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, BUFFERS, WAVES>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(S::THREADS), S::LDS, stream, q,
+    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(S::THREADS), S::LDS, stream, q,
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }
 template <int NT> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t stream)
 {
-    typedef Staged<kIn16, NT, 2, 2, 2> S;
+    typedef Staged<kIn16, NT, 2, 2> S;
     static std::atomic<unsigned long long> served{ 0 };
     if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_direct_kernel<NT>), S::LDS, served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
@@ -960,8 +959,8 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
         if constexpr (OUT == kIn16)                     // one or two steps: 128 to 128 channels at 262144 positions 24.0 us with 64 rows, 26.1 with 128; 512 to 512 at 16384 14.6 and 12.7
             if (q.contraction % kStep == 0 && ((q.ldx | q.columns | (long)q.x | (long)q.W) & 15) == 0)
                 return whole_tiles && q.contraction > 2 * kStep ? launch_direct<4>(q, stream) : launch_direct<2>(q, stream);
-        if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 2>(q, stream);
-        return launch_staged<OUT, 2, 2, 2, OUT == kIn32 ? 2 : 1, OUT == kIn32 ? 3 : 4>(q, stream);
+        if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2>(q, stream);
+        return launch_staged<OUT, 2, 2, 2, 3>(q, stream);
     }
 }
 

@@ -287,7 +287,8 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *   turbofno_quantise_8bit   scale[b][p] = max over the channels k of block b of |x[k][p]| / 448 (real and imaginary parts; 1 where that is below 2^-126, and
  *                            all q of the block are zeros then; NaN where an x of it is infinite or NaN), q = x / scale in e4m3: scale [ceil(K / 128)][P].
  *   turbofno_mix_8bit_blocks turbofno_mix_8bit with x = xscale[k / 128][p] xq[k][p] and W = wscale[n / 128][k / 128] Wq[n][k]: xscale [ceil(K / 128)][P],
- *                            wscale [ceil(N / 128)][ceil(K / 128)].
+ *                            wscale [ceil(N / 128)][ceil(K / 128)]. A bf16 result's sums of 128 products drop of each what lies more than about 2^-19 below their
+ *                            largest (2^-12 of the sum of magnitudes at most); results in 32 bits are sums in fp32.
  */
 #define TURBOFNO_C64  0
 #define TURBOFNO_F32  1

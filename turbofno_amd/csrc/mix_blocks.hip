@@ -17,8 +17,8 @@
 //                  in the caches); float32 176
 //   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 27.7 us, 2.8 TB/s of 77.6 MB:
 //                  235 x 3 tiles, less than two rounds
-//   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 7.0 us, of which an empty launch
-//                  after launch takes 3; 4.2 MB of weights
+//   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 6.8 us, of which an empty launch
+//                  after launch takes 3; 4096 to 4096 at 64 10.7 us, 16.8 MB of weights
 // Up to 64 real values of the contraction the kernels of the product with one scale per row are ahead, and take this one's scales.
 #include "kernels.h"
 #include "mix_kernel.h"
@@ -39,8 +39,9 @@ template <bool COMPLEX> struct RawStep {
     unsigned row[2][kRowsOfHalf<COMPLEX>];              // four columns of the lane's channels
     float4_v scale;                                     // of the columns
 };
-// 64 columns of a wave, from column0 on. kWindow: all of them exist; otherwise `there` of them, at least one, and a word that would end behind the last value of all starts
-// earlier and is shifted (what it holds beyond its row's end is not used): kNarrow by 32-bit offsets from the first value, kFar whatever lies between the channels
+// 64 columns of a wave, from column0 on. kWindow: all of them exist, a row's place is a scalar part and the lane's 32 bits. Otherwise `there` of them do, at least one, and a word that
+// would end behind the last value of all starts earlier and is shifted (what it holds beyond its row's end is not used): kNarrow by 32-bit offsets from the first value, kFar64
+// whatever lies between the channels. For few columns kNarrow is ahead of kWindow also where all 64 exist, by the rows' scalar parts: 4096 to 4096 channels at 64 10.7 us, 14.8
 enum { kWindow = 0, kNarrow = 1, kFar64 = 2 };
 template <bool COMPLEX, int MODE> struct Input {
     static constexpr int V = COMPLEX ? 2 : 1, HALF = kRowsOfHalf<COMPLEX>;
@@ -53,7 +54,7 @@ template <bool COMPLEX, int MODE> struct Input {
     template <bool GUARD> __device__ __forceinline__ void fetch(int step, RawStep<COMPLEX>& raw) const
     {
         const int first = step * (kStep / V);
-        const unsigned quarter = fresh((unsigned)(kq * HALF) * (unsigned)q.ldx + (MODE == kWindow || 4 * c < there ? 4 * c : 0));
+        const unsigned quarter = fresh((unsigned)(kq * HALF) * (unsigned)q.ldx + (MODE == kWindow || 4 * c < there ? 4 * c : 0) + (MODE == kNarrow ? (unsigned)column0 : 0));
         const unsigned end = MODE == kNarrow ? (unsigned)((q.contraction - 1) * q.ldx + q.columns - 4) : 0;     // of the last word
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -857,14 +858,13 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
 
 constexpr int kSplitWaves = 8;
 template <int OUT, bool COMPLEX, int MODE>
-__device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, long from, int row0)
+__device__ __forceinline__ void split(const MixBlocksParams& q, float4_v* sums, long column0, int row0)
 {
     constexpr int V = COMPLEX ? 2 : 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const long column0 = MODE != kWindow || from + kColumns <= q.columns ? from : q.columns - kColumns;
     const Input<COMPLEX, MODE> in(q, column0);
     // what wave i < 4 finishes in the end, the rows 4 kq + i: asked for ahead of the products
-    const Results<OUT, COMPLEX, 1> results = { q, column0, from, in.c, 4 * in.kq + (wave & 3) };
+    const Results<OUT, COMPLEX, 1> results = { q, column0, column0, in.c, 4 * in.kq + (wave & 3) };
     float bias[V];
     RawOf<OUT> residual[1];
     if (q.bias)
@@ -928,7 +928,7 @@ template <int NT> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t
 // Up to this number of real values the contraction is one step or less than half of one: the product with scales per position and row has kernels for it, whose scales
 // are those of one block. bf16, 64 to 64 channels at 2^20 positions 54 us (here 59 - 70), 16 to 16 at 10^6 16 us (40); 128 to 128 at 262144 29 us (26)
 constexpr int kOneBlock = 64;
-// Blocks of 64 columns and 16 rows up to which their waves divide the steps: bf16, 1024 to 1024 channels at 256 positions 6.7 us (tiles 7.5), at 512 11 (7.7)
+// Blocks of 64 columns and 16 rows up to which their waves divide the steps: bf16, 1024 to 1024 channels at 256 positions 6.8 us (tiles 7.5), at 512 11 (7.7)
 constexpr long kSplitBlocks = 256;
 // Tiles of 128 rows from which they are enough for the GPU: bf16, 1024 to 1024 at 8192 positions 18.7 us (with 64 rows 21.6), at 4096 13.6 (12.8), at 2048 11.2 (8.5)
 constexpr long kWholeTiles = 384;
@@ -945,8 +945,7 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
     const long columns = (q.columns + kColumns - 1) / kColumns;
     if (!near || q.columns < 2 * kColumns || columns * tiles16 <= kSplitBlocks) {
         const dim3 grid = grid_of(columns * tiles16), block(64 * kSplitWaves);
-        if (near && q.columns >= kColumns) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kWindow>), grid, block, 0, stream, q, tiles16);
-        else if (near && (q.contraction + kStep) * q.ldx < (1L << 31)) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kNarrow>), grid, block, 0, stream, q, tiles16);
+        if (near && (q.contraction + kStep) * q.ldx < (1L << 31)) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kNarrow>), grid, block, 0, stream, q, tiles16);
         else hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kFar64>), grid, block, 0, stream, q, tiles16);
         return hipGetLastError();
     }

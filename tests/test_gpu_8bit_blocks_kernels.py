@@ -146,3 +146,32 @@ def test_on_two_streams_at_once():
                     got.append(((n + i) % len(operands), tf.mix_8bit_blocks(*o, activation="silu")))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[n]) for n, y in got)
+
+
+@pytest.mark.parametrize("kind,K,N,P", [("bf16", 384, 1030, 8208), ("bf16", 384, 300, 1040), ("bf16", 256, 1030, 5637), ("f32", 100, 1030, 5637), ("c64", 64, 500, 4100), ("bf16", 512, 200, 200)])
+def test_each_kernel_in_a_graph(kind, K, N, P):
+    """quantised and multiplied in a captured graph, replayed with other fields and eager calls in between: the eager result each time"""
+    operands = product_operands(kind, K, N, (P,), 70)
+    wide = torch.complex64 if kind == "c64" else torch.float32
+    x, place = randn((K, P), wide, 71), operands[5].clone()
+    q, scale = tf.quantise_8bit(x)
+    y = torch.empty_like(operands[5])
+
+    def run(q, scale, y):
+        tf.quantise_8bit(x, q=q, scale=scale)
+        tf.mix_8bit_blocks(q, scale, *operands[2:5], residual=place, activation="silu", y=y)
+    run(q, scale, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(q, scale, y)
+    for i in range(3):
+        x.copy_(randn((K, P), wide, 80 + i))
+        place.copy_(randn((N, P), place.dtype, 90 + i))
+        want = torch.empty_like(y)
+        run(torch.empty_like(q), torch.empty_like(scale), want)
+        torch.cuda.synchronize()
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), i

@@ -138,3 +138,39 @@ def test_dropout_of_channels_far_apart(kind, K):
     within(gbias, E.gbias, E.gbias_off, "gbias")
     del far, gx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind,K,columns", [(kind, K, columns) for kind in TYPES for K, columns in ((40, 1001), (200, 65537), (2500, 5003))])
+def test_one_tensor_for_two_operands(kind, K, columns):
+    """x its own residual, the gradient of y that of s too: what copies of them give"""
+    x, gain, bias, _ = operands(kind, K, places(kind, columns), 100)
+    want = tf.layer_norm(x, gain, bias, x.clone(), drop=0.2, rng=rng_of())
+    got = tf.layer_norm(x, gain, bias, x, drop=0.2, rng=rng_of())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    back = lambda gs: tf.layer_norm_backward(x, want[1], gain, want[2], want[3], gs=gs, drop=0.2, rng=rng_of())  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(back(x), back(x.clone())))
+    assert torch.equal(tf.dropout(x, 0.2, rng_of(), residual=x), tf.dropout(x, 0.2, rng_of(), residual=x.clone()))
+
+
+def test_two_graphs_in_turns():
+    """two captured gradients of other sizes, each with its workspace, replayed in turns beside eager calls: the eager results"""
+    sets = []
+    for K, columns, seed in ((200, 30011, 110), (2500, 5003, 120)):
+        x, gain, bias, gs = operands("bf16", K, places("bf16", columns), seed)
+        _, s, mean, rstd = tf.layer_norm(x, gain, bias)
+        call = lambda gy=x, s=s, gain=gain, mean=mean, rstd=rstd, gs=gs, **k: tf.layer_norm_backward(gy, s, gain, mean, rstd, gs=gs, **k)  # noqa: E731
+        want = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        sets.append((graph, got, want, call))
+    for i in range(4):
+        for graph, got, want, call in sets:
+            for t in set(got):
+                t.zero_()
+            graph.replay()
+        eager = [call() for _, _, _, call in sets]
+        torch.cuda.synchronize()
+        for (_, got, want, _), again in zip(sets, eager):
+            assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(got, want, again)), i

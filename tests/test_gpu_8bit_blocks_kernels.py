@@ -19,6 +19,9 @@ SHAPES = {
 # whole steps and pieces of 16 columns: read into LDS directly, tiles of 128 rows from three steps on, tiles of 64 rows for one and two steps and for fewer columns
 SHAPES["bf16"] = SHAPES["f32"] + [(384, 1030, 8208), (640, 520, 16400), (1024, 392, 16384), (512, 1030, 8064), (128, 1030, 8208), (256, 520, 16400), (384, 300, 1040), (640, 77, 3008),
                                   (896, 650, 528)]
+# few tiles of 64 rows and many steps: two groups of waves with half of the steps each, an odd number of them too, the last one not whole
+SHAPES["f32"] = SHAPES["f32"] + [(385, 300, 1001), (640, 100, 1001), (1100, 200, 700), (1024, 130, 2000)]
+SHAPES["bf16"] = SHAPES["bf16"] + [(1024, 300, 1040), (1152, 130, 2000), (1200, 200, 1003), (1030, 500, 701), (1900, 260, 400), (2176, 300, 528)]
 CASES = [(kind,) + shape for kind in TYPES for shape in SHAPES[kind]]
 
 

@@ -19,6 +19,7 @@
 //                  235 x 3 tiles, less than two rounds
 //   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 6.8 us, of which an empty launch
 //                  after launch takes 3; 4096 to 4096 at 64 10.7 us, 16.8 MB of weights
+// Direct and staged tiles that are fewer than compute units: two groups of waves with half of the steps each.
 // Up to 64 real values of the contraction the kernels of the product with one scale per row are ahead, and take this one's scales.
 #include "kernels.h"
 #include "mix_kernel.h"
@@ -516,7 +517,8 @@ template <int OUT, int NT, int RG, int CG> struct Staged {
     static constexpr int X_EACH = kStep * PIECES / THREADS, W_EACH = ROWS * 8 / THREADS, X_ROWS = THREADS / PIECES;      // 16-byte pieces of a thread; rows of x at a time
     static constexpr int X_BYTES = kStep * COLUMNS, W_BYTES = ROWS * kStep;
     static_assert(X_BYTES >= RG * CG * 4096, "the results' way out");
-    static constexpr size_t LDS = 2 * (X_BYTES + W_BYTES + COLUMNS * 4) + ROWS * 4;
+    static constexpr int GROUP_BYTES = 2 * (X_BYTES + W_BYTES + COLUMNS * 4);
+    static constexpr size_t lds(int groups) { return groups * GROUP_BYTES + ROWS * 4; }
     // what a row's pieces are exchanged by
     static __device__ __forceinline__ int place_of(int row) { return PIECES == 16 ? (row & 7) | (row >> 1 & 8) : (row & 7) ^ (row >> 4 & 1); }
     static_assert(PIECES == 8 || PIECES == 16, "columns of a block");
@@ -567,24 +569,50 @@ __device__ __forceinline__ void put_staged(const MixBlocksParams& q, bool out, c
     if (wave_column >= from && wave_row + 16 * NT <= q.rows) put(std::true_type());
     else put(std::false_type());
 }
-template <int OUT, int NT, int RG, int CG, int WAVES>
-__global__ __launch_bounds__((Staged<OUT, NT, RG, CG>::THREADS), WAVES) void mix_blocks_staged_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
+// GROUPS = 2: the block's threads twice, the second half of the steps by the second half of them, with LDS of their own. Both take as many, `each` (and meet at the same barriers): of an
+// odd number the one in the middle twice, for nothing the second time. The sums of the second group are added to the first one's, which goes on alone; false for the other
+template <int NT, int GROUPS, typename S>
+__device__ __forceinline__ bool join_groups(int group, int tid, unsigned char* own, unsigned char* others, float4_v (&total)[NT][4], bool& out)
+{
+    if constexpr (GROUPS == 2) {
+        static_assert(NT * 4 * S::THREADS * sizeof(float4_v) <= 2 * S::X_BYTES, "the sums' place");
+        __syncthreads();                                // the last step's reads are done
+        if (group) {
+            float4_v* sums = reinterpret_cast<float4_v*>(own);
+            int* flags = reinterpret_cast<int*>(own + 2 * S::X_BYTES);
+#pragma unroll
+            for (int i = 0; i < NT * 4; ++i) sums[i * S::THREADS + tid] = total[i / 4][i % 4];
+            flags[tid] = out;
+        }
+        __syncthreads();
+        if (group) return false;
+        const float4_v* sums = reinterpret_cast<const float4_v*>(others);
+        out |= reinterpret_cast<const int*>(others + 2 * S::X_BYTES)[tid] != 0;
+#pragma unroll
+        for (int i = 0; i < NT * 4; ++i) total[i / 4][i % 4] += sums[i * S::THREADS + tid];
+    }
+    return true;
+}
+template <int OUT, int NT, int RG, int CG, int WAVES, int GROUPS>
+__global__ __launch_bounds__((GROUPS * Staged<OUT, NT, RG, CG>::THREADS), WAVES) void mix_blocks_staged_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
 {
     typedef Staged<OUT, NT, RG, CG> S;
     constexpr bool EXACT = OUT == kIn32;
     extern __shared__ uint4_v staged[];
+    const int group = GROUPS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS) : 0;
     unsigned char* const bytes = reinterpret_cast<unsigned char*>(staged);
-    unsigned char* const xs = bytes;                    // two buffers each
-    unsigned char* const ws = bytes + 2 * S::X_BYTES;
+    unsigned char* const xs = bytes + group * S::GROUP_BYTES;       // two buffers each
+    unsigned char* const ws = xs + 2 * S::X_BYTES;
     float* const scales = reinterpret_cast<float*>(ws + 2 * S::W_BYTES);
-    float* const biases = scales + 2 * S::COLUMNS;
+    float* const biases = reinterpret_cast<float*>(bytes + GROUPS * S::GROUP_BYTES);
     const long id = block_index();
     const long slot = by_xcd ? id / 8 : id, column_tile = column_tile_of<OUT == kIn32>(id, slot / row_tiles, column_tiles, by_xcd);
     if (column_tile >= column_tiles) return;
-    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
+    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
     const int wr = wave / CG, wc = wave % CG, wave_row = row0 + wr * 16 * NT;
     const long from = column_tile * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);      // the last tile ends with the columns
-    const int count = q.contraction, steps = (count + kStep - 1) / kStep, whole = count / kStep;
+    const int count = q.contraction, steps = (count + kStep - 1) / kStep, whole = count / kStep, each = (steps + GROUPS - 1) / GROUPS, first = group ? steps - each : 0;
+    const bool twice = group && 2 * each > steps;
     const float* wscale = q.wscale + (long)(wave_row / kScaleBlock) * ((q.contraction + kScaleBlock - 1) / kScaleBlock);
     const int x_row = tid / S::PIECES, x_piece = tid % S::PIECES;
 
@@ -628,19 +656,19 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG>::THREADS), WAVES) void mix
     };
     auto begin = [&](auto guard) {
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) ask(0, j, guard);
-        keep(0, guard);
+        for (int j = 0; j < PIECES; ++j) ask(first, j, guard);
+        keep(first, guard);
     };
-    if (whole) begin(std::false_type());
+    if (first < whole) begin(std::false_type());
     else begin(std::true_type());
     if (q.bias)
-        for (int e = tid; e < S::ROWS; e += S::THREADS)
+        for (int e = threadIdx.x; e < S::ROWS; e += GROUPS * S::THREADS)
             biases[e] = value_of(static_cast<const typename Columns<OUT>::Value*>(q.bias)[row0 + e < q.rows ? row0 + e : q.rows - 1]);
     __syncthreads();
 
     float4_v total[NT][4] = {};
     bool out = false;
-    float weight_scale = common_scale(wscale);
+    float weight_scale = common_scale(wscale + first);
     // a lane reads one half of a row's piece: lanes 2 j and 2 j + 1 row j of eight
     const int piece = wc * 4 ^ S::place_of(16 * kq + (c >> 1));
     const unsigned char* const x_from = xs + (16 * kq + (c >> 1)) * S::COLUMNS + 8 * (c & 1);
@@ -653,6 +681,7 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG>::THREADS), WAVES) void mix
 #pragma unroll
         for (int b = 0; b < 4; ++b) joint[b] = scales[(s & 1) * S::COLUMNS + wc * 64 + 16 * b + c];
         joint = joint_scale(joint, weight_scale, out);
+        if (GROUPS == 2 && twice && s == first) joint = (float4_v){ 0.f, 0.f, 0.f, 0.f };
         if constexpr (NEXT) weight_scale = common_scale(wscale + s + 1);
         Operands<false, EXACT> ops;
 #pragma unroll
@@ -705,12 +734,15 @@ __global__ __launch_bounds__((Staged<OUT, NT, RG, CG>::THREADS), WAVES) void mix
             __syncthreads();
         }
     };
-    for (int s = 0; s < whole - 1; ++s) body(s, std::true_type(), std::false_type());
-    if (whole && whole < steps) body(whole - 1, std::true_type(), std::true_type());
-    body(steps - 1, std::false_type(), std::false_type());
+    const int end = first + each;
+    int s = first;
+    for (; s < end - 1 && s + 1 < whole; ++s) body(s, std::true_type(), std::false_type());
+    if (s < end - 1) body(s++, std::true_type(), std::true_type());
+    body(s, std::false_type(), std::false_type());
 
+    if (!join_groups<NT, GROUPS, S>(group, tid, xs, bytes + S::GROUP_BYTES, total, out)) return;
     // the results' way out: the buffer that the last step did not read
-    put_staged<OUT, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs + (steps & 1) * S::X_BYTES) + wave * 1024, biases + wr * 16 * NT, wave_row,
+    put_staged<OUT, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs + (end & 1) * S::X_BYTES) + wave * 1024, biases + wr * 16 * NT, wave_row,
                         scalar(column0 + wc * 64), from);
 }
 
@@ -729,21 +761,23 @@ __device__ __forceinline__ void direct_word_to_lds(ScalarAddress base, unsigned 
 // operands of x of the next step, read in the second half of this one. So a buffer of x is free again a step earlier than one of W: x is asked for two steps ahead, W one.
 // Loads arrive in their order, and the loop has no others: in the middle of a step those of the step before have, at its end those of W too. Each wait is followed by a barrier,
 // for the other waves' loads; the last step ends with none on the way.
-template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_blocks_direct_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
+template <int NT, int GROUPS> __global__ __launch_bounds__(256 * GROUPS, (NT == 4 || GROUPS == 2 ? 2 : 3)) void mix_blocks_direct_kernel(const MixBlocksParams q, int row_tiles, long column_tiles, bool by_xcd)
 {
     typedef Staged<kIn16, NT, 2, 2> S;
     extern __shared__ uint4_v staged[];
+    const int group = GROUPS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS) : 0;
     unsigned char* const bytes = reinterpret_cast<unsigned char*>(staged);
-    unsigned char *const xs = bytes, *const ws = bytes + 2 * S::X_BYTES;
+    unsigned char *const xs = bytes + group * S::GROUP_BYTES, *const ws = xs + 2 * S::X_BYTES;
     float* const scales = reinterpret_cast<float*>(ws + 2 * S::W_BYTES);
-    float* const biases = scales + 2 * S::COLUMNS;
+    float* const biases = reinterpret_cast<float*>(bytes + GROUPS * S::GROUP_BYTES);
     const long id = block_index();
     const long slot = by_xcd ? id / 8 : id, column_tile = column_tile_of<false>(id, slot / row_tiles, column_tiles, by_xcd);
     if (column_tile >= column_tiles) return;
-    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
+    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
     const int wr = wave / 2, wc = wave % 2, wave_row = row0 + wr * 16 * NT;
     const long from = column_tile * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);
-    const int count = q.contraction, steps = count / kStep;
+    const int count = q.contraction, steps = count / kStep, each = (steps + GROUPS - 1) / GROUPS, first = group ? steps - each : 0;
+    const bool twice = group && 2 * each > steps;
     const float* wscale = q.wscale + (long)(row0 / kScaleBlock) * steps;
     const unsigned x_offset = (unsigned)(lane / 8) * (unsigned)q.ldx + 16 * ((lane % 8) ^ S::place_of(8 * wave + lane / 8));
     constexpr int X_CALLS = S::X_BYTES / 4096, W_CALLS = S::W_BYTES / 4096;
@@ -753,7 +787,7 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
         const int u = (4 * j + wave) * 64 + lane, p = u / 16 % 8, row = u / 128 * 16 + ((u & 15) ^ p);
         w_offset[j] = (unsigned)(row0 + row < q.rows ? row : q.rows - 1 - row0) * (unsigned)count + 16 * p;
     }
-    long x_at = scalar(wave * 8 * q.ldx + column0);     // of the step that is asked for next
+    long x_at = scalar((first * kStep + wave * 8) * q.ldx + column0);     // of the step that is asked for next
     const long x_part = scalar(32 * q.ldx);
     auto ask_x = [&](int s, int j) {
         direct_to_lds(scalar(q.x, x_at), x_offset, place_in_lds(xs) + (s & 1) * S::X_BYTES + (4 * j + wave) * 1024);
@@ -774,23 +808,23 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
     };
     constexpr std::integral_constant<int, 0> none;
     if (q.bias)
-        for (int e = tid; e < S::ROWS; e += S::THREADS) biases[e] = value_of(static_cast<const unsigned short*>(q.bias)[row0 + e < q.rows ? row0 + e : q.rows - 1]);
+        for (int e = threadIdx.x; e < S::ROWS; e += GROUPS * S::THREADS) biases[e] = value_of(static_cast<const unsigned short*>(q.bias)[row0 + e < q.rows ? row0 + e : q.rows - 1]);
 #pragma unroll
-    for (int j = 0; j < X_CALLS; ++j) ask_x(0, j);
-    ask_scales(0);
+    for (int j = 0; j < X_CALLS; ++j) ask_x(first, j);
+    ask_scales(first);
 #pragma unroll
-    for (int j = 0; j < W_CALLS; ++j) ask_w(0, j);
-    if (steps > 1) {
+    for (int j = 0; j < W_CALLS; ++j) ask_w(first, j);
+    if (each > 1) {
 #pragma unroll
-        for (int j = 0; j < X_CALLS; ++j) ask_x(1, j);
-        ask_scales(1);
+        for (int j = 0; j < X_CALLS; ++j) ask_x(first + 1, j);
+        ask_scales(first + 1);
     }
     const int piece = wc * 4 ^ S::place_of(16 * kq + (c >> 1));
     const unsigned char* const x_from = xs + (16 * kq + (c >> 1)) * S::COLUMNS + 8 * (c & 1);
     const uint4_v* const w_from = reinterpret_cast<const uint4_v*>(ws) + wr * NT * 128 + kq * 16;
     int8_v next[4];
     float4_v next_scale;
-    float weight_scale = common_scale(wscale);
+    float weight_scale = common_scale(wscale + first);
     auto read_x = [&](int s, int b) {                   // 16 columns
         const unsigned char* const here = x_from + (s & 1) * S::X_BYTES;
 #pragma unroll
@@ -801,10 +835,10 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
         }
         next_scale[b] = scales[(s & 1) * S::COLUMNS + wc * 64 + 16 * b + c];
     };
-    if (steps > 1) arrived(std::integral_constant<int, X_CALLS + 1>());
+    if (each > 1) arrived(std::integral_constant<int, X_CALLS + 1>());
     else arrived(none);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) read_x(0, b);
+    for (int b = 0; b < 4; ++b) read_x(first, b);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     float4_v total[NT][4] = {};
@@ -815,7 +849,8 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
         Operands<false, false> ops;
 #pragma unroll
         for (int b = 0; b < 4; ++b) ops.b[b] = next[b];
-        const float4_v joint = joint_scale(next_scale, weight_scale, out);
+        float4_v joint = joint_scale(next_scale, weight_scale, out);
+        if (GROUPS == 2 && twice && s == first) joint = (float4_v){ 0.f, 0.f, 0.f, 0.f };
         const uint4_v *const lower = w_from + (s & 1) * (S::W_BYTES / 16) + (c ^ kq), *const upper = w_from + (s & 1) * (S::W_BYTES / 16) + 64 + (c ^ (4 + kq));
         constexpr int CALLS = X_CALLS + W_CALLS + 1;
         auto ask_some = [&](int turn) {
@@ -847,10 +882,12 @@ template <int NT> __global__ __launch_bounds__(256, (NT == 4 ? 2 : 3)) void mix_
         }
         if constexpr (LEFT >= 1) arrived(std::integral_constant<int, LEFT == 2 ? X_CALLS + 1 : 0>());
     };
-    int s = 0;
-    for (; s < steps - 2; ++s) body(s, std::integral_constant<int, 2>());
-    if (s == steps - 2) body(s++, std::integral_constant<int, 1>());
+    const int end = first + each;
+    int s = first;
+    for (; s < end - 2; ++s) body(s, std::integral_constant<int, 2>());
+    if (s == end - 2) body(s++, std::integral_constant<int, 1>());
     body(s, std::integral_constant<int, 0>());
+    if (!join_groups<NT, GROUPS, S>(group, tid, xs, bytes + S::GROUP_BYTES, total, out)) return;
     put_staged<kIn16, NT>(q, out, wscale, total, reinterpret_cast<float*>(xs) + wave * 1024, biases + wr * 16 * NT, wave_row, scalar(column0 + wc * 64), from);
 }
 
@@ -901,27 +938,27 @@ template <int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t 
                        column_tiles, by_xcd);
     return hipGetLastError();
 }
-template <int OUT, int NT, int RG, int CG, int WAVES> hipError_t launch_staged(const MixBlocksParams& q, hipStream_t stream)
+template <int OUT, int NT, int RG, int CG, int WAVES, int GROUPS> hipError_t launch_staged(const MixBlocksParams& q, hipStream_t stream)
 {
     typedef Staged<OUT, NT, RG, CG> S;
     static std::atomic<unsigned long long> served{ 0 };
-    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES>), S::LDS, served); e != hipSuccess) return e;
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES, GROUPS>), S::lds(GROUPS), served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
     const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
     const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(S::THREADS), S::LDS, stream, q,
+    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES, GROUPS>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(GROUPS * S::THREADS), S::lds(GROUPS), stream, q,
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }
-template <int NT> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t stream)
+template <int NT, int GROUPS> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t stream)
 {
     typedef Staged<kIn16, NT, 2, 2> S;
     static std::atomic<unsigned long long> served{ 0 };
-    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_direct_kernel<NT>), S::LDS, served); e != hipSuccess) return e;
+    if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_direct_kernel<NT, GROUPS>), S::lds(GROUPS), served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
     const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
     const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_direct_kernel<NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(S::THREADS), S::LDS, stream, q,
+    hipLaunchKernelGGL((mix_blocks_direct_kernel<NT, GROUPS>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(GROUPS * S::THREADS), S::lds(GROUPS), stream, q,
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }
@@ -932,6 +969,9 @@ constexpr int kOneBlock = 64;
 constexpr long kSplitBlocks = 256;
 // Tiles of 128 rows from which they are enough for the GPU: bf16, 1024 to 1024 at 8192 positions 18.7 us (with 64 rows 21.6), at 4096 13.6 (12.8), at 2048 11.2 (8.5)
 constexpr long kWholeTiles = 384;
+// Tiles of 64 rows up to which there is at most one for each compute unit, so that a second group of waves takes half of the steps. Two groups and one: bf16, 4096 to 4096 channels at 256
+// positions 20.5 us and 23.7, 1024 to 1024 at 2001 (staged) 10.7 and 12.1, at 1024 (direct) 7.8 and 7.6; float32 1024 to 1024 at 500 10.3 and 12.1, 512 to 512 at 1000 7.4 and 7.9
+constexpr long kOneTileEach = 256;
 template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int type, hipStream_t stream)
 {
     if (q.contraction * (COMPLEX ? 2 : 1) <= kOneBlock) {
@@ -955,11 +995,12 @@ template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int
         return launch_tiles<2>(q, stream);
     } else {
         const bool whole_tiles = (columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles;
+        const bool both = (columns + 1) / 2 * ((tiles16 + 3) / 4) <= kOneTileEach && q.contraction > (OUT == kIn32 ? 3 : 7) * kStep;       // bf16, 512 to 512 at 2048 5.8 us with one, 6.1 with two
         if constexpr (OUT == kIn16)                     // one or two steps: 128 to 128 channels at 262144 positions 24.0 us with 64 rows, 26.1 with 128; 512 to 512 at 16384 14.6 and 12.7
             if (q.contraction % kStep == 0 && ((q.ldx | q.columns | (long)q.x | (long)q.W) & 15) == 0)
-                return whole_tiles && q.contraction > 2 * kStep ? launch_direct<4>(q, stream) : launch_direct<2>(q, stream);
-        if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2>(q, stream);
-        return launch_staged<OUT, 2, 2, 2, 3>(q, stream);
+                return whole_tiles && q.contraction > 2 * kStep ? launch_direct<4, 1>(q, stream) : both ? launch_direct<2, 2>(q, stream) : launch_direct<2, 1>(q, stream);
+        if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 1>(q, stream);
+        return both ? launch_staged<OUT, 2, 2, 2, 2, 2>(q, stream) : launch_staged<OUT, 2, 2, 2, 3, 1>(q, stream);
     }
 }
 

@@ -161,10 +161,10 @@ __device__ __forceinline__ void layer_norm_strip(const LayerNormParams& q, float
 #pragma unroll
             for (int c = 0; c < COUNT; ++c) {
                 if ((block + c) * kScaleBlock >= q.K) break;
-                const float4_v factor = write_scales<COMPLEX, FULL>(q.rstd + (block + c) * q.positions, column, lane_there, strip.group() == 0, most[c]);
+                const Divisor by = write_scales<COMPLEX, FULL>(q.rstd + (block + c) * q.positions, column, lane_there, strip.group() == 0, most[c]);
 #pragma unroll
                 for (int r = c * OF_BLOCK; r < (c + 1) * OF_BLOCK && r < COUNT_ROWS; ++r)
-                    if (strip.has(first + r)) write_row<kIn8, FULL>(strip, q.y, q.ldy, column0, there, first + r, eight_bits(four(v[r]), factor));
+                    if (strip.has(first + r)) write_row<kIn8, FULL>(strip, q.y, q.ldy, column0, there, first + r, eight_bits(four(v[r]), by));
             }
         };
         if constexpr (HELD > 0) finish(0, held);

@@ -27,10 +27,10 @@ __device__ __forceinline__ void quantise_strip(const QuantiseParams& q, int bloc
     for (int r = 0; r < HELD; ++r)
         if (strip.has(r)) most[0] = larger4(most[0], magnitude(to_float<IN>(raw[r])));
     block_maxima<COMPLEX, LANES>(most, shared);
-    const float4_v factor = write_scales<COMPLEX, FULL>(q.scale + block * q.positions, column0 + 4 * strip.lane, there - 4 * strip.lane, strip.group() == 0, most[0]);
+    const Divisor by = write_scales<COMPLEX, FULL>(q.scale + block * q.positions, column0 + 4 * strip.lane, there - 4 * strip.lane, strip.group() == 0, most[0]);
 #pragma unroll
     for (int r = 0; r < HELD; ++r)
-        if (strip.has(r)) strip.template write<kIn8, FULL>(to, q.ldq, column0, there, r, eight_bits(to_float<IN>(raw[r]), factor));
+        if (strip.has(r)) strip.template write<kIn8, FULL>(to, q.ldq, column0, there, r, eight_bits(to_float<IN>(raw[r]), by));
 }
 template <int IN, bool COMPLEX, int LANES> __global__ __launch_bounds__(kThreads, 4) void quantise_kernel(const QuantiseParams q, long strips, long run)
 {

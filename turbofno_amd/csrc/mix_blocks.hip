@@ -22,6 +22,7 @@
 // Direct and staged tiles that are fewer than compute units: two groups of waves with half of the steps each.
 // Up to 64 real values of the contraction the kernels of the product with one scale per row are ahead, and take this one's scales.
 #include "kernels.h"
+#include "mix_blocks_choice.h"
 #include "mix_kernel.h"
 #include <algorithm>
 
@@ -31,7 +32,8 @@ namespace {
 
 typedef int int8_v __attribute__((ext_vector_type(8)));
 typedef uint4_v uint4_any __attribute__((aligned(1)));
-constexpr int kStep = 128;                              // real values of a step
+constexpr int kStep = kBlocksStep;
+static_assert(kColumns == 64, "mix_blocks_choice.h counts tiles of 64 columns");
 
 // ---- the input of the tile and split kernels: a lane has four consecutive columns, 4 c ... 4 c + 3 with c = lane % 16, and transposes them ----
 
@@ -929,8 +931,10 @@ template <int OUT, bool COMPLEX, int MODE> __global__ __launch_bounds__(64 * kSp
     if (column0 < q.columns) split<OUT, COMPLEX, MODE>(q, sums, column0, (int)(id % row_tiles) * 16);
 }
 
+// The launches refuse fewer columns than a wave or a block reads: it would read ahead of its operands
 template <int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t stream)
 {
+    if (q.columns < kColumns) return hipErrorInvalidValue;
     const long column_tiles = (q.columns + 4 * kColumns - 1) / (4 * kColumns);
     const int row_tiles = (q.rows + 16 * NT - 1) / (16 * NT);
     const bool by_xcd = column_tiles >= 64;
@@ -941,6 +945,7 @@ template <int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t 
 template <int OUT, int NT, int RG, int CG, int WAVES, int GROUPS> hipError_t launch_staged(const MixBlocksParams& q, hipStream_t stream)
 {
     typedef Staged<OUT, NT, RG, CG> S;
+    if (q.columns < S::COLUMNS) return hipErrorInvalidValue;
     static std::atomic<unsigned long long> served{ 0 };
     if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES, GROUPS>), S::lds(GROUPS), served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
@@ -953,6 +958,7 @@ template <int OUT, int NT, int RG, int CG, int WAVES, int GROUPS> hipError_t lau
 template <int NT, int GROUPS> hipError_t launch_direct(const MixBlocksParams& q, hipStream_t stream)
 {
     typedef Staged<kIn16, NT, 2, 2> S;
+    if (q.columns < S::COLUMNS) return hipErrorInvalidValue;
     static std::atomic<unsigned long long> served{ 0 };
     if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_direct_kernel<NT, GROUPS>), S::lds(GROUPS), served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
@@ -962,45 +968,27 @@ template <int NT, int GROUPS> hipError_t launch_direct(const MixBlocksParams& q,
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }
-// Up to this number of real values the contraction is one step or less than half of one: the product with scales per position and row has kernels for it, whose scales
-// are those of one block. bf16, 64 to 64 channels at 2^20 positions 54 us (here 59 - 70), 16 to 16 at 10^6 16 us (40); 128 to 128 at 262144 29 us (26)
-constexpr int kOneBlock = 64;
-// Blocks of 64 columns and 16 rows up to which their waves divide the steps: bf16, 1024 to 1024 channels at 256 positions 6.8 us (tiles 7.5), at 512 11 (7.7)
-constexpr long kSplitBlocks = 256;
-// Tiles of 128 rows from which they are enough for the GPU: bf16, 1024 to 1024 at 8192 positions 18.7 us (with 64 rows 21.6), at 4096 13.6 (12.8), at 2048 11.2 (8.5)
-constexpr long kWholeTiles = 384;
-// Tiles of 64 rows up to which there is at most one for each compute unit, so that a second group of waves takes half of the steps. Two groups and one: bf16, 4096 to 4096 channels at 256
-// positions 20.5 us and 23.7, 1024 to 1024 at 2001 (staged) 10.7 and 12.1, at 1024 (direct) 7.8 and 7.6; float32 1024 to 1024 at 500 10.3 and 12.1, 512 to 512 at 1000 7.4 and 7.9
-constexpr long kOneTileEach = 256;
 template <int OUT, bool COMPLEX> hipError_t launch(const MixBlocksParams& q, int type, hipStream_t stream)
 {
-    if (q.contraction * (COMPLEX ? 2 : 1) <= kOneBlock) {
+    const BlocksChoice choice = blocks_choice({ COMPLEX, OUT == kIn32, q.columns, q.ldx, q.ldr, q.ldy, q.rows, q.contraction, (((long)q.x | (long)q.W) & 15) == 0 });
+    if (choice.kernel == BlocksKernel::kOneScale) {
         const MixParams p = { q.x, nullptr, q.W, q.bias, q.residual, q.xscale, q.wscale, q.y, nullptr, q.columns, q.ldx, 0, q.ldr, q.ldy, 0, q.rows, q.contraction, q.contraction, q.act,
                               kScaleShift };
         return launch_mix_8bit(p, type, stream);
     }
-    // a lane's part of an address in 32 bits, 48 rows of the input (complex: 24) and 12 of the results
-    const bool near = 48 * q.ldx < (1L << 32) - 4096 && 12 * std::max(q.ldr, q.ldy) * (long)sizeof(typename Columns<OUT>::Value) < (1L << 32) - 4096;
-    const int tiles16 = (q.rows + 15) / 16;
-    const long columns = (q.columns + kColumns - 1) / kColumns;
-    if (!near || q.columns < 2 * kColumns || columns * tiles16 <= kSplitBlocks) {
-        const dim3 grid = grid_of(columns * tiles16), block(64 * kSplitWaves);
-        if (near && (q.contraction + kStep) * q.ldx < (1L << 31)) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kNarrow>), grid, block, 0, stream, q, tiles16);
+    if (choice.kernel == BlocksKernel::kSplitNear || choice.kernel == BlocksKernel::kSplitFar) {
+        const int tiles16 = (q.rows + 15) / 16;
+        const dim3 grid = grid_of((q.columns + kColumns - 1) / kColumns * tiles16), block(64 * kSplitWaves);
+        if (choice.kernel == BlocksKernel::kSplitNear) hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kNarrow>), grid, block, 0, stream, q, tiles16);
         else hipLaunchKernelGGL((mix_blocks_split_kernel<OUT, COMPLEX, kFar64>), grid, block, 0, stream, q, tiles16);
         return hipGetLastError();
     }
-    if constexpr (COMPLEX) {
-        const long wide = (columns + 3) / 4;
-        if (tiles16 > 2 && wide * ((tiles16 + 3) / 4) >= 256) return launch_tiles<4>(q, stream);
-        return launch_tiles<2>(q, stream);
-    } else {
-        const bool whole_tiles = (columns + 1) / 2 * ((tiles16 + 7) / 8) >= kWholeTiles;
-        const bool both = (columns + 1) / 2 * ((tiles16 + 3) / 4) <= kOneTileEach && q.contraction > (OUT == kIn32 ? 3 : 7) * kStep;       // bf16, 512 to 512 at 2048 5.8 us with one, 6.1 with two
-        if constexpr (OUT == kIn16)                     // one or two steps: 128 to 128 channels at 262144 positions 24.0 us with 64 rows, 26.1 with 128; 512 to 512 at 16384 14.6 and 12.7
-            if (q.contraction % kStep == 0 && ((q.ldx | q.columns | (long)q.x | (long)q.W) & 15) == 0)
-                return whole_tiles && q.contraction > 2 * kStep ? launch_direct<4, 1>(q, stream) : both ? launch_direct<2, 2>(q, stream) : launch_direct<2, 1>(q, stream);
-        if (whole_tiles) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 1>(q, stream);
-        return both ? launch_staged<OUT, 2, 2, 2, 2, 2>(q, stream) : launch_staged<OUT, 2, 2, 2, 3, 1>(q, stream);
+    if constexpr (COMPLEX) return choice.nt == 4 ? launch_tiles<4>(q, stream) : launch_tiles<2>(q, stream);
+    else {
+        if constexpr (OUT == kIn16)
+            if (choice.kernel == BlocksKernel::kDirect) return choice.nt == 4 ? launch_direct<4, 1>(q, stream) : choice.groups == 2 ? launch_direct<2, 2>(q, stream) : launch_direct<2, 1>(q, stream);
+        if (choice.nt == 4) return launch_staged<OUT, 4, 2, OUT == kIn32 ? 4 : 2, 2, 1>(q, stream);
+        return choice.groups == 2 ? launch_staged<OUT, 2, 2, 2, 2, 2>(q, stream) : launch_staged<OUT, 2, 2, 2, 3, 1>(q, stream);
     }
 }
 

@@ -1,0 +1,22 @@
+"""Which blocks take which pieces of work, on the CPU: each piece is one block's, also in launches of several rows of blocks. A piece that two blocks took would be added or activated twice
+where its result replaces an operand."""
+import os
+import subprocess
+
+import pytest
+
+HOST = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host")
+
+
+def run(tmp_path, name, lines):
+    exe = str(tmp_path / name)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", os.path.join(HOST, name + ".cpp"), "-o", exe], check=True)
+    text = "".join(" ".join(map(str, ln)) + "\n" for ln in lines)
+    return [tuple(map(int, ln.split())) for ln in subprocess.run([exe], input=text, check=True, capture_output=True, text=True).stdout.splitlines()]
+
+
+@pytest.mark.parametrize("together", [0, 1])
+def test_each_strip_is_one_block_s(tmp_path, together):
+    row = 1 << 22
+    strips = [1, 7, 8, 9, 64, 1000, row - 1, row, row + 1, row + 9, 2 * row, 2 * row + 2, 2 * row + 17]
+    assert run(tmp_path, "block_order_check", [(n, together) for n in strips]) == [(0, 0)] * len(strips)

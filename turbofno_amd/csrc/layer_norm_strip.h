@@ -183,7 +183,7 @@ template <int IN, bool COMPLEX, bool DROP, bool EIGHT, int LANES, int HELD>
 __global__ __launch_bounds__(kThreads, (IN == kIn16 && HELD < 16 && !(EIGHT && LANES < 16) ? 4 : 2)) void layer_norm_kernel(const LayerNormParams q, long run)
 {
     typedef Strip<LANES> S;
-    const long id = block_index(), column0 = (run ? id % 8 * run + id / 8 : id) * S::COLUMNS;
+    const long id = block_index(), column0 = (run ? side_by_side(id, run) : id) * S::COLUMNS;
     if (column0 >= q.columns) return;
     __shared__ float4_v shared[kAreas<EIGHT, LANES, HELD> * (kThreads / 64) * LANES];
     __shared__ Affine<COMPLEX> affines[HELD ? HELD * S::GROUPS : 1];

@@ -35,7 +35,7 @@ __device__ __forceinline__ void quantise_strip(const QuantiseParams& q, int bloc
 template <int IN, bool COMPLEX, int LANES> __global__ __launch_bounds__(kThreads, 4) void quantise_kernel(const QuantiseParams q, long strips, long run)
 {
     __shared__ float4_v shared[kThreads / 64 * LANES];
-    const long id = block_index(), block = id / strips, place = id - block * strips, column0 = (run ? place % 8 * run + place / 8 : place) * (4 * LANES);
+    const long id = block_index(), block = id / strips, place = id - block * strips, column0 = (run ? side_by_side(place, run) : place) * (4 * LANES);
     if (block * kScaleBlock >= q.K || column0 >= q.columns) return;
     if (column0 + 4 * LANES <= q.columns) quantise_strip<IN, COMPLEX, LANES, true>(q, (int)block, shared, column0, 4 * LANES);
     else quantise_strip<IN, COMPLEX, LANES, false>(q, (int)block, shared, column0, (int)(q.columns - column0));

@@ -19,4 +19,11 @@ def run(tmp_path, name, lines):
 def test_each_strip_is_one_block_s(tmp_path, together):
     row = 1 << 22
     strips = [1, 7, 8, 9, 64, 1000, row - 1, row, row + 1, row + 9, 2 * row, 2 * row + 2, 2 * row + 17]
-    assert run(tmp_path, "block_order_check", [(n, together) for n in strips]) == [(0, 0)] * len(strips)
+    assert run(tmp_path, "block_order_check", [(0, n, together) for n in strips]) == [(0, 0)] * len(strips)
+
+
+@pytest.mark.parametrize("turns", [0, 1])
+def test_each_tile_is_one_block_s(tmp_path, turns):
+    row = 1 << 22
+    tiles = [(1, 1), (3, 63), (3, 64), (2, 65), (17, 1001), (1, row - 7), (1, row), (1, row + 1), (1, row + 9), (3, row // 3), (3, row // 3 + 5), (5, row // 2 + 3), (1024, 4095), (1024, 4097)]
+    assert run(tmp_path, "block_order_check", [(1,) + t + (turns,) for t in tiles]) == [(0, 0)] * len(tiles)

@@ -10,4 +10,18 @@ constexpr long grid_rows(long blocks) { return blocks <= kGridRow ? 1 : (blocks 
 constexpr long kNoPlace = 1L << 48;
 constexpr long side_by_side(long id, long run) { return id / 8 < run ? id % 8 * run + id / 8 : kNoPlace; }
 
+// Tiles of a product, `row_tiles` over each of `column_tiles` tiles of columns. With many columns (from 64 tiles on) those of the same columns follow one another on one XCD, whose L2 cache
+// then holds them; `turns`: neighbours go to the XCDs in turns, otherwise side by side to one of them. Tiles beyond the last are those of blocks that have none
+struct Tile {
+    long column;
+    int row;
+};
+constexpr bool tiles_by_xcd(long column_tiles) { return column_tiles >= 64; }
+constexpr long tile_blocks(int row_tiles, long column_tiles) { return (tiles_by_xcd(column_tiles) ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles; }
+constexpr Tile tile_of(long id, int row_tiles, long column_tiles, bool by_xcd, bool turns)
+{
+    const long slot = by_xcd ? id / 8 : id, nth = slot / row_tiles, among = nth * 8 + id % 8;
+    return { !by_xcd ? nth : turns ? among : side_by_side(among, (column_tiles + 7) / 8), (int)(slot % row_tiles) };
+}
+
 }  // namespace tfno

@@ -382,12 +382,8 @@ __device__ __forceinline__ void sum_steps(const MixBlocksParams& q, const Input<
 
 // ---- many columns, complex: four waves side by side share 16 NT rows of W ----
 
-// The tile of columns of a block. Blocks go to the eight XCDs in turns: with many columns (by_xcd) those of the same columns follow one another on one XCD, whose L2 cache then holds
-// them. So do tiles side by side: bf16, 512 to 512 channels at 65551 positions 44.8 us (in turns 48.4), 2048 to 2048 at 32768 197 (205); float32 512 to 512 at 65536 63.0 (58.7)
-template <bool TURNS> __device__ __forceinline__ long column_tile_of(long id, long nth, long column_tiles, bool by_xcd)
-{
-    return !by_xcd ? nth : TURNS ? nth * 8 + id % 8 : id % 8 * ((column_tiles + 7) / 8) + nth;
-}
+// Blocks go to the eight XCDs in turns (block_order.h). With many columns, tiles side by side go to one: bf16, 512 to 512 channels at 65551 positions 44.8 us (in turns 48.4), 2048 to 2048 at
+// 32768 197 (205); not for float32, 512 to 512 at 65536 63.0 (58.7)
 // The weights of a step pass LDS, in the order in which lanes read them: 16 bytes per lane, half and 16 rows. Two buffers: a step's are written while those of the
 // step before are read, after they were asked for ahead of its products, like the rows of x of the next step. A wave whose 64 columns are not all there takes the last
 // 64 and leaves those that it shares with others alone; one that has none goes along for its part of the weights.
@@ -399,10 +395,10 @@ __global__ __launch_bounds__(256, 2) void mix_blocks_tile_kernel(const MixBlocks
     __shared__ uint4_v weights[2 * CHUNKS];
     __shared__ float biases[16 * NT * V];
     const long id = block_index();
-    const long slot = by_xcd ? id / 8 : id, column_tile = column_tile_of<false>(id, slot / row_tiles, column_tiles, by_xcd);
-    if (column_tile >= column_tiles) return;
-    const int row0 = (int)(slot % row_tiles) * (16 * NT), lane = threadIdx.x & 63;
-    const long from = column_tile * (4 * kColumns) + (long)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kColumns;
+    const Tile tile = tile_of(id, row_tiles, column_tiles, by_xcd, false);
+    if (tile.column >= column_tiles) return;
+    const int row0 = tile.row * (16 * NT), lane = threadIdx.x & 63;
+    const long from = tile.column * (4 * kColumns) + (long)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kColumns;
     const Input<true, kWindow> in(q, scalar(from + kColumns <= q.columns ? from : q.columns - kColumns));
     const int count = q.contraction * V, steps = (count + kStep - 1) / kStep;
     const float* wscale = q.wscale + (long)(row0 / kScaleBlock) * ((q.contraction + kScaleBlock - 1) / kScaleBlock);
@@ -608,11 +604,11 @@ __global__ __launch_bounds__((GROUPS * Staged<OUT, NT, RG, CG>::THREADS), WAVES)
     float* const scales = reinterpret_cast<float*>(ws + 2 * S::W_BYTES);
     float* const biases = reinterpret_cast<float*>(bytes + GROUPS * S::GROUP_BYTES);
     const long id = block_index();
-    const long slot = by_xcd ? id / 8 : id, column_tile = column_tile_of<OUT == kIn32>(id, slot / row_tiles, column_tiles, by_xcd);
-    if (column_tile >= column_tiles) return;
-    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
+    const Tile tile = tile_of(id, row_tiles, column_tiles, by_xcd, OUT == kIn32);
+    if (tile.column >= column_tiles) return;
+    const int row0 = tile.row * S::ROWS, tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
     const int wr = wave / CG, wc = wave % CG, wave_row = row0 + wr * 16 * NT;
-    const long from = column_tile * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);      // the last tile ends with the columns
+    const long from = tile.column * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);      // the last tile ends with the columns
     const int count = q.contraction, steps = (count + kStep - 1) / kStep, whole = count / kStep, each = (steps + GROUPS - 1) / GROUPS, first = group ? steps - each : 0;
     const bool twice = group && 2 * each > steps;
     const float* wscale = q.wscale + (long)(wave_row / kScaleBlock) * ((q.contraction + kScaleBlock - 1) / kScaleBlock);
@@ -773,11 +769,11 @@ template <int NT, int GROUPS> __global__ __launch_bounds__(256 * GROUPS, (NT == 
     float* const scales = reinterpret_cast<float*>(ws + 2 * S::W_BYTES);
     float* const biases = reinterpret_cast<float*>(bytes + GROUPS * S::GROUP_BYTES);
     const long id = block_index();
-    const long slot = by_xcd ? id / 8 : id, column_tile = column_tile_of<false>(id, slot / row_tiles, column_tiles, by_xcd);
-    if (column_tile >= column_tiles) return;
-    const int row0 = (int)(slot % row_tiles) * S::ROWS, tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
+    const Tile tile = tile_of(id, row_tiles, column_tiles, by_xcd, false);
+    if (tile.column >= column_tiles) return;
+    const int row0 = tile.row * S::ROWS, tid = threadIdx.x % S::THREADS, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, kq = lane >> 4;
     const int wr = wave / 2, wc = wave % 2, wave_row = row0 + wr * 16 * NT;
-    const long from = column_tile * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);
+    const long from = tile.column * S::COLUMNS, column0 = scalar(from + S::COLUMNS <= q.columns ? from : q.columns - S::COLUMNS);
     const int count = q.contraction, steps = count / kStep, each = (steps + GROUPS - 1) / GROUPS, first = group ? steps - each : 0;
     const bool twice = group && 2 * each > steps;
     const float* wscale = q.wscale + (long)(row0 / kScaleBlock) * steps;
@@ -937,8 +933,8 @@ template <int NT> hipError_t launch_tiles(const MixBlocksParams& q, hipStream_t 
     if (q.columns < kColumns) return hipErrorInvalidValue;
     const long column_tiles = (q.columns + 4 * kColumns - 1) / (4 * kColumns);
     const int row_tiles = (q.rows + 16 * NT - 1) / (16 * NT);
-    const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_tile_kernel<NT>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(256), 0, stream, q, row_tiles,
+    const bool by_xcd = tiles_by_xcd(column_tiles);
+    hipLaunchKernelGGL((mix_blocks_tile_kernel<NT>), grid_of(tile_blocks(row_tiles, column_tiles)), dim3(256), 0, stream, q, row_tiles,
                        column_tiles, by_xcd);
     return hipGetLastError();
 }
@@ -950,8 +946,8 @@ template <int OUT, int NT, int RG, int CG, int WAVES, int GROUPS> hipError_t lau
     if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES, GROUPS>), S::lds(GROUPS), served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
     const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
-    const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES, GROUPS>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(GROUPS * S::THREADS), S::lds(GROUPS), stream, q,
+    const bool by_xcd = tiles_by_xcd(column_tiles);
+    hipLaunchKernelGGL((mix_blocks_staged_kernel<OUT, NT, RG, CG, WAVES, GROUPS>), grid_of(tile_blocks(row_tiles, column_tiles)), dim3(GROUPS * S::THREADS), S::lds(GROUPS), stream, q,
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }
@@ -963,8 +959,8 @@ template <int NT, int GROUPS> hipError_t launch_direct(const MixBlocksParams& q,
     if (hipError_t e = allow_dynamic_lds(reinterpret_cast<const void*>(mix_blocks_direct_kernel<NT, GROUPS>), S::lds(GROUPS), served); e != hipSuccess) return e;
     const long column_tiles = (q.columns + S::COLUMNS - 1) / S::COLUMNS;
     const int row_tiles = (q.rows + S::ROWS - 1) / S::ROWS;
-    const bool by_xcd = column_tiles >= 64;
-    hipLaunchKernelGGL((mix_blocks_direct_kernel<NT, GROUPS>), grid_of((by_xcd ? (column_tiles + 7) / 8 * 8 : column_tiles) * row_tiles), dim3(GROUPS * S::THREADS), S::lds(GROUPS), stream, q,
+    const bool by_xcd = tiles_by_xcd(column_tiles);
+    hipLaunchKernelGGL((mix_blocks_direct_kernel<NT, GROUPS>), grid_of(tile_blocks(row_tiles, column_tiles)), dim3(GROUPS * S::THREADS), S::lds(GROUPS), stream, q,
                        row_tiles, column_tiles, by_xcd);
     return hipGetLastError();
 }

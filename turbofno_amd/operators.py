@@ -148,6 +148,11 @@ def _meet(a, b):
     return False
 
 
+def _over(y, x):
+    """is the result to take the place of x"""
+    return isinstance(y, torch.Tensor) and isinstance(x, torch.Tensor) and y.numel() > 0 and y.data_ptr() == x.data_ptr()
+
+
 def _input(x, name):
     """type, device, channels and positions of the field a call starts from"""
     if not isinstance(x, torch.Tensor):
@@ -402,13 +407,14 @@ def dropout(x, drop, rng, residual=None, y=None):
 
 def layer_norm(x, gain, bias=None, residual=None, eps=1e-6, drop=0.0, rng=None, y=None, s=None, mean=None, rstd=None):
     """s = residual + dropout(x), mean over channels of s, rstd = 1 / sqrt(mean over channels of |s - mean|^2 + eps), y = gain rstd (s - mean) + bias: x[K][...],
-    gain[K] in float32, bias[K] in float32, complex64 for complex fields -> (y, s, mean, rstd). Without residual and dropout s is x itself. `s` and `y` may be `x` or
-    `residual` themselves; mean (of the type of bias) and rstd have the shape of the positions. drop, rng: as dropout takes them. Not recorded for autograd:
+    gain[K] in float32, bias[K] in float32, complex64 for complex fields -> (y, s, mean, rstd). Without residual and dropout s is x itself, or what x was where y replaces it. `s` and `y`
+    may be `x` or `residual` themselves; mean (of the type of bias) and rstd have the shape of the positions. drop, rng: as dropout takes them. Not recorded for autograd:
     the gradients are layer_norm_backward's."""
+    summed = residual is not None or drop or _over(y, x)
     if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() >= 2:
         y, mean = _result(y, x.shape, x.dtype, x.device), _result(mean, x.shape[1:], _wide(x.dtype), x.device)
         rstd = _result(rstd, x.shape[1:], torch.float32, x.device)
-        if residual is not None or drop:
+        if summed:
             s = _result(s, x.shape, x.dtype, x.device)
         if _compiled("layer_norm", ("layer_norm",), x, gain, bias, residual, eps, drop, rng, s, y, mean, rstd):
             return y, x if s is None else s, mean, rstd
@@ -420,7 +426,7 @@ def layer_norm(x, gain, bias=None, residual=None, eps=1e-6, drop=0.0, rng=None, 
         raise TypeError("gain must be a float32 tensor on the GPU")
     pg, pb = _packed(gain, "gain", (K,), torch.float32, device), _packed(bias, "bias", (K,), _wide(dtype), device)
     pd = _rng(rng, device)
-    if residual is not None or drop:
+    if summed:
         s = _result(s, x.shape, dtype, device)
     y, mean, rstd = _result(y, x.shape, dtype, device), _result(mean, places, _wide(dtype), device), _result(rstd, places, torch.float32, device)
     ps, lds = _field(s, "s", x.shape, dtype, device)

@@ -32,3 +32,19 @@ def test_layer_norm(kind, K, P, drop):
     assert got[1] is s and all(torch.equal(a, b) for a, b in zip(got, want))
     empty = x[:, :0].contiguous()
     assert tf.layer_norm(empty, gain, bias, y=empty)[1].shape == (K, 0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("K,P", [(20, 300), (600, 70)])
+@pytest.mark.parametrize("passed", [True, False])
+def test_rms_norm(kind, K, P, passed):
+    x, gain, _, gy = operands(kind, K, P)
+    want = tf.rms_norm(x, gain)
+    grads = tf.rms_norm_backward(gy, want[1], gain, want[2])
+    place, rstd = x.clone(), torch.empty(P, device="cuda") if passed else None
+    got = tf.rms_norm(place, gain, y=place, rstd=rstd)
+    assert got[0] is place and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(tf.rms_norm_backward(gy, got[1], gain, got[2]), grads))
+    place, s = x.clone(), torch.empty_like(x)
+    got = tf.rms_norm(place, gain, y=place, s=s, rstd=rstd)
+    assert got[1] is s and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -296,6 +296,8 @@ def mix_backward(gy, x, W, z=None, activation="none", gz=None, gx=None, gW=None,
 
 def _norm(x, gain, residual, eps, y, scale, s, rstd, eight):
     row = scale if eight else rstd
+    if residual is None and s is None and _over(y, x):
+        s = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if row is not None and (residual is None or s is not None) and getattr(y, "is_cuda", False):
         if _compiled("rms_norm", ("rms_norm_8bit" if eight else "rms_norm",), int(eight), x, gain, residual, eps, s, y, row):
             return y, row, x if s is None else s
@@ -329,8 +331,8 @@ def _norm(x, gain, residual, eps, y, scale, s, rstd, eight):
 
 def rms_norm(x, gain, residual=None, eps=1e-6, y=None, s=None, rstd=None):
     """s = x + residual, rstd = 1 / sqrt(mean over channels of |s|^2 + eps), y = gain rstd s: x[K][...], gain[K] in float32 -> (y, s, rstd).
-    Without a residual s is x itself. `s` and `y` may be `x` or `residual` themselves; rstd has the shape of the positions. Not recorded for autograd: the
-    gradients are rms_norm_backward's."""
+    Without a residual s is x itself, or what x was where y replaces it. `s` and `y` may be `x` or `residual` themselves; rstd has the shape of the positions.
+    Not recorded for autograd: the gradients are rms_norm_backward's."""
     y, rstd, s = _norm(x, gain, residual, eps, y, None, s, rstd, False)
     return y, s, rstd
 

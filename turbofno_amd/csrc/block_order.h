@@ -1,5 +1,6 @@
 // Which blocks a launch has and which pieces of work they take. Plain arithmetic, so that it can be checked without a GPU.
 #pragma once
+#include <algorithm>
 
 namespace tfno {
 
@@ -22,6 +23,31 @@ constexpr Tile tile_of(long id, int row_tiles, long column_tiles, bool by_xcd, b
 {
     const long slot = by_xcd ? id / 8 : id, nth = slot / row_tiles, among = nth * 8 + id % 8;
     return { !by_xcd ? nth : turns ? among : side_by_side(among, (column_tiles + 7) / 8), (int)(slot % row_tiles) };
+}
+
+// Persistent blocks over strips of a field (gradient of the layer norm): those of a block, of `strips` from the one `base`, are every `step`th of all, or, `together`, of an eighth of them
+constexpr long kGradBlocks = 512;
+struct StripTurns {
+    long base, strips, run, step;
+    constexpr StripTurns(long from, long all, bool together) : base(from), strips(all), run(together ? (all + 7) / 8 : 0), step(std::min(together ? run : all, together ? kGradBlocks / 8 : kGradBlocks)) { }
+    constexpr long blocks() const { return run ? 8 * step : step; }
+    constexpr long first(unsigned block) const { return base + (run ? block % 8 * run + block / 8 : block); }
+    constexpr long last(unsigned block) const { return base + (run && (block % 8 + 1) * run < strips ? (block % 8 + 1) * run : strips); }
+};
+// Strips of a launch, up to 64 for each block: one sum over many more would round off as a whole, the more the larger it has grown (a constant gradient of 0.1 over 2^28 positions: in one launch
+// off by 6.5e-5, so by 3.7e-6). Each launch has sums of its own
+constexpr long kLaunchStrips = 64 * kGradBlocks;
+constexpr long grad_launches(long strips) { return (strips + kLaunchStrips - 1) / kLaunchStrips; }
+constexpr long strips_of_launch(long strips)            // whole rounds of blocks
+{
+    const long launches = grad_launches(strips);
+    return launches ? ((strips + launches - 1) / launches + kGradBlocks - 1) / kGradBlocks * kGradBlocks : 0;
+}
+// blocks of all launches, at most: strips of 8 columns are the narrowest, of 32 where there are several launches
+constexpr long grad_rows(long columns)
+{
+    const long launches = grad_launches((columns + 31) / 32);
+    return launches > 1 ? launches * kGradBlocks : std::max(1l, std::min((columns + 7) / 8, kGradBlocks));
 }
 
 }  // namespace tfno

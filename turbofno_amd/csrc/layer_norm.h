@@ -13,15 +13,6 @@ constexpr long kNarrowColumns = 8192;                   // strips of 8 to 32 col
 inline bool far_apart(long ld) { return ld >= (1L << 30) / 32; }
 constexpr int kChunk = 8;                               // channels of a lane whose loads overlap where not all are held
 
-// The strips of a block: every `step`th of all, or of an eighth of them (block i runs on XCD i % 8)
-struct StripTurns {
-    long strips, run, step;
-    StripTurns(long all, bool together, long most_blocks) : strips(all), run(together ? (all + 7) / 8 : 0), step(std::min(together ? run : all, together ? most_blocks / 8 : most_blocks)) { }
-    long blocks() const { return run ? 8 * step : step; }
-    __device__ __forceinline__ long first(unsigned block) const { return run ? block % 8 * run + block / 8 : block; }
-    __device__ __forceinline__ long last(unsigned block) const { return run ? (block % 8 + 1) * run < strips ? (block % 8 + 1) * run : strips : strips; }
-};
-
 // with dropout, what a lane keeps of its columns
 struct KeepAll { };
 template <bool COMPLEX, bool DROP> __device__ __forceinline__ auto keep_of(const Drop& drop, long column)

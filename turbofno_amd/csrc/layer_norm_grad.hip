@@ -3,7 +3,7 @@
 //   g_k = gain_k gy_k,  gr_k = rstd (g_k - mean g - h_k mean Re(conj(h) g)) + gs_k,  gx_k = keep gr_k / (1 - drop)
 //   ggain_k = sum_p Re(conj(h_k) gy_k),  gbias_k = sum_p gy_k
 //
-// Strips of positions with all of their channels, as in the norm; the blocks are persistent and hold their sums over positions in registers, a second kernel adds
+// Strips of positions with all of their channels, as in the norm; the blocks are persistent and hold their sums over positions in registers, a last kernel adds
 // them up in a fixed order. Where the channels do not fit into registers the strip is read twice and the sums lie in the workspace.
 //
 // complex64, 64 channels at 2^20 positions with residual stream and dropout 528 us, 5.1 TB/s: the stream, and 5 us of the second kernel. bf16 takes as long per value for half the
@@ -260,20 +260,23 @@ __global__ __launch_bounds__(1024) void add_sums_kernel(const float* __restrict_
     else if (gbias) gbias[value - K] = v;
 }
 
-constexpr long kGradBlocks = 512;                       // persistent blocks
-
-// Lanes side by side and channels held per lane (0: read twice). The workspace is for as many blocks as there are strips of the narrowest kind
+// Lanes side by side and channels held per lane (0: read twice)
 template <int IN, bool COMPLEX, bool DROP, int LANES, int HELD> hipError_t launch_as(const LayerNormGradParams& q, hipStream_t stream)
 {
-    const long strips = (q.columns + 4 * LANES - 1) / (4 * LANES);
-    const StripTurns turns(strips, LANES >= 4 && run_together(q.columns, IN, strips), kGradBlocks);
-    const long blocks = turns.blocks();
-    if (blocks) {
-        if constexpr (HELD > 0) hipLaunchKernelGGL((layer_norm_grad_kernel<IN, COMPLEX, DROP, LANES, HELD>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, turns);
-        else hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, LANES>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, q, turns);
+    const long strips = (q.columns + 4 * LANES - 1) / (4 * LANES), each = strips_of_launch(strips);
+    const int count = q.K * (COMPLEX ? 3 : 2);
+    long blocks = 0;
+    for (long base = 0; base < strips; base += each) {
+        const long these = std::min(each, strips - base);
+        const StripTurns turns(base, these, LANES >= 4 && run_together(q.columns, IN, these));
+        LayerNormGradParams part = q;
+        part.sums += blocks * count;
+        blocks += turns.blocks();
+        const dim3 grid((unsigned)turns.blocks()), block(kThreads);
+        if constexpr (HELD > 0) hipLaunchKernelGGL((layer_norm_grad_kernel<IN, COMPLEX, DROP, LANES, HELD>), grid, block, 0, stream, part, turns);
+        else hipLaunchKernelGGL((layer_norm_grad_long_kernel<IN, COMPLEX, DROP, LANES>), grid, block, 0, stream, part, turns);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
-    const int count = q.K * (COMPLEX ? 3 : 2);
     hipLaunchKernelGGL(add_sums_kernel, dim3((unsigned)((count + 15) / 16)), dim3(1024), 0, stream, q.sums, blocks, q.K, count, q.ggain, q.gbias);
     return hipGetLastError();
 }
@@ -307,8 +310,7 @@ template <int IN, bool COMPLEX> hipError_t launch_grad(const LayerNormGradParams
 
 size_t layer_norm_backward_workspace(int type, long P, int K)
 {
-    const long blocks = std::min((P * values_of(type) + 7) / 8, kGradBlocks);          // strips of 8 columns are the narrowest
-    return (size_t)(blocks ? blocks : 1) * K * (1 + values_of(type)) * sizeof(float);
+    return (size_t)grad_rows(P * values_of(type)) * K * (1 + values_of(type)) * sizeof(float);
 }
 
 hipError_t launch_layer_norm_backward(const LayerNormGradParams& q, int type, hipStream_t stream)

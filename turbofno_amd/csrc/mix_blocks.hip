@@ -47,6 +47,7 @@ template <bool COMPLEX> struct RawStep {
 // whatever lies between the channels. For few columns kNarrow is ahead of kWindow also where all 64 exist, by the rows' scalar parts: 4096 to 4096 channels at 64 10.7 us, 14.8
 enum { kWindow = 0, kNarrow = 1, kFar64 = 2 };
 template <bool COMPLEX, int MODE> struct Input {
+    static_assert(COMPLEX || MODE != kWindow, "the tiles of real fields read x their own way");
     static constexpr int V = COMPLEX ? 2 : 1, HALF = kRowsOfHalf<COMPLEX>;
     const MixBlocksParams& q;
     const int c, kq, there;
@@ -83,11 +84,11 @@ template <bool COMPLEX, int MODE> struct Input {
                 const long column = column0 + 4 * c + i;
                 raw.scale[i] = q.xscale[scales + (column >= q.columns ? q.columns - 1 : column) / V];
             }
-        else if constexpr (COMPLEX) {
+        else {
             const uint2_v v = near_load4<kIn16>(scalar(q.xscale, (scales + column0 / 2) * 4), fresh(8 * c));        // two floats, any multiple of 4 bytes
             const float2_v f = __builtin_bit_cast(float2_v, v);
             raw.scale = (float4_v){ f[0], f[0], f[1], f[1] };
-        } else raw.scale = near_load4<kIn32>(scalar(q.xscale, (scales + column0) * 4), fresh(16 * c));
+        }
     }
     __device__ __forceinline__ void clear(int step, RawStep<COMPLEX>& raw) const
     {

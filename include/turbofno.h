@@ -272,9 +272,9 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *   turbofno_dropout         y = residual + dropout(x) (residual may be NULL): dropout(x) is x / (1 - drop) where the element is kept and 0 elsewhere, whatever x
  *                            is there; 0 <= drop < 1. No mask is stored: the element of channel k at position p is kept where word p % 4 of
  *                            Philox 4x32-10 (Salmon, Moraes, Dror, Shaw 2011) with key = seed and counter = (low 32 bits of p / 4, k + 2^16 (p / 4 >> 32),
- *                            offset) is at least the whole number nearest to drop 2^32; a complex element is kept or dropped as a whole. `rng`: two 64-bit
- *                            numbers on the GPU, seed and offset, which are read when the kernel runs, so that a captured graph takes what stands there at
- *                            each replay. Each use in a model and each step takes an offset (or a seed) of its own. The gradient of x is the same call on the
+ *                            offset) is at least the whole number nearest to drop 2^32, at most 2^32 - 1; a complex element is kept or dropped as a whole.
+ *                            `rng`: two 64-bit numbers on the GPU, seed and offset, which are read when the kernel runs, so that a captured graph takes what
+ *                            stands there at each replay. Each use in a model and each step takes an offset (or a seed) of its own. The gradient of x is the same call on the
  *                            gradient of y, with the same rng, that of residual is the gradient of y. y may be x or residual itself.
  *   turbofno_layer_norm      s = residual + dropout(x), mean[p] = mean over k of s[k][p], rstd[p] = 1 / sqrt(mean over k of |s - mean|^2 + eps),
  *                            y[k] = gain[k] rstd (s[k] - mean) + bias[k]. gain [K] in fp32, bias [K] and mean [P] in fp32 or, for complex fields, complex64.
@@ -285,7 +285,8 @@ int turbofno_query_1d_tile(int logDY, long M, int N, int K, int compute_units, i
  *                            not used and may be NULL. ggain [K], gbias [K] (in the type of bias; may be NULL). gx and gr may be gy, s or gs themselves, but do
  *                            not overlap. The sums do not depend on anything but the operands and sizes. Workspace: as queried, 4-byte aligned.
  *   turbofno_quantise_8bit   scale[b][p] = max over the channels k of block b of |x[k][p]| / 448 (real and imaginary parts; 1 where that is below 2^-126, and
- *                            all q of the block are zeros then; NaN where an x of it is infinite or NaN), q = x / scale in e4m3: scale [ceil(K / 128)][P].
+ *                            all q of the block are zeros then; NaN where an x of it is infinite or NaN), q = x / scale, rounded to fp32 and then, ties to
+ *                            even, to e4m3: scale [ceil(K / 128)][P].
  *   turbofno_mix_8bit_blocks turbofno_mix_8bit with x = xscale[k / 128][p] xq[k][p] and W = wscale[n / 128][k / 128] Wq[n][k]: xscale [ceil(K / 128)][P],
  *                            wscale [ceil(N / 128)][ceil(K / 128)]. A bf16 result's sums of 128 products drop of each what lies more than about 2^-19 below their
  *                            largest (2^-12 of the sum of magnitudes at most); results in 32 bits are sums in fp32.

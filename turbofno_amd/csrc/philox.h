@@ -2,7 +2,7 @@
 // SC 2011), a function of a key and a counter, so that no mask is stored and the gradient forms the same one again:
 //
 //   key = seed (two words),  counter = (low word of q, channel + 2^16 high word of q, offset (two words)),  q = position / 4
-//   element kept  <=>  word position % 4 of the result >= threshold, the whole number nearest to drop 2^32
+//   element kept  <=>  word position % 4 of the result >= threshold, the whole number nearest to drop 2^32, at most 2^32 - 1
 //
 // q has at most 34 bits and a channel 16. A complex element is kept or dropped as a whole. The numbers depend on nothing else: not on strides, types or the
 // kernel that asks. The key and the offset lie in memory of the GPU, so that a captured graph draws other numbers when its user has changed them.

@@ -6,9 +6,10 @@
 // Strips of positions with all of their channels, as in the norm; the blocks are persistent and hold their sums over positions in registers, a last kernel adds
 // them up in a fixed order. Where the channels do not fit into registers the strip is read twice and the sums lie in the workspace.
 //
-// complex64, 64 channels at 2^20 positions with residual stream and dropout 528 us, 5.1 TB/s: the stream, and 5 us of the second kernel. bf16 takes as long per value for half the
-// bytes, 256 channels at 131072 55 us, 3.7 TB/s. 200 channels at 30011 positions, bf16, 19.3 us: 469 strips are one round, in which loads, sums, joins and stores follow one another
-// (16.0 us at 30016, where rows start at whole cache lines), and 4 us of the second kernel.
+// complex64, 64 channels at 2^20 positions with residual stream and dropout 528 us, 5.1 TB/s: the stream, and 5 us of the last kernel. bf16 takes as long per value for half the
+// bytes, 256 channels at 131072 without either 55 us, 3.7 TB/s. From 257 channels on a compute unit has one block, whose loads nothing covers while its sums are joined and its
+// results written: bf16, 512 at 65536 71 us, 2.9 TB/s, with both 99. 200 channels at 30011 positions, bf16, 19.2 us: 469 strips are one round, in which loads, sums, joins and stores follow one another
+// (16.0 us at 30016, where rows start at whole cache lines), and 4 us of the last kernel.
 #include "layer_norm.h"
 
 namespace tfno {
@@ -286,7 +287,7 @@ template <int IN, bool COMPLEX, bool DROP> hipError_t launch_grad(const LayerNor
         return q.K <= 64 ? launch_as<IN, COMPLEX, DROP, 64, 8>(q, stream) : launch_as<IN, COMPLEX, DROP, 64, 0>(q, stream);
     if (q.K <= 64 && q.columns >= kFewColumns) return q.K <= 32 ? launch_as<IN, COMPLEX, DROP, 64, 4>(q, stream) : launch_as<IN, COMPLEX, DROP, 64, 8>(q, stream);
     if (q.K <= 64) return launch_as<IN, COMPLEX, DROP, 16, 2>(q, stream);
-    // bf16, 128 channels at 262144 columns 84 us, 90 with 32 lanes
+    // all with residual stream and dropout: bf16, 128 channels at 262144 columns 84 us, 90 with 32 lanes
     if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, 16, 4>(q, stream);
     if (q.K <= 256) return launch_as<IN, COMPLEX, DROP, 16, 8>(q, stream);
     const bool few = q.columns < kNarrowColumns;

@@ -213,7 +213,7 @@ template <int IN, bool COMPLEX, bool DROP, bool EIGHT> hipError_t launch(const L
         if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 4>(q, stream);
         return launch_as<IN, COMPLEX, DROP, EIGHT, 16, 8>(q, stream);
     }
-    // bf16, 128 channels at 262144 columns 60 us, 65 with 64 lanes; float32, 256 at 65536 53 us, 58 with 16
+    // all with residual: bf16, 128 channels at 262144 columns 60 us, 65 with 64 lanes; float32, 256 at 65536 53 us, 58 with 16
     if (q.K <= 128) return launch_as<IN, COMPLEX, DROP, EIGHT, 32, 8>(q, stream);
     if (q.K <= 256) return launch_as<IN, COMPLEX, DROP, EIGHT, 32, 16>(q, stream);
     // float32, 512 channels at 4000 columns 8.7 us, 11.2 with 16 lanes; at 16000 24.1 and 23.0

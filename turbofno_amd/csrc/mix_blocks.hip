@@ -10,17 +10,19 @@
 //   fp32 result    the operands are widened to bf16, which holds them exactly, and take four matrix instructions whose sums are fp32.
 // Kernels, from many columns to few:
 //   direct         bf16, whole steps and 16-byte pieces: tiles of 128 or 64 rows and 128 columns, x and W read into LDS past the registers and ahead of time, x taken from
-//                  there by transposing reads. 1024 to 1024 channels at 65536 positions with GELU 134 us, 1.03 PFLOP/s; without it 127, of which 26 are the result's stores at
-//                  a copy's rate; each further 1024 channels 78 us, 1.8 PFLOP/s. There waves wait for data 34 % of their time, for their turn to issue 34 %; matrix
-//                  instructions take 28 % of the cycles, vector instructions (16 multiply-adds of totals for each 4 of the former) 29 %, LDS 17 %.
+//                  there by transposing reads. 1024 to 1024 channels at 65536 positions with GELU 134 us, 1.02 PFLOP/s; without it 123, of which 26 are the result's stores at
+//                  a copy's rate; each further 1024 channels 85 us, 1.6 PFLOP/s (passes among others, two sets of inputs in turns). With 2048 channels waves wait for data
+//                  34 % of their time, for their turn to issue 35 %; matrix instructions take 28 % of the cycles, vector instructions, which count those too, 29 %, LDS 20 %;
+//                  with 1024 and GELU 34, 30, 20, 36 and 17 %.
 //   staged         the same through registers: any strides, ends of steps and fp32 results. 1024 to 1024 at 65536 with W one byte on 120 us where direct takes 110 (inputs
-//                  in the caches); float32 176
-//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 27.7 us, 2.8 TB/s of 77.6 MB:
+//                  in the caches); float32 181
+//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 27.5 us, 2.8 TB/s of 77.6 MB:
 //                  235 x 3 tiles, less than two rounds
 //   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 6.8 us, of which an empty launch
 //                  after launch takes 3; 4096 to 4096 at 64 10.7 us, 16.8 MB of weights
 // Direct and staged tiles that are fewer than compute units: two groups of waves with half of the steps each.
 // Up to 64 real values of the contraction the kernels of the product with one scale per row are ahead, and take this one's scales.
+#include "direct_lds.h"
 #include "kernels.h"
 #include "mix_blocks_choice.h"
 #include "mix_kernel.h"
@@ -745,17 +747,6 @@ __global__ __launch_bounds__((GROUPS * Staged<OUT, NT, RG, CG>::THREADS), WAVES)
                         scalar(column0 + wc * 64), from);
 }
 
-// Memory -> LDS, 16 bytes (one word) per lane, of all lanes one after the other from `to` on, which is uniform. No register is loaded. The compiler's form of it waits for all loads
-// ahead of each transposing read (149 us instead of 135); here arrived() waits, ahead of the barrier behind which the values are read
-__device__ __forceinline__ unsigned place_in_lds(const void* p) { return (unsigned)(unsigned long)(__attribute__((address_space(3))) const char*)p; }
-__device__ __forceinline__ void direct_to_lds(ScalarAddress base, unsigned offset, unsigned to)
-{
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
-}
-__device__ __forceinline__ void direct_word_to_lds(ScalarAddress base, unsigned offset, unsigned to)
-{
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" : : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "m0", "memory");
-}
 // The same where whole steps and 16-byte pieces are all there is, for bf16 results: memory is read into LDS directly, past the registers. The registers that this leaves hold the
 // operands of x of the next step, read in the second half of this one. So a buffer of x is free again a step earlier than one of W: x is asked for two steps ahead, W one.
 // Loads arrive in their order, and the loop has no others: in the middle of a step those of the step before have, at its end those of W too. Each wait is followed by a barrier,

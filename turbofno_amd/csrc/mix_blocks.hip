@@ -11,12 +11,12 @@
 // Kernels, from many columns to few:
 //   direct         bf16, whole steps and 16-byte pieces: tiles of 128 or 64 rows and 128 columns, x and W read into LDS past the registers and ahead of time, x taken from
 //                  there by transposing reads. 1024 to 1024 channels at 65536 positions with GELU 134 us, 1.02 PFLOP/s; without it 123, of which 26 are the result's stores at
-//                  a copy's rate; each further 1024 channels 85 us, 1.6 PFLOP/s (passes among others, two sets of inputs in turns). With 2048 channels waves wait for data
-//                  34 % of their time, for their turn to issue 35 %; matrix instructions take 28 % of the cycles, vector instructions, which count those too, 29 %, LDS 20 %;
-//                  with 1024 and GELU 34, 30, 20, 36 and 17 %.
+//                  a copy's rate; each further 1024 channels 81 us, 1.7 PFLOP/s (passes among others, two sets of inputs in turns). With 2048 channels waves wait for data
+//                  36 % of their time, for their turn to issue 33 %; matrix instructions take 28 % of the cycles, vector instructions, which count those too, 28 %, LDS 19 %;
+//                  with 1024 and GELU 35, 28, 20, 36 and 17 %.
 //   staged         the same through registers: any strides, ends of steps and fp32 results. 1024 to 1024 at 65536 with W one byte on 120 us where direct takes 110 (inputs
 //                  in the caches); float32 181
-//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 27.5 us, 2.8 TB/s of 77.6 MB:
+//   tile           complex: x through registers, whose lanes transpose 4 x 4 bytes; W through LDS. 200 to 136 at 30011 with SiLU and residual 27.4 us, 2.8 TB/s of 77.6 MB:
 //                  235 x 3 tiles, less than two rounds
 //   split          few columns: the eight waves of a block divide the steps of 64 columns and 16 rows. 2048 to 2048 at 16 positions 6.8 us, of which an empty launch
 //                  after launch takes 3; 4096 to 4096 at 64 10.7 us, 16.8 MB of weights
